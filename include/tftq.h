@@ -205,6 +205,40 @@ int tftq_dequantize_scaled(const tftq_plan *plan, void *const *tensors, const vo
 int tftq_reduce_static(const tftq_plan *plan, void *packed, int64_t packed_bytes, int rank,
                        int is_avg, int device, void *stream);
 
+/*
+ * 4-bit microscaled matrices (no counterpart in the reference): the weights, activations and
+ * gradients of a linear layer whose products run on the 4-bit matrix cores.
+ *
+ * Blocks of 32 consecutive elements of a row share a scale 2^e, e = clamp(floor(log2 max|x|) - 2,
+ * -127, 127), held as the byte e + 127; an element is the nearest of 0, .5, 1, 1.5, 2, 3, 4, 6 to
+ * x / 2^e with its sign (ties to the even mantissa, larger values 6), held in 4 bits (sign, two
+ * bits of exponent, one of mantissa), two to a byte, the first in the low half.  The last block of
+ * a row may be shorter.  A block that holds an infinity or a NaN has the byte 255 and reads as NaN.
+ *
+ * A matrix [rows, cols] is one buffer of tftq_mx_bytes(rows, cols) bytes, 16-byte aligned, that the
+ * caller owns.  With P = ceil(cols / 256) panels:
+ *    codes   [P][rows][128]            columns 256 p to 256 p + 255 of every row, zero past the last one
+ *    scales  [P][rows rounded up to an even number][8]   of those columns' blocks
+ */
+/* bytes of a matrix, or TFTQ_E_SHAPE */
+int64_t tftq_mx_bytes(int64_t rows, int64_t cols);
+
+/*
+ * Quantises x [rows, cols] (row_stride elements from row to row, columns contiguous) along its rows
+ * into by_rows, a matrix [rows, cols], and along its columns into by_cols, a matrix [cols, rows]:
+ * either may be NULL.  x is read once for both.
+ */
+int tftq_mx_quantize(int dtype, const void *x, int64_t rows, int64_t cols, int64_t row_stride, void *by_rows,
+                     void *by_cols, int device, void *stream);
+
+/* The values that a matrix [rows, cols] stands for, rounded once to `dtype`. */
+int tftq_mx_dequantize(int dtype, const void *matrix, int64_t rows, int64_t cols, void *out, int64_t row_stride,
+                       int device, void *stream);
+
+/* out [m, n] = a [m, k] b [n, k]^T of two matrices, summed in fp32 and rounded once to `dtype`. */
+int tftq_mx_product(int dtype, const void *a, int64_t m, const void *b, int64_t n, int64_t k, void *out,
+                    int64_t row_stride, int device, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,6 +9,14 @@ from .quantization import (  # noqa: F401
     prepare,
 )
 
+from .mxfp4 import (  # noqa: F401
+    MXFP4Tensor,
+    linear_mxfp4,
+    matmul_mxfp4,
+    quantize_mxfp4,
+    quantize_mxfp4_both,
+)
+
 from .collectives import (  # noqa: F401
     allocate_reduce_scatter_output,
     allreduce_quantized,
@@ -26,4 +34,9 @@ __all__ = [
     "fused_reduce_fp8",
     "prepare",
     "PreparedBucket",
+    "MXFP4Tensor",
+    "linear_mxfp4",
+    "matmul_mxfp4",
+    "quantize_mxfp4",
+    "quantize_mxfp4_both",
 ]

@@ -45,6 +45,14 @@ SYMBOLS = [
     ("tftq_dequantize_scaled", _c.c_int, [_P, _P, _P, _P, _P, _c.c_int64, _c.c_float, _c.c_int, _P]),
     # plan, packed, packed_bytes, rank, is_avg, device, stream
     ("tftq_reduce_static", _c.c_int, [_P, _P, _c.c_int64, _c.c_int, _c.c_int, _c.c_int, _P]),
+    # rows, cols
+    ("tftq_mx_bytes", _c.c_int64, [_c.c_int64, _c.c_int64]),
+    # dtype, x, rows, cols, row_stride, by_rows, by_cols, device, stream
+    ("tftq_mx_quantize", _c.c_int, [_c.c_int, _P, _c.c_int64, _c.c_int64, _c.c_int64, _P, _P, _c.c_int, _P]),
+    # dtype, matrix, rows, cols, out, row_stride, device, stream
+    ("tftq_mx_dequantize", _c.c_int, [_c.c_int, _P, _c.c_int64, _c.c_int64, _P, _c.c_int64, _c.c_int, _P]),
+    # dtype, a, m, b, n, k, out, row_stride, device, stream
+    ("tftq_mx_product", _c.c_int, [_c.c_int, _P, _c.c_int64, _P, _c.c_int64, _c.c_int64, _P, _c.c_int64, _c.c_int, _P]),
 ]
 ABI_VERSION = 2
 

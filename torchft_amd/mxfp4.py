@@ -1,0 +1,220 @@
+"""Linear layers on 4-bit microscaled matrices (no counterpart in the reference).
+
+A matrix is kept as 4-bit numbers (sign, two bits of exponent, one of mantissa: 0, .5, 1, 1.5, 2, 3, 4
+and 6) with a power of two for every 32 of them along the axis that a product contracts, 4.25 bits an
+element; the matrix cores of gfx950 multiply such matrices four times as fast as 16-bit ones.
+
+* :func:`quantize_mxfp4` / :func:`quantize_mxfp4_both` make an :class:`MXFP4Tensor` of a matrix, along
+  its rows, its columns or both in one pass over it;
+* :func:`matmul_mxfp4` is the product ``a @ b.T`` of two of them;
+* :func:`linear_mxfp4` is ``x @ weight.T`` of ordinary tensors, with gradients: each of the three
+  products of a training step takes both operands quantised along the axis that it contracts, and the
+  rounding to 4 bits counts as the identity.  With a weight that is an :class:`MXFP4Tensor` already (a
+  model that is served) only ``x`` is quantised in the call.
+
+Kernels are enqueued on the current stream of the tensors' device; nothing synchronises the host, and
+no function keeps anything from one call for the next.  There is no CPU or eager fallback.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .quantization import _DTYPE_CODE, _check, _stream_of
+
+_BLOCK = 32    # elements of a scale
+_PANEL = 256   # columns of a panel
+_PANEL_BYTES = _PANEL // 2
+_PANEL_BLOCKS = _PANEL // _BLOCK
+
+
+class MXFP4Tensor:
+    """A matrix ``[rows, columns]`` in 4-bit microscaled form, blocks of 32 along its rows.
+
+    ``buffer`` holds it in the order in which the product reads it (``tftq_mx_bytes`` of
+    ``include/tftq.h`` describes it); :attr:`codes` and :attr:`scales` are copies in the usual order.
+    ``dtype`` is what it was quantised from and what :meth:`dequantize` and products return by
+    default.  It is no ``torch.Tensor``: it has no gradient and takes part in the functions of this module."""
+
+    __slots__ = ("buffer", "shape", "dtype")
+
+    def __init__(self, buffer: torch.Tensor, shape: tuple, dtype: torch.dtype) -> None:
+        self.buffer = buffer
+        self.shape = torch.Size(shape)
+        self.dtype = dtype
+
+    @classmethod
+    def from_blocks(cls, codes: torch.Tensor, scales: torch.Tensor, columns: int,
+                    dtype: torch.dtype = torch.bfloat16) -> "MXFP4Tensor":
+        """The matrix of ``columns`` columns that ``codes`` ``[rows, blocks, 16]`` (two codes a byte, the
+        first in the low half) and ``scales`` ``[rows, blocks]`` (exponents plus 127, 255 for NaN) hold, as
+        checkpoints keep it.  Codes past the last column are taken as zero."""
+        assert codes.dtype == torch.uint8 and scales.dtype == torch.uint8, "Codes and scales are uint8"
+        assert codes.dim() == 3 and codes.shape[2] == _BLOCK // 2, "Codes are [rows, blocks, 16]"
+        assert scales.shape == codes.shape[:2], "Scales are [rows, blocks]"
+        assert 0 <= columns <= codes.shape[1] * _BLOCK and codes.shape[1] == -(-columns // _BLOCK), \
+            "The blocks do not fit the number of columns"
+        assert scales.device == codes.device, "Codes and scales must be on the same device"
+        assert dtype in _DTYPE_CODE, "Only fp32, fp16 and bf16 are supported"
+        rows, blocks = scales.shape
+        self = _empty(rows, columns, dtype, codes.device)
+        if rows == 0 or columns == 0:
+            return self
+        panels = -(-columns // _PANEL)
+        past = columns % _BLOCK
+        if past:
+            codes = codes.clone()
+            if past % 2:
+                codes[:, -1, past // 2] &= 15
+            codes[:, -1, (past + 1) // 2:] = 0
+        more = panels * _PANEL_BLOCKS - blocks
+        by_panel = self._panel_views()
+        by_panel[0].copy_(torch.nn.functional.pad(codes, (0, 0, 0, more)).view(rows, panels, _PANEL_BYTES).transpose(0, 1))
+        by_panel[1].zero_()
+        by_panel[1][:, :rows].copy_(torch.nn.functional.pad(scales, (0, more)).view(rows, panels, _PANEL_BLOCKS).transpose(0, 1))
+        return self
+
+    def _panel_views(self):
+        rows, columns = self.shape
+        panels, even = -(-columns // _PANEL), rows + rows % 2
+        split = panels * rows * _PANEL_BYTES
+        return (self.buffer[:split].view(panels, rows, _PANEL_BYTES),
+                self.buffer[split:split + panels * even * _PANEL_BLOCKS].view(panels, even, _PANEL_BLOCKS))
+
+    @property
+    def device(self) -> torch.device:
+        return self.buffer.device
+
+    @property
+    def codes(self) -> torch.Tensor:
+        """``[rows, blocks, 16]`` bytes of two codes each."""
+        rows, columns = self.shape
+        codes = self._panel_views()[0].transpose(0, 1)
+        return codes.reshape(rows, codes.shape[1] * _PANEL_BLOCKS, _BLOCK // 2)[:, :-(-columns // _BLOCK)]
+
+    @property
+    def scales(self) -> torch.Tensor:
+        """``[rows, blocks]`` exponents plus 127; 255 for a block that is NaN."""
+        rows, columns = self.shape
+        scales = self._panel_views()[1][:, :rows].transpose(0, 1)
+        return scales.reshape(rows, scales.shape[1] * _PANEL_BLOCKS)[:, :-(-columns // _BLOCK)]
+
+    def dequantize(self, dtype: torch.dtype | None = None) -> torch.Tensor:
+        """The values that the matrix stands for, rounded once to ``dtype``."""
+        dtype = self.dtype if dtype is None else dtype
+        assert dtype in _DTYPE_CODE, "Only fp32, fp16 and bf16 are supported"
+        rows, columns = self.shape
+        out = torch.empty(rows, columns, dtype=dtype, device=self.device)
+        _check(_lib.load().tftq_mx_dequantize(_DTYPE_CODE[dtype], self.buffer.data_ptr(), rows, columns, out.data_ptr(),
+                                              columns, self.device.index, _stream_of(self.device)),
+               "tftq_mx_dequantize")
+        return out
+
+    def record_stream(self, stream: torch.cuda.Stream) -> None:
+        """As ``torch.Tensor.record_stream``: the memory is used on another stream than the one it was made on."""
+        self.buffer.record_stream(stream)
+
+    def __repr__(self) -> str:
+        return f"MXFP4Tensor({self.shape[0]}x{self.shape[1]}, of {self.dtype}, on {self.device})"
+
+
+def _empty(rows: int, columns: int, dtype: torch.dtype, device: torch.device) -> MXFP4Tensor:
+    assert device.type == "cuda", "A GPU tensor is required"
+    _lib.check_device(device.index)
+    size = _lib.load().tftq_mx_bytes(rows, columns)
+    if size < 0:
+        _check(size, "tftq_mx_bytes")
+    return MXFP4Tensor(torch.empty(size, dtype=torch.uint8, device=device), (rows, columns), dtype)
+
+
+def _quantize(x: torch.Tensor, by_rows: bool, by_columns: bool):
+    """(rows, columns), None for what is not asked for."""
+    assert x.dim() == 2, "Only 2D tensors are supported"
+    assert x.dtype in _DTYPE_CODE, "Only fp32, fp16 and bf16 are supported"
+    x = x.detach()
+    rows, columns = x.shape
+    if columns > 1 and x.stride(1) != 1 or rows > 1 and x.stride(0) < columns:
+        if x.stride(0) == 1 and x.stride(1) >= rows:  # stored column by column: its transpose is stored by rows
+            flipped = _quantize(x.t(), by_columns, by_rows)
+            return flipped[1], flipped[0]
+        x = x.contiguous()
+    r = _empty(rows, columns, x.dtype, x.device) if by_rows else None
+    c = _empty(columns, rows, x.dtype, x.device) if by_columns else None
+    _check(_lib.load().tftq_mx_quantize(_DTYPE_CODE[x.dtype], x.data_ptr(), rows, columns, x.stride(0),
+                                        r.buffer.data_ptr() if by_rows else None, c.buffer.data_ptr() if by_columns else None,
+                                        x.device.index, _stream_of(x.device)),
+           "tftq_mx_quantize")
+    return r, c
+
+
+def quantize_mxfp4(x: torch.Tensor, dim: int = -1) -> MXFP4Tensor:
+    """The matrix ``x`` in 4-bit microscaled form, blocks of 32 along ``dim``; with ``dim=0`` the result is
+    the transposed matrix, whose rows are the columns of ``x``."""
+    assert dim in (-2, -1, 0, 1), "Only 2D tensors are supported"
+    return _quantize(x, True, False)[0] if dim in (-1, 1) else _quantize(x, False, True)[1]
+
+
+def quantize_mxfp4_both(x: torch.Tensor) -> "tuple[MXFP4Tensor, MXFP4Tensor]":
+    """``(quantize_mxfp4(x), quantize_mxfp4(x, 0))`` in one pass over ``x``."""
+    return _quantize(x, True, True)
+
+
+def matmul_mxfp4(a: MXFP4Tensor, b: MXFP4Tensor, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``a @ b.T``, summed in float32 and rounded once to ``out_dtype`` (``a.dtype`` by default)."""
+    out_dtype = a.dtype if out_dtype is None else out_dtype
+    assert out_dtype in _DTYPE_CODE, "Only fp32, fp16 and bf16 are supported"
+    assert a.device == b.device, "All inputs must be on the same device"
+    assert a.shape[1] == b.shape[1], "The matrices have different numbers of columns"
+    (m, k), n = a.shape, b.shape[0]
+    out = torch.empty(m, n, dtype=out_dtype, device=a.device)
+    _check(_lib.load().tftq_mx_product(_DTYPE_CODE[out_dtype], a.buffer.data_ptr(), m, b.buffer.data_ptr(), n, k,
+                                       out.data_ptr(), n, a.device.index, _stream_of(a.device)),
+           "tftq_mx_product")
+    return out
+
+
+class _Linear(torch.autograd.Function):
+    """``x @ w.T`` of matrices; what the backward pass contracts along other axes is quantised along
+    them while the forward pass reads x and w, and kept in place of x and w: 4.25 bits an element."""
+
+    @staticmethod
+    def forward(ctx, x, w):
+        for_dw, for_dx = ctx.needs_input_grad[1], ctx.needs_input_grad[0]
+        ctx.dtypes = x.dtype, w.dtype
+        x_rows, ctx.x_columns = _quantize(x, True, for_dw)
+        w_rows, ctx.w_columns = _quantize(w, True, for_dx)
+        return matmul_mxfp4(x_rows, w_rows, x.dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x_columns, w_columns = ctx.x_columns, ctx.w_columns
+        dy_rows, dy_columns = _quantize(dy, w_columns is not None, x_columns is not None)
+        dx = matmul_mxfp4(dy_rows, w_columns, ctx.dtypes[0]) if w_columns is not None else None
+        dw = matmul_mxfp4(dy_columns, x_columns, ctx.dtypes[1]) if x_columns is not None else None
+        return dx, dw
+
+
+def linear_mxfp4(x: torch.Tensor, weight: "torch.Tensor | MXFP4Tensor") -> torch.Tensor:
+    """``x @ weight.T`` on the 4-bit matrix cores: ``x`` ``[..., k]`` and ``weight`` ``[n, k]`` are quantised
+    along ``k`` in the call (a weight that is an :class:`MXFP4Tensor` is taken as it is), the sums
+    are float32, the result has the type of ``x``.
+
+    With a weight that is a tensor both gradients are available:
+    ``dx = dy @ weight`` and ``dw = dy.T @ x`` with every operand quantised along the contracted axis.
+    A weight that is kept in 4 bits along ``k`` cannot be contracted along ``n``: gradients through it are
+    refused."""
+    assert x.dim() >= 1, "x has at least one dimension"
+    assert x.dtype in _DTYPE_CODE, "Only fp32, fp16 and bf16 are supported"
+    assert len(weight.shape) == 2 and x.shape[-1] == weight.shape[1], "The last dimension of x is not the weight's number of columns"
+    assert x.device == weight.device, "All inputs must be on the same device"
+    flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1]) if x.numel() else x.new_empty(x.shape[:-1].numel(), x.shape[-1])
+    if isinstance(weight, MXFP4Tensor):
+        assert not (torch.is_grad_enabled() and x.requires_grad), "A weight in 4 bits has no gradient product"
+        y = matmul_mxfp4(_quantize(flat, True, False)[0], weight, x.dtype)
+    else:
+        assert weight.dtype in _DTYPE_CODE, "Only fp32, fp16 and bf16 are supported"
+        y = _Linear.apply(flat, weight)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], weight.shape[0])
