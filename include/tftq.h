@@ -239,6 +239,46 @@ int tftq_mx_dequantize(int dtype, const void *matrix, int64_t rows, int64_t cols
 int tftq_mx_product(int dtype, const void *a, int64_t m, const void *b, int64_t n, int64_t k, void *out,
                     int64_t row_stride, int device, void *stream);
 
+/*
+ * Newton-Schulz orthogonalisation of a list of matrices, and the step of the Muon optimiser (no
+ * counterpart in the reference): what a replica does with the averaged gradients of its weight
+ * matrices.  For every matrix u [rows, cols]:
+ *    X = u / max(|u|_F, eps);  iterations times:  X = a X + (b (X X^T) + c (X X^T)^2) X
+ * (of u^T where rows > cols).  Products run on the 16-bit matrix cores with fp32 sums; with `precise`
+ * set every one is three, of high and low parts, and the result has the accuracy of fp32 products
+ * (as has, in any case, that of a matrix with fewer than 64 rows or columns).
+ */
+typedef struct tftq_ns {
+    int n;                          /* matrices; empty ones are left alone */
+    const int64_t *shapes;          /* [n][2] rows, columns: at most 2^24 each */
+    const void *const *in;          /* gradients; columns contiguous */
+    const int64_t *in_stride;       /* [n] elements from row to row */
+    int in_dtype;
+    float *const *momenta;          /* NULL: u is the gradient.  Else m = momentum m + (1 - momentum) g, in place, */
+    const int64_t *momenta_stride;  /* and u = m, or g + momentum (m - g) with nesterov */
+    float momentum;
+    int nesterov;
+    void *const *out;
+    const int64_t *out_stride;
+    int out_dtype;
+    const float *steps;             /* NULL: out = X.  Else [n], and out = keep out - step X */
+    float keep;
+    int iterations;                 /* at least 1 */
+    const float *coefficients;      /* [iterations][3] a, b, c */
+    float eps;
+    int precise;
+} tftq_ns;
+
+/* bytes that tftq_newton_schulz needs for these matrices, or TFTQ_E_ARG / TFTQ_E_SHAPE */
+int64_t tftq_newton_schulz_workspace(int n, const int64_t *shapes, int precise);
+
+/*
+ * `what` and the host arrays it names are read before the call returns.  `workspace` is device
+ * memory, 128-byte aligned, of workspace_bytes bytes (TFTQ_E_SIZE if too few), and holds nothing
+ * between calls.  A gradient may be the matrix that `out` names when it has no momentum.
+ */
+int tftq_newton_schulz(const tftq_ns *what, void *workspace, int64_t workspace_bytes, int device, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -17,6 +17,8 @@ from .mxfp4 import (  # noqa: F401
     quantize_mxfp4_both,
 )
 
+from .muon import Muon, muon_, orthogonalize  # noqa: F401
+
 from .collectives import (  # noqa: F401
     allocate_reduce_scatter_output,
     allreduce_quantized,
@@ -39,4 +41,7 @@ __all__ = [
     "matmul_mxfp4",
     "quantize_mxfp4",
     "quantize_mxfp4_both",
+    "Muon",
+    "muon_",
+    "orthogonalize",
 ]

@@ -13,7 +13,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_HERE, "csrc")
 LIB_PATH = os.path.join(_HERE, "libtftq.so")
 SOURCES = ["tftq_quantize.hip", "tftq_dequantize.hip", "tftq_reduce.hip", "tftq_reduce_all.hip", "tftq_reduce_wide.hip",
-           "tftq_reduce_long.hip", "tftq_reduce_one.hip", "tftq_runtime.hip", "tftq_mxfp4.hip", "tftq_mxfp4_product.hip",
+           "tftq_reduce_long.hip", "tftq_reduce_one.hip", "tftq_runtime.hip", "tftq_mxfp4.hip", "tftq_mxfp4_product.hip", "tftq_orthogonal.hip",
            "tftq_plan.cpp"]
 # Streaming kernels without arithmetic that bench.py times beside the product kernels
 # (benchmark infrastructure; torchft_amd never loads this library).

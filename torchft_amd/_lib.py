@@ -19,6 +19,19 @@ ERR_NAMES = {
 # every symbol that include/tftq.h declares: (name, restype, argtypes)
 _c = ctypes
 _P = _c.c_void_p
+_L = _c.POINTER(_c.c_int64)
+
+
+class NewtonSchulz(_c.Structure):
+    """``tftq_ns``."""
+
+    _fields_ = [("n", _c.c_int), ("shapes", _L), ("inputs", _c.POINTER(_P)), ("in_stride", _L), ("in_dtype", _c.c_int),
+                ("momenta", _c.POINTER(_P)), ("momenta_stride", _L), ("momentum", _c.c_float), ("nesterov", _c.c_int),
+                ("out", _c.POINTER(_P)), ("out_stride", _L), ("out_dtype", _c.c_int), ("steps", _c.POINTER(_c.c_float)),
+                ("keep", _c.c_float), ("iterations", _c.c_int), ("coefficients", _c.POINTER(_c.c_float)),
+                ("eps", _c.c_float), ("precise", _c.c_int)]
+
+
 SYMBOLS = [
     ("tftq_version", _c.c_int, []),
     ("tftq_build_id", _c.c_char_p, []),
@@ -51,6 +64,10 @@ SYMBOLS = [
     ("tftq_mx_quantize", _c.c_int, [_c.c_int, _P, _c.c_int64, _c.c_int64, _c.c_int64, _P, _P, _c.c_int, _P]),
     # dtype, matrix, rows, cols, out, row_stride, device, stream
     ("tftq_mx_dequantize", _c.c_int, [_c.c_int, _P, _c.c_int64, _c.c_int64, _P, _c.c_int64, _c.c_int, _P]),
+    # n, shapes, precise
+    ("tftq_newton_schulz_workspace", _c.c_int64, [_c.c_int, _L, _c.c_int]),
+    # what, workspace, workspace_bytes, device, stream
+    ("tftq_newton_schulz", _c.c_int, [_c.POINTER(NewtonSchulz), _P, _c.c_int64, _c.c_int, _P]),
     # dtype, a, m, b, n, k, out, row_stride, device, stream
     ("tftq_mx_product", _c.c_int, [_c.c_int, _P, _c.c_int64, _P, _c.c_int64, _c.c_int64, _P, _c.c_int64, _c.c_int, _P]),
 ]

@@ -42,7 +42,7 @@ __global__ __launch_bounds__(T::THREADS) void k_mx_product(TileOperand a, TileOp
     tile_place(tile_piece(blockIdx.x, gridDim.x), tiles_m, tiles_n, &tm, &tn);
     T t;
     t.zero();
-    t.multiply(a, b, 0, panels, tm * T::ROWS, tn * T::COLS, lds);
+    t.multiply(TilePair{a, b}, 0, panels, tm * T::ROWS, tn * T::COLS, lds);
     t.store_strips(tm * T::ROWS, tn * T::COLS, lds, [&](const float *strip, int row, int col) {
         const int lane = threadIdx.x & 63;
         if (whole) {

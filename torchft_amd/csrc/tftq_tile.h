@@ -38,6 +38,39 @@ struct TileOperand {
     int rows;
 };
 
+// Two operands as fp16 numbers and what their rounding left, as fp16 numbers too: the products high x
+// high, low x high and high x low, one after the other, as one sum over three times the panels.
+struct TileSplit {
+    const uint8_t *a_high, *a_low, *b_high, *b_low;
+    int a_rows, b_rows, panels;
+};
+// What a step of a tile's loop multiplies: panel s of either operand.
+struct TilePanels {
+    const uint8_t *a, *b, *a_scales, *b_scales;
+};
+struct TilePair {  // one product
+    TileOperand a, b;
+    __device__ int a_rows() const { return a.rows; }
+    __device__ int b_rows() const { return b.rows; }
+    __device__ TilePanels at(int s) const
+    {
+        return {a.panels + (int64_t)s * a.rows * PANEL_BYTES, b.panels + (int64_t)s * b.rows * PANEL_BYTES,
+                a.scales + (int64_t)s * ((a.rows + 1) & ~1) * 8, b.scales + (int64_t)s * ((b.rows + 1) & ~1) * 8};
+    }
+};
+struct TileTriple {  // three
+    TileSplit o;
+    __device__ int a_rows() const { return o.a_rows; }
+    __device__ int b_rows() const { return o.b_rows; }
+    __device__ TilePanels at(int s) const
+    {
+        const uint8_t *a = o.a_high, *b = o.b_high;
+        if (s >= 2 * o.panels) b = o.b_low, s -= 2 * o.panels;
+        else if (s >= o.panels) a = o.a_low, s -= o.panels;
+        return {a + (int64_t)s * o.a_rows * PANEL_BYTES, b + (int64_t)s * o.b_rows * PANEL_BYTES, nullptr, nullptr};
+    }
+};
+
 __device__ static inline void tile_load16(const uint8_t *from, uint8_t *lds)
 {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
@@ -97,20 +130,23 @@ struct Tile {
             tile_load16(scales + (int64_t)pair * 16, lds + wave * 1024);
         }
     }
-    __device__ static void load(const TileOperand &a, const TileOperand &b, int s, int row0, int col0, uint8_t *buf)
+    template <class P>
+    __device__ static void load(const P &p, int s, int row0, int col0, uint8_t *buf)
     {
-        load_rows<BM>(a.panels + (int64_t)s * a.rows * PANEL_BYTES, a.rows, row0, buf);
-        load_rows<BN>(b.panels + (int64_t)s * b.rows * PANEL_BYTES, b.rows, col0, buf + BM * PANEL_BYTES);
+        const TilePanels at = p.at(s);
+        load_rows<BM>(at.a, p.a_rows(), row0, buf);
+        load_rows<BN>(at.b, p.b_rows(), col0, buf + BM * PANEL_BYTES);
         if (FP4) {
             uint8_t *sc = buf + (BM + BN) * PANEL_BYTES;
-            load_scales<BM>(a.scales + (int64_t)s * ((a.rows + 1) & ~1) * 8, a.rows, row0, sc, 0);
-            load_scales<BN>(b.scales + (int64_t)s * ((b.rows + 1) & ~1) * 8, b.rows, col0, sc + SCALES_M, WAVES / 2);
+            load_scales<BM>(at.a_scales, p.a_rows(), row0, sc, 0);
+            load_scales<BN>(at.b_scales, p.b_rows(), col0, sc + SCALES_M, WAVES / 2);
         }
     }
 
     // acc += the product over panels [s0, s1) of the tile at (row0, col0).  Every wavefront of the
     // workgroup calls it with the same arguments.
-    __device__ void multiply(const TileOperand &a, const TileOperand &b, int s0, int s1, int row0, int col0, uint8_t *lds)
+    template <class P>
+    __device__ void multiply(const P &p, int s0, int s1, int row0, int col0, uint8_t *lds)
     {
         if (s0 >= s1) return;
         const int lane = threadIdx.x & 63, wave = tile_wave();
@@ -121,11 +157,11 @@ struct Tile {
         for (int q = 0; q < 4; q++) place[q] = ((2 * q + half) ^ (lane & 7)) * 16;
         const int a_at = (wm + in_row) * PANEL_BYTES, b_at = (BM + wn + in_row) * PANEL_BYTES;
 
-        load(a, b, s0, row0, col0, lds);
+        load(p, s0, row0, col0, lds);
         int cur = 0;
         for (int s = s0; s < s1; s++) {
             __syncthreads();  // panel s has landed; nobody reads the other buffer any more
-            if (s + 1 < s1) load(a, b, s + 1, row0, col0, lds + (cur ^ BUFFER));
+            if (s + 1 < s1) load(p, s + 1, row0, col0, lds + (cur ^ BUFFER));
             const uint8_t *buf = lds + cur;
             uint32_t sa[TM][2], sb[TN][2];
             if (FP4) {
