@@ -5,30 +5,16 @@
 #include "tftq_device.h"
 #include "tftq_mxfp4.h"
 
+// A result as it is stored.
 template <int DTYPE>
 struct MxOut {
     static constexpr int SIZE = DTYPE == TFTQ_F32 ? 4 : 2, V = 16 / SIZE;
-    __device__ static void put(uint8_t *to, float v)
+    typedef _Float16 H2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 B2 __attribute__((ext_vector_type(2)));
+    __device__ static uint32_t two(float a, float b)
     {
-        if constexpr (DTYPE == TFTQ_F32) *(float *)to = v;
-        else if constexpr (DTYPE == TFTQ_F16) *(_Float16 *)to = (_Float16)v;
-        else *(__bf16 *)to = (__bf16)v;
-    }
-    __device__ static void put_vector(uint8_t *to, const float *v)
-    {
-        tile_i4 w;
-        if constexpr (DTYPE == TFTQ_F32) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) w[i] = __float_as_int(v[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint16_t lo = DTYPE == TFTQ_F16 ? __builtin_bit_cast(uint16_t, (_Float16)v[2 * i]) : __builtin_bit_cast(uint16_t, (__bf16)v[2 * i]);
-                const uint16_t hi = DTYPE == TFTQ_F16 ? __builtin_bit_cast(uint16_t, (_Float16)v[2 * i + 1]) : __builtin_bit_cast(uint16_t, (__bf16)v[2 * i + 1]);
-                w[i] = (int)(lo | (uint32_t)hi << 16);
-            }
-        }
-        *(tile_i4 *)to = w;
+        if constexpr (DTYPE == TFTQ_F16) return __builtin_bit_cast(uint32_t, H2{(_Float16)a, (_Float16)b});
+        else return __builtin_bit_cast(uint32_t, B2{(__bf16)a, (__bf16)b});
     }
 };
 
@@ -36,27 +22,31 @@ template <class T, int DTYPE>
 __global__ __launch_bounds__(T::THREADS) void k_mx_product(TileOperand a, TileOperand b, int panels, uint8_t *out, int64_t ld,
                                                            int whole, int tiles_m, int tiles_n)
 {
-    __shared__ __attribute__((aligned(128))) uint8_t lds[T::LDS];
+    __shared__ __attribute__((aligned(128))) uint8_t lds[T::LDS_PIECES];
     using O = MxOut<DTYPE>;
-    int tm, tn;
-    tile_place(tile_piece(blockIdx.x, gridDim.x), tiles_m, tiles_n, &tm, &tn);
+    int apart, pieces;
+    const int first = tile_pieces(blockIdx.x, gridDim.x, tiles_m * tiles_n, &apart, &pieces);
+    auto place = [&](int n, int *row0, int *col0) {
+        int tm, tn;
+        tile_place(first + n * apart, tiles_m, tiles_n, &tm, &tn);
+        *row0 = tm * T::ROWS, *col0 = tn * T::COLS;
+    };
     T t;
-    t.zero();
-    t.multiply(TilePair{a, b}, 0, panels, tm * T::ROWS, tn * T::COLS, lds);
-    t.store_strips(tm * T::ROWS, tn * T::COLS, lds, [&](const float *strip, int row, int col) {
-        const int lane = threadIdx.x & 63;
-        if (whole) {
-            constexpr int ACROSS = T::WN / O::V, AT_ONCE = 64 / ACROSS;
-            const int c = lane % ACROSS * O::V;
-            if (col + c >= b.rows) return;
+    t.multiply(TilePair{a, b}, panels, pieces, place, lds, [&](int row0, int col0) {
+        t.template store_pieces<O::SIZE>(row0, col0, lds + 2 * T::BUFFER, O::two, [&](tile_i4 v, int row, int col) {
+            if (row >= a.rows) return;
+            uint8_t *at = out + ((int64_t)row * ld + col) * O::SIZE;
+            if (whole) {
+                if (col < b.rows) *(tile_i4 *)at = v;
+                return;
+            }
 #pragma unroll
-            for (int r = lane / ACROSS; r < 32; r += AT_ONCE)
-                if (row + r < a.rows) O::put_vector(out + ((int64_t)(row + r) * ld + col + c) * O::SIZE, strip + r * T::PITCH + c);
-        } else {
-            for (int r = 0; r < 32 && row + r < a.rows; r++)
-                for (int c = lane; c < T::WN && col + c < b.rows; c += 64)
-                    O::put(out + ((int64_t)(row + r) * ld + col + c) * O::SIZE, strip[r * T::PITCH + c]);
-        }
+            for (int n = 0; n < O::V; n++) {
+                if (col + n >= b.rows) return;
+                if constexpr (O::SIZE == 4) ((int *)at)[n] = v[n];
+                else ((uint16_t *)at)[n] = (uint16_t)(v[n / 2] >> (16 * (n & 1)));
+            }
+        });
     });
 }
 
@@ -72,7 +62,9 @@ static int product(int dtype, const TileOperand &a, const TileOperand &b, int pa
     const void *k = dtype == TFTQ_F32 ? (const void *)k_mx_product<T, TFTQ_F32>
                     : dtype == TFTQ_F16 ? (const void *)k_mx_product<T, TFTQ_F16>
                                         : (const void *)k_mx_product<T, TFTQ_BF16>;
-    return (int)hipLaunchKernel(k, dim3((unsigned)(tiles_m * tiles_n)), dim3(T::THREADS), args, 0, st);
+    // as many workgroups as the 256 compute units hold at once; each takes its tiles one after the other
+    const int resident = 256 * (160 * 1024 / T::LDS_PIECES), tiles = tiles_m * tiles_n;
+    return (int)hipLaunchKernel(k, dim3((unsigned)(tiles < resident ? tiles : resident)), dim3(T::THREADS), args, 0, st);
 }
 
 extern "C" int tftq_mx_product(int dtype, const void *a, int64_t m, const void *b, int64_t n, int64_t k, void *out,

@@ -287,9 +287,10 @@ __global__ __launch_bounds__(T::THREADS) void k_ns_product(const NsLaunch l, con
     const uint8_t *bh = WHAT == NS_A ? w.x : WHAT == NS_B ? w.e : turn ? w.t2 : w.t, *bl = WHAT == NS_A ? w.xl : WHAT == NS_B ? w.el : turn ? w.tl2 : w.tl;
     const int panels = WHAT == NS_A ? (k + 63) >> 6 : rp, b_rows = WHAT == NS_X ? k : r;
     T t;
-    t.zero();
-    if (PRECISE) t.multiply(TileTriple{{ah, al, bh, bl, r, b_rows, panels}}, 0, 3 * panels, row0, col0, lds);
-    else t.multiply(TilePair{{ah, nullptr, r}, {bh, nullptr, b_rows}}, 0, panels, row0, col0, lds);
+    auto place = [&](int, int *r0, int *c0) { *r0 = row0, *c0 = col0; };
+    auto done = [](int, int) {};
+    if constexpr (PRECISE) t.multiply(TileTriple{{ah, al, bh, bl, r, b_rows, panels}}, 3 * panels, 1, place, lds, done);
+    else t.multiply(TilePair{{ah, nullptr, r}, {bh, nullptr, b_rows}}, panels, 1, place, lds, done);
 
     // The result's panels: along its rows, and along its columns (its transpose), each with its remainder.
     uint8_t *out = WHAT == NS_A ? w.e : WHAT == NS_B ? w.g : w.x, *out_l = WHAT == NS_A ? w.el : WHAT == NS_B ? w.gl : w.xl;

@@ -12,8 +12,8 @@
 // lane / 32 of a slice of 32 bytes.  One kernel body therefore serves both; the 4-bit one also hands the
 // instruction the scale of the lane's 32 codes.
 //
-// Staging: global_load_lds of 16 bytes per lane, 8 rows per instruction, two buffers, one barrier per
-// panel; the loads of panel s + 1 run while panel s is multiplied.  A wavefront's bytes land in LDS in
+// Staging: loads straight into LDS, 16 bytes per lane and 8 rows per instruction, two buffers, one barrier per
+// panel; panel s + 2 is loaded from the moment when panel s has been read, a whole panel ahead.  A wavefront's bytes land in LDS in
 // lane order, so the order in which lanes take the 16-byte pieces of their row is what arranges the
 // buffer: piece p of row r lies at place p ^ (r % 8), and the 8 lanes that one cycle of ds_read_b128
 // serves, 8 neighbouring rows, find their pieces in 8 different groups of banks.
@@ -23,6 +23,7 @@
 #include <stdint.h>
 
 typedef int tile_i4 __attribute__((ext_vector_type(4)));
+typedef uint32_t tile_u2 __attribute__((ext_vector_type(2)));
 typedef int tile_i8 __attribute__((ext_vector_type(8)));
 typedef float tile_f4 __attribute__((ext_vector_type(4)));
 typedef float tile_f16 __attribute__((ext_vector_type(16)));
@@ -71,10 +72,16 @@ struct TileTriple {  // three
     }
 };
 
-__device__ static inline void tile_load16(const uint8_t *from, uint8_t *lds)
+// A buffer of `bytes` bytes (what lies past them reads as zero), and a load of 16 bytes per lane from it
+// into LDS, in lane order from `lds` on.  (The global instruction that does the same makes the compiler
+// wait for every LDS read in flight at the next use of one.)
+__device__ static inline __amdgpu_buffer_rsrc_t tile_buffer(const uint8_t *from, int bytes)
 {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
-                                     (__attribute__((address_space(3))) void *)lds, 16, 0, 0);
+    return __builtin_amdgcn_make_buffer_rsrc((void *)from, 0, bytes, 0x00020000);
+}
+__device__ static inline void tile_load16(__amdgpu_buffer_rsrc_t from, int at, int more, uint8_t *lds)
+{
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void *)lds, 16, at, more, 0, 0);
 }
 
 // The wavefront's number in its workgroup, in a scalar register.
@@ -85,13 +92,16 @@ template <int BM, int BN, int WGM, int WGN, bool FP4>
 struct Tile {
     static constexpr int ROWS = BM, COLS = BN, WAVES = WGM * WGN, THREADS = 64 * WAVES;
     static constexpr int WM = BM / WGM, WN = BN / WGN, TM = WM / 32, TN = WN / 32;
-    static constexpr int SCALES_M = BM * 8 < 1024 ? 1024 : BM * 8, SCALES_N = BN * 8 < 1024 ? 1024 : BN * 8;
-    static constexpr int BUFFER = (BM + BN) * PANEL_BYTES + (FP4 ? SCALES_M + SCALES_N : 0);
+    // the first half of the wavefronts loads a's scales of a panel, the other half b's, 1024 bytes each
+    // (zeros past the last ones: without a branch in the loop)
+    static constexpr int SCALES = WAVES / 2 * 1024;
+    static constexpr int BUFFER = (BM + BN) * PANEL_BYTES + (FP4 ? 2 * SCALES : 0);
     // a wavefront's strip of 32 rows of results, behind the buffers' use (store_strips)
     static constexpr int PITCH = WN + 4;
     static constexpr int LDS = 2 * BUFFER > WAVES * 32 * PITCH * 4 ? 2 * BUFFER : WAVES * 32 * PITCH * 4;
+    static constexpr int LDS_PIECES = 2 * BUFFER + WAVES * 2048;
     static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "every wavefront loads the same number of rows");
-    static_assert(LDS <= 160 * 1024, "");
+    static_assert(LDS <= 160 * 1024 && LDS_PIECES <= 160 * 1024 && BM * 8 <= SCALES && BN * 8 <= SCALES, "");
 
     tile_f16 acc[TM][TN];
 
@@ -105,93 +115,161 @@ struct Tile {
                 for (int r = 0; r < 16; r++) acc[i][j][r] = 0.f;
     }
 
-    // Rows [row0, row0 + ROWS) of a panel; rows past the last one are read as the last one (their
-    // results are not stored).
-    template <int COUNT>
-    __device__ static void load_rows(const uint8_t *panel, int rows, int row0, uint8_t *lds)
-    {
-        const int lane = threadIdx.x & 63, wave = tile_wave();
-        const int piece = ((lane & 7) ^ (lane >> 3)) * 16;
-#pragma unroll
-        for (int q = 0; q < COUNT / (8 * WAVES); q++) {
-            const int at = (q * WAVES + wave) * 8;
-            const int row = min(row0 + at + (lane >> 3), rows - 1);
-            tile_load16(panel + (int64_t)row * PANEL_BYTES + piece, lds + at * PANEL_BYTES);
-        }
-    }
-    // The scales of those rows, two rows per lane; by the wavefronts from `first` on.
-    template <int COUNT>
-    __device__ static void load_scales(const uint8_t *scales, int rows, int row0, uint8_t *lds, int first)
-    {
-        const int lane = threadIdx.x & 63, wave = tile_wave() - first;
-        constexpr int PIECES = (COUNT * 8 + 1023) / 1024;
-        if (wave >= 0 && wave < PIECES) {
-            const int pair = min((row0 >> 1) + wave * 64 + lane, ((rows + 1) >> 1) - 1);
-            tile_load16(scales + (int64_t)pair * 16, lds + wave * 1024);
-        }
-    }
+    // What a step of the loop loads: a panel of the rows of a tile.  Rows past the last one read as zero.
+    struct Step {
+        const uint8_t *a, *b, *scales;
+        int a_bytes, b_bytes, scale_bytes;
+    };
     template <class P>
-    __device__ static void load(const P &p, int s, int row0, int col0, uint8_t *buf)
+    __device__ static Step step(const P &p, int s, int row0, int col0)
     {
         const TilePanels at = p.at(s);
-        load_rows<BM>(at.a, p.a_rows(), row0, buf);
-        load_rows<BN>(at.b, p.b_rows(), col0, buf + BM * PANEL_BYTES);
-        if (FP4) {
-            uint8_t *sc = buf + (BM + BN) * PANEL_BYTES;
-            load_scales<BM>(at.a_scales, p.a_rows(), row0, sc, 0);
-            load_scales<BN>(at.b_scales, p.b_rows(), col0, sc + SCALES_M, WAVES / 2);
+        const int rows = min(p.a_rows() - row0, BM), cols = min(p.b_rows() - col0, BN);
+        Step t = {at.a + (int64_t)row0 * PANEL_BYTES, at.b + (int64_t)col0 * PANEL_BYTES, nullptr, rows * PANEL_BYTES, cols * PANEL_BYTES, 0};
+        if (FP4) {  // two rows per lane: a's for the first half of the wavefronts, b's for the other
+            const bool m = tile_wave() < WAVES / 2;
+            t.scales = m ? at.a_scales + (int64_t)row0 * 8 : at.b_scales + (int64_t)col0 * 8;
+            t.scale_bytes = (((m ? rows : cols) + 1) & ~1) * 8;
         }
+        return t;
+    }
+    // Part `part` of `parts` of a wavefront's loads of a step, 8 rows an instruction.
+    static constexpr int LOADS_M = BM / (8 * WAVES), LOADS_N = BN / (8 * WAVES);
+    __device__ static void load_part(const Step &t, int at, uint8_t *buf, int part, int parts)
+    {
+        const int wave = tile_wave();
+        const __amdgpu_buffer_rsrc_t a = tile_buffer(t.a, t.a_bytes), b = tile_buffer(t.b, t.b_bytes);
+#pragma unroll
+        for (int n = 0; n < LOADS_M + LOADS_N; n++) {
+            if (n * parts / (LOADS_M + LOADS_N) != part) continue;
+            constexpr int EACH = WAVES * 8 * PANEL_BYTES;
+            if (n < LOADS_M) tile_load16(a, at, n * EACH, buf + n * EACH + wave * 8 * PANEL_BYTES);
+            else tile_load16(b, at, (n - LOADS_M) * EACH, buf + (BM * PANEL_BYTES + (n - LOADS_M) * EACH) + wave * 8 * PANEL_BYTES);
+        }
+        if (FP4 && part == 0)
+            tile_load16(tile_buffer(t.scales, t.scale_bytes), (threadIdx.x & 63) * 16, wave % (WAVES / 2) * 1024,
+                        buf + (BM + BN) * PANEL_BYTES + wave * 1024);
     }
 
-    // acc += the product over panels [s0, s1) of the tile at (row0, col0).  Every wavefront of the
-    // workgroup calls it with the same arguments.
-    template <class P>
-    __device__ void multiply(const P &p, int s0, int s1, int row0, int col0, uint8_t *lds)
+    // The 16 bytes of every row and column that slice q of a panel takes, and the scales of a panel.
+    struct Slice {
+        tile_i4 a[TM], b[TN];
+    };
+    struct Scales {
+        uint32_t a[TM][2], b[TN][2];
+    };
+
+    // The products over `panels` panels of `tiles` tiles, one after the other: place(t, &row0, &col0) says
+    // where tile t lies, done(row0, col0) takes its values out of acc.  Every wavefront of the workgroup
+    // calls it with the same arguments.
+    //
+    // Slice q + 1 is read from LDS while slice q is multiplied, and the first slice of the next panel while
+    // the last one of this panel is: the barrier between the panels stands before that last slice, whose
+    // operands are in registers by then, so the matrix cores have work on both sides of it, and the
+    // loads of the panel after the next, half of them behind it and half in the next slice, have the time
+    // to the next barrier.  The order (a few reads, a few loads, TN products, TM times a slice) is written
+    // out and kept.  A tile's first panels are on their way while the last tile's values are stored.
+    template <class P, class G, class D>
+    __device__ void multiply(const P &p, int panels, int tiles, G place, uint8_t *lds, D done)
     {
-        if (s0 >= s1) return;
         const int lane = threadIdx.x & 63, wave = tile_wave();
         const int wm = wave / WGN * WM, wn = wave % WGN * WN;
         const int in_row = lane & 31, half = lane >> 5;
-        int place[4];
+        int at[4];
 #pragma unroll
-        for (int q = 0; q < 4; q++) place[q] = ((2 * q + half) ^ (lane & 7)) * 16;
+        for (int q = 0; q < 4; q++) at[q] = ((2 * q + half) ^ (lane & 7)) * 16;
         const int a_at = (wm + in_row) * PANEL_BYTES, b_at = (BM + wn + in_row) * PANEL_BYTES;
+        const int load_at = (wave * 8 + (lane >> 3)) * PANEL_BYTES + ((lane & 7) ^ (lane >> 3)) * 16;
+        Slice slice[2];
+        Scales scale[2];
 
-        load(p, s0, row0, col0, lds);
-        int cur = 0;
-        for (int s = s0; s < s1; s++) {
-            __syncthreads();  // panel s has landed; nobody reads the other buffer any more
-            if (s + 1 < s1) load(p, s + 1, row0, col0, lds + (cur ^ BUFFER));
-            const uint8_t *buf = lds + cur;
-            uint32_t sa[TM][2], sb[TN][2];
-            if (FP4) {
-                const uint8_t *sc = buf + (BM + BN) * PANEL_BYTES;
-#pragma unroll
-                for (int i = 0; i < TM; i++) {  // the lane's half of every slice: bytes 0 and 2 of both words
-                    const uint64_t v = *(const uint64_t *)(sc + (wm + 32 * i + in_row) * 8) >> (8 * half);
-                    sa[i][0] = (uint32_t)v, sa[i][1] = (uint32_t)(v >> 32);
-                }
-#pragma unroll
-                for (int j = 0; j < TN; j++) {
-                    const uint64_t v = *(const uint64_t *)(sc + SCALES_M + (wn + 32 * j + in_row) * 8) >> (8 * half);
-                    sb[j][0] = (uint32_t)v, sb[j][1] = (uint32_t)(v >> 32);
-                }
+        // the tile that is multiplied; the panel after the next one of its, or of a later tile's
+        int tile = 0, row0, col0, ahead = 0, ahead_panel = 0, ahead_row, ahead_col;
+        place(0, &row0, &col0);
+        ahead_row = row0, ahead_col = col0;
+        auto advance = [&] {
+            if (++ahead_panel < panels) return;
+            if (ahead + 1 < tiles) place(++ahead, &ahead_row, &ahead_col), ahead_panel = 0;
+            else ahead_panel = panels - 1;  // the last panel is loaded again: no branch among the products
+        };
+        zero();
+        if (panels <= 0) {
+            for (; tile < tiles; tile++) {
+                place(tile, &row0, &col0);
+                done(row0, col0);
             }
+            return;
+        }
+        load_part(step(p, 0, row0, col0), load_at, lds, 0, 1);
+        advance();
+        Step next = step(p, ahead_panel, ahead_row, ahead_col);
+        advance();
+        Step later = step(p, ahead_panel, ahead_row, ahead_col);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < TM; i++) load_part(next, load_at, lds + BUFFER, i, 2 * TM);
+        int cur = 0;
+#pragma unroll
+        for (int i = 0; i < TM; i++) read_part(slice[0], lds, a_at + at[0], b_at + at[0], i);
+        if (FP4) read_scales(scale[0], lds, wm + in_row, wn + in_row, half);
+        for (int s = 0;;) {
+            const uint8_t *buf = lds + cur;
 #pragma unroll
             for (int q = 0; q < 4; q++) {
-                tile_i4 fa[TM], fb[TN];
+                if (q == 3) {
+                    __syncthreads();  // the next panel has landed, and everybody has read all of this one
+                    buf = lds + (cur ^ BUFFER);
+                    if (FP4) read_scales(scale[1], buf, wm + in_row, wn + in_row, half);
+                }
 #pragma unroll
-                for (int i = 0; i < TM; i++) fa[i] = *(const tile_i4 *)(buf + a_at + 32 * i * PANEL_BYTES + place[q]);
+                for (int i = 0; i < TM; i++) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    const int to = (q + 1) & 3;
+                    read_part(slice[(q + 1) & 1], buf, a_at + at[to], b_at + at[to], i);
+                    if (q == 0) load_part(next, load_at, lds + (cur ^ BUFFER), TM + i, 2 * TM);
+                    if (q == 3) load_part(later, load_at, lds + cur, i, 2 * TM);
 #pragma unroll
-                for (int j = 0; j < TN; j++) fb[j] = *(const tile_i4 *)(buf + b_at + 32 * j * PANEL_BYTES + place[q]);
-#pragma unroll
-                for (int i = 0; i < TM; i++)
-#pragma unroll
-                    for (int j = 0; j < TN; j++) acc[i][j] = one(fa[i], fb[j], acc[i][j], q, sa[i], sb[j]);
+                    for (int j = 0; j < TN; j++)
+                        acc[i][j] = one(slice[q & 1].b[j], slice[q & 1].a[i], acc[i][j], q, scale[0].b[j], scale[0].a[i]);
+                }
             }
+            if (FP4) scale[0] = scale[1];
             cur ^= BUFFER;
+            if (++s == panels) {
+                done(row0, col0);
+                if (++tile == tiles) break;
+                place(tile, &row0, &col0);
+                zero();
+                s = 0;
+            }
+            next = later;
+            advance();
+            later = step(p, ahead_panel, ahead_row, ahead_col);
         }
-        __syncthreads();  // the buffers may be used again
+        __syncthreads();  // nothing is on its way to LDS any more
+    }
+
+    // Part `part` of the TM parts of a slice's reads.
+    __device__ static void read_part(Slice &f, const uint8_t *buf, int a, int b, int part)
+    {
+        constexpr int EACH = (TM + TN + TM - 1) / TM;
+#pragma unroll
+        for (int n = 0; n < EACH; n++) {
+            const int at = part * EACH + n;
+            if (at < TN) f.b[at] = *(const tile_i4 *)(buf + b + 32 * at * PANEL_BYTES);
+            else if (at < TM + TN) f.a[at - TN] = *(const tile_i4 *)(buf + a + 32 * (at - TN) * PANEL_BYTES);
+        }
+    }
+    // Of the 8 scales of a row in a panel the lane needs its half's: bytes 0 and 2 of both words.
+    __device__ static void read_scales(Scales &f, const uint8_t *buf, int a, int b, int half)
+    {
+        const uint8_t *sc = buf + (BM + BN) * PANEL_BYTES;
+#pragma unroll
+        for (int i = 0; i < TM + TN; i++) {
+            const uint64_t v = *(const uint64_t *)(sc + (i < TM ? (a + 32 * i) * 8 : SCALES + (b + 32 * (i - TM)) * 8)) >> (8 * half);
+            uint32_t *to = i < TM ? f.a[i] : f.b[i - TM];
+            to[0] = (uint32_t)v, to[1] = (uint32_t)(v >> 32);
+        }
     }
 
     __device__ static tile_f16 one(tile_i4 x, tile_i4 y, tile_f16 c, int q, const uint32_t *sx, const uint32_t *sy)
@@ -207,8 +285,8 @@ struct Tile {
     }
 
     // f(strip, row, col) for every 32 x WN values of the wavefront, strip[r * PITCH + c] in LDS being
-    // C[row + r][col + c].  The accumulators hold single rows of 32 columns over half a wavefront;
-    // from the strip every lane takes what makes whole 16 bytes of the result.
+    // C[row + r][col + c].  A lane's accumulators hold 4 neighbouring values of one row, 8 columns apart
+    // (b is the instruction's first operand); from the strip it takes what makes whole 16 bytes of the result.
     template <class F>
     __device__ void store_strips(int row0, int col0, uint8_t *lds, F f)
     {
@@ -220,12 +298,51 @@ struct Tile {
 #pragma unroll
             for (int j = 0; j < TN; j++)
 #pragma unroll
-                for (int r = 0; r < 16; r++)
-                    strip[(8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)) * PITCH + 32 * j + (lane & 31)] = acc[i][j][r];
+                for (int g = 0; g < 4; g++)
+                    *(tile_f4 *)(strip + (lane & 31) * PITCH + 32 * j + 8 * g + 4 * (lane >> 5)) =
+                        tile_f4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
             wave_fence();
             f(strip, row0 + wm + 32 * i, col0 + wn);
             wave_fence();
         }
+    }
+    // f(the lane's 16 bytes, row, column) of the results, as elements of SIZE bytes; `to` makes a word of two
+    // sums of those of 2.  By way of 2048 bytes of LDS per wavefront beside the buffers: 64 bytes of 32
+    // rows at a time, so that 4 lanes have a whole line's half.
+    template <int SIZE, class C, class F>
+    __device__ void store_pieces(int row0, int col0, uint8_t *lds, C to, F f)
+    {
+        constexpr int COLS = 64 / SIZE;
+        const int lane = threadIdx.x & 63, wave = tile_wave();
+        const int wm = wave / WGN * WM, wn = wave % WGN * WN;
+        uint8_t *own = lds + wave * 2048;
+        const int row = lane & 31, half = lane >> 5;
+#pragma unroll
+        for (int i = 0; i < TM; i++)
+#pragma unroll
+            for (int c = 0; c < WN / COLS; c++) {
+                // 16 bytes of a row lie at place (their number) ^ (row / 4 % 4)
+#pragma unroll
+                for (int g = 0; g < COLS / 8; g++) {
+                    const int first = c * COLS + 8 * g;
+                    const tile_f16 &from = acc[i][first / 32];
+                    const int r = first % 32 / 8 * 4;
+                    if constexpr (SIZE == 2) {
+                        const tile_u2 v = {to(from[r], from[r + 1]), to(from[r + 2], from[r + 3])};
+                        *(tile_u2 *)(own + row * 64 + ((g ^ (row >> 2)) & 3) * 16 + half * 8) = v;
+                    } else {
+                        *(tile_f4 *)(own + row * 64 + (((2 * g + half) ^ (row >> 2)) & 3) * 16) = tile_f4{from[r], from[r + 1], from[r + 2], from[r + 3]};
+                    }
+                }
+                wave_fence();
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    const int at = n * 16 + (lane >> 2);
+                    const tile_i4 v = *(const tile_i4 *)(own + at * 64 + (((lane & 3) ^ (at >> 2)) & 3) * 16);
+                    f(v, row0 + wm + 32 * i + at, col0 + wn + c * COLS + (lane & 3) * (16 / SIZE));
+                }
+                wave_fence();
+            }
     }
 
     // LDS of a wavefront's own: its accesses are performed in order, the compiler keeps them so.
@@ -242,6 +359,15 @@ struct Tile {
 __device__ static inline int tile_piece(int id, int count)
 {
     const int xcd = id & 7, n = id >> 3, whole = count >> 3, more = count & 7;
+    return xcd * whole + min(xcd, more) + n;
+}
+// The same for `groups` workgroups that share `count` pieces (no fewer than workgroups): the first of the
+// workgroup's pieces, how far the next one is, and how many it has.
+__device__ static inline int tile_pieces(int id, int groups, int count, int *apart, int *pieces)
+{
+    const int xcd = id & 7, n = id >> 3, whole = count >> 3, more = count & 7;
+    *apart = (groups - xcd + 7) >> 3;
+    *pieces = (whole + (xcd < more) - n + *apart - 1) / *apart;
     return xcd * whole + min(xcd, more) + n;
 }
 
