@@ -49,7 +49,7 @@ struct NsMatrix {
     uint8_t *work;
     int rows, cols;  // of X
     int flip;        // X is the transpose of the matrix as it lies
-    int whole_out;   // vectors of out's rows are aligned
+    int whole_in, whole_momentum, whole_out;  // vectors of the rows are aligned
     float step;      // out = keep * out - step * X with NsParams::update, else out = X
     int first;       // the launch's first workgroup of this matrix
 };
@@ -101,11 +101,21 @@ __device__ static inline int ns_find(const NsLaunch &l, int id, int *piece)
     return i;
 }
 
-__device__ static inline float ns_read(const uint8_t *from, int64_t i, int dtype)
+// 4 neighbouring elements, n of which exist.
+__device__ static inline tile_f4 ns_read(const uint8_t *from, int64_t at, int dtype, bool whole, int n)
 {
-    if (dtype == TFTQ_F32) return ((const float *)from)[i];
-    if (dtype == TFTQ_F16) return (float)((const _Float16 *)from)[i];
-    return (float)((const __bf16 *)from)[i];
+    typedef _Float16 H4 __attribute__((ext_vector_type(4)));
+    typedef __bf16 B4 __attribute__((ext_vector_type(4)));
+    tile_f4 v = {0.f, 0.f, 0.f, 0.f};
+    if (whole && n >= 4) {
+        if (dtype == TFTQ_F32) return *(const tile_f4 *)(from + at * 4);
+        if (dtype == TFTQ_F16) return __builtin_convertvector(*(const H4 *)(from + at * 2), tile_f4);
+        return __builtin_convertvector(*(const B4 *)(from + at * 2), tile_f4);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (i < n) v[i] = dtype == TFTQ_F32 ? ((const float *)from)[at + i] : dtype == TFTQ_F16 ? (float)((const _Float16 *)from)[at + i] : (float)((const __bf16 *)from)[at + i];
+    return v;
 }
 // The momentum's next value and the update that is orthogonalised.
 __device__ static inline float ns_momentum(float m, float g, const NsParams &p) { return m * p.momentum + (1.f - p.momentum) * g; }
@@ -122,18 +132,39 @@ __global__ __launch_bounds__(256) void k_ns_squares(const NsLaunch l, const NsPa
     const int across = (wide + NORM_COLS - 1) / NORM_COLS;
     const int row0 = piece / across * NORM_ROWS, col0 = piece % across * NORM_COLS;
     const int rows = min(NORM_ROWS, high - row0);
+    // a thread has 4 neighbouring columns of every `apart`th row
+    const int groups = (min(NORM_COLS, wide - col0) + 3) >> 2, apart = 256 / groups;
+    const int c = col0 + (int)threadIdx.x % groups * 4, n = wide - c;
     double sum = 0;
-    for (int c = threadIdx.x; c < NORM_COLS && col0 + c < wide; c += 256)
-#pragma unroll 4
-        for (int r = 0; r < rows; r++) {
-            float u = ns_read(m.in, (row0 + r) * m.ld_in + col0 + c, p.in_dtype);
-            if (m.momentum) {
-                float *at = m.momentum + (row0 + r) * m.ld_momentum + col0 + c;
-                const float next = ns_momentum(*at, u, p);
-                *at = next;
-                u = ns_update(next, u, p);
+    constexpr int AT_ONCE = 8;  // rows whose loads are in flight together
+    if ((int)threadIdx.x < groups * apart)
+        for (int r0 = row0 + (int)threadIdx.x / groups; r0 < row0 + rows; r0 += AT_ONCE * apart) {
+            tile_f4 u[AT_ONCE], next[AT_ONCE];
+#pragma unroll
+            for (int q = 0; q < AT_ONCE; q++) {
+                const int64_t r = min(r0 + q * apart, row0 + rows - 1);
+                u[q] = ns_read(m.in, r * m.ld_in + c, p.in_dtype, m.whole_in, n);
+                if (m.momentum) next[q] = ns_read((const uint8_t *)m.momentum, r * m.ld_momentum + c, TFTQ_F32, m.whole_momentum, n);
             }
-            sum += (double)u * (double)u;
+#pragma unroll
+            for (int q = 0; q < AT_ONCE; q++) {
+                const int64_t r = r0 + q * apart;
+                if (r >= row0 + rows) continue;
+                if (m.momentum) {
+                    float *at = m.momentum + r * m.ld_momentum + c;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) next[q][i] = ns_momentum(next[q][i], u[q][i], p), u[q][i] = ns_update(next[q][i], u[q][i], p);
+                    if (m.whole_momentum && n >= 4) {
+                        *(tile_f4 *)at = next[q];
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (i < n) at[i] = next[q][i];
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) sum += (double)u[q][i] * (double)u[q][i];
+            }
         }
     for (int s = 32; s; s >>= 1) sum += __shfl_xor(sum, s);
     if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum;
@@ -180,16 +211,24 @@ __global__ __launch_bounds__(256) void k_ns_start(const NsLaunch l, const NsPara
 
     // read along the rows of the matrix as it lies
     const int at_row = m.flip ? col0 : row0, at_col = m.flip ? row0 : col0;
-    for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-        const int r = i >> 6, c = i & 63;
-        float v = 0.f;
-        if (at_row + r < high && at_col + c < wide) {
-            float u = ns_read(m.in, (at_row + r) * m.ld_in + at_col + c, p.in_dtype);
-            if (m.momentum) u = ns_update(m.momentum[(at_row + r) * m.ld_momentum + at_col + c], u, p);
-            v = (float)(u * by);
+    for (int q = threadIdx.x; q < 64 * 16; q += 256) {
+        const int r = q >> 4, c = (q & 15) * 4, n = wide - at_col - c;
+        tile_f4 v = {0.f, 0.f, 0.f, 0.f};
+        if (at_row + r < high && n > 0) {
+            const int64_t row = at_row + r;
+            v = ns_read(m.in, row * m.ld_in + at_col + c, p.in_dtype, m.whole_in, n);
+            if (m.momentum) {
+                const tile_f4 old = ns_read((const uint8_t *)m.momentum, row * m.ld_momentum + at_col + c, TFTQ_F32, m.whole_momentum, n);
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[i] = ns_update(old[i], v[i], p);
+            }
         }
-        if (m.flip) tile[c][r] = v;
-        else tile[r][c] = v;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float x = i < n ? (float)(v[i] * by) : 0.f;
+            if (m.flip) tile[c + i][r] = x;
+            else tile[r][c + i] = x;
+        }
     }
     __syncthreads();
     for (int q = threadIdx.x; q < 64 * 8; q += 256) {
@@ -264,117 +303,236 @@ __device__ static inline void ns_put(const NsMatrix m, const NsParams p, int64_t
 
 enum { NS_A, NS_B, NS_X };
 
+// What becomes of a product's sums: E and D, G and F, or X, X^T and the result.
+template <int WHAT, bool PRECISE>
+struct NsFinish {
+    static constexpr bool LOW = PRECISE || WHAT == NS_X;  // the result's rows have a remainder
+    NsMatrix m;
+    NsParams p;
+    NsWork w;
+    uint8_t *out, *out_l, *turned, *turned_l;  // panels along the result's rows, and along its columns
+    float scale_x, per_x;                      // powers of two
+    int r, cols, padded;
+    bool mirror;
+
+    __device__ NsFinish(const NsMatrix &matrix, const NsParams &params, const NsWork &work, int turn, bool diagonal)
+        : m(matrix), p(params), w(work)
+    {
+        out = WHAT == NS_A ? w.e : WHAT == NS_B ? w.g : w.x, out_l = WHAT == NS_A ? w.el : WHAT == NS_B ? w.gl : w.xl;
+        turned = WHAT != NS_X ? out : turn ? w.t : w.t2, turned_l = WHAT != NS_X ? out_l : turn ? w.tl : w.tl2;
+        scale_x = *w.scale, per_x = 1.f / scale_x;
+        r = m.rows, cols = WHAT == NS_X ? m.cols : m.rows, padded = (cols + 63) & ~63;
+        mirror = WHAT == NS_X ? !p.last || m.flip : !diagonal;
+    }
+    __device__ float scale() const { return WHAT == NS_A ? SCALE_E : WHAT == NS_B ? SCALE_G : scale_x; }
+    __device__ int64_t at(int i, int j) const { return ((int64_t)(j >> 6) * r + i) * PANEL_BYTES + (j & 63) * 2; }
+
+    // What the results of row i, columns j to j + 7, are made of beside their sums.
+    struct Old {
+        ns_h8 high, low;
+        float di;
+    };
+    __device__ __forceinline__ Old old(int i, int j) const
+    {
+        Old o = {};
+        if (WHAT == NS_A || i >= r || j >= padded) return o;
+        o.high = *(const ns_h8 *)((WHAT == NS_B ? w.e : w.x) + at(i, j));
+        if (LOW) o.low = *(const ns_h8 *)((WHAT == NS_B ? w.el : w.xl) + at(i, j));
+        o.di = WHAT == NS_B ? w.d[i] : p.a + w.f[i];
+        return o;
+    }
+    // Their values in place of the sums v, and those along the rows to where they go.
+    __device__ __forceinline__ void row(int i, int j, float *v, const Old &was) const
+    {
+        const bool inside = i < r && j < padded;
+        ns_h8 high, low;
+#pragma unroll
+        for (int n = 0; n < 8; n++) {
+            float o = 0.f;
+            if (inside && j + n < cols) {
+                if (WHAT == NS_A) {
+                    o = v[n] * per_x * per_x;
+                    if (i == j + n) w.d[i] = o;
+                } else {
+                    const float x = ((float)was.high[n] + (LOW ? (float)was.low[n] : 0.f)) * (WHAT == NS_B ? 1.f / SCALE_E : per_x);
+                    if (WHAT == NS_B) {
+                        const float dj = w.d[j + n], square = v[n] * (1.f / (SCALE_E * SCALE_E));
+                        if (i == j + n) w.f[i] = p.b * was.di + p.c * (square + was.di * was.di);
+                        o = p.b * x + p.c * (square + (was.di + dj) * x);
+                    } else {
+                        o = was.di * x + v[n] * (1.f / SCALE_G) * per_x;
+                    }
+                }
+                if (WHAT != NS_X && i == j + n) o = 0.f;
+            }
+            _Float16 a, b;
+            ns_split(o, scale(), &a, &b);
+            high[n] = a, low[n] = b;
+            v[n] = o;
+        }
+        if (!inside) return;
+        if (WHAT == NS_X && p.last) {
+            if (!m.flip) ns_put(m, p, i, j, cols - j, v);
+            return;
+        }
+        *(ns_h8 *)(out + at(i, j)) = high;
+        if (LOW) *(ns_h8 *)(out_l + at(i, j)) = low;
+    }
+    // The values of column j, rows i to i + 7, along the columns.
+    __device__ __forceinline__ void column(int i, int j, const float *v) const
+    {
+        if (j >= cols || i >= ((r + 63) & ~63)) return;
+        if (WHAT == NS_X && p.last) {
+            if (i < r) ns_put(m, p, j, i, r - i, v);
+            return;
+        }
+        ns_h8 high, low;
+#pragma unroll
+        for (int n = 0; n < 8; n++) {
+            _Float16 a, b;
+            ns_split(v[n], scale(), &a, &b);
+            high[n] = a, low[n] = b;
+        }
+        const int64_t to = ((int64_t)(i >> 6) * cols + j) * PANEL_BYTES + (i & 63) * 2;
+        *(ns_h8 *)(turned + to) = high;
+        if (PRECISE) *(ns_h8 *)(turned_l + to) = low;
+    }
+};
+
+// How many tiles of `size` rows cover n of them and what fills the last panel up, whose zeros they write.
+__host__ __device__ static inline int ns_tiles(int n, int size) { return (((n + 63) & ~63) + size - 1) / size; }
+
+// What a product contracts, and the tile of a matrix that piece `piece` is.
+template <int WHAT>
+struct NsProduct {
+    const uint8_t *ah, *al, *bh, *bl;
+    int a_rows, b_rows, panels;
+    __device__ NsProduct(const NsMatrix &m, const NsWork &w, int turn)
+    {
+        ah = WHAT == NS_A ? w.x : WHAT == NS_B ? w.e : w.g, al = WHAT == NS_A ? w.xl : WHAT == NS_B ? w.el : w.gl;
+        bh = WHAT == NS_A ? w.x : WHAT == NS_B ? w.e : turn ? w.t2 : w.t, bl = WHAT == NS_A ? w.xl : WHAT == NS_B ? w.el : turn ? w.tl2 : w.tl;
+        a_rows = m.rows, b_rows = WHAT == NS_X ? m.cols : m.rows;
+        panels = ((WHAT == NS_A ? m.cols : m.rows) + 63) >> 6;
+    }
+    __device__ void tile(int piece, int high, int wide, int *tm, int *tn) const
+    {
+        if (WHAT == NS_X) {
+            tile_place(piece, ns_tiles(a_rows, high), ns_tiles(b_rows, wide), tm, tn);
+            return;
+        }
+        int n = (int)((sqrtf(8.f * piece + 1.f) - 1.f) * 0.5f);  // column n of the upper triangle has n + 1 tiles
+        while ((n + 1) * (n + 2) / 2 <= piece) n++;
+        while (n * (n + 1) / 2 > piece) n--;
+        *tn = n, *tm = piece - n * (n + 1) / 2;
+    }
+};
+
 template <class T, int WHAT, bool PRECISE>
 __global__ __launch_bounds__(T::THREADS) void k_ns_product(const NsLaunch l, const NsParams p, int turn)
 {
     __shared__ __attribute__((aligned(128))) uint8_t lds[T::LDS];
-    int piece;
+    int piece, tm, tn;
     const NsMatrix m = l.m[ns_find(l, tile_piece(blockIdx.x, gridDim.x), &piece)];
-    const int r = m.rows, k = m.cols, rp = (r + 63) >> 6;
-    const NsWork w = ns_work(m.work, r, k, m.flip, PRECISE);
-    int tm, tn;
-    if (WHAT == NS_X) {
-        tile_place(piece, (r + T::ROWS - 1) / T::ROWS, (k + T::COLS - 1) / T::COLS, &tm, &tn);
-    } else {  // column tn of the upper triangle has tn + 1 tiles
-        tn = (int)((sqrtf(8.f * piece + 1.f) - 1.f) * 0.5f);
-        while ((tn + 1) * (tn + 2) / 2 <= piece) tn++;
-        while (tn * (tn + 1) / 2 > piece) tn--;
-        tm = piece - tn * (tn + 1) / 2;
-    }
+    const NsWork w = ns_work(m.work, m.rows, m.cols, m.flip, PRECISE);
+    const NsProduct<WHAT> o(m, w, turn);
+    o.tile(piece, T::ROWS, T::COLS, &tm, &tn);
     const int row0 = tm * T::ROWS, col0 = tn * T::COLS;
-
-    const uint8_t *ah = WHAT == NS_A ? w.x : WHAT == NS_B ? w.e : w.g, *al = WHAT == NS_A ? w.xl : WHAT == NS_B ? w.el : w.gl;
-    const uint8_t *bh = WHAT == NS_A ? w.x : WHAT == NS_B ? w.e : turn ? w.t2 : w.t, *bl = WHAT == NS_A ? w.xl : WHAT == NS_B ? w.el : turn ? w.tl2 : w.tl;
-    const int panels = WHAT == NS_A ? (k + 63) >> 6 : rp, b_rows = WHAT == NS_X ? k : r;
     T t;
     auto place = [&](int, int *r0, int *c0) { *r0 = row0, *c0 = col0; };
     auto done = [](int, int) {};
-    if constexpr (PRECISE) t.multiply(TileTriple{{ah, al, bh, bl, r, b_rows, panels}}, 3 * panels, 1, place, lds, done);
-    else t.multiply(TilePair{{ah, nullptr, r}, {bh, nullptr, b_rows}}, panels, 1, place, lds, done);
+    if constexpr (PRECISE) t.multiply(TileTriple{{o.ah, o.al, o.bh, o.bl, o.a_rows, o.b_rows, o.panels}}, 3 * o.panels, 1, place, lds, done);
+    else t.multiply(TilePair{{o.ah, nullptr, o.a_rows}, {o.bh, nullptr, o.b_rows}}, o.panels, 1, place, lds, done);
 
-    // The result's panels: along its rows, and along its columns (its transpose), each with its remainder.
-    uint8_t *out = WHAT == NS_A ? w.e : WHAT == NS_B ? w.g : w.x, *out_l = WHAT == NS_A ? w.el : WHAT == NS_B ? w.gl : w.xl;
-    uint8_t *flip = WHAT != NS_X ? out : turn ? w.t : w.t2, *flip_l = WHAT != NS_X ? out_l : turn ? w.tl : w.tl2;
-    const float scale_x = *w.scale, per_x = 1.f / scale_x;  // powers of two
-    const float scale = WHAT == NS_A ? SCALE_E : WHAT == NS_B ? SCALE_G : scale_x;
-    constexpr bool LOW = PRECISE || WHAT == NS_X;
-    const int cols = WHAT == NS_X ? k : r, padded = (cols + 63) & ~63;
-    const bool last = WHAT == NS_X && p.last, mirror = WHAT == NS_X ? !last || m.flip : tm != tn;
+    const NsFinish<WHAT, PRECISE> finish(m, p, w, turn, tm == tn);
+    constexpr int ACROSS = T::WN / 8, PASSES = 32 * ACROSS / 64;  // 8 neighbours of a row per lane
+    static_assert(32 * ACROSS % 64 == 0, "");
     const int lane = threadIdx.x & 63;
-
-    t.store_strips(row0, col0, lds, [&](float *strip, int row, int col) {
-        constexpr int ACROSS = T::WN / 8;
-        const int c = lane % ACROSS * 8, j0 = col + c;
-#pragma unroll 1
-        for (int q = lane / ACROSS; q < 32; q += 64 / ACROSS) {
-            const int i = row + q;
-            float *v = strip + q * T::PITCH + c;
-            const bool inside = i < r && j0 < padded;
-            const int64_t at = ((int64_t)(j0 >> 6) * r + i) * PANEL_BYTES + (j0 & 63) * 2;
-            float o[8];
-            if (WHAT == NS_A) {
+    typename NsFinish<WHAT, PRECISE>::Old was[2][PASSES];  // of the next strip while one is finished
+    t.store_strips(row0, col0, lds, [&](int i, int row, int col) __attribute__((always_inline)) {
 #pragma unroll
-                for (int n = 0; n < 8; n++) {
-                    o[n] = v[n] * per_x * per_x;
-                    if (i == j0 + n && i < r) w.d[i] = o[n];
-                }
-            } else if (inside) {
-                ns_h8 hi = *(const ns_h8 *)((WHAT == NS_B ? w.e : w.x) + at), lo = hi;
-                if (LOW) lo = *(const ns_h8 *)((WHAT == NS_B ? w.el : w.xl) + at);
-                const float di = WHAT == NS_B ? w.d[i] : p.a + w.f[i];
+        for (int q = 0; q < PASSES; q++) was[i & 1][q] = finish.old(row + (lane + 64 * q) / ACROSS, col + (lane + 64 * q) % ACROSS * 8);
+    }, [&](int i, float *strip, int row, int col) __attribute__((always_inline)) {
 #pragma unroll
-                for (int n = 0; n < 8; n++) {
-                    const float old = ((float)hi[n] + (LOW ? (float)lo[n] : 0.f)) * (WHAT == NS_B ? 1.f / SCALE_E : per_x);
-                    if (WHAT == NS_B) {
-                        const float dj = j0 + n < r ? w.d[j0 + n] : 0.f, square = v[n] * (1.f / (SCALE_E * SCALE_E));
-                        if (i == j0 + n) w.f[i] = p.b * di + p.c * (square + di * di);
-                        o[n] = p.b * old + p.c * (square + (di + dj) * old);
-                    } else {
-                        o[n] = di * old + v[n] * (1.f / SCALE_G) * per_x;
-                    }
-                }
-            }
-            ns_h8 hi, lo;
-#pragma unroll
-            for (int n = 0; n < 8; n++) {
-                if (!inside || j0 + n >= cols || (WHAT != NS_X && i == j0 + n)) o[n] = 0.f;
-                _Float16 a, b;
-                ns_split(o[n], scale, &a, &b);
-                hi[n] = a, lo[n] = b;
-                v[n] = o[n];
-            }
-            if (last) {
-                if (!m.flip && inside) ns_put(m, p, i, j0, cols - j0, o);
-            } else if (inside) {
-                *(ns_h8 *)(out + at) = hi;
-                if (LOW) *(ns_h8 *)(out_l + at) = lo;
-            }
+        for (int q = 0; q < PASSES; q++) {
+            const int at = (lane + 64 * q) / ACROSS, c = (lane + 64 * q) % ACROSS * 8;
+            finish.row(row + at, col + c, strip + at * T::PITCH + c, was[i & 1][q]);
         }
         T::wave_fence();
-        if (!mirror) return;
-        // the same values down the columns, 8 rows of a column per lane
+        if (!finish.mirror) return;
 #pragma unroll 1
-        for (int q = lane; q < T::WN * 4; q += 64) {
-            const int i0 = row + (q & 3) * 8, j = col + (q >> 2);
-            if (j >= cols || i0 >= rp * 64) continue;
-            float o[8];
-            ns_h8 hi, lo;
+        for (int q = lane; q < T::WN * 4; q += 64) {  // 8 rows of a column per lane
+            float v[8];
 #pragma unroll
-            for (int n = 0; n < 8; n++) {
-                o[n] = strip[((q & 3) * 8 + n) * T::PITCH + (q >> 2)];
-                _Float16 a, b;
-                ns_split(o[n], scale, &a, &b);
-                hi[n] = a, lo[n] = b;
-            }
-            if (last) {
-                if (i0 < r) ns_put(m, p, j, i0, r - i0, o);
-                continue;
-            }
-            const int64_t at = ((int64_t)(i0 >> 6) * cols + j) * PANEL_BYTES + (i0 & 63) * 2;
-            *(ns_h8 *)(flip + at) = hi;
-            if (PRECISE) *(ns_h8 *)(flip_l + at) = lo;
+            for (int n = 0; n < 8; n++) v[n] = strip[((q & 3) * 8 + n) * T::PITCH + (q >> 2)];
+            finish.column(row + (q & 3) * 8, col + (q >> 2), v);
         }
     });
+}
+
+// The same for matrices of few tiles, where a kernel's time is that of the loads it waits for: a tile of
+// 32 x 32 per workgroup, whose 8 wavefronts share the panels between them, take their operands straight
+// from memory with all of a panel's loads in flight, and add up in LDS.
+template <int WHAT, bool PRECISE>
+__global__ __launch_bounds__(512) void k_ns_small(const NsLaunch l, const NsParams p, int turn)
+{
+    constexpr int WAVES = 8, PITCH = 36;
+    __shared__ __attribute__((aligned(128))) float sums[WAVES][32 * PITCH];
+    int piece, tm, tn;
+    const NsMatrix m = l.m[ns_find(l, tile_piece(blockIdx.x, gridDim.x), &piece)];
+    const NsWork w = ns_work(m.work, m.rows, m.cols, m.flip, PRECISE);
+    const NsProduct<WHAT> o(m, w, turn);
+    o.tile(piece, 32, 32, &tm, &tn);
+    const int lane = threadIdx.x & 63, wave = tile_wave(), half = lane >> 5;
+    const int64_t a_at = (int64_t)min(tm * 32 + (lane & 31), o.a_rows - 1) * PANEL_BYTES + half * 16;
+    const int64_t b_at = (int64_t)min(tn * 32 + (lane & 31), o.b_rows - 1) * PANEL_BYTES + half * 16;
+    tile_f16 acc = {};
+    for (int s = wave; s < o.panels; s += WAVES) {
+        const int64_t a = a_at + (int64_t)s * o.a_rows * PANEL_BYTES, b = b_at + (int64_t)s * o.b_rows * PANEL_BYTES;
+        tile_h8 ah[4], bh[4], al[4], bl[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            ah[q] = *(const tile_h8 *)(o.ah + a + q * 32), bh[q] = *(const tile_h8 *)(o.bh + b + q * 32);
+            if (PRECISE) al[q] = *(const tile_h8 *)(o.al + a + q * 32), bl[q] = *(const tile_h8 *)(o.bl + b + q * 32);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q++) {  // b first: a lane's sums are neighbours in a row (tftq_tile.h)
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(bh[q], ah[q], acc, 0, 0, 0);
+            if (PRECISE) {
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(bh[q], al[q], acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(bl[q], ah[q], acc, 0, 0, 0);
+            }
+        }
+    }
+#pragma unroll
+    for (int g = 0; g < 4; g++)
+        *(tile_f4 *)(sums[wave] + (lane & 31) * PITCH + 8 * g + 4 * half) = tile_f4{acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
+
+    const NsFinish<WHAT, PRECISE> finish(m, p, w, turn, tm == tn);
+    const int id = threadIdx.x, at = id >> 2, c = (id & 3) * 8;  // the first 128 threads
+    typename NsFinish<WHAT, PRECISE>::Old was = {};
+    if (id < 128) was = finish.old(tm * 32 + at, tn * 32 + c);
+    __syncthreads();
+    if (id < 128) {
+        float v[8];
+#pragma unroll
+        for (int n = 0; n < 8; n++) {
+            v[n] = sums[0][at * PITCH + c + n];
+#pragma unroll
+            for (int k = 1; k < WAVES; k++) v[n] += sums[k][at * PITCH + c + n];
+        }
+        finish.row(tm * 32 + at, tn * 32 + c, v, was);
+#pragma unroll
+        for (int n = 0; n < 8; n++) sums[0][at * PITCH + c + n] = v[n];
+    }
+    if (!finish.mirror) return;
+    __syncthreads();
+    if (id < 128) {
+        const int j = id >> 2, i = (id & 3) * 8;
+        float v[8];
+#pragma unroll
+        for (int n = 0; n < 8; n++) v[n] = sums[0][(i + n) * PITCH + j];
+        finish.column(tm * 32 + i, tn * 32 + j, v);
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -393,28 +551,72 @@ static int launch_over(NsLaunch &l, F workgroups, const void *kernel, int thread
     return (int)hipLaunchKernel(kernel, dim3((unsigned)total), dim3(threads), args, 0, st);
 }
 
-static int64_t tiles(const NsMatrix &m, int what, int size)
+static int64_t tiles(const NsMatrix &m, int what, int high, int wide)
 {
-    const int64_t r = (m.rows + size - 1) / size, k = (m.cols + size - 1) / size;
+    const int64_t r = ns_tiles(m.rows, high), k = ns_tiles(m.cols, wide);
     return what == NS_X ? r * k : r * (r + 1) / 2;
 }
 
 template <class T, int WHAT>
-static int launch_product(NsLaunch &l, bool precise, const NsParams &p, int turn, hipStream_t st)
+static int launch_tiles(NsLaunch &l, bool precise, const NsParams &p, int turn, hipStream_t st)
 {
     const void *k = precise ? (const void *)k_ns_product<T, WHAT, true> : (const void *)k_ns_product<T, WHAT, false>;
-    return launch_over(l, [](const NsMatrix &m) { return tiles(m, WHAT, T::ROWS); }, k, T::THREADS, p, turn, st);
+    return launch_over(l, [](const NsMatrix &m) { return tiles(m, WHAT, T::ROWS, T::COLS); }, k, T::THREADS, p, turn, st);
 }
 
-// One of the three products for all matrices of a launch, with the largest tiles that give most compute units one.
+// The tiles that a product of the matrices of a launch is cut into.  `cost` is what a panel of the tiles
+// that run at once on a compute unit takes, that of one tile of 256 x 256 being 1, from the rates of
+// launches that fill all units evenly (8192^3, TFLOP/s: 256x256 1230, 192x256 1190, 192x192 1040,
+// 128x128 1000, 64x64 600); `at_once`: how many that is.
+struct NsTiles {
+    int high, wide, at_once;
+    double cost;
+};
+constexpr NsTiles NS_256 = {256, 256, 1, 1.0}, NS_192X256 = {192, 256, 1, 0.775}, NS_192 = {192, 192, 1, 0.665},
+                  NS_128 = {128, 128, 2, 0.61}, NS_64 = {64, 64, 4, 0.51};
+
+// About how many panels of a 256 x 256 tile a product takes: as many rounds of tiles as the compute
+// units need, or the longest tile.
+static double ns_time(const NsLaunch &l, int what, const NsTiles &t)
+{
+    double work = 0, longest = 0;
+    int64_t count = 0;
+    for (int i = 0; i < l.count; i++) {
+        const int64_t n = tiles(l.m[i], what, t.high, t.wide);
+        const double panels = ((what == NS_A ? l.m[i].cols : l.m[i].rows) + 63) / 64;
+        count += n, work += (double)n * panels, longest = std::max(longest, panels);
+    }
+    const double rounds = (double)((count + 256 * t.at_once - 1) / (256 * t.at_once));
+    return std::max(longest, rounds * work / count) * t.cost;
+}
+
+// One of the three products for all matrices of a launch.
 template <int WHAT>
 static int product(NsLaunch &l, bool precise, const NsParams &p, int turn, hipStream_t st)
 {
-    int64_t big = 0, middle = 0;
-    for (int i = 0; i < l.count; i++) big += tiles(l.m[i], WHAT, 256), middle += tiles(l.m[i], WHAT, 128);
-    if (big >= 160) return launch_product<Tile<256, 256, 2, 4, false>, WHAT>(l, precise, p, turn, st);
-    if (middle >= 160) return launch_product<Tile<128, 128, 2, 2, false>, WHAT>(l, precise, p, turn, st);
-    return launch_product<Tile<64, 64, 2, 2, false>, WHAT>(l, precise, p, turn, st);
+    // the matrices with most panels first: the last workgroups are then short ones
+    std::stable_sort(l.m, l.m + l.count, [](const NsMatrix &x, const NsMatrix &y) { return WHAT == NS_A ? x.cols > y.cols : x.rows > y.rows; });
+    int64_t small = 0, longest = 0;
+    for (int i = 0; i < l.count; i++) {
+        small += tiles(l.m[i], WHAT, 32, 32);
+        longest = std::max<int64_t>(longest, WHAT == NS_A ? l.m[i].cols : l.m[i].rows);
+    }
+    if (small <= 512) {
+        const void *k = precise ? (const void *)k_ns_small<WHAT, true> : (const void *)k_ns_small<WHAT, false>;
+        return launch_over(l, [](const NsMatrix &m) { return tiles(m, WHAT, 32, 32); }, k, 512, p, turn, st);
+    }
+    const NsTiles choice[] = {NS_256, WHAT == NS_X ? NS_192X256 : NS_192, NS_128, NS_64};
+    int best = 0;
+    for (int i = 1; i < 4; i++)
+        if (ns_time(l, WHAT, choice[i]) < ns_time(l, WHAT, choice[best])) best = i;
+    switch (best) {
+    case 0: return launch_tiles<Tile<256, 256, 2, 4, false>, WHAT>(l, precise, p, turn, st);
+    case 1:
+        if (WHAT == NS_X) return launch_tiles<Tile<192, 256, 2, 4, false>, NS_X>(l, precise, p, turn, st);
+        return launch_tiles<Tile<192, 192, 2, 2, false>, WHAT == NS_X ? NS_A : WHAT>(l, precise, p, turn, st);
+    case 2: return launch_tiles<Tile<128, 128, 2, 2, false>, WHAT>(l, precise, p, turn, st);
+    default: return launch_tiles<Tile<64, 64, 2, 2, false>, WHAT>(l, precise, p, turn, st);
+    }
 }
 
 static bool ns_shapes_ok(int n, const int64_t *shapes)
@@ -502,6 +704,9 @@ extern "C" int tftq_newton_schulz(const tftq_ns *what, void *workspace, int64_t 
             m.ld_in = s.in_stride[i], m.ld_out = s.out_stride[i], m.ld_momentum = s.momenta ? s.momenta_stride[i] : 0;
             m.flip = rows > cols;
             m.rows = (int)std::min(rows, cols), m.cols = (int)std::max(rows, cols);
+            const int in_size = s.in_dtype == TFTQ_F32 ? 4 : 2;
+            m.whole_in = m.ld_in * in_size % 16 == 0 && (uintptr_t)m.in % 16 == 0;
+            m.whole_momentum = m.ld_momentum % 4 == 0 && (uintptr_t)m.momentum % 16 == 0;
             m.whole_out = m.ld_out * out_size % 16 == 0 && (uintptr_t)m.out % 16 == 0;
             m.step = s.steps ? s.steps[i] : 0.f;
             m.work = work;

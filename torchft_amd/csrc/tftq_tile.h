@@ -170,7 +170,7 @@ struct Tile {
     // to the next barrier.  The order (a few reads, a few loads, TN products, TM times a slice) is written
     // out and kept.  A tile's first panels are on their way while the last tile's values are stored.
     template <class P, class G, class D>
-    __device__ void multiply(const P &p, int panels, int tiles, G place, uint8_t *lds, D done)
+    __device__ __forceinline__ void multiply(const P &p, int panels, int tiles, G place, uint8_t *lds, D done)
     {
         const int lane = threadIdx.x & 63, wave = tile_wave();
         const int wm = wave / WGN * WM, wn = wave % WGN * WN;
@@ -284,17 +284,20 @@ struct Tile {
         }
     }
 
-    // f(strip, row, col) for every 32 x WN values of the wavefront, strip[r * PITCH + c] in LDS being
-    // C[row + r][col + c].  A lane's accumulators hold 4 neighbouring values of one row, 8 columns apart
-    // (b is the instruction's first operand); from the strip it takes what makes whole 16 bytes of the result.
-    template <class F>
-    __device__ void store_strips(int row0, int col0, uint8_t *lds, F f)
+    // f(i, strip, row, col) for every 32 x WN values of the wavefront, strip[r * PITCH + c] in LDS being
+    // C[row + r][col + c]; before(i, row, col) is called a strip ahead, to load what f needs.  A lane's
+    // accumulators hold 4 neighbouring values of one row, 8 columns apart (b is the instruction's first
+    // operand); from the strip it takes what makes whole 16 bytes of the result.
+    template <class B, class F>
+    __device__ __forceinline__ void store_strips(int row0, int col0, uint8_t *lds, B before, F f)
     {
         const int lane = threadIdx.x & 63, wave = tile_wave();
         const int wm = wave / WGN * WM, wn = wave % WGN * WN;
         float *strip = (float *)lds + wave * 32 * PITCH;
+        before(0, row0 + wm, col0 + wn);
 #pragma unroll
         for (int i = 0; i < TM; i++) {
+            if (i + 1 < TM) before(i + 1, row0 + wm + 32 * (i + 1), col0 + wn);
 #pragma unroll
             for (int j = 0; j < TN; j++)
 #pragma unroll
@@ -302,7 +305,7 @@ struct Tile {
                     *(tile_f4 *)(strip + (lane & 31) * PITCH + 32 * j + 8 * g + 4 * (lane >> 5)) =
                         tile_f4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
             wave_fence();
-            f(strip, row0 + wm + 32 * i, col0 + wn);
+            f(i, strip, row0 + wm + 32 * i, col0 + wn);
             wave_fence();
         }
     }
@@ -310,7 +313,7 @@ struct Tile {
     // sums of those of 2.  By way of 2048 bytes of LDS per wavefront beside the buffers: 64 bytes of 32
     // rows at a time, so that 4 lanes have a whole line's half.
     template <int SIZE, class C, class F>
-    __device__ void store_pieces(int row0, int col0, uint8_t *lds, C to, F f)
+    __device__ __forceinline__ void store_pieces(int row0, int col0, uint8_t *lds, C to, F f)
     {
         constexpr int COLS = 64 / SIZE;
         const int lane = threadIdx.x & 63, wave = tile_wave();
