@@ -240,6 +240,15 @@ int tftq_mx_product(int dtype, const void *a, int64_t m, const void *b, int64_t 
                     int64_t row_stride, int device, void *stream);
 
 /*
+ * out [m, n] = Q(x) b^T: x [m, k] is quantised along its rows on the way, out has its type.  Few rows
+ * (the tokens of a model that is served) take one kernel and no workspace; others quantise into
+ * `workspace`, tftq_mx_linear_workspace bytes for the same x, 16-byte aligned.
+ */
+int64_t tftq_mx_linear_workspace(int dtype, const void *x, int64_t m, int64_t row_stride, int64_t n, int64_t k);
+int tftq_mx_linear(int dtype, const void *x, int64_t m, int64_t row_stride, const void *b, int64_t n, int64_t k,
+                   void *out, int64_t out_stride, void *workspace, int64_t workspace_bytes, int device, void *stream);
+
+/*
  * Newton-Schulz orthogonalisation of a list of matrices, and the step of the Muon optimiser (no
  * counterpart in the reference): what a replica does with the averaged gradients of its weight
  * matrices.  For every matrix u [rows, cols]:

@@ -64,6 +64,11 @@ SYMBOLS = [
     ("tftq_mx_quantize", _c.c_int, [_c.c_int, _P, _c.c_int64, _c.c_int64, _c.c_int64, _P, _P, _c.c_int, _P]),
     # dtype, matrix, rows, cols, out, row_stride, device, stream
     ("tftq_mx_dequantize", _c.c_int, [_c.c_int, _P, _c.c_int64, _c.c_int64, _P, _c.c_int64, _c.c_int, _P]),
+    # dtype, x, m, row_stride, n, k
+    ("tftq_mx_linear_workspace", _c.c_int64, [_c.c_int, _P, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64]),
+    # dtype, x, m, row_stride, b, n, k, out, out_stride, workspace, workspace_bytes, device, stream
+    ("tftq_mx_linear", _c.c_int, [_c.c_int, _P, _c.c_int64, _c.c_int64, _P, _c.c_int64, _c.c_int64, _P, _c.c_int64, _P,
+                                  _c.c_int64, _c.c_int, _P]),
     # n, shapes, precise
     ("tftq_newton_schulz_workspace", _c.c_int64, [_c.c_int, _L, _c.c_int]),
     # what, workspace, workspace_bytes, device, stream

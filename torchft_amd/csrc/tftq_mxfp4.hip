@@ -12,63 +12,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
-#include "tftq_device.h"
 #include "tftq_mxfp4.h"
-
-typedef uint32_t mx_u4 __attribute__((ext_vector_type(4)));
-typedef uint16_t mx_s2 __attribute__((ext_vector_type(2)));
-typedef _Float16 mx_h2 __attribute__((ext_vector_type(2)));
-typedef __bf16 mx_b2 __attribute__((ext_vector_type(2)));
-typedef float mx_f2 __attribute__((ext_vector_type(2)));
-
-// What the kernels ask of an element type: a 16-byte vector holds V elements in four words.  Magnitudes
-// are compared as the integers that their bits are, two of a 16-bit type at once; an infinity or NaN is
-// then larger than every finite value.
-struct MxF32 {
-    static constexpr int SIZE = 4, V = 4;
-    __device__ static uint32_t mag(uint32_t w) { return w & 0x7fffffffu; }
-    __device__ static uint32_t mag_max(uint32_t a, uint32_t b) { return max(a, b); }
-    __device__ static uint32_t mag_all(uint32_t m) { return m; }  // the larger of a word's magnitudes
-    __device__ static uint32_t bits(uint32_t m) { return m; }     // of a magnitude: its binary32 bits
-};
-struct MxHalf {
-    static constexpr int SIZE = 2, V = 8;
-    __device__ static uint32_t mag(uint32_t w) { return w & 0x7fff7fffu; }
-    __device__ static uint32_t mag_max(uint32_t a, uint32_t b)
-    {
-        return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(mx_s2, a), __builtin_bit_cast(mx_s2, b)));
-    }
-    __device__ static uint32_t mag_all(uint32_t m) { return max(m & 0xffffu, m >> 16); }
-};
-struct MxF16 : MxHalf {
-    __device__ static uint32_t bits(uint32_t m) { return __float_as_uint((float)__builtin_bit_cast(_Float16, (uint16_t)m)); }
-    template <int SEL>
-    __device__ static uint32_t codes(uint32_t old, uint32_t w, float x)
-    {
-        return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(old, __builtin_bit_cast(mx_h2, w), x, SEL);
-    }
-};
-struct MxBF16 : MxHalf {
-    __device__ static uint32_t bits(uint32_t m) { return m << 16; }
-    template <int SEL>
-    __device__ static uint32_t codes(uint32_t old, uint32_t w, float x)
-    {
-        return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(old, __builtin_bit_cast(mx_b2, w), x, SEL);
-    }
-};
-
-// The scale's byte for a block whose largest magnitude has these binary32 bits.  Subnormal numbers
-// (exponent field 0) are below 2^-126, so their blocks have the smallest scale whatever they hold.
-__device__ static inline uint32_t mx_byte(uint32_t bits)
-{
-    const int e = (int)(bits >> 23);
-    return e == 255 ? 255u : (uint32_t)max(e - 2, 0);
-}
-// 2^(byte - 127) in binary32; 2^-127 is subnormal, and 255 is NaN.
-__device__ static inline float mx_scale(uint32_t byte)
-{
-    return __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7fc00000u : byte << 23);
-}
 
 // The largest over the 32 / V neighbouring lanes that hold a row's block.
 template <class T>
@@ -84,8 +28,8 @@ __device__ static inline uint32_t mx_over_block(uint32_t m)
 // of a column lies in one lane (P = 32) and a block of a row in 4 or 8 neighbouring ones: neither needs
 // LDS, and the matrix is read once for both directions.
 template <class T, bool BY_ROWS, bool BY_COLS, int P>
-__global__ __launch_bounds__(64) void k_mx_quantize(const uint8_t *x, int64_t ld, int rows, int cols, int tiles_c, int whole,
-                                                    MxMatrix by_rows, MxMatrix by_cols)
+__global__ __launch_bounds__(64, 2) void k_mx_quantize(const uint8_t *x, int64_t ld, int rows, int cols, int tiles_c,
+                                                       MxMatrix by_rows, MxMatrix by_cols)
 {
     constexpr int V = T::V, ACROSS = 128 / V, GROUPS = 64 / ACROSS;
     static_assert(!BY_COLS || P == 32, "");
@@ -96,25 +40,17 @@ __global__ __launch_bounds__(64) void k_mx_quantize(const uint8_t *x, int64_t ld
 
     mx_u4 raw[P];
     const uint8_t *at = x + ((int64_t)row * ld + col) * T::SIZE;
-    if (whole && col + V <= cols) {  // vectors of the rows are aligned
+    if (col + V <= cols) {
 #pragma unroll
         for (int p = 0; p < P; p++) {
             raw[p] = mx_u4{0, 0, 0, 0};
-            if (row + p < rows) raw[p] = *(const mx_u4 *)(at + (int64_t)p * ld * T::SIZE);
+            if (row + p < rows) raw[p] = *(const mx_u4_any *)(at + (int64_t)p * ld * T::SIZE);
         }
     } else {
 #pragma unroll
         for (int p = 0; p < P; p++) {
             raw[p] = mx_u4{0, 0, 0, 0};
-            if (row + p < rows) {
-                const uint8_t *from = at + (int64_t)p * ld * T::SIZE;
-#pragma unroll
-                for (int v = 0; v < V; v++) {
-                    if (col + v >= cols) continue;
-                    if (T::SIZE == 4) raw[p][v] = ((const uint32_t *)from)[v];
-                    else raw[p][v / 2] |= (uint32_t)((const uint16_t *)from)[v] << (16 * (v & 1));
-                }
-            }
+            if (row + p < rows) raw[p] = mx_read<T>(at - (int64_t)col * T::SIZE + (int64_t)p * ld * T::SIZE, col, cols);
         }
     }
 
@@ -128,16 +64,7 @@ __global__ __launch_bounds__(64) void k_mx_quantize(const uint8_t *x, int64_t ld
             for (int w = 1; w < 4; w++) m = T::mag_max(m, T::mag(raw[p][w]));
             const uint32_t byte = mx_byte(T::bits(mx_over_block<T>(T::mag_all(m))));
             const float scale = mx_scale(byte);
-            uint32_t c = 0;
-            if constexpr (T::SIZE == 4) {
-                c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, __uint_as_float(raw[p][0]), __uint_as_float(raw[p][1]), scale, 0);
-                c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, __uint_as_float(raw[p][2]), __uint_as_float(raw[p][3]), scale, 1);
-            } else {
-                c = T::template codes<0>(c, raw[p][0], scale);
-                c = T::template codes<1>(c, raw[p][1], scale);
-                c = T::template codes<2>(c, raw[p][2], scale);
-                c = T::template codes<3>(c, raw[p][3], scale);
-            }
+            const uint32_t c = mx_codes<T>(raw[p], scale);
             if (row + p < rows) {
                 if (T::SIZE == 4) *(uint16_t *)(codes + p * PANEL_BYTES) = (uint16_t)c;
                 else *(uint32_t *)(codes + p * PANEL_BYTES) = c;
@@ -263,11 +190,10 @@ static int quantize(const void *x, int64_t ld, int rows, int cols, const MxMatri
     const int64_t high = c.panels ? mx_panels(rows) * 256 : rows;
     const int64_t tiles = tiles_c * ((high + GROUPS * per_lane - 1) / (GROUPS * per_lane));
     if (tiles > (1 << 25)) return TFTQ_E_SHAPE;
-    const int whole = ld * T::SIZE % 16 == 0 && (uintptr_t)x % 16 == 0;
     const dim3 grid((unsigned)tiles), block(64);
     const uint8_t *px = (const uint8_t *)x;
     int tc = (int)tiles_c;
-    void *args[] = {(void *)&px, (void *)&ld, (void *)&rows, (void *)&cols, (void *)&tc, (void *)&whole, (void *)&r, (void *)&c};
+    void *args[] = {(void *)&px, (void *)&ld, (void *)&rows, (void *)&cols, (void *)&tc, (void *)&r, (void *)&c};
     const void *k = !c.panels ? (const void *)k_mx_quantize<T, true, false, 4>
                     : r.panels ? (const void *)k_mx_quantize<T, true, true, 32>
                                : (const void *)k_mx_quantize<T, false, true, 32>;

@@ -14,6 +14,9 @@
 // launch function of libtftq.so, whose address it has been given (bind).  Anything out of the
 // ordinary gives None, and Python does the call in its own steps, with its own words for what is wrong.
 //
+// And it makes the calls of the 4-bit microscaled matrices (mxfp4.py) whose arguments are plain: the
+// checks, the allocations and the launch in one step.
+//
 // Host code only; built with the host compiler against the Python and libtorch headers
 // (torchft_amd/_build.py).  Not part of libtftq.so, whose C ABI has no Python or torch
 // types.
@@ -22,6 +25,7 @@
 #include <Python.h>
 
 #include <algorithm>
+#include <type_traits>
 #include <utility>
 #include <vector>
 
@@ -437,6 +441,214 @@ constexpr c10::DispatchKeySet WRAPPERS({c10::DispatchKey::Python, c10::DispatchK
                                         c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::BatchedNestedTensor,
                                         c10::DispatchKey::Functionalize});
 
+// ---------------------------------------------------------------------------
+// 4-bit microscaled matrices (mxfp4.py)
+// ---------------------------------------------------------------------------
+// What libtftq.so does (tftq.h), and the devices that have been found able to run it.
+struct {
+    int64_t (*bytes)(int64_t rows, int64_t cols) = nullptr;
+    int (*quantize)(int dtype, const void *x, int64_t rows, int64_t cols, int64_t row_stride, void *by_rows, void *by_cols, int device,
+                    void *stream) = nullptr;
+    int (*product)(int dtype, const void *a, int64_t m, const void *b, int64_t n, int64_t k, void *out, int64_t row_stride, int device,
+                   void *stream) = nullptr;
+    int64_t (*linear_workspace)(int dtype, const void *x, int64_t m, int64_t row_stride, int64_t n, int64_t k) = nullptr;
+    int (*linear)(int dtype, const void *x, int64_t m, int64_t row_stride, const void *b, int64_t n, int64_t k, void *out,
+                  int64_t out_stride, void *workspace, int64_t workspace_bytes, int device, void *stream) = nullptr;
+    int (*dequantize)(int dtype, const void *matrix, int64_t rows, int64_t cols, void *out, int64_t row_stride, int device,
+                      void *stream) = nullptr;
+    uint64_t devices = 0;
+} mx;
+
+bool mx_calls(int64_t device) { return mx.bytes && device >= 0 && device < 64 && (mx.devices >> device & 1) != 0 && plain_calls(); }
+
+// A matrix of ordinary numbers that a kernel takes as it is.
+struct Matrix {
+    int64_t rows = 0, cols = 0, stride = 0, device = -1;
+    int dtype = -1;  // tftq.h's
+    at::ScalarType type = at::kFloat;
+    void *data = nullptr;
+
+    bool read(PyObject *o)
+    {
+        if (!THPVariable_CheckExact(o)) return false;  // a tensor or a parameter
+        const at::Tensor &t = THPVariable_Unpack(o);
+        if (!t.defined() || t.key_set().has_any(WRAPPERS) ||
+            t.layout() != at::kStrided || !t.device().is_cuda() || t.dim() != 2 || t.is_neg())
+            return false;
+        type = t.scalar_type();
+        dtype = type == at::kFloat ? 0 : type == at::kHalf ? 1 : type == at::kBFloat16 ? 2 : -1;
+        rows = t.size(0), cols = t.size(1), stride = t.stride(0), device = t.device().index();
+        if (dtype < 0 || rows == 0 || cols == 0 || (cols > 1 && t.stride(1) != 1) || (rows > 1 && stride < cols)) return false;
+        data = t.data_ptr();
+        return data != nullptr;
+    }
+};
+
+at::Tensor on_device(c10::IntArrayRef sizes, at::ScalarType type, int64_t device)
+{
+    return at::empty(sizes, at::TensorOptions(type).device(c10::Device(c10::kCUDA, static_cast<c10::DeviceIndex>(device))));
+}
+
+// The buffer of a matrix [rows, cols] in 4 bits.
+bool mx_buffer(PyObject *o, int64_t rows, int64_t cols, int64_t device, void **data)
+{
+    return packed_buffer(o, device, mx.bytes(rows, cols), data) && (reinterpret_cast<uintptr_t>(*data) & 15) == 0;
+}
+
+bool whole_numbers(PyObject *const *args, Py_ssize_t n, int64_t *out)
+{
+    for (Py_ssize_t i = 0; i < n; i++) {
+        if (!PyLong_CheckExact(args[i])) return false;
+        out[i] = PyLong_AsLongLong(args[i]);
+    }
+    if (!PyErr_Occurred()) return true;
+    PyErr_Clear();
+    return false;
+}
+
+// mx_quantize(x, by_rows, by_columns) -> (buffer or None, buffer or None), the code of tftq_mx_quantize, or None
+PyObject *mx_quantize(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    if (!arguments("mx_quantize", n, 3)) return nullptr;
+    const bool by_rows = args[1] == Py_True, by_cols = args[2] == Py_True;
+    void *stream = nullptr;
+    try {
+        Matrix x;
+        if (!x.read(args[0]) || !mx_calls(x.device) || !current_stream(x.device, &stream)) Py_RETURN_NONE;
+        const int64_t r_bytes = by_rows ? mx.bytes(x.rows, x.cols) : 0, c_bytes = by_cols ? mx.bytes(x.cols, x.rows) : 0;
+        if (r_bytes < 0 || c_bytes < 0) Py_RETURN_NONE;
+        at::Tensor r, c;
+        int rc;
+        {
+            WithoutInterpreter others_run;
+            if (by_rows) r = on_device({r_bytes}, at::kByte, x.device);
+            if (by_cols) c = on_device({c_bytes}, at::kByte, x.device);
+            rc = mx.quantize(x.dtype, x.data, x.rows, x.cols, x.stride, by_rows ? r.data_ptr() : nullptr, by_cols ? c.data_ptr() : nullptr,
+                             static_cast<int>(x.device), stream);
+        }
+        if (rc) return PyLong_FromLong(rc);
+        PyObject *first = by_rows ? THPVariable_Wrap(std::move(r)) : Py_NewRef(Py_None);
+        PyObject *second = by_cols ? THPVariable_Wrap(std::move(c)) : Py_NewRef(Py_None);
+        PyObject *pair = first && second ? PyTuple_Pack(2, first, second) : nullptr;
+        Py_XDECREF(first);
+        Py_XDECREF(second);
+        return pair;
+    } catch (...) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+}
+
+// mx_product(a, m, b, n, k, dtype) -> a b^T of two buffers, the code of tftq_mx_product, or None
+PyObject *mx_product(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    if (!arguments("mx_product", n, 6)) return nullptr;
+    static const at::ScalarType types[3] = {at::kFloat, at::kHalf, at::kBFloat16};
+    int64_t m, sizes[3];
+    void *stream = nullptr, *a = nullptr, *b = nullptr;
+    if (!whole_numbers(args + 1, 1, &m) || !whole_numbers(args + 3, 3, sizes) || !THPVariable_CheckExact(args[0])) Py_RETURN_NONE;
+    const int64_t cols = sizes[0], k = sizes[1], dtype = sizes[2];
+    if (m <= 0 || cols <= 0 || k <= 0 || dtype < 0 || dtype > 2) Py_RETURN_NONE;
+    try {
+        const int64_t device = THPVariable_Unpack(args[0]).device().index();
+        if (!mx_calls(device) || !mx_buffer(args[0], m, k, device, &a) || !mx_buffer(args[2], cols, k, device, &b) ||
+            !current_stream(device, &stream))
+            Py_RETURN_NONE;
+        at::Tensor out;
+        int rc;
+        {
+            WithoutInterpreter others_run;
+            out = on_device({m, cols}, types[dtype], device);
+            rc = mx.product(static_cast<int>(dtype), a, m, b, cols, k, out.data_ptr(), cols, static_cast<int>(device), stream);
+        }
+        return rc ? PyLong_FromLong(rc) : THPVariable_Wrap(std::move(out));
+    } catch (...) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+}
+
+// mx_linear(x, b, n, k) -> Q(x) b^T, the code of tftq_mx_linear, or None
+PyObject *mx_linear(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    if (!arguments("mx_linear", n, 4)) return nullptr;
+    int64_t sizes[2];
+    void *stream = nullptr, *b = nullptr;
+    if (!whole_numbers(args + 2, 2, sizes)) Py_RETURN_NONE;
+    try {
+        Matrix x;
+        if (!x.read(args[0]) || x.cols != sizes[1] || sizes[0] <= 0 || !mx_calls(x.device) ||
+            !mx_buffer(args[1], sizes[0], x.cols, x.device, &b) || !current_stream(x.device, &stream))
+            Py_RETURN_NONE;
+        const int64_t bytes = mx.linear_workspace(x.dtype, x.data, x.rows, x.stride, sizes[0], x.cols);
+        if (bytes < 0) Py_RETURN_NONE;
+        at::Tensor out, workspace;
+        int rc;
+        {
+            WithoutInterpreter others_run;
+            out = on_device({x.rows, sizes[0]}, x.type, x.device);
+            if (bytes) workspace = on_device({bytes}, at::kByte, x.device);
+            rc = mx.linear(x.dtype, x.data, x.rows, x.stride, b, sizes[0], x.cols, out.data_ptr(), sizes[0],
+                           bytes ? workspace.data_ptr() : nullptr, bytes, static_cast<int>(x.device), stream);
+        }
+        return rc ? PyLong_FromLong(rc) : THPVariable_Wrap(std::move(out));
+    } catch (...) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+}
+
+// mx_dequantize(buffer, rows, columns, dtype) -> the values, the code of tftq_mx_dequantize, or None
+PyObject *mx_dequantize(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    if (!arguments("mx_dequantize", n, 4)) return nullptr;
+    static const at::ScalarType types[3] = {at::kFloat, at::kHalf, at::kBFloat16};
+    int64_t sizes[3];
+    void *stream = nullptr, *matrix = nullptr;
+    if (!whole_numbers(args + 1, 3, sizes) || !THPVariable_CheckExact(args[0])) Py_RETURN_NONE;
+    if (sizes[0] <= 0 || sizes[1] <= 0 || sizes[2] < 0 || sizes[2] > 2) Py_RETURN_NONE;
+    try {
+        const int64_t device = THPVariable_Unpack(args[0]).device().index();
+        if (!mx_calls(device) || !mx_buffer(args[0], sizes[0], sizes[1], device, &matrix) || !current_stream(device, &stream)) Py_RETURN_NONE;
+        at::Tensor out;
+        int rc;
+        {
+            WithoutInterpreter others_run;
+            out = on_device({sizes[0], sizes[1]}, types[sizes[2]], device);
+            rc = mx.dequantize(static_cast<int>(sizes[2]), matrix, sizes[0], sizes[1], out.data_ptr(), sizes[1], static_cast<int>(device), stream);
+        }
+        return rc ? PyLong_FromLong(rc) : THPVariable_Wrap(std::move(out));
+    } catch (...) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+}
+
+// mx_bind(bytes, quantize, product, linear_workspace, linear, dequantize): the addresses of libtftq.so's
+// functions; mx_device(index): a device that has been checked.  Both after bind().
+PyObject *mx_bind(PyObject *, PyObject *args)
+{
+    unsigned long long f[6];
+    if (!PyArg_ParseTuple(args, "KKKKKK", &f[0], &f[1], &f[2], &f[3], &f[4], &f[5])) return nullptr;
+    auto to = [](unsigned long long at, auto &function) {
+        function = reinterpret_cast<typename std::remove_reference<decltype(function)>::type>(static_cast<uintptr_t>(at));
+    };
+    to(f[1], mx.quantize);
+    to(f[2], mx.product);
+    to(f[3], mx.linear_workspace);
+    to(f[4], mx.linear);
+    to(f[5], mx.dequantize);
+    to(f[0], mx.bytes);
+    Py_RETURN_NONE;
+}
+PyObject *mx_device(PyObject *, PyObject *index)
+{
+    const long i = PyLong_AsLong(index);
+    if (i == -1 && PyErr_Occurred()) return nullptr;
+    if (i >= 0 && i < 64) mx.devices |= 1ull << i;
+    Py_RETURN_NONE;
+}
+
 // in_place(owners, pieces, known) -> addresses, or None
 // The owners' addresses as a list of ints, if a kernel may read and write the owners, all at once, as
 // the elements of `pieces` (as many plain contiguous tensors), and `known` itself if they are the
@@ -514,6 +726,12 @@ PyMethodDef methods[] = {
     {"bucket_quantize", fast(bucket_quantize), METH_FASTCALL, "bucket_quantize(plan, device, pointers)"},
     {"bucket_reduce", fast(bucket_reduce), METH_FASTCALL, "bucket_reduce(plan, device, packed, rank, is_avg)"},
     {"bucket_dequantize", fast(bucket_dequantize), METH_FASTCALL, "bucket_dequantize(plan, device, pointers, packed, post_scale)"},
+    {"mx_bind", mx_bind, METH_VARARGS, "mx_bind(bytes, quantize, product, linear_workspace, linear, dequantize)"},
+    {"mx_device", mx_device, METH_O, "mx_device(index): the device can run the kernels"},
+    {"mx_quantize", fast(mx_quantize), METH_FASTCALL, "mx_quantize(x, by_rows, by_columns): the buffers, or None"},
+    {"mx_product", fast(mx_product), METH_FASTCALL, "mx_product(a, m, b, n, k, dtype): a b^T of two buffers, or None"},
+    {"mx_linear", fast(mx_linear), METH_FASTCALL, "mx_linear(x, b, n, k): Q(x) b^T, or None"},
+    {"mx_dequantize", fast(mx_dequantize), METH_FASTCALL, "mx_dequantize(buffer, rows, columns, dtype): the values, or None"},
     {"in_place", in_place, METH_VARARGS,
      "in_place(owners, pieces, known): the owners' addresses if kernels may work on them in place of the pieces, or None"},
     {"describe", describe, METH_VARARGS,

@@ -18,16 +18,47 @@ no function keeps anything from one call for the next.  There is no CPU or eager
 
 from __future__ import annotations
 
+import ctypes
+import threading
+
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
+from . import quantization as _q
 from .quantization import _DTYPE_CODE, _check, _stream_of
 
 _BLOCK = 32    # elements of a scale
 _PANEL = 256   # columns of a panel
 _PANEL_BYTES = _PANEL // 2
 _PANEL_BLOCKS = _PANEL // _BLOCK
+
+
+# The module that makes whole calls with plain arguments (_pylist.mx_quantize and the like: checks,
+# allocations and launch in one step), once it knows the library and a device that can run it.  It answers
+# None to anything else, and the functions below then go their own way.  Host time on small matrices:
+# HOST_TIMES.
+_native = None
+_bind_lock = threading.Lock()
+
+
+def _ready(device: torch.device) -> None:
+    """Raises unless the kernels run on ``device``."""
+    global _native
+    assert device.type == "cuda", "A GPU tensor is required"
+    _lib.check_device(device.index)
+    if not hasattr(_q._pylist, "mx_bind"):
+        return
+    with _bind_lock:
+        if _native is None:
+            lib = _lib.load()
+            _q._bind(lib)
+            if _q._calls is None:
+                return
+            _q._pylist.mx_bind(*(ctypes.cast(getattr(lib, "tftq_mx_" + name), ctypes.c_void_p).value for name in (
+                "bytes", "quantize", "product", "linear_workspace", "linear", "dequantize")))
+            _native = _q._pylist
+        _native.mx_device(device.index)
 
 
 class MXFP4Tensor:
@@ -42,7 +73,7 @@ class MXFP4Tensor:
 
     def __init__(self, buffer: torch.Tensor, shape: tuple, dtype: torch.dtype) -> None:
         self.buffer = buffer
-        self.shape = torch.Size(shape)
+        self.shape = shape if type(shape) is torch.Size else torch.Size(shape)
         self.dtype = dtype
 
     @classmethod
@@ -106,6 +137,10 @@ class MXFP4Tensor:
         dtype = self.dtype if dtype is None else dtype
         assert dtype in _DTYPE_CODE, "Only fp32, fp16 and bf16 are supported"
         rows, columns = self.shape
+        if _native is not None:
+            out = _native.mx_dequantize(self.buffer, rows, columns, _DTYPE_CODE[dtype])
+            if out is not None:
+                return _result(out, "tftq_mx_dequantize")
         out = torch.empty(rows, columns, dtype=dtype, device=self.device)
         _check(_lib.load().tftq_mx_dequantize(_DTYPE_CODE[dtype], self.buffer.data_ptr(), rows, columns, out.data_ptr(),
                                               columns, self.device.index, _stream_of(self.device)),
@@ -120,9 +155,15 @@ class MXFP4Tensor:
         return f"MXFP4Tensor({self.shape[0]}x{self.shape[1]}, of {self.dtype}, on {self.device})"
 
 
+def _result(got, what: str):
+    """What a whole call gave: its result, or the error code of the library."""
+    if type(got) is int:
+        _check(got, what)
+    return got
+
+
 def _empty(rows: int, columns: int, dtype: torch.dtype, device: torch.device) -> MXFP4Tensor:
-    assert device.type == "cuda", "A GPU tensor is required"
-    _lib.check_device(device.index)
+    _ready(device)
     size = _lib.load().tftq_mx_bytes(rows, columns)
     if size < 0:
         _check(size, "tftq_mx_bytes")
@@ -131,6 +172,13 @@ def _empty(rows: int, columns: int, dtype: torch.dtype, device: torch.device) ->
 
 def _quantize(x: torch.Tensor, by_rows: bool, by_columns: bool):
     """(rows, columns), None for what is not asked for."""
+    if _native is not None:
+        got = _native.mx_quantize(x, by_rows, by_columns)
+        if got is not None:
+            r, c = _result(got, "tftq_mx_quantize")
+            shape, dtype = x.shape, x.dtype
+            return (MXFP4Tensor(r, shape, dtype) if by_rows else None,
+                    MXFP4Tensor(c, (shape[1], shape[0]), dtype) if by_columns else None)
     assert x.dim() == 2, "Only 2D tensors are supported"
     assert x.dtype in _DTYPE_CODE, "Only fp32, fp16 and bf16 are supported"
     x = x.detach()
@@ -168,10 +216,36 @@ def matmul_mxfp4(a: MXFP4Tensor, b: MXFP4Tensor, out_dtype: torch.dtype | None =
     assert a.device == b.device, "All inputs must be on the same device"
     assert a.shape[1] == b.shape[1], "The matrices have different numbers of columns"
     (m, k), n = a.shape, b.shape[0]
+    if _native is not None:
+        out = _native.mx_product(a.buffer, m, b.buffer, n, k, _DTYPE_CODE[out_dtype])
+        if out is not None:
+            return _result(out, "tftq_mx_product")
     out = torch.empty(m, n, dtype=out_dtype, device=a.device)
     _check(_lib.load().tftq_mx_product(_DTYPE_CODE[out_dtype], a.buffer.data_ptr(), m, b.buffer.data_ptr(), n, k,
                                        out.data_ptr(), n, a.device.index, _stream_of(a.device)),
            "tftq_mx_product")
+    return out
+
+
+def _linear_rows(x: torch.Tensor, weight: MXFP4Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """``x @ weight.T`` of a matrix x that is quantised along its rows in the call and not kept: in the
+    product's own kernel where x has few rows."""
+    (m, k), n = x.shape, weight.shape[0]
+    if _native is not None and x.dtype == dtype:
+        out = _native.mx_linear(x, weight.buffer, n, k)
+        if out is not None:
+            return _result(out, "tftq_mx_linear")
+    if k > 1 and x.stride(1) != 1 or m > 1 and x.stride(0) < k:
+        x = x.contiguous()
+    lib = _lib.load()
+    size = lib.tftq_mx_linear_workspace(_DTYPE_CODE[dtype], x.data_ptr(), m, x.stride(0), n, k)
+    if size < 0:
+        _check(size, "tftq_mx_linear_workspace")
+    out = torch.empty(m, n, dtype=dtype, device=x.device)
+    workspace = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+    _check(lib.tftq_mx_linear(_DTYPE_CODE[dtype], x.data_ptr(), m, x.stride(0), weight.buffer.data_ptr(), n, k, out.data_ptr(), n,
+                              None if workspace is None else workspace.data_ptr(), size, x.device.index, _stream_of(x.device)),
+           "tftq_mx_linear")
     return out
 
 
@@ -183,8 +257,11 @@ class _Linear(torch.autograd.Function):
     def forward(ctx, x, w):
         for_dw, for_dx = ctx.needs_input_grad[1], ctx.needs_input_grad[0]
         ctx.dtypes = x.dtype, w.dtype
-        x_rows, ctx.x_columns = _quantize(x, True, for_dw)
+        ctx.x_columns = None
         w_rows, ctx.w_columns = _quantize(w, True, for_dx)
+        if not for_dw:
+            return _linear_rows(x.detach(), w_rows, x.dtype)
+        x_rows, ctx.x_columns = _quantize(x, True, True)
         return matmul_mxfp4(x_rows, w_rows, x.dtype)
 
     @staticmethod
@@ -213,7 +290,7 @@ def linear_mxfp4(x: torch.Tensor, weight: "torch.Tensor | MXFP4Tensor") -> torch
     flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1]) if x.numel() else x.new_empty(x.shape[:-1].numel(), x.shape[-1])
     if isinstance(weight, MXFP4Tensor):
         assert not (torch.is_grad_enabled() and x.requires_grad), "A weight in 4 bits has no gradient product"
-        y = matmul_mxfp4(_quantize(flat, True, False)[0], weight, x.dtype)
+        y = _linear_rows(flat.detach(), weight, x.dtype)
     else:
         assert weight.dtype in _DTYPE_CODE, "Only fp32, fp16 and bf16 are supported"
         y = _Linear.apply(flat, weight)
