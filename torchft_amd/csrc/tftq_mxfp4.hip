@@ -44,7 +44,7 @@ __global__ __launch_bounds__(64, 2) void k_mx_quantize(const uint8_t *x, int64_t
 #pragma unroll
         for (int p = 0; p < P; p++) {
             raw[p] = mx_u4{0, 0, 0, 0};
-            if (row + p < rows) raw[p] = *(const mx_u4_any *)(at + (int64_t)p * ld * T::SIZE);
+            if (row + p < rows) raw[p] = __builtin_nontemporal_load((const mx_u4_any *)(at + (int64_t)p * ld * T::SIZE));
         }
     } else {
 #pragma unroll
@@ -55,21 +55,31 @@ __global__ __launch_bounds__(64, 2) void k_mx_quantize(const uint8_t *x, int64_t
     }
 
     if (BY_ROWS) {
-        uint8_t *codes = by_rows.panels + ((int64_t)(col >> 8) * rows + row) * PANEL_BYTES + (col & 255) / 2;
-        uint8_t *scales = by_rows.scales + ((int64_t)(col >> 8) * ((rows + 1) & ~1) + row) * 8 + (col & 255) / 32;
+        // of two rows the even lane stores its and its neighbour's codes of the first, the odd one those of
+        // the second; of four rows every lane of a block's first four stores one's scale
+        const int odd = lane & 1, mine = lane & 3, team = lane % (32 / V);
+        uint8_t *codes = by_rows.panels + ((int64_t)(col >> 8) * rows + row + odd) * PANEL_BYTES + (col & 255 & ~(2 * V - 1)) / 2;
+        uint8_t *scales = by_rows.scales + ((int64_t)(col >> 8) * ((rows + 1) & ~1) + row + mine) * 8 + (col & 255) / 32;
+        uint32_t byte = 0;
 #pragma unroll
-        for (int p = 0; p < P; p++) {
-            uint32_t m = T::mag(raw[p][0]);
+        for (int p = 0; p < P; p += 2) {
+            uint32_t c[2];
 #pragma unroll
-            for (int w = 1; w < 4; w++) m = T::mag_max(m, T::mag(raw[p][w]));
-            const uint32_t byte = mx_byte(T::bits(mx_over_block<T>(T::mag_all(m))));
-            const float scale = mx_scale(byte);
-            const uint32_t c = mx_codes<T>(raw[p], scale);
-            if (row + p < rows) {
-                if (T::SIZE == 4) *(uint16_t *)(codes + p * PANEL_BYTES) = (uint16_t)c;
-                else *(uint32_t *)(codes + p * PANEL_BYTES) = c;
-                if (lane % (32 / V) == 0) scales[p * 8] = (uint8_t)byte;
+            for (int q = 0; q < 2; q++) {
+                uint32_t m = T::mag(raw[p + q][0]);
+#pragma unroll
+                for (int w = 1; w < 4; w++) m = T::mag_max(m, T::mag(raw[p + q][w]));
+                const uint32_t b = mx_byte(T::bits(mx_over_block<T>(T::mag_all(m))));
+                c[q] = mx_codes<T>(raw[p + q], mx_scale(b));
+                if ((p + q) % 4 == mine) byte = b;
             }
+            const uint32_t got = (uint32_t)__builtin_amdgcn_mov_dpp((int)(odd ? c[0] : c[1]), 0xb1, 0xf, 0xf, true);
+            const uint32_t low = odd ? got : c[0], high = odd ? c[1] : got;
+            if (row + p + odd < rows) {
+                if (T::SIZE == 4) *(uint32_t *)(codes + p * PANEL_BYTES) = low | high << 16;
+                else *(uint64_t *)(codes + p * PANEL_BYTES) = low | (uint64_t)high << 32;
+            }
+            if (p % 4 == 2 && team < 4 && row + p - 2 + mine < rows) scales[(p - 2) * 8] = (uint8_t)byte;
         }
     }
     if constexpr (BY_COLS) {
@@ -112,58 +122,43 @@ __global__ __launch_bounds__(64, 2) void k_mx_quantize(const uint8_t *x, int64_t
     }
 }
 
+// A lane turns V neighbouring codes into a vector of 16 bytes; codes are read in the order in which they lie.
 template <int DTYPE>
-__device__ static inline void mx_store(uint8_t *to, const float *v, int n, bool whole)
+__global__ __launch_bounds__(256) void k_mx_dequantize(MxMatrix m, int rows, int cols, uint8_t *out, int64_t ld)
 {
-    if constexpr (DTYPE == TFTQ_F32) {
-        if (whole) {
-            ((float4 *)to)[0] = float4{v[0], v[1], v[2], v[3]};
-            ((float4 *)to)[1] = float4{v[4], v[5], v[6], v[7]};
-        } else {
-            for (int i = 0; i < 8; i++)
-                if (i < n) ((float *)to)[i] = v[i];
-        }
-    } else {
-        uint16_t h[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-            h[i] = DTYPE == TFTQ_F16 ? __builtin_bit_cast(uint16_t, (_Float16)v[i]) : __builtin_bit_cast(uint16_t, (__bf16)v[i]);
-        if (whole) {
-            mx_u4 w;
-#pragma unroll
-            for (int i = 0; i < 4; i++) w[i] = h[2 * i] | (uint32_t)h[2 * i + 1] << 16;
-            *(mx_u4 *)to = w;
-        } else {
-            for (int i = 0; i < 8; i++)
-                if (i < n) ((uint16_t *)to)[i] = h[i];
-        }
-    }
-}
-
-// A lane turns 8 codes, a word of the panels, into 8 neighbouring elements; words are read in the
-// order in which they lie.
-template <int DTYPE>
-__global__ __launch_bounds__(256) void k_mx_dequantize(MxMatrix m, int rows, int cols, uint8_t *out, int64_t ld, int whole)
-{
-    constexpr int SIZE = DTYPE == TFTQ_F32 ? 4 : 2;
-    const int64_t words = (int64_t)((cols + 255) >> 8) * rows * 32;
+    constexpr int SIZE = DTYPE == TFTQ_F32 ? 4 : 2, V = 16 / SIZE, PER_ROW = 256 / V;
+    const int64_t pieces = (int64_t)((cols + 255) >> 8) * rows * PER_ROW;
     const int64_t first = (int64_t)blockIdx.x * 1024 + threadIdx.x;
 #pragma unroll
     for (int q = 0; q < 4; q++) {
-        const int64_t word = first + 256 * q;
-        if (word >= words) return;
-        const int64_t line = word >> 5;  // (panel, row)
-        const int panel = (int)(line / rows), row = (int)(line - (int64_t)panel * rows), in = (int)word & 31;
-        const int col = panel * 256 + in * 8;
+        const int64_t piece = first + 256 * q;
+        if (piece >= pieces) return;
+        const int64_t line = piece / PER_ROW;  // (panel, row)
+        const int panel = (int)(line / rows), row = (int)(line - (int64_t)panel * rows), in = (int)(piece % PER_ROW);
+        const int col = panel * 256 + in * V;
         if (col >= cols) continue;
-        const uint32_t c = ((const uint32_t *)m.panels)[word];
-        const float scale = mx_scale(m.scales[((int64_t)panel * ((rows + 1) & ~1) + row) * 8 + in / 4]);
+        const uint32_t c = SIZE == 4 ? ((const uint16_t *)m.panels)[piece] : ((const uint32_t *)m.panels)[piece];
+        const float scale = mx_scale(m.scales[((int64_t)panel * ((rows + 1) & ~1) + row) * 8 + in * V / 32]);
         const mx_f2 p[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 0), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 1),
                             __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 2), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 3)};
-        float v[8];
+        mx_u4 w = {0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[2 * i] = p[i].x * scale, v[2 * i + 1] = p[i].y * scale;
-        mx_store<DTYPE>(out + ((int64_t)row * ld + col) * SIZE, v, cols - col, whole && col + 8 <= cols);
+        for (int i = 0; i < V; i++) {
+            const float v = (i & 1 ? p[i / 2].y : p[i / 2].x) * scale;
+            if constexpr (DTYPE == TFTQ_F32) w[i] = __float_as_uint(v);
+            else w[i / 2] |= (uint32_t)(DTYPE == TFTQ_F16 ? __builtin_bit_cast(uint16_t, (_Float16)v) : __builtin_bit_cast(uint16_t, (__bf16)v)) << (16 * (i & 1));
+        }
+        uint8_t *to = out + ((int64_t)row * ld + col) * SIZE;
+        if (col + V <= cols) {
+            __builtin_nontemporal_store(w, (mx_u4_any *)to);
+            continue;
+        }
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            if (col + i >= cols) continue;
+            if (SIZE == 4) ((uint32_t *)to)[i] = w[i];
+            else ((uint16_t *)to)[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+        }
     }
 }
 
@@ -227,14 +222,13 @@ extern "C" int tftq_mx_dequantize(int dtype, const void *matrix, int64_t rows, i
     if (rows < 0 || cols < 0 || rows > MX_MOST || cols > MX_MOST) return TFTQ_E_SHAPE;
     if (rows == 0 || cols == 0) return 0;
     if (!matrix || !out || ((uintptr_t)matrix & 15) || row_stride < (rows > 1 ? cols : 0)) return TFTQ_E_ARG;
-    const int64_t groups = (mx_panels(cols) * rows * 32 + 1023) / 1024;
+    const int64_t groups = (mx_panels(cols) * rows * (dtype == TFTQ_F32 ? 64 : 32) + 1023) / 1024;
     if (groups > (1 << 23)) return TFTQ_E_SHAPE;
     DeviceScope scope(device);
     if (scope.err != hipSuccess) return (int)scope.err;
     MxMatrix m = mx_matrix((void *)matrix, rows, cols);
-    const int size = dtype == TFTQ_F32 ? 4 : 2;
-    int whole = row_stride * size % 16 == 0 && (uintptr_t)out % 16 == 0, r = (int)rows, c = (int)cols;
-    void *args[] = {(void *)&m, (void *)&r, (void *)&c, (void *)&out, (void *)&row_stride, (void *)&whole};
+    int r = (int)rows, c = (int)cols;
+    void *args[] = {(void *)&m, (void *)&r, (void *)&c, (void *)&out, (void *)&row_stride};
     const void *k = dtype == TFTQ_F32 ? (const void *)k_mx_dequantize<TFTQ_F32>
                     : dtype == TFTQ_F16 ? (const void *)k_mx_dequantize<TFTQ_F16>
                                         : (const void *)k_mx_dequantize<TFTQ_BF16>;

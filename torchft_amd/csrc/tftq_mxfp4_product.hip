@@ -229,10 +229,20 @@ extern "C" int tftq_mx_product(int dtype, const void *a, int64_t m, const void *
         default: return few<MxQuantized, TFTQ_BF16>(ta.panels, 0, ta.scales, (int)m, tb, (int)k, (uint8_t *)out, row_stride, st);
         }
     }
-    const int64_t big = ((m + 255) / 256) * ((n + 255) / 256), middle = ((m + 127) / 128) * ((n + 127) / 128);
-    if (big >= 160) return product<Tile<256, 256, 2, 4, true>>(dtype, ta, tb, panels, (uint8_t *)out, row_stride, st);
-    if (middle >= 160) return product<Tile<128, 128, 2, 2, true>>(dtype, ta, tb, panels, (uint8_t *)out, row_stride, st);
-    return product<Tile<64, 64, 2, 2, true>>(dtype, ta, tb, panels, (uint8_t *)out, row_stride, st);
+    const TileShape choice[] = {TILES_256, TILES_192X256, TILES_128, TILES_64_FP4};
+    int best = 0;
+    double least = 0;
+    for (int i = 0; i < 4; i++) {
+        const double count = (double)((m + choice[i].high - 1) / choice[i].high) * (double)((n + choice[i].wide - 1) / choice[i].wide);
+        const double time = tile_time(choice[i], count, count * panels, panels);
+        if (i == 0 || time < least) best = i, least = time;
+    }
+    switch (best) {
+    case 0: return product<Tile<256, 256, 2, 4, true>>(dtype, ta, tb, panels, (uint8_t *)out, row_stride, st);
+    case 1: return product<Tile<192, 256, 2, 4, true>>(dtype, ta, tb, panels, (uint8_t *)out, row_stride, st);
+    case 2: return product<Tile<128, 128, 2, 2, true>>(dtype, ta, tb, panels, (uint8_t *)out, row_stride, st);
+    default: return product<Tile<64, 64, 2, 2, true>>(dtype, ta, tb, panels, (uint8_t *)out, row_stride, st);
+    }
 }
 
 // Whether x [m, k] is quantised by the workgroups of the product with n rows.  That saves a launch and the

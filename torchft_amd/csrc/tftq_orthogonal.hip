@@ -14,7 +14,8 @@
 // A = D + E, B = F + G with E and G zero on the diagonal, and
 //     (A A)[i][j] = (E E)[i][j] + (D[i] + D[j]) E[i][j],     (B X)[i][j] = F[i] X[i][j] + (G X)[i][j];
 // and X keeps what its rounding leaves as a second fp16 number (22 bits together), which the products
-// leave out and the term (a + F) X takes in.  Relative error of the result against 64 bits, one
+// leave out and the term (a + F) X takes in.  (Not in the last iteration, to which it adds nothing that
+// one rounding of the result would leave: errors 0 to 10 % larger, and 4 of 46 bytes an element less.)  Relative error of the result against 64 bits, one
 // product each, matrices of 64x64 to 1024x1024 with even, low-rank and 1/i spectra: 2.4e-4 to 1.3e-3
 // (bf16 results are rounded by 1.7e-3; A, B and X in plain bf16: 1.3e-2 to 7.7e-2, in plain fp16 up to
 // 9e-3).  `precise`: A, B and X^T have second numbers too and every product is three, high x high +
@@ -39,7 +40,18 @@ constexpr int64_t NS_LONGEST = 1 << 24;  // rows or columns
 // |X| <= ~1.2, |A| <= ~1.5, |B| <= ~3 with the usual coefficients; others may pass these a few times over.
 // X of a gradient so small that eps divides it stays small: its scale is larger by a power of two (ns_scale).
 constexpr float SCALE_X = 16384.f, SCALE_E = 4096.f, SCALE_G = 2048.f;
-constexpr int NORM_ROWS = 64, NORM_COLS = 1024;  // of the matrix as it lies: the part that a workgroup sums the squares of
+constexpr int NORM_COLS = 1024;
+// The rows of the matrix as it lies, `wide` columns of at most 1024 each, whose squares a workgroup sums up:
+// 64, or 8 where that makes no more than 1024 sums of a matrix (1001x130: 57 -> 12 us).
+__host__ __device__ static inline int ns_part_rows(int64_t high, int64_t wide)
+{
+    return (high + 7) / 8 * ((wide + NORM_COLS - 1) / NORM_COLS) <= 1024 ? 8 : 64;
+}
+__host__ __device__ static inline int64_t ns_parts_of(int64_t high, int64_t wide)
+{
+    const int rows = ns_part_rows(high, wide);
+    return (high + rows - 1) / rows * ((wide + NORM_COLS - 1) / NORM_COLS);
+}
 
 struct NsMatrix {
     const uint8_t *in;
@@ -49,7 +61,6 @@ struct NsMatrix {
     uint8_t *work;
     int rows, cols;  // of X
     int flip;        // X is the transpose of the matrix as it lies
-    int whole_in, whole_momentum, whole_out;  // vectors of the rows are aligned
     float step;      // out = keep * out - step * X with NsParams::update, else out = X
     int first;       // the launch's first workgroup of this matrix
 };
@@ -59,7 +70,8 @@ struct NsLaunch {
 };
 struct NsParams {
     float momentum, keep, a, b, c, eps, growth;
-    int nesterov, in_dtype, out_dtype, update, last;
+    int nesterov, in_dtype, out_dtype, update;
+    int last, next_last;  // the last iteration, the one before it
 };
 static_assert(sizeof(NsLaunch) + sizeof(NsParams) <= 3800, "kernel arguments");
 
@@ -78,7 +90,7 @@ __host__ __device__ static inline NsWork ns_work(uint8_t *base, int64_t r, int64
 {
     const int64_t rp = (r + 63) / 64, kp = (k + 63) / 64, x = kp * r * PANEL_BYTES, t = rp * k * PANEL_BYTES, a = rp * r * PANEL_BYTES;
     const int64_t high = flip ? k : r, wide = flip ? r : k;
-    const int64_t parts = ((high + NORM_ROWS - 1) / NORM_ROWS) * ((wide + NORM_COLS - 1) / NORM_COLS);
+    const int64_t parts = ns_parts_of(high, wide);
     NsWork w;
     w.x = base, w.xl = w.x + x;
     w.t = w.xl + x, w.t2 = w.t + t;
@@ -101,16 +113,17 @@ __device__ static inline int ns_find(const NsLaunch &l, int id, int *piece)
     return i;
 }
 
-// 4 neighbouring elements, n of which exist.
-__device__ static inline tile_f4 ns_read(const uint8_t *from, int64_t at, int dtype, bool whole, int n)
+// 4 neighbouring elements at any element's address, n of which exist.
+typedef float ns_f4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef _Float16 ns_h4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef __bf16 ns_b4_any __attribute__((ext_vector_type(4), aligned(2)));
+__device__ static inline tile_f4 ns_read(const uint8_t *from, int64_t at, int dtype, int n)
 {
-    typedef _Float16 H4 __attribute__((ext_vector_type(4)));
-    typedef __bf16 B4 __attribute__((ext_vector_type(4)));
     tile_f4 v = {0.f, 0.f, 0.f, 0.f};
-    if (whole && n >= 4) {
-        if (dtype == TFTQ_F32) return *(const tile_f4 *)(from + at * 4);
-        if (dtype == TFTQ_F16) return __builtin_convertvector(*(const H4 *)(from + at * 2), tile_f4);
-        return __builtin_convertvector(*(const B4 *)(from + at * 2), tile_f4);
+    if (n >= 4) {
+        if (dtype == TFTQ_F32) return *(const ns_f4_any *)(from + at * 4);
+        if (dtype == TFTQ_F16) return __builtin_convertvector(*(const ns_h4_any *)(from + at * 2), tile_f4);
+        return __builtin_convertvector(*(const ns_b4_any *)(from + at * 2), tile_f4);
     }
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -130,8 +143,9 @@ __global__ __launch_bounds__(256) void k_ns_squares(const NsLaunch l, const NsPa
     const NsMatrix m = l.m[ns_find(l, blockIdx.x, &piece)];
     const int high = m.flip ? m.cols : m.rows, wide = m.flip ? m.rows : m.cols;
     const int across = (wide + NORM_COLS - 1) / NORM_COLS;
-    const int row0 = piece / across * NORM_ROWS, col0 = piece % across * NORM_COLS;
-    const int rows = min(NORM_ROWS, high - row0);
+    const int part = ns_part_rows(high, wide);
+    const int row0 = piece / across * part, col0 = piece % across * NORM_COLS;
+    const int rows = min(part, high - row0);
     // a thread has 4 neighbouring columns of every `apart`th row
     const int groups = (min(NORM_COLS, wide - col0) + 3) >> 2, apart = 256 / groups;
     const int c = col0 + (int)threadIdx.x % groups * 4, n = wide - c;
@@ -143,8 +157,8 @@ __global__ __launch_bounds__(256) void k_ns_squares(const NsLaunch l, const NsPa
 #pragma unroll
             for (int q = 0; q < AT_ONCE; q++) {
                 const int64_t r = min(r0 + q * apart, row0 + rows - 1);
-                u[q] = ns_read(m.in, r * m.ld_in + c, p.in_dtype, m.whole_in, n);
-                if (m.momentum) next[q] = ns_read((const uint8_t *)m.momentum, r * m.ld_momentum + c, TFTQ_F32, m.whole_momentum, n);
+                u[q] = ns_read(m.in, r * m.ld_in + c, p.in_dtype, n);
+                if (m.momentum) next[q] = ns_read((const uint8_t *)m.momentum, r * m.ld_momentum + c, TFTQ_F32, n);
             }
 #pragma unroll
             for (int q = 0; q < AT_ONCE; q++) {
@@ -154,8 +168,8 @@ __global__ __launch_bounds__(256) void k_ns_squares(const NsLaunch l, const NsPa
                     float *at = m.momentum + r * m.ld_momentum + c;
 #pragma unroll
                     for (int i = 0; i < 4; i++) next[q][i] = ns_momentum(next[q][i], u[q][i], p), u[q][i] = ns_update(next[q][i], u[q][i], p);
-                    if (m.whole_momentum && n >= 4) {
-                        *(tile_f4 *)at = next[q];
+                    if (n >= 4) {
+                        *(ns_f4_any *)at = next[q];
                     } else {
 #pragma unroll
                         for (int i = 0; i < 4; i++)
@@ -198,7 +212,7 @@ __global__ __launch_bounds__(256) void k_ns_start(const NsLaunch l, const NsPara
     const int across = (m.cols + 63) / 64;
     const int row0 = piece / across * 64, col0 = piece % across * 64;
     const int high = m.flip ? m.cols : m.rows, wide = m.flip ? m.rows : m.cols;
-    const int parts = (high + NORM_ROWS - 1) / NORM_ROWS * ((wide + NORM_COLS - 1) / NORM_COLS);
+    const int parts = (int)ns_parts_of(high, wide);
     double sum = 0;
     for (int i = threadIdx.x; i < parts; i += 256) sum += w.squares[i];
     for (int s = 32; s; s >>= 1) sum += __shfl_xor(sum, s);
@@ -216,9 +230,9 @@ __global__ __launch_bounds__(256) void k_ns_start(const NsLaunch l, const NsPara
         tile_f4 v = {0.f, 0.f, 0.f, 0.f};
         if (at_row + r < high && n > 0) {
             const int64_t row = at_row + r;
-            v = ns_read(m.in, row * m.ld_in + at_col + c, p.in_dtype, m.whole_in, n);
+            v = ns_read(m.in, row * m.ld_in + at_col + c, p.in_dtype, n);
             if (m.momentum) {
-                const tile_f4 old = ns_read((const uint8_t *)m.momentum, row * m.ld_momentum + at_col + c, TFTQ_F32, m.whole_momentum, n);
+                const tile_f4 old = ns_read((const uint8_t *)m.momentum, row * m.ld_momentum + at_col + c, TFTQ_F32, n);
 #pragma unroll
                 for (int i = 0; i < 4; i++) v[i] = ns_update(old[i], v[i], p);
             }
@@ -263,42 +277,31 @@ __global__ __launch_bounds__(256) void k_ns_start(const NsLaunch l, const NsPara
 __device__ static inline void ns_put(const NsMatrix m, const NsParams p, int64_t row, int64_t col, int n, const float *v)
 {
     const int64_t at = row * m.ld_out + col;
-    if (p.out_dtype == TFTQ_F32) {
-        float *to = (float *)m.out + at;
-        const bool vector = m.whole_out && n >= 8;
+    const int size = p.out_dtype == TFTQ_F32 ? 4 : 2;
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            tile_f4 o = {0.f, 0.f, 0.f, 0.f};
-            if (p.update && vector) o = ((const tile_f4 *)to)[h];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int q = 4 * h + i;
-                if (p.update && !vector && q < n) o[i] = to[q];
-                o[i] = p.update ? p.keep * o[i] - m.step * v[q] : v[q];
-                if (!vector && q < n) to[q] = o[i];
-            }
-            if (vector) ((tile_f4 *)to)[h] = o;
-        }
-        return;
-    }
-    uint16_t *to = (uint16_t *)m.out + at;
-    const bool half = p.out_dtype == TFTQ_F16;
-    typedef uint16_t s8 __attribute__((ext_vector_type(8)));
-    s8 o;
-    const bool vector = m.whole_out && n >= 8;
-    if (p.update && vector) o = *(const s8 *)to;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        float r = v[i];
+    for (int h = 0; h < 8; h += 4) {
+        uint8_t *to = m.out + (at + h) * size;
+        tile_f4 o = {v[h], v[h + 1], v[h + 2], v[h + 3]};
+        if (n - h <= 0) return;
         if (p.update) {
-            if (!vector) o[i] = i < n ? to[i] : (uint16_t)0;
-            const float old = half ? (float)__builtin_bit_cast(_Float16, (uint16_t)o[i]) : (float)__builtin_bit_cast(__bf16, (uint16_t)o[i]);
-            r = p.keep * old - m.step * r;
+            const tile_f4 old = ns_read(to, 0, p.out_dtype, n - h);
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[i] = p.keep * old[i] - m.step * o[i];
         }
-        o[i] = half ? __builtin_bit_cast(uint16_t, (_Float16)r) : __builtin_bit_cast(uint16_t, (__bf16)r);
-        if (!vector && i < n) to[i] = o[i];
+        if (n - h >= 4) {
+            if (p.out_dtype == TFTQ_F32) *(ns_f4_any *)to = o;
+            else if (p.out_dtype == TFTQ_F16) *(ns_h4_any *)to = __builtin_convertvector(o, ns_h4_any);
+            else *(ns_b4_any *)to = __builtin_convertvector(o, ns_b4_any);
+            continue;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (i >= n - h) continue;
+            if (p.out_dtype == TFTQ_F32) ((float *)to)[i] = o[i];
+            else if (p.out_dtype == TFTQ_F16) ((_Float16 *)to)[i] = (_Float16)o[i];
+            else ((__bf16 *)to)[i] = (__bf16)o[i];
+        }
     }
-    if (vector) *(s8 *)to = o;
 }
 
 enum { NS_A, NS_B, NS_X };
@@ -337,7 +340,7 @@ struct NsFinish {
         Old o = {};
         if (WHAT == NS_A || i >= r || j >= padded) return o;
         o.high = *(const ns_h8 *)((WHAT == NS_B ? w.e : w.x) + at(i, j));
-        if (LOW) o.low = *(const ns_h8 *)((WHAT == NS_B ? w.el : w.xl) + at(i, j));
+        if (PRECISE || (LOW && !p.last)) o.low = *(const ns_h8 *)((WHAT == NS_B ? w.el : w.xl) + at(i, j));
         o.di = WHAT == NS_B ? w.d[i] : p.a + w.f[i];
         return o;
     }
@@ -376,7 +379,7 @@ struct NsFinish {
             return;
         }
         *(ns_h8 *)(out + at(i, j)) = high;
-        if (LOW) *(ns_h8 *)(out_l + at(i, j)) = low;
+        if (PRECISE || (LOW && !p.next_last)) *(ns_h8 *)(out_l + at(i, j)) = low;
     }
     // The values of column j, rows i to i + 7, along the columns.
     __device__ __forceinline__ void column(int i, int j, const float *v) const
@@ -564,33 +567,21 @@ static int launch_tiles(NsLaunch &l, bool precise, const NsParams &p, int turn, 
     return launch_over(l, [](const NsMatrix &m) { return tiles(m, WHAT, T::ROWS, T::COLS); }, k, T::THREADS, p, turn, st);
 }
 
-// The tiles that a product of the matrices of a launch is cut into.  `cost` is what a panel of the tiles
-// that run at once on a compute unit takes, that of one tile of 256 x 256 being 1, from the rates of
-// launches that fill all units evenly (8192^3, TFLOP/s: 256x256 1230, 192x256 1190, 192x192 1040,
-// 128x128 1000, 64x64 600); `at_once`: how many that is.
-struct NsTiles {
-    int high, wide, at_once;
-    double cost;
-};
-constexpr NsTiles NS_256 = {256, 256, 1, 1.0}, NS_192X256 = {192, 256, 1, 0.775}, NS_192 = {192, 192, 1, 0.665},
-                  NS_128 = {128, 128, 2, 0.61}, NS_64 = {64, 64, 4, 0.51};
-
-// About how many panels of a 256 x 256 tile a product takes: as many rounds of tiles as the compute
-// units need, or the longest tile.
-static double ns_time(const NsLaunch &l, int what, const NsTiles &t)
+// About how long a product of the matrices of a launch takes in tiles of a size.
+static double ns_time(const NsLaunch &l, int what, const TileShape &t)
 {
-    double work = 0, longest = 0;
-    int64_t count = 0;
+    double work = 0, longest = 0, count = 0;
     for (int i = 0; i < l.count; i++) {
-        const int64_t n = tiles(l.m[i], what, t.high, t.wide);
+        const double n = (double)tiles(l.m[i], what, t.high, t.wide);
         const double panels = ((what == NS_A ? l.m[i].cols : l.m[i].rows) + 63) / 64;
-        count += n, work += (double)n * panels, longest = std::max(longest, panels);
+        count += n, work += n * panels, longest = std::max(longest, panels);
     }
-    const double rounds = (double)((count + 256 * t.at_once - 1) / (256 * t.at_once));
-    return std::max(longest, rounds * work / count) * t.cost;
+    return tile_time(t, count, work, longest);
 }
 
-// One of the three products for all matrices of a launch.
+// One of the three products for all matrices of a launch.  Up to 512 tiles of 32 x 32 take k_ns_small
+// (graph replays, whole orthogonalisation: 512x512 fp32 138 us, with tiles of 64 x 64 219; 256x512 108,
+// 183; with 1024 as the limit, 1024x1024 454, 389).
 template <int WHAT>
 static int product(NsLaunch &l, bool precise, const NsParams &p, int turn, hipStream_t st)
 {
@@ -605,7 +596,7 @@ static int product(NsLaunch &l, bool precise, const NsParams &p, int turn, hipSt
         const void *k = precise ? (const void *)k_ns_small<WHAT, true> : (const void *)k_ns_small<WHAT, false>;
         return launch_over(l, [](const NsMatrix &m) { return tiles(m, WHAT, 32, 32); }, k, 512, p, turn, st);
     }
-    const NsTiles choice[] = {NS_256, WHAT == NS_X ? NS_192X256 : NS_192, NS_128, NS_64};
+    const TileShape choice[] = {TILES_256, WHAT == NS_X ? TILES_192X256 : TILES_192, TILES_128, TILES_64};
     int best = 0;
     for (int i = 1; i < 4; i++)
         if (ns_time(l, WHAT, choice[i]) < ns_time(l, WHAT, choice[best])) best = i;
@@ -690,7 +681,6 @@ extern "C" int tftq_newton_schulz(const tftq_ns *what, void *workspace, int64_t 
     DeviceScope scope(device);
     if (scope.err != hipSuccess) return (int)scope.err;
     hipStream_t st = (hipStream_t)stream;
-    const int out_size = s.out_dtype == TFTQ_F32 ? 4 : 2;
 
     return ns_parts(s.n, s.shapes, s.precise, [&](const int *at, int count, bool precise, int64_t) {
         NsLaunch l;
@@ -704,20 +694,16 @@ extern "C" int tftq_newton_schulz(const tftq_ns *what, void *workspace, int64_t 
             m.ld_in = s.in_stride[i], m.ld_out = s.out_stride[i], m.ld_momentum = s.momenta ? s.momenta_stride[i] : 0;
             m.flip = rows > cols;
             m.rows = (int)std::min(rows, cols), m.cols = (int)std::max(rows, cols);
-            const int in_size = s.in_dtype == TFTQ_F32 ? 4 : 2;
-            m.whole_in = m.ld_in * in_size % 16 == 0 && (uintptr_t)m.in % 16 == 0;
-            m.whole_momentum = m.ld_momentum % 4 == 0 && (uintptr_t)m.momentum % 16 == 0;
-            m.whole_out = m.ld_out * out_size % 16 == 0 && (uintptr_t)m.out % 16 == 0;
             m.step = s.steps ? s.steps[i] : 0.f;
             m.work = work;
             work += ns_work(nullptr, m.rows, m.cols, m.flip, precise).bytes;
         }
         float growth = 1.f;
         for (int it = 0; it < s.iterations; it++) growth *= fmaxf(1.f, fabsf(s.coefficients[3 * it]));
-        NsParams p = {s.momentum, s.keep, 0, 0, 0, s.eps, growth, s.nesterov, s.in_dtype, s.out_dtype, s.steps != nullptr, 0};
+        NsParams p = {s.momentum, s.keep, 0, 0, 0, s.eps, growth, s.nesterov, s.in_dtype, s.out_dtype, s.steps != nullptr, 0, 0};
         int rc = launch_over(l, [](const NsMatrix &m) {
             const int64_t high = m.flip ? m.cols : m.rows, wide = m.flip ? m.rows : m.cols;
-            return (high + NORM_ROWS - 1) / NORM_ROWS * ((wide + NORM_COLS - 1) / NORM_COLS);
+            return ns_parts_of(high, wide);
         }, (const void *)k_ns_squares, 256, p, precise, st);
         if (rc) return rc;
         rc = launch_over(l, [](const NsMatrix &m) { return (int64_t)((m.rows + 63) / 64) * ((m.cols + 63) / 64); },
@@ -725,7 +711,7 @@ extern "C" int tftq_newton_schulz(const tftq_ns *what, void *workspace, int64_t 
         if (rc) return rc;
         for (int it = 0; it < s.iterations; it++) {
             p.a = s.coefficients[3 * it], p.b = s.coefficients[3 * it + 1], p.c = s.coefficients[3 * it + 2];
-            p.last = it + 1 == s.iterations;
+            p.last = it + 1 == s.iterations, p.next_last = it + 2 == s.iterations;
             if ((rc = product<NS_A>(l, precise, p, it & 1, st)) || (rc = product<NS_B>(l, precise, p, it & 1, st)) ||
                 (rc = product<NS_X>(l, precise, p, it & 1, st)))
                 return rc;

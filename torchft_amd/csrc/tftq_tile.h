@@ -383,3 +383,24 @@ __device__ static inline void tile_place(int piece, int tiles_m, int tiles_n, in
     *tn = in / height;
     *tm = first + in % height;
 }
+
+// A size of tiles.  `cost` is what a panel of the tiles that run at once on a compute unit takes, that of one
+// of 256 x 256 being 1; `at_once`: how many that is.  From the rates of launches that fill all units
+// evenly (8192^3, fp16, TFLOP/s: 256x256 1230, 192x256 1190, 192x192 1040, 128x128 1000, 64x64 600;
+// 4-bit, 256x256 4300, 128x128 3500, 64x64 1900).
+struct TileShape {
+    int high, wide, at_once;
+    double cost;
+};
+constexpr TileShape TILES_256 = {256, 256, 1, 1.0}, TILES_192X256 = {192, 256, 1, 0.775}, TILES_192 = {192, 192, 1, 0.665},
+                    TILES_128 = {128, 128, 2, 0.61}, TILES_64 = {64, 64, 4, 0.51}, TILES_64_FP4 = {64, 64, 3, 0.425};
+
+// About how many panels of a 256 x 256 tile `count` tiles of that size take together: `work` panels in
+// all, `longest` the longest of them, in as many rounds as the 256 units need.  Storing a tile's values
+// and waiting for its first operands takes about as long as 4 panels.
+static inline double tile_time(const TileShape &t, double count, double work, double longest)
+{
+    const double rounds = (double)(((int64_t)count + 256 * t.at_once - 1) / (256 * t.at_once));
+    const double each = work / count + 4, most = longest + 4;
+    return (rounds * each > most ? rounds * each : most) * t.cost;
+}

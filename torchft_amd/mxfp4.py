@@ -65,7 +65,7 @@ class MXFP4Tensor:
     """A matrix ``[rows, columns]`` in 4-bit microscaled form, blocks of 32 along its rows.
 
     ``buffer`` holds it in the order in which the product reads it (``tftq_mx_bytes`` of
-    ``include/tftq.h`` describes it); :attr:`codes` and :attr:`scales` are copies in the usual order.
+    ``include/tftq.h`` describes it); :attr:`codes` and :attr:`scales` are in the usual order (copies where that is another).
     ``dtype`` is what it was quantised from and what :meth:`dequantize` and products return by
     default.  It is no ``torch.Tensor``: it has no gradient and takes part in the functions of this module."""
 
@@ -122,15 +122,24 @@ class MXFP4Tensor:
     def codes(self) -> torch.Tensor:
         """``[rows, blocks, 16]`` bytes of two codes each."""
         rows, columns = self.shape
-        codes = self._panel_views()[0].transpose(0, 1)
-        return codes.reshape(rows, codes.shape[1] * _PANEL_BLOCKS, _BLOCK // 2)[:, :-(-columns // _BLOCK)]
+        panels, blocks = -(-columns // _PANEL), -(-columns // _BLOCK)
+        codes = self.buffer.as_strided((rows, panels, _PANEL_BYTES), (_PANEL_BYTES, rows * _PANEL_BYTES, 1))
+        codes = codes.reshape(rows, panels * _PANEL_BLOCKS, _BLOCK // 2)
+        return codes if blocks == panels * _PANEL_BLOCKS else codes[:, :blocks]
 
     @property
     def scales(self) -> torch.Tensor:
         """``[rows, blocks]`` exponents plus 127; 255 for a block that is NaN."""
         rows, columns = self.shape
-        scales = self._panel_views()[1][:, :rows].transpose(0, 1)
-        return scales.reshape(rows, scales.shape[1] * _PANEL_BLOCKS)[:, :-(-columns // _BLOCK)]
+        panels, blocks, even = -(-columns // _PANEL), -(-columns // _BLOCK), rows + rows % 2
+        if rows == 0 or panels == 0:
+            return self.buffer.new_empty(rows, blocks)
+        if panels == 1:
+            return self._panel_views()[1][0, :rows, :blocks]
+        # a row's 8 scales of a panel are moved as one number
+        scales = self.buffer.view(torch.int64).as_strided((rows, panels), (1, even), panels * rows * _PANEL_BYTES // 8)
+        scales = scales.contiguous().view(torch.uint8)
+        return scales if blocks == panels * _PANEL_BLOCKS else scales[:, :blocks]
 
     def dequantize(self, dtype: torch.dtype | None = None) -> torch.Tensor:
         """The values that the matrix stands for, rounded once to ``dtype``."""
@@ -283,6 +292,10 @@ def linear_mxfp4(x: torch.Tensor, weight: "torch.Tensor | MXFP4Tensor") -> torch
     ``dx = dy @ weight`` and ``dw = dy.T @ x`` with every operand quantised along the contracted axis.
     A weight that is kept in 4 bits along ``k`` cannot be contracted along ``n``: gradients through it are
     refused."""
+    if _native is not None and type(weight) is MXFP4Tensor and not (x.requires_grad and torch.is_grad_enabled()):
+        out = _native.mx_linear(x, weight.buffer, *weight.shape)
+        if out is not None:
+            return _result(out, "tftq_mx_linear")
     assert x.dim() >= 1, "x has at least one dimension"
     assert x.dtype in _DTYPE_CODE, "Only fp32, fp16 and bf16 are supported"
     assert len(weight.shape) == 2 and x.shape[-1] == weight.shape[1], "The last dimension of x is not the weight's number of columns"
