@@ -62,7 +62,7 @@ struct NsMatrix {
     int rows, cols;  // of X
     int flip;        // X is the transpose of the matrix as it lies
     float step;      // out = keep * out - step * X with NsParams::update, else out = X
-    int first;       // the launch's first workgroup of this matrix
+    int first, pieces;  // the launch's first workgroup of this matrix (products: in eighths, ns_tile), and how many it has
 };
 struct NsLaunch {
     int count;
@@ -130,6 +130,19 @@ __device__ static inline tile_f4 ns_read(const uint8_t *from, int64_t at, int dt
         if (i < n) v[i] = dtype == TFTQ_F32 ? ((const float *)from)[at + i] : dtype == TFTQ_F16 ? (float)((const _Float16 *)from)[at + i] : (float)((const __bf16 *)from)[at + i];
     return v;
 }
+// The matrix and the tile of a product's workgroup: every XCD takes an eighth of every matrix's tiles,
+// neighbouring ones (workgroups go to the 8 XCDs in turn), so that the matrices with most panels are
+// shared by all (one run of the whole list's tiles each: A of 3 matrices of 88 panels and 4 of 32, 161 us).
+// False for a workgroup that fills up a matrix's last eight.
+__device__ static inline bool ns_tile(const NsLaunch &l, int id, int *matrix, int *piece)
+{
+    int n;
+    *matrix = ns_find(l, id >> 3, &n);
+    const int xcd = id & 7, count = l.m[*matrix].pieces, whole = count >> 3, more = count & 7;
+    *piece = xcd * whole + min(xcd, more) + n;
+    return n < whole + (xcd < more);
+}
+
 // The momentum's next value and the update that is orthogonalised.
 __device__ static inline float ns_momentum(float m, float g, const NsParams &p) { return m * p.momentum + (1.f - p.momentum) * g; }
 __device__ static inline float ns_update(float m, float g, const NsParams &p) { return p.nesterov ? g + p.momentum * (m - g) : m; }
@@ -434,8 +447,9 @@ template <class T, int WHAT, bool PRECISE>
 __global__ __launch_bounds__(T::THREADS) void k_ns_product(const NsLaunch l, const NsParams p, int turn)
 {
     __shared__ __attribute__((aligned(128))) uint8_t lds[T::LDS];
-    int piece, tm, tn;
-    const NsMatrix m = l.m[ns_find(l, tile_piece(blockIdx.x, gridDim.x), &piece)];
+    int matrix, piece, tm, tn;
+    if (!ns_tile(l, blockIdx.x, &matrix, &piece)) return;
+    const NsMatrix m = l.m[matrix];
     const NsWork w = ns_work(m.work, m.rows, m.cols, m.flip, PRECISE);
     const NsProduct<WHAT> o(m, w, turn);
     o.tile(piece, T::ROWS, T::COLS, &tm, &tn);
@@ -480,8 +494,9 @@ __global__ __launch_bounds__(512) void k_ns_small(const NsLaunch l, const NsPara
 {
     constexpr int WAVES = 8, PITCH = 36;
     __shared__ __attribute__((aligned(128))) float sums[WAVES][32 * PITCH];
-    int piece, tm, tn;
-    const NsMatrix m = l.m[ns_find(l, tile_piece(blockIdx.x, gridDim.x), &piece)];
+    int matrix, piece, tm, tn;
+    if (!ns_tile(l, blockIdx.x, &matrix, &piece)) return;
+    const NsMatrix m = l.m[matrix];
     const NsWork w = ns_work(m.work, m.rows, m.cols, m.flip, PRECISE);
     const NsProduct<WHAT> o(m, w, turn);
     o.tile(piece, 32, 32, &tm, &tn);
@@ -542,16 +557,18 @@ __global__ __launch_bounds__(512) void k_ns_small(const NsLaunch l, const NsPara
 // host side
 // ---------------------------------------------------------------------------
 template <class F>
-static int launch_over(NsLaunch &l, F workgroups, const void *kernel, int threads, const NsParams &p, int extra, hipStream_t st)
+static int launch_over(NsLaunch &l, F workgroups, bool eighths, const void *kernel, int threads, const NsParams &p, int extra, hipStream_t st)
 {
     int64_t total = 0;
     for (int i = 0; i < l.count; i++) {
-        l.m[i].first = (int)total;
-        total += workgroups(l.m[i]);
+        const int64_t n = workgroups(l.m[i]);
+        if (n > (1 << 22)) return TFTQ_E_SHAPE;
+        l.m[i].first = (int)total, l.m[i].pieces = (int)n;
+        total += eighths ? (n + 7) / 8 : n;
         if (total > (1 << 22)) return TFTQ_E_SHAPE;
     }
     void *args[] = {(void *)&l, (void *)&p, (void *)&extra};
-    return (int)hipLaunchKernel(kernel, dim3((unsigned)total), dim3(threads), args, 0, st);
+    return (int)hipLaunchKernel(kernel, dim3((unsigned)(eighths ? total * 8 : total)), dim3(threads), args, 0, st);
 }
 
 static int64_t tiles(const NsMatrix &m, int what, int high, int wide)
@@ -564,7 +581,7 @@ template <class T, int WHAT>
 static int launch_tiles(NsLaunch &l, bool precise, const NsParams &p, int turn, hipStream_t st)
 {
     const void *k = precise ? (const void *)k_ns_product<T, WHAT, true> : (const void *)k_ns_product<T, WHAT, false>;
-    return launch_over(l, [](const NsMatrix &m) { return tiles(m, WHAT, T::ROWS, T::COLS); }, k, T::THREADS, p, turn, st);
+    return launch_over(l, [](const NsMatrix &m) { return tiles(m, WHAT, T::ROWS, T::COLS); }, true, k, T::THREADS, p, turn, st);
 }
 
 // About how long a product of the matrices of a launch takes in tiles of a size.
@@ -594,7 +611,7 @@ static int product(NsLaunch &l, bool precise, const NsParams &p, int turn, hipSt
     }
     if (small <= 512) {
         const void *k = precise ? (const void *)k_ns_small<WHAT, true> : (const void *)k_ns_small<WHAT, false>;
-        return launch_over(l, [](const NsMatrix &m) { return tiles(m, WHAT, 32, 32); }, k, 512, p, turn, st);
+        return launch_over(l, [](const NsMatrix &m) { return tiles(m, WHAT, 32, 32); }, true, k, 512, p, turn, st);
     }
     const TileShape choice[] = {TILES_256, WHAT == NS_X ? TILES_192X256 : TILES_192, TILES_128, TILES_64};
     int best = 0;
@@ -704,9 +721,9 @@ extern "C" int tftq_newton_schulz(const tftq_ns *what, void *workspace, int64_t 
         int rc = launch_over(l, [](const NsMatrix &m) {
             const int64_t high = m.flip ? m.cols : m.rows, wide = m.flip ? m.rows : m.cols;
             return ns_parts_of(high, wide);
-        }, (const void *)k_ns_squares, 256, p, precise, st);
+        }, false, (const void *)k_ns_squares, 256, p, precise, st);
         if (rc) return rc;
-        rc = launch_over(l, [](const NsMatrix &m) { return (int64_t)((m.rows + 63) / 64) * ((m.cols + 63) / 64); },
+        rc = launch_over(l, [](const NsMatrix &m) { return (int64_t)((m.rows + 63) / 64) * ((m.cols + 63) / 64); }, false,
                          (const void *)k_ns_start, 256, p, precise, st);
         if (rc) return rc;
         for (int it = 0; it < s.iterations; it++) {
