@@ -97,8 +97,8 @@ __host__ __device__ static inline NsWork ns_work(uint8_t *base, int64_t r, int64
     w.tl = w.t2 + t, w.tl2 = w.tl + (precise ? t : 0);
     w.e = w.tl2 + (precise ? t : 0), w.g = w.e + a;
     w.el = w.g + a, w.gl = w.el + (precise ? a : 0);
-    w.d = (float *)(w.gl + (precise ? a : 0)), w.f = w.d + ((r + 31) & ~31ll);
-    w.scale = w.f + ((r + 31) & ~31ll);
+    w.d = (float *)(w.gl + (precise ? a : 0)), w.f = w.d + ((r + 63) & ~63ll);
+    w.scale = w.f + ((r + 63) & ~63ll);
     w.squares = (double *)(w.scale + 32);
     w.bytes = (uint8_t *)(w.squares + ((parts + 15) & ~15ll)) - base;
     return w;
@@ -319,7 +319,10 @@ __device__ static inline void ns_put(const NsMatrix m, const NsParams p, int64_t
 
 enum { NS_A, NS_B, NS_X };
 
-// What becomes of a product's sums: E and D, G and F, or X, X^T and the result.
+// What becomes of a product's sums: E and D, G and F, or X, X^T and the result.  Everything is kept in the
+// scale of the fp16 numbers that come of it, so that a value costs a few instructions: a tile's 65 536
+// values and their transposes are as much work for the vector units as 20 panels of products are for
+// the matrix cores (before: 45).
 template <int WHAT, bool PRECISE>
 struct NsFinish {
     static constexpr bool LOW = PRECISE || WHAT == NS_X;  // the result's rows have a remainder
@@ -327,7 +330,7 @@ struct NsFinish {
     NsParams p;
     NsWork w;
     uint8_t *out, *out_l, *turned, *turned_l;  // panels along the result's rows, and along its columns
-    float scale_x, per_x;                      // powers of two
+    float per_x;                               // one over X's scale, a power of two
     int r, cols, padded;
     bool mirror;
 
@@ -336,11 +339,10 @@ struct NsFinish {
     {
         out = WHAT == NS_A ? w.e : WHAT == NS_B ? w.g : w.x, out_l = WHAT == NS_A ? w.el : WHAT == NS_B ? w.gl : w.xl;
         turned = WHAT != NS_X ? out : turn ? w.t : w.t2, turned_l = WHAT != NS_X ? out_l : turn ? w.tl : w.tl2;
-        scale_x = *w.scale, per_x = 1.f / scale_x;
+        per_x = 1.f / *w.scale;
         r = m.rows, cols = WHAT == NS_X ? m.cols : m.rows, padded = (cols + 63) & ~63;
         mirror = WHAT == NS_X ? !p.last || m.flip : !diagonal;
     }
-    __device__ float scale() const { return WHAT == NS_A ? SCALE_E : WHAT == NS_B ? SCALE_G : scale_x; }
     __device__ int64_t at(int i, int j) const { return ((int64_t)(j >> 6) * r + i) * PANEL_BYTES + (j & 63) * 2; }
 
     // What the results of row i, columns j to j + 7, are made of beside their sums.
@@ -357,61 +359,80 @@ struct NsFinish {
         o.di = WHAT == NS_B ? w.d[i] : p.a + w.f[i];
         return o;
     }
-    // Their values in place of the sums v, and those along the rows to where they go.
-    __device__ __forceinline__ void row(int i, int j, float *v, const Old &was) const
+    // v: the sums of row i, columns j to j + 7, and then their values as numbers (of the last iteration)
+    // or in the result's scale.  They go to the rows' panels; `high` and `low` are what is stored there.
+    __device__ __forceinline__ void row(int i, int j, float *v, const Old &was, ns_h8 *high, ns_h8 *low) const
     {
         const bool inside = i < r && j < padded;
-        ns_h8 high, low;
+        if (WHAT == NS_A) {
+            if ((unsigned)(i - j) < 8u && i < r) {
 #pragma unroll
-        for (int n = 0; n < 8; n++) {
-            float o = 0.f;
-            if (inside && j + n < cols) {
-                if (WHAT == NS_A) {
-                    o = v[n] * per_x * per_x;
-                    if (i == j + n) w.d[i] = o;
-                } else {
-                    const float x = ((float)was.high[n] + (LOW ? (float)was.low[n] : 0.f)) * (WHAT == NS_B ? 1.f / SCALE_E : per_x);
-                    if (WHAT == NS_B) {
-                        const float dj = w.d[j + n], square = v[n] * (1.f / (SCALE_E * SCALE_E));
-                        if (i == j + n) w.f[i] = p.b * was.di + p.c * (square + was.di * was.di);
-                        o = p.b * x + p.c * (square + (was.di + dj) * x);
-                    } else {
-                        o = was.di * x + v[n] * (1.f / SCALE_G) * per_x;
-                    }
-                }
-                if (WHAT != NS_X && i == j + n) o = 0.f;
+                for (int n = 0; n < 8; n++)
+                    if (i == j + n) w.d[i] = v[n] * per_x * per_x;
             }
-            _Float16 a, b;
-            ns_split(o, scale(), &a, &b);
-            high[n] = a, low[n] = b;
-            v[n] = o;
+            const float by = per_x * per_x * SCALE_E;
+#pragma unroll
+            for (int n = 0; n < 8; n++) v[n] *= by;
+        } else if (WHAT == NS_B) {
+            const float by = p.c * (SCALE_G / (SCALE_E * SCALE_E)), c = p.c * (SCALE_G / SCALE_E), b = p.b * (SCALE_G / SCALE_E);
+            if ((unsigned)(i - j) < 8u && i < r) {
+#pragma unroll
+                for (int n = 0; n < 8; n++)
+                    if (i == j + n) w.f[i] = p.b * was.di + p.c * (v[n] * (1.f / (SCALE_E * SCALE_E)) + was.di * was.di);
+            }
+            tile_f4 d[2] = {};
+            if (inside) d[0] = *(const tile_f4 *)(w.d + j), d[1] = *(const tile_f4 *)(w.d + j + 4);
+#pragma unroll
+            for (int n = 0; n < 8; n++) {
+                const float x = PRECISE ? (float)was.high[n] + (float)was.low[n] : (float)was.high[n];
+                v[n] = fmaf(x, fmaf(c, was.di + d[n / 4][n % 4], b), v[n] * by);
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < 8; n++) v[n] = fmaf(was.di, (float)was.high[n], fmaf(was.di, (float)was.low[n], v[n] * (1.f / SCALE_G)));
         }
-        if (!inside) return;
+        if (!(i < r && j + 8 <= cols)) {  // zeros past the last row and column
+#pragma unroll
+            for (int n = 0; n < 8; n++) v[n] = i < r && j + n < cols ? v[n] : 0.f;
+        }
+        if (WHAT != NS_X && (unsigned)(i - j) < 8u) {  // and on the diagonal
+#pragma unroll
+            for (int n = 0; n < 8; n++) v[n] = i == j + n ? 0.f : v[n];
+        }
         if (WHAT == NS_X && p.last) {
-            if (!m.flip) ns_put(m, p, i, j, cols - j, v);
+#pragma unroll
+            for (int n = 0; n < 8; n++) v[n] *= per_x;
+            if (inside && !m.flip) ns_put(m, p, i, j, cols - j, v);
             return;
         }
-        *(ns_h8 *)(out + at(i, j)) = high;
-        if (PRECISE || (LOW && !p.next_last)) *(ns_h8 *)(out_l + at(i, j)) = low;
+        split(v, high, low);
+        if (!inside) return;
+        *(ns_h8 *)(out + at(i, j)) = *high;
+        if (PRECISE || (LOW && !p.next_last)) *(ns_h8 *)(out_l + at(i, j)) = *low;
     }
-    // The values of column j, rows i to i + 7, along the columns.
-    __device__ __forceinline__ void column(int i, int j, const float *v) const
+    __device__ __forceinline__ static void split(const float *v, ns_h8 *high, ns_h8 *low)
+    {
+        typedef float F2 __attribute__((ext_vector_type(2)));
+        typedef _Float16 H2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int n = 0; n < 8; n += 2) {
+            const H2 h = __builtin_convertvector(F2{v[n], v[n + 1]}, H2);
+            const H2 l = __builtin_convertvector(F2{v[n] - (float)h[0], v[n + 1] - (float)h[1]}, H2);
+            (*high)[n] = h[0], (*high)[n + 1] = h[1], (*low)[n] = l[0], (*low)[n + 1] = l[1];
+        }
+    }
+    // Column j, rows i to i + 7, of an iteration that is not the last, to the columns' panels.
+    __device__ __forceinline__ void column(int i, int j, const ns_h8 &high, const ns_h8 &low) const
     {
         if (j >= cols || i >= ((r + 63) & ~63)) return;
-        if (WHAT == NS_X && p.last) {
-            if (i < r) ns_put(m, p, j, i, r - i, v);
-            return;
-        }
-        ns_h8 high, low;
-#pragma unroll
-        for (int n = 0; n < 8; n++) {
-            _Float16 a, b;
-            ns_split(v[n], scale(), &a, &b);
-            high[n] = a, low[n] = b;
-        }
         const int64_t to = ((int64_t)(i >> 6) * cols + j) * PANEL_BYTES + (i & 63) * 2;
         *(ns_h8 *)(turned + to) = high;
         if (PRECISE) *(ns_h8 *)(turned_l + to) = low;
+    }
+    // The last one's values of column j, rows i to i + 7.
+    __device__ __forceinline__ void column_out(int i, int j, const float *v) const
+    {
+        if (j < cols && i < r) ns_put(m, p, j, i, r - i, v);
     }
 };
 
@@ -443,10 +464,30 @@ struct NsProduct {
     }
 };
 
+// Column lane % 16, rows 8 (lane / 16) to + 7, of 32 rows of 16 numbers in LDS.  Of ds_read_b64_tr_b16 every 16
+// lanes name 4 rows of 16 numbers, 4 of them each, and get a column's 4 each.
+__device__ static inline ns_h8 ns_down(const _Float16 *from, int pitch, int lane)
+{
+    typedef short S4 __attribute__((ext_vector_type(4)));
+    typedef _Float16 H4 __attribute__((ext_vector_type(4)));
+    const _Float16 *at = from + ((lane >> 4) * 8 + (lane & 15) / 4) * pitch + (lane & 3) * 4;
+    const H4 a = __builtin_bit_cast(H4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) S4 *)at));
+    const H4 b = __builtin_bit_cast(H4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) S4 *)(at + 4 * pitch)));
+    return ns_h8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+
+// LDS of a product's workgroup: the tile's buffers, and when they are done with its strips as sums and as
+// two fp16 numbers each.
+template <class T>
+struct NsLds {
+    static constexpr int STRIPS = T::WAVES * (32 * T::PITCH * 4 + 2 * 32 * (T::WN + 8) * 2);
+    static constexpr int BYTES = T::LDS > STRIPS ? T::LDS : STRIPS;
+};
+
 template <class T, int WHAT, bool PRECISE>
 __global__ __launch_bounds__(T::THREADS) void k_ns_product(const NsLaunch l, const NsParams p, int turn)
 {
-    __shared__ __attribute__((aligned(128))) uint8_t lds[T::LDS];
+    __shared__ __attribute__((aligned(128))) uint8_t lds[NsLds<T>::BYTES];
     int matrix, piece, tm, tn;
     if (!ns_tile(l, blockIdx.x, &matrix, &piece)) return;
     const NsMatrix m = l.m[matrix];
@@ -462,26 +503,51 @@ __global__ __launch_bounds__(T::THREADS) void k_ns_product(const NsLaunch l, con
 
     const NsFinish<WHAT, PRECISE> finish(m, p, w, turn, tm == tn);
     constexpr int ACROSS = T::WN / 8, PASSES = 32 * ACROSS / 64;  // 8 neighbours of a row per lane
-    static_assert(32 * ACROSS % 64 == 0, "");
+    static_assert(32 * ACROSS % 64 == 0 && T::WN % 16 == 0, "");
+    // the fp16 numbers of a strip, behind the strips themselves
+    constexpr int PITCH16 = T::WN + 8, HALF = 32 * PITCH16;
+    static_assert(T::WAVES * (32 * T::PITCH * 4 + 2 * HALF * 2) <= NsLds<T>::BYTES, "");
     const int lane = threadIdx.x & 63;
+    _Float16 *halves = (_Float16 *)(lds + T::WAVES * 32 * T::PITCH * 4) + tile_wave() * 2 * HALF;
     typename NsFinish<WHAT, PRECISE>::Old was[2][PASSES];  // of the next strip while one is finished
     t.store_strips(row0, col0, lds, [&](int i, int row, int col) __attribute__((always_inline)) {
 #pragma unroll
         for (int q = 0; q < PASSES; q++) was[i & 1][q] = finish.old(row + (lane + 64 * q) / ACROSS, col + (lane + 64 * q) % ACROSS * 8);
     }, [&](int i, float *strip, int row, int col) __attribute__((always_inline)) {
+        const bool last = WHAT == NS_X && p.last;
 #pragma unroll
         for (int q = 0; q < PASSES; q++) {
             const int at = (lane + 64 * q) / ACROSS, c = (lane + 64 * q) % ACROSS * 8;
-            finish.row(row + at, col + c, strip + at * T::PITCH + c, was[i & 1][q]);
+            float v[8];
+            tile_f4 *from = (tile_f4 *)__builtin_assume_aligned(strip + at * T::PITCH + c, 16);
+            *(tile_f4 *)v = from[0], *(tile_f4 *)(v + 4) = from[1];
+            ns_h8 high, low;
+            finish.row(row + at, col + c, v, was[i & 1][q], &high, &low);
+            if (!finish.mirror) continue;
+            if (last) {
+                from[0] = *(tile_f4 *)v, from[1] = *(tile_f4 *)(v + 4);
+            } else {
+                *(ns_h8 *)__builtin_assume_aligned(halves + at * PITCH16 + c, 16) = high;
+                if (PRECISE) *(ns_h8 *)__builtin_assume_aligned(halves + HALF + at * PITCH16 + c, 16) = low;
+            }
         }
         T::wave_fence();
         if (!finish.mirror) return;
+        if (last) {
 #pragma unroll 1
-        for (int q = lane; q < T::WN * 4; q += 64) {  // 8 rows of a column per lane
-            float v[8];
+            for (int q = lane; q < T::WN * 4; q += 64) {  // 8 rows of a column per lane
+                float v[8];
 #pragma unroll
-            for (int n = 0; n < 8; n++) v[n] = strip[((q & 3) * 8 + n) * T::PITCH + (q >> 2)];
-            finish.column(row + (q & 3) * 8, col + (q >> 2), v);
+                for (int n = 0; n < 8; n++) v[n] = strip[((q & 3) * 8 + n) * T::PITCH + (q >> 2)];
+                finish.column_out(row + (q & 3) * 8, col + (q >> 2), v);
+            }
+            return;
+        }
+#pragma unroll
+        for (int c = 0; c < T::WN; c += 16) {  // 8 rows of 16 columns per 16 lanes
+            ns_h8 high = ns_down(halves + c, PITCH16, lane), low = high;
+            if (PRECISE) low = ns_down(halves + HALF + c, PITCH16, lane);
+            finish.column(row + (lane >> 4) * 8, col + c + (lane & 15), high, low);
         }
     });
 }
@@ -538,7 +604,8 @@ __global__ __launch_bounds__(512) void k_ns_small(const NsLaunch l, const NsPara
 #pragma unroll
             for (int k = 1; k < WAVES; k++) v[n] += sums[k][at * PITCH + c + n];
         }
-        finish.row(tm * 32 + at, tn * 32 + c, v, was);
+        ns_h8 high, low;
+        finish.row(tm * 32 + at, tn * 32 + c, v, was, &high, &low);
 #pragma unroll
         for (int n = 0; n < 8; n++) sums[0][at * PITCH + c + n] = v[n];
     }
@@ -549,7 +616,13 @@ __global__ __launch_bounds__(512) void k_ns_small(const NsLaunch l, const NsPara
         float v[8];
 #pragma unroll
         for (int n = 0; n < 8; n++) v[n] = sums[0][(i + n) * PITCH + j];
-        finish.column(tm * 32 + i, tn * 32 + j, v);
+        if (WHAT == NS_X && p.last) {
+            finish.column_out(tm * 32 + i, tn * 32 + j, v);
+        } else {
+            ns_h8 high, low;
+            finish.split(v, &high, &low);
+            finish.column(tm * 32 + i, tn * 32 + j, high, low);
+        }
     }
 }
 
