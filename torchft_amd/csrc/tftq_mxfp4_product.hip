@@ -38,7 +38,7 @@ __global__ __launch_bounds__(T::THREADS) void k_mx_product(TileOperand a, TileOp
     };
     T t;
     t.multiply(TilePair{a, b}, panels, pieces, place, lds, [&](int row0, int col0) {
-        t.template store_pieces<O::SIZE>(row0, col0, lds + 2 * T::BUFFER, O::two, [&](tile_i4 v, int row, int col) {
+        t.template store_pieces<O::SIZE>(row0, col0, lds + T::PIECES_AT, O::two, [&](tile_i4 v, int row, int col) {
             if (row >= a.rows) return;
             uint8_t *at = out + ((int64_t)row * ld + col) * O::SIZE;
             if (whole) {
@@ -241,7 +241,7 @@ extern "C" int tftq_mx_product(int dtype, const void *a, int64_t m, const void *
     case 0: return product<Tile<256, 256, 2, 4, true>>(dtype, ta, tb, panels, (uint8_t *)out, row_stride, st);
     case 1: return product<Tile<192, 256, 2, 4, true>>(dtype, ta, tb, panels, (uint8_t *)out, row_stride, st);
     case 2: return product<Tile<128, 128, 2, 2, true>>(dtype, ta, tb, panels, (uint8_t *)out, row_stride, st);
-    default: return product<Tile<64, 64, 2, 2, true>>(dtype, ta, tb, panels, (uint8_t *)out, row_stride, st);
+    default: return product<Tile<64, 64, 2, 2, true, 3>>(dtype, ta, tb, panels, (uint8_t *)out, row_stride, st);
     }
 }
 

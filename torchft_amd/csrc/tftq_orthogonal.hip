@@ -669,9 +669,10 @@ static double ns_time(const NsLaunch &l, int what, const TileShape &t)
     return tile_time(t, count, work, longest);
 }
 
-// One of the three products for all matrices of a launch.  Up to 512 tiles of 32 x 32 take k_ns_small
-// (graph replays, whole orthogonalisation: 512x512 fp32 138 us, with tiles of 64 x 64 219; 256x512 108,
-// 183; with 1024 as the limit, 1024x1024 454, 389).
+// One of the three products for all matrices of a launch.  Up to 512 tiles of 32 x 32 (256 where a product
+// is one, not three) take k_ns_small.  Graph replays of the whole orthogonalisation, us, so and with tiles of
+// 64 x 64: fp32 512x512 127, 182; 512x768 159, 164; 768x1024 264, 263; 1024x1024 432, 292.  bf16 512x512
+// 90, 102; 512x768 105, 104; 640x640 117, 112; 768x1024 162, 140.
 template <int WHAT>
 static int product(NsLaunch &l, bool precise, const NsParams &p, int turn, hipStream_t st)
 {
@@ -682,7 +683,7 @@ static int product(NsLaunch &l, bool precise, const NsParams &p, int turn, hipSt
         small += tiles(l.m[i], WHAT, 32, 32);
         longest = std::max<int64_t>(longest, WHAT == NS_A ? l.m[i].cols : l.m[i].rows);
     }
-    if (small <= 512) {
+    if (small <= (precise ? 512 : 256)) {
         const void *k = precise ? (const void *)k_ns_small<WHAT, true> : (const void *)k_ns_small<WHAT, false>;
         return launch_over(l, [](const NsMatrix &m) { return tiles(m, WHAT, 32, 32); }, true, k, 512, p, turn, st);
     }
@@ -696,7 +697,7 @@ static int product(NsLaunch &l, bool precise, const NsParams &p, int turn, hipSt
         if (WHAT == NS_X) return launch_tiles<Tile<192, 256, 2, 4, false>, NS_X>(l, precise, p, turn, st);
         return launch_tiles<Tile<192, 192, 2, 2, false>, WHAT == NS_X ? NS_A : WHAT>(l, precise, p, turn, st);
     case 2: return launch_tiles<Tile<128, 128, 2, 2, false>, WHAT>(l, precise, p, turn, st);
-    default: return launch_tiles<Tile<64, 64, 2, 2, false>, WHAT>(l, precise, p, turn, st);
+    default: return launch_tiles<Tile<64, 64, 2, 2, false, 3>, WHAT>(l, precise, p, turn, st);
     }
 }
 

@@ -12,15 +12,17 @@
 // lane / 32 of a slice of 32 bytes.  One kernel body therefore serves both; the 4-bit one also hands the
 // instruction the scale of the lane's 32 codes.
 //
-// Staging: loads straight into LDS, 16 bytes per lane and 8 rows per instruction, two buffers, one barrier per
-// panel; panel s + 2 is loaded from the moment when panel s has been read, a whole panel ahead.  A wavefront's bytes land in LDS in
-// lane order, so the order in which lanes take the 16-byte pieces of their row is what arranges the
-// buffer: piece p of row r lies at place p ^ (r % 8), and the 8 lanes that one cycle of ds_read_b128
+// Staging: loads straight into LDS, 16 bytes per lane and 8 rows per instruction, one barrier per panel and
+// two buffers (small tiles: three); a buffer's next panel is loaded from the moment when everybody has read
+// the one that it holds.  A wavefront's bytes land in LDS in lane order, so the order in which lanes take
+// the 16-byte pieces of their row is what arranges the buffer: piece p of row r lies at place p ^ (r % 8), and the 8 lanes that one cycle of ds_read_b128
 // serves, 8 neighbouring rows, find their pieces in 8 different groups of banks.
 #pragma once
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+
+#include <algorithm>
 
 typedef int tile_i4 __attribute__((ext_vector_type(4)));
 typedef uint32_t tile_u2 __attribute__((ext_vector_type(2)));
@@ -87,8 +89,11 @@ __device__ static inline void tile_load16(__amdgpu_buffer_rsrc_t from, int at, i
 // The wavefront's number in its workgroup, in a scalar register.
 __device__ static inline int tile_wave() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
 
-// BM x BN values of C by WGM x WGN wavefronts, each of them TM x TN squares of 32.
-template <int BM, int BN, int WGM, int WGN, bool FP4>
+// BM x BN values of C by WGM x WGN wavefronts, each of them TM x TN squares of 32.  BUFFERS: panels in LDS;
+// with more than two a panel is loaded BUFFERS - 1 panels ahead, for small tiles, which multiply a panel in
+// less time than it takes to come (tiles of 64 x 64 with 2, 3 and 4: 1024x1024 orthogonalised 382, 292,
+// 293 us; 4-bit 128x4096x14336 33.5, 28.1, 28.1; 4 leave LDS for fewer tiles to a unit).
+template <int BM, int BN, int WGM, int WGN, bool FP4, int BUFFERS = 2>
 struct Tile {
     static constexpr int ROWS = BM, COLS = BN, WAVES = WGM * WGN, THREADS = 64 * WAVES;
     static constexpr int WM = BM / WGM, WN = BN / WGN, TM = WM / 32, TN = WN / 32;
@@ -98,8 +103,8 @@ struct Tile {
     static constexpr int BUFFER = (BM + BN) * PANEL_BYTES + (FP4 ? 2 * SCALES : 0);
     // a wavefront's strip of 32 rows of results, behind the buffers' use (store_strips)
     static constexpr int PITCH = WN + 4;
-    static constexpr int LDS = 2 * BUFFER > WAVES * 32 * PITCH * 4 ? 2 * BUFFER : WAVES * 32 * PITCH * 4;
-    static constexpr int LDS_PIECES = 2 * BUFFER + WAVES * 2048;
+    static constexpr int LDS = BUFFERS * BUFFER > WAVES * 32 * PITCH * 4 ? BUFFERS * BUFFER : WAVES * 32 * PITCH * 4;
+    static constexpr int LDS_PIECES = BUFFERS * BUFFER + WAVES * 2048, PIECES_AT = BUFFERS * BUFFER;
     static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "every wavefront loads the same number of rows");
     static_assert(LDS <= 160 * 1024 && LDS_PIECES <= 160 * 1024 && BM * 8 <= SCALES && BN * 8 <= SCALES, "");
 
@@ -134,7 +139,7 @@ struct Tile {
         return t;
     }
     // Part `part` of `parts` of a wavefront's loads of a step, 8 rows an instruction.
-    static constexpr int LOADS_M = BM / (8 * WAVES), LOADS_N = BN / (8 * WAVES);
+    static constexpr int LOADS_M = BM / (8 * WAVES), LOADS_N = BN / (8 * WAVES), LOADS = LOADS_M + LOADS_N + (FP4 ? 1 : 0);
     __device__ static void load_part(const Step &t, int at, uint8_t *buf, int part, int parts)
     {
         const int wave = tile_wave();
@@ -201,14 +206,24 @@ struct Tile {
             return;
         }
         load_part(step(p, 0, row0, col0), load_at, lds, 0, 1);
-        advance();
-        Step next = step(p, ahead_panel, ahead_row, ahead_col);
+        Step next;
+        if constexpr (BUFFERS == 2) {
+            advance();
+            next = step(p, ahead_panel, ahead_row, ahead_col);
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < TM; i++) load_part(next, load_at, lds + BUFFER, i, 2 * TM);
+        } else {
+#pragma unroll
+            for (int n = 1; n < BUFFERS; n++) {
+                advance();
+                load_part(step(p, ahead_panel, ahead_row, ahead_col), load_at, lds + n * BUFFER, 0, 1);
+            }
+            landed<(BUFFERS - 1) * LOADS>();
+        }
         advance();
         Step later = step(p, ahead_panel, ahead_row, ahead_col);
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < TM; i++) load_part(next, load_at, lds + BUFFER, i, 2 * TM);
-        int cur = 0;
+        int cur = 0, then = BUFFER;
 #pragma unroll
         for (int i = 0; i < TM; i++) read_part(slice[0], lds, a_at + at[0], b_at + at[0], i);
         if (FP4) read_scales(scale[0], lds, wm + in_row, wn + in_row, half);
@@ -217,8 +232,10 @@ struct Tile {
 #pragma unroll
             for (int q = 0; q < 4; q++) {
                 if (q == 3) {
-                    __syncthreads();  // the next panel has landed, and everybody has read all of this one
-                    buf = lds + (cur ^ BUFFER);
+                    // the next panel has landed, and everybody has read all of this one
+                    if constexpr (BUFFERS == 2) __syncthreads();
+                    else landed<(BUFFERS - 2) * LOADS>();
+                    buf = lds + then;
                     if (FP4) read_scales(scale[1], buf, wm + in_row, wn + in_row, half);
                 }
 #pragma unroll
@@ -226,15 +243,16 @@ struct Tile {
                     __builtin_amdgcn_sched_barrier(0);
                     const int to = (q + 1) & 3;
                     read_part(slice[(q + 1) & 1], buf, a_at + at[to], b_at + at[to], i);
-                    if (q == 0) load_part(next, load_at, lds + (cur ^ BUFFER), TM + i, 2 * TM);
-                    if (q == 3) load_part(later, load_at, lds + cur, i, 2 * TM);
+                    if (BUFFERS == 2 && q == 0) load_part(next, load_at, lds + then, TM + i, 2 * TM);
+                    if (q == 3) load_part(later, load_at, lds + cur, i, BUFFERS == 2 ? 2 * TM : TM);
 #pragma unroll
                     for (int j = 0; j < TN; j++)
                         acc[i][j] = one(slice[q & 1].b[j], slice[q & 1].a[i], acc[i][j], q, scale[0].b[j], scale[0].a[i]);
                 }
             }
             if (FP4) scale[0] = scale[1];
-            cur ^= BUFFER;
+            cur = then;
+            then = then + BUFFER == BUFFERS * BUFFER ? 0 : then + BUFFER;
             if (++s == panels) {
                 done(row0, col0);
                 if (++tile == tiles) break;
@@ -242,11 +260,22 @@ struct Tile {
                 zero();
                 s = 0;
             }
-            next = later;
+            if (BUFFERS == 2) next = later;
             advance();
             later = step(p, ahead_panel, ahead_row, ahead_col);
         }
         __syncthreads();  // nothing is on its way to LDS any more
+    }
+
+    // Waits until all but this wavefront's last N memory operations are done, then for the other wavefronts.
+    // Operations are done in the order in which they were issued, and a wavefront issues LOADS of them for
+    // every panel, none of them on a condition: with the loads of k later panels issued, a panel has landed
+    // when all but k LOADS are done (a tile's stores between them only make the wait longer).
+    template <int N>
+    __device__ static void landed()
+    {
+        static_assert(N < 64, "");
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
     }
 
     // Part `part` of the TM parts of a slice's reads.
@@ -384,23 +413,29 @@ __device__ static inline void tile_place(int piece, int tiles_m, int tiles_n, in
     *tm = first + in % height;
 }
 
-// A size of tiles.  `cost` is what a panel of the tiles that run at once on a compute unit takes, that of one
-// of 256 x 256 being 1; `at_once`: how many that is.  From the rates of launches that fill all units
-// evenly (8192^3, fp16, TFLOP/s: 256x256 1230, 192x256 1190, 192x192 1040, 128x128 1000, 64x64 600;
-// 4-bit, 256x256 4300, 128x128 3500, 64x64 1900).
+// A size of tiles.  `at_once`: the tiles that a compute unit runs at once; `cost`: what a panel of them all
+// takes then, `one` with one tile to a unit, a panel of one tile of 256 x 256 on every unit being 1.  From
+// launches that fill all units (8192^3, fp16, TFLOP/s: 256x256 1230, 192x256 1190, 192x192 1040, 128x128
+// 1000, 64x64 760; 4-bit, 256x256 4300, 128x128 3500) and from short ones (4-bit, us, tiles of 256, 128,
+// 64: 256x4096x4096 23.5, 13.4, 10.8; 256x14336x4096 26.6, 17.9, 24.7; 2048x5632x2048 22.1, 22.6, 35.5).
+// 128x128 is 0.61 by its rate, but 3 to a unit take 1.02 (a list of products of depth 2048 in 696 tiles
+// 79 us, in 216 of 256x256 71).
 struct TileShape {
     int high, wide, at_once;
-    double cost;
+    double one, cost;
 };
-constexpr TileShape TILES_256 = {256, 256, 1, 1.0}, TILES_192X256 = {192, 256, 1, 0.775}, TILES_192 = {192, 192, 1, 0.665},
-                    TILES_128 = {128, 128, 2, 0.61}, TILES_64 = {64, 64, 4, 0.51}, TILES_64_FP4 = {64, 64, 3, 0.425};
+constexpr TileShape TILES_256 = {256, 256, 1, 1.0, 1.0}, TILES_192X256 = {192, 256, 1, 0.775, 0.775},
+                    TILES_192 = {192, 192, 1, 0.665, 0.665}, TILES_128 = {128, 128, 2, 0.41, 0.68},
+                    TILES_64 = {64, 64, 3, 0.22, 0.30}, TILES_64_FP4 = {64, 64, 2, 0.26, 0.31};
 
 // About how many panels of a 256 x 256 tile `count` tiles of that size take together: `work` panels in
-// all, `longest` the longest of them, in as many rounds as the 256 units need.  Storing a tile's values
-// and waiting for its first operands takes about as long as 4 panels.
+// all, `longest` the longest of them.  Storing a tile's values and waiting for its first operands takes
+// about as long as 4 panels.
 static inline double tile_time(const TileShape &t, double count, double work, double longest)
 {
-    const double rounds = (double)(((int64_t)count + 256 * t.at_once - 1) / (256 * t.at_once));
-    const double each = work / count + 4, most = longest + 4;
-    return (rounds * each > most ? rounds * each : most) * t.cost;
+    const int64_t units = ((int64_t)count + 255) / 256;
+    const double each = work / count + 4;
+    const double alone = units < t.at_once ? t.one + (t.cost - t.one) * (units - 1) / (t.at_once - 1) : t.cost;
+    const double rounds = units < t.at_once ? 1 : (double)units / t.at_once;
+    return std::max(rounds * each, longest + 4) * alone;
 }
