@@ -53,3 +53,25 @@ def test_blocks_that_do_not_fit():
             MXFP4Tensor.from_blocks(*bad)
     with pytest.raises(AssertionError, match="GPU"):
         MXFP4Tensor.from_blocks(codes, scales, 64)
+
+
+def test_linear_refuses_before_it_launches():
+    L = _lib.load()
+    buf = (ctypes.c_uint8 * 65536)()
+    at = (ctypes.addressof(buf) + 15) & ~15
+
+    def size(dtype=BF16, x=at, m=100, stride=512, n=40, k=512):
+        return L.tftq_mx_linear_workspace(dtype, x, m, stride, n, k)
+
+    def call(dtype=BF16, x=at, m=100, stride=512, b=at, n=40, k=512, out=at, out_stride=40, workspace=at, bytes=1 << 40):
+        return L.tftq_mx_linear(dtype, x, m, stride, b, n, k, out, out_stride, workspace, bytes, -1, None)
+    assert size() == L.tftq_mx_bytes(100, 512)  # x, quantised in a launch of its own
+    assert size(m=1) == 0 and size(m=0) == 0 and size(k=0) == 0
+    assert size(dtype=7) == call(dtype=7) == -2
+    for bad in (dict(m=-1), dict(n=-1), dict(k=-1), dict(m=2 ** 31), dict(n=2 ** 31), dict(k=2 ** 31)):
+        assert size(**bad) == call(**bad) == -3
+    assert call(m=0, x=None) == 0 and call(n=0, b=None) == 0
+    assert call(x=None) == call(b=None) == call(out=None) == call(b=at + 8) == -1
+    assert call(stride=511) == call(out_stride=39) == -1
+    assert call(bytes=L.tftq_mx_bytes(100, 512) - 1) == -4
+    assert call(workspace=None) == call(workspace=at + 8) == -1

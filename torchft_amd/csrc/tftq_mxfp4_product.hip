@@ -259,6 +259,7 @@ static bool few_rows(int dtype, const void *x, int64_t m, int64_t row_stride, in
 
 extern "C" int64_t tftq_mx_linear_workspace(int dtype, const void *x, int64_t m, int64_t row_stride, int64_t n, int64_t k)
 {
+    if (dtype != TFTQ_F32 && dtype != TFTQ_F16 && dtype != TFTQ_BF16) return TFTQ_E_DTYPE;
     if (m < 0 || n < 0 || k < 0 || m > MX_MOST || n > MX_MOST || k > MX_MOST) return TFTQ_E_SHAPE;
     return few_rows(dtype, x, m, row_stride, n, k) ? 0 : tftq_mx_bytes(m, k);
 }

@@ -36,8 +36,9 @@ _PANEL_BLOCKS = _PANEL // _BLOCK
 
 # The module that makes whole calls with plain arguments (_pylist.mx_quantize and the like: checks,
 # allocations and launch in one step), once it knows the library and a device that can run it.  It answers
-# None to anything else, and the functions below then go their own way.  Host time on small matrices:
-# HOST_TIMES.
+# None to anything else, and the functions below then go their own way.  Host time on small matrices, us, in
+# Python and so: quantisation 7.7, 4.3; along both axes 10, 5.5; product 6.0, 4.3; linear with a kept weight
+# 12, 7.8; linear with its gradients 147, 107 (torch's own linear: 115; most of it is autograd's).
 _native = None
 _bind_lock = threading.Lock()
 
@@ -65,8 +66,8 @@ class MXFP4Tensor:
     """A matrix ``[rows, columns]`` in 4-bit microscaled form, blocks of 32 along its rows.
 
     ``buffer`` holds it in the order in which the product reads it (``tftq_mx_bytes`` of
-    ``include/tftq.h`` describes it); :attr:`codes` and :attr:`scales` are in the usual order (copies where that is another).
-    ``dtype`` is what it was quantised from and what :meth:`dequantize` and products return by
+    ``include/tftq.h`` describes it); :attr:`codes` and :attr:`scales` are in the usual order (copies where
+    that is another).  ``dtype`` is what it was quantised from and what :meth:`dequantize` and products return by
     default.  It is no ``torch.Tensor``: it has no gradient and takes part in the functions of this module."""
 
     __slots__ = ("buffer", "shape", "dtype")
@@ -106,6 +107,15 @@ class MXFP4Tensor:
         by_panel[1].zero_()
         by_panel[1][:, :rows].copy_(torch.nn.functional.pad(scales, (0, more)).view(rows, panels, _PANEL_BLOCKS).transpose(0, 1))
         return self
+
+    def _data(self) -> int:
+        """The buffer's address, if it holds the matrix that the kernels will look for there."""
+        buffer = self.buffer
+        assert buffer.dtype == torch.uint8 and buffer.dim() == 1 and buffer.is_contiguous() and buffer.data_ptr() % 16 == 0, \
+            "The buffer of a 4-bit matrix is a contiguous run of bytes"
+        assert buffer.numel() >= _lib.load().tftq_mx_bytes(*self.shape), "The buffer is too small for the matrix"
+        _ready(buffer.device)
+        return buffer.data_ptr()
 
     def _panel_views(self):
         rows, columns = self.shape
@@ -151,7 +161,7 @@ class MXFP4Tensor:
             if out is not None:
                 return _result(out, "tftq_mx_dequantize")
         out = torch.empty(rows, columns, dtype=dtype, device=self.device)
-        _check(_lib.load().tftq_mx_dequantize(_DTYPE_CODE[dtype], self.buffer.data_ptr(), rows, columns, out.data_ptr(),
+        _check(_lib.load().tftq_mx_dequantize(_DTYPE_CODE[dtype], self._data(), rows, columns, out.data_ptr(),
                                               columns, self.device.index, _stream_of(self.device)),
                "tftq_mx_dequantize")
         return out
@@ -230,7 +240,7 @@ def matmul_mxfp4(a: MXFP4Tensor, b: MXFP4Tensor, out_dtype: torch.dtype | None =
         if out is not None:
             return _result(out, "tftq_mx_product")
     out = torch.empty(m, n, dtype=out_dtype, device=a.device)
-    _check(_lib.load().tftq_mx_product(_DTYPE_CODE[out_dtype], a.buffer.data_ptr(), m, b.buffer.data_ptr(), n, k,
+    _check(_lib.load().tftq_mx_product(_DTYPE_CODE[out_dtype], a._data(), m, b._data(), n, k,
                                        out.data_ptr(), n, a.device.index, _stream_of(a.device)),
            "tftq_mx_product")
     return out
@@ -252,7 +262,7 @@ def _linear_rows(x: torch.Tensor, weight: MXFP4Tensor, dtype: torch.dtype) -> to
         _check(size, "tftq_mx_linear_workspace")
     out = torch.empty(m, n, dtype=dtype, device=x.device)
     workspace = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-    _check(lib.tftq_mx_linear(_DTYPE_CODE[dtype], x.data_ptr(), m, x.stride(0), weight.buffer.data_ptr(), n, k, out.data_ptr(), n,
+    _check(lib.tftq_mx_linear(_DTYPE_CODE[dtype], x.data_ptr(), m, x.stride(0), weight._data(), n, k, out.data_ptr(), n,
                               None if workspace is None else workspace.data_ptr(), size, x.device.index, _stream_of(x.device)),
            "tftq_mx_linear")
     return out
