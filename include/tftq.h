@@ -242,7 +242,8 @@ int tftq_mx_product(int dtype, const void *a, int64_t m, const void *b, int64_t 
 /*
  * out [m, n] = Q(x) b^T: x [m, k] is quantised along its rows on the way, out has its type.  Few rows
  * (the tokens of a model that is served) take one kernel and no workspace; others quantise into
- * `workspace`, tftq_mx_linear_workspace bytes for the same x, 16-byte aligned.
+ * `workspace`, tftq_mx_linear_workspace bytes (TFTQ_E_DTYPE or TFTQ_E_SHAPE in place of a number of bytes)
+ * for the same x, 16-byte aligned, which holds nothing between calls.
  */
 int64_t tftq_mx_linear_workspace(int dtype, const void *x, int64_t m, int64_t row_stride, int64_t n, int64_t k);
 int tftq_mx_linear(int dtype, const void *x, int64_t m, int64_t row_stride, const void *b, int64_t n, int64_t k,
@@ -259,12 +260,12 @@ int tftq_mx_linear(int dtype, const void *x, int64_t m, int64_t row_stride, cons
  */
 typedef struct tftq_ns {
     int n;                          /* matrices; empty ones are left alone */
-    const int64_t *shapes;          /* [n][2] rows, columns: at most 2^24 each */
+    const int64_t *shapes;          /* [n][2] rows, columns: at most 2^24 each, 2^35 elements */
     const void *const *in;          /* gradients; columns contiguous */
     const int64_t *in_stride;       /* [n] elements from row to row */
     int in_dtype;
     float *const *momenta;          /* NULL: u is the gradient.  Else m = momentum m + (1 - momentum) g, in place, */
-    const int64_t *momenta_stride;  /* and u = m, or g + momentum (m - g) with nesterov */
+    const int64_t *momenta_stride;  /* and u = m, or momentum m + (1 - momentum) g with nesterov */
     float momentum;
     int nesterov;
     void *const *out;

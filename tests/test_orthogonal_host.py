@@ -55,3 +55,13 @@ def test_refuses_before_it_launches():
     assert call(size=64) == -4
     assert call(workspace=None) == -1 and call(workspace=at + 64) == -1
     assert call(shapes=shapes((0, 6))) == 0
+
+
+def test_workspace_of_the_largest():
+    """Refused before anything is queued; a list of large ones is taken in parts."""
+    L = _lib.load()
+    assert L.tftq_newton_schulz_workspace(1, shapes((2 ** 24, 2 ** 12)), 0) == -3
+    one = L.tftq_newton_schulz_workspace(1, shapes((2 ** 17, 2 ** 17)), 0)
+    assert one > 4 * 2 * 2 ** 34
+    assert L.tftq_newton_schulz_workspace(2, shapes((2 ** 17, 2 ** 17), (2 ** 17, 2 ** 17)), 0) == 2 * one
+    assert L.tftq_newton_schulz_workspace(5, shapes(*[(2 ** 17, 2 ** 17)] * 5), 0) == 2 * one

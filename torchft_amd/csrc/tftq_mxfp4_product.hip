@@ -65,6 +65,7 @@ __global__ __launch_bounds__(T::THREADS) void k_mx_product(TileOperand a, TileOp
 constexpr int FEW_WAVES = 8, FEW_PITCH = PANEL_BYTES + 16;  // a token's codes of a panel, its scales and padding
 constexpr int FEW_SUMS = FEW_WAVES * 16 * 20 * 4;           // a group's sums of every wavefront
 constexpr int FEW_MOST = 64;                                // rows of x
+constexpr int64_t FEW_WIDEST = 1 << 26;                     // rows of b: a launch has fewer than 2^32 threads
 struct MxQuantized {};
 
 template <class X>
@@ -222,7 +223,7 @@ extern "C" int tftq_mx_product(int dtype, const void *a, int64_t m, const void *
     // of 64 x 64 are too few for the units: with the quantisation of a before it, n 14336, k 4096,
     // 24 rows 15.8 us (tiles 14.6), 64 rows 30.9 (14.8); n 4096, k 14336, 24 rows 15.0 (36.8), 64 rows
     // 23.8 (37.2); n 1024, k 4096, 64 rows 10.0 (11.7).
-    if (m <= 16 || (m <= FEW_MOST && (n + 63) / 64 < 160)) {
+    if ((m <= 16 && n <= FEW_WIDEST) || (m <= FEW_MOST && (n + 63) / 64 < 160)) {
         switch (dtype) {
         case TFTQ_F32: return few<MxQuantized, TFTQ_F32>(ta.panels, 0, ta.scales, (int)m, tb, (int)k, (uint8_t *)out, row_stride, st);
         case TFTQ_F16: return few<MxQuantized, TFTQ_F16>(ta.panels, 0, ta.scales, (int)m, tb, (int)k, (uint8_t *)out, row_stride, st);
@@ -254,7 +255,7 @@ static bool few_rows(int dtype, const void *x, int64_t m, int64_t row_stride, in
 {
     const int64_t panels = (k + 255) / 256, size = dtype == TFTQ_F32 ? 4 : 2;
     const bool aligned = (uintptr_t)x % 16 == 0 && (m <= 1 || row_stride * size % 16 == 0);
-    return m <= FEW_MOST && FEW_SUMS + m * panels * FEW_PITCH <= 80 * 1024 && m * k * (1.0 + n / 4096.0) <= (aligned ? 1e5 : 4e4);
+    return m <= FEW_MOST && n <= FEW_WIDEST && FEW_SUMS + m * panels * FEW_PITCH <= 80 * 1024 && m * k * (1.0 + n / 4096.0) <= (aligned ? 1e5 : 4e4);
 }
 
 extern "C" int64_t tftq_mx_linear_workspace(int dtype, const void *x, int64_t m, int64_t row_stride, int64_t n, int64_t k)

@@ -15,8 +15,8 @@
 //     (A A)[i][j] = (E E)[i][j] + (D[i] + D[j]) E[i][j],     (B X)[i][j] = F[i] X[i][j] + (G X)[i][j];
 // and X keeps what its rounding leaves as a second fp16 number (22 bits together), which the products
 // leave out and the term (a + F) X takes in.  (Not in the last iteration, to which it adds nothing that
-// one rounding of the result would leave: errors 0 to 10 % larger, and 4 of 46 bytes an element less.)  Relative error of the result against 64 bits, one
-// product each, matrices of 64x64 to 1024x1024 with even, low-rank and 1/i spectra: 2.4e-4 to 1.3e-3
+// one rounding of the result would leave: errors 0 to 10 % larger, and 4 of 46 bytes an element less.)
+// Relative error of the result against 64 bits, one product each, matrices of 64x64 to 1024x1024 with even, low-rank and 1/i spectra: 2.4e-4 to 1.3e-3
 // (bf16 results are rounded by 1.7e-3; A, B and X in plain bf16: 1.3e-2 to 7.7e-2, in plain fp16 up to
 // 9e-3).  `precise`: A, B and X^T have second numbers too and every product is three, high x high +
 // low x high + high x low: 5e-7 to 5e-6, where fp32 products give 1e-6 to 6e-6, at three times the work
@@ -149,7 +149,7 @@ __device__ static inline bool ns_tile(const NsLaunch &l, int id, int *matrix, in
 __device__ static inline float ns_momentum(float m, float g, const NsParams &p) { return m * p.momentum + (1.f - p.momentum) * g; }
 __device__ static inline float ns_update(float m, float g, const NsParams &p) { return p.nesterov ? m * p.momentum + (1.f - p.momentum) * g : m; }
 
-// momentum <- its next value; the sums of the squares of u, one for 64 x 1024 elements, in 64 bits: no
+// momentum <- its next value; the sums of the squares of u, one for 8 or 64 rows of 1024, in 64 bits: no
 // gradient's norm leaves their range, and the order of the additions is always the same.
 __global__ __launch_bounds__(256) void k_ns_squares(const NsLaunch l, const NsParams p, int precise)
 {
@@ -637,10 +637,8 @@ static int launch_over(NsLaunch &l, F workgroups, bool eighths, const void *kern
     int64_t total = 0;
     for (int i = 0; i < l.count; i++) {
         const int64_t n = workgroups(l.m[i]);
-        if (n > (1 << 22)) return TFTQ_E_SHAPE;
         l.m[i].first = (int)total, l.m[i].pieces = (int)n;
         total += eighths ? (n + 7) / 8 : n;
-        if (total > (1 << 22)) return TFTQ_E_SHAPE;
     }
     void *args[] = {(void *)&l, (void *)&p, (void *)&extra};
     return (int)hipLaunchKernel(kernel, dim3((unsigned)(eighths ? total * 8 : total)), dim3(threads), args, 0, st);
@@ -680,11 +678,8 @@ static int product(NsLaunch &l, bool precise, const NsParams &p, int turn, hipSt
 {
     // the matrices with most panels first: the last workgroups are then short ones
     std::stable_sort(l.m, l.m + l.count, [](const NsMatrix &x, const NsMatrix &y) { return WHAT == NS_A ? x.cols > y.cols : x.rows > y.rows; });
-    int64_t small = 0, longest = 0;
-    for (int i = 0; i < l.count; i++) {
-        small += tiles(l.m[i], WHAT, 32, 32);
-        longest = std::max<int64_t>(longest, WHAT == NS_A ? l.m[i].cols : l.m[i].rows);
-    }
+    int64_t small = 0;
+    for (int i = 0; i < l.count; i++) small += tiles(l.m[i], WHAT, 32, 32);
     if (small <= (precise ? 512 : 256)) {
         const void *k = precise ? (const void *)k_ns_small<WHAT, true> : (const void *)k_ns_small<WHAT, false>;
         return launch_over(l, [](const NsMatrix &m) { return tiles(m, WHAT, 32, 32); }, true, k, 512, p, turn, st);
@@ -716,21 +711,29 @@ static bool ns_shapes_ok(int n, const int64_t *shapes)
 // one tile high, and its products wait for memory, not for the matrix cores.
 static bool ns_precise(int64_t r, int precise) { return precise || r < 64; }
 
+// Squares of 64 of a launch's matrices: no kernel has more workgroups of 256 threads, or half as many of
+// 512, and a launch has fewer than 2^32 threads.
+constexpr int64_t NS_SQUARES = 1 << 23;
+
 // f(the matrices of one launch, how many, whether they take three products, bytes of workspace) for the whole list.
 template <class F>
 static int ns_parts(int n, const int64_t *shapes, int precise, F f)
 {
     for (int kind = 0; kind < 2; kind++) {
         int at[NS_MOST], count = 0;
-        int64_t bytes = 0;
+        int64_t bytes = 0, squares = 0;
         for (int i = 0; i < n; i++) {
             const int64_t a = shapes[2 * i], b = shapes[2 * i + 1], r = a < b ? a : b;
             if (r == 0 || ns_precise(r, precise) != (kind != 0)) continue;
+            const int64_t more = ((a + 63) / 64) * ((b + 63) / 64);
+            if (more > NS_SQUARES) return TFTQ_E_SHAPE;
+            if (count == NS_MOST || squares + more > NS_SQUARES) {
+                if (const int rc = f(at, count, kind != 0, bytes)) return rc;
+                count = 0, bytes = 0, squares = 0;
+            }
             bytes += ns_work(nullptr, r, a < b ? b : a, a > b, kind != 0).bytes;
+            squares += more;
             at[count++] = i;
-            if (count < NS_MOST) continue;
-            if (const int rc = f(at, count, kind != 0, bytes)) return rc;
-            count = 0, bytes = 0;
         }
         if (count)
             if (const int rc = f(at, count, kind != 0, bytes)) return rc;
@@ -743,11 +746,11 @@ extern "C" int64_t tftq_newton_schulz_workspace(int n, const int64_t *shapes, in
     if (n < 0 || (n > 0 && !shapes)) return TFTQ_E_ARG;
     if (!ns_shapes_ok(n, shapes)) return TFTQ_E_SHAPE;
     int64_t most = 0;
-    ns_parts(n, shapes, precise, [&](const int *, int, bool, int64_t bytes) {
+    const int rc = ns_parts(n, shapes, precise, [&](const int *, int, bool, int64_t bytes) {
         most = std::max(most, bytes);
         return 0;
     });
-    return most;
+    return rc ? rc : most;
 }
 
 static bool ns_dtype_ok(int d) { return d == TFTQ_F32 || d == TFTQ_F16 || d == TFTQ_BF16; }
@@ -768,7 +771,7 @@ extern "C" int tftq_newton_schulz(const tftq_ns *what, void *workspace, int64_t 
         if (s.momenta && (!s.momenta[i] || s.momenta_stride[i] < least)) return TFTQ_E_ARG;
     }
     const int64_t needed = tftq_newton_schulz_workspace(s.n, s.shapes, s.precise);
-    if (needed == 0) return 0;
+    if (needed <= 0) return (int)needed;
     if (workspace_bytes < needed) return TFTQ_E_SIZE;
     if (!workspace || ((uintptr_t)workspace & 127)) return TFTQ_E_ARG;
     DeviceScope scope(device);

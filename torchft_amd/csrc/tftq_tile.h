@@ -210,7 +210,7 @@ struct Tile {
         if constexpr (BUFFERS == 2) {
             advance();
             next = step(p, ahead_panel, ahead_row, ahead_col);
-            __syncthreads();
+            landed<0>();
 #pragma unroll
             for (int i = 0; i < TM; i++) load_part(next, load_at, lds + BUFFER, i, 2 * TM);
         } else {
@@ -233,8 +233,7 @@ struct Tile {
             for (int q = 0; q < 4; q++) {
                 if (q == 3) {
                     // the next panel has landed, and everybody has read all of this one
-                    if constexpr (BUFFERS == 2) __syncthreads();
-                    else landed<(BUFFERS - 2) * LOADS>();
+                    landed<(BUFFERS - 2) * LOADS>();
                     buf = lds + then;
                     if (FP4) read_scales(scale[1], buf, wm + in_row, wn + in_row, half);
                 }
@@ -264,7 +263,7 @@ struct Tile {
             advance();
             later = step(p, ahead_panel, ahead_row, ahead_col);
         }
-        __syncthreads();  // nothing is on its way to LDS any more
+        landed<0>();  // nothing is on its way to LDS any more
     }
 
     // Waits until all but this wavefront's last N memory operations are done, then for the other wavefronts.
