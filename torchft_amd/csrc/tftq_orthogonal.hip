@@ -25,6 +25,7 @@
 // A and A A are symmetric: only tiles on and above the diagonal are computed, and stored twice.
 // X^T is stored beside X so that all three products contract rows of both operands (tftq_tile.h).
 #include <hip/hip_runtime.h>
+#include <limits.h>
 #include <math.h>
 #include <stdint.h>
 
@@ -62,10 +63,11 @@ struct NsMatrix {
     int rows, cols;  // of X
     int flip;        // X is the transpose of the matrix as it lies
     float step;      // out = keep * out - step * X with NsParams::update, else out = X
-    int first, pieces;  // the launch's first workgroup of this matrix (products: in eighths, ns_tile), and how many it has
+    int pieces;      // the launch's workgroups of this matrix
 };
 struct NsLaunch {
     int count;
+    int first[NS_MOST];  // of every matrix the first workgroup (products: in eighths, ns_tile); past the last one INT_MAX
     NsMatrix m[NS_MOST];
 };
 struct NsParams {
@@ -104,12 +106,19 @@ __host__ __device__ static inline NsWork ns_work(uint8_t *base, int64_t r, int64
     return w;
 }
 
-// The matrix of this workgroup, and which of the matrix's workgroups it is.
-__device__ static inline int ns_find(const NsLaunch &l, int id, int *piece)
+// The matrix of this workgroup, and which of the matrix's workgroups it is.  A kernel's arguments may lie in
+// host memory: all of `first` comes in one load (a search of 24 matrices that loads one at a time takes 8.0 us
+// in an empty kernel, this one 2.8; 24 matrices of 128x256 orthogonalised: 218, 153), and `count`, the
+// first argument, comes in registers.
+__device__ static inline int ns_find(const NsLaunch &l, int count, int id, int *piece)
 {
-    int i = 0;
-    while (i + 1 < l.count && id >= l.m[i + 1].first) i++;
-    *piece = id - l.m[i].first;
+    int i = 0, start = 0;
+    *piece = id;
+    if (count == 1) return 0;
+#pragma unroll
+    for (int n = 1; n < NS_MOST; n++)
+        if (id >= l.first[n]) i = n, start = l.first[n];
+    *piece = id - start;
     return i;
 }
 
@@ -134,10 +143,10 @@ __device__ static inline tile_f4 ns_read(const uint8_t *from, int64_t at, int dt
 // neighbouring ones (workgroups go to the 8 XCDs in turn), so that the matrices with most panels are
 // shared by all (one run of the whole list's tiles each: A of 3 matrices of 88 panels and 4 of 32, 161 us).
 // False for a workgroup that fills up a matrix's last eight.
-__device__ static inline bool ns_tile(const NsLaunch &l, int id, int *matrix, int *piece)
+__device__ static inline bool ns_tile(const NsLaunch &l, int matrices, int id, int *matrix, int *piece)
 {
     int n;
-    *matrix = ns_find(l, id >> 3, &n);
+    *matrix = ns_find(l, matrices, id >> 3, &n);
     const int xcd = id & 7, count = l.m[*matrix].pieces, whole = count >> 3, more = count & 7;
     *piece = xcd * whole + min(xcd, more) + n;
     return n < whole + (xcd < more);
@@ -151,11 +160,11 @@ __device__ static inline float ns_update(float m, float g, const NsParams &p) { 
 
 // momentum <- its next value; the sums of the squares of u, one for 8 or 64 rows of 1024, in 64 bits: no
 // gradient's norm leaves their range, and the order of the additions is always the same.
-__global__ __launch_bounds__(256) void k_ns_squares(const NsLaunch l, const NsParams p, int precise)
+__global__ __launch_bounds__(256) void k_ns_squares(int count, int precise, const NsLaunch l, const NsParams p)
 {
     __shared__ double sums[4];
     int piece;
-    const NsMatrix m = l.m[ns_find(l, blockIdx.x, &piece)];
+    const NsMatrix m = l.m[ns_find(l, count, blockIdx.x, &piece)];
     const int high = m.flip ? m.cols : m.rows, wide = m.flip ? m.rows : m.cols;
     const int across = (wide + NORM_COLS - 1) / NORM_COLS;
     const int part = ns_part_rows(high, wide);
@@ -217,12 +226,12 @@ __device__ static inline void ns_split(float v, float scale, _Float16 *high, _Fl
 }
 
 // X and X^T in panels from u / |u|, a square of 64 per workgroup.
-__global__ __launch_bounds__(256) void k_ns_start(const NsLaunch l, const NsParams p, int precise)
+__global__ __launch_bounds__(256) void k_ns_start(int count, int precise, const NsLaunch l, const NsParams p)
 {
     __shared__ float tile[64][65];
     __shared__ double sums[4];
     int piece;
-    const NsMatrix m = l.m[ns_find(l, blockIdx.x, &piece)];
+    const NsMatrix m = l.m[ns_find(l, count, blockIdx.x, &piece)];
     const NsWork w = ns_work(m.work, m.rows, m.cols, m.flip, precise);
     const int across = (m.cols + 63) / 64;
     const int row0 = piece / across * 64, col0 = piece % across * 64;
@@ -487,11 +496,11 @@ struct NsLds {
 };
 
 template <class T, int WHAT, bool PRECISE>
-__global__ __launch_bounds__(T::THREADS) void k_ns_product(const NsLaunch l, const NsParams p, int turn)
+__global__ __launch_bounds__(T::THREADS) void k_ns_product(int count, int turn, const NsLaunch l, const NsParams p)
 {
     __shared__ __attribute__((aligned(128))) uint8_t lds[NsLds<T>::BYTES];
     int matrix, piece, tm, tn;
-    if (!ns_tile(l, blockIdx.x, &matrix, &piece)) return;
+    if (!ns_tile(l, count, blockIdx.x, &matrix, &piece)) return;
     const NsMatrix m = l.m[matrix];
     const NsWork w = ns_work(m.work, m.rows, m.cols, m.flip, PRECISE);
     const NsProduct<WHAT> o(m, w, turn);
@@ -558,12 +567,12 @@ __global__ __launch_bounds__(T::THREADS) void k_ns_product(const NsLaunch l, con
 // 32 x 32 per workgroup, whose 8 wavefronts share the panels between them, take their operands straight
 // from memory with all of a panel's loads in flight, and add up in LDS.
 template <int WHAT, bool PRECISE>
-__global__ __launch_bounds__(512) void k_ns_small(const NsLaunch l, const NsParams p, int turn)
+__global__ __launch_bounds__(512) void k_ns_small(int count, int turn, const NsLaunch l, const NsParams p)
 {
     constexpr int WAVES = 8, PITCH = 36;
     __shared__ __attribute__((aligned(128))) float sums[WAVES][32 * PITCH];
     int matrix, piece, tm, tn;
-    if (!ns_tile(l, blockIdx.x, &matrix, &piece)) return;
+    if (!ns_tile(l, count, blockIdx.x, &matrix, &piece)) return;
     const NsMatrix m = l.m[matrix];
     const NsWork w = ns_work(m.work, m.rows, m.cols, m.flip, PRECISE);
     const NsProduct<WHAT> o(m, w, turn);
@@ -637,10 +646,11 @@ static int launch_over(NsLaunch &l, F workgroups, bool eighths, const void *kern
     int64_t total = 0;
     for (int i = 0; i < l.count; i++) {
         const int64_t n = workgroups(l.m[i]);
-        l.m[i].first = (int)total, l.m[i].pieces = (int)n;
+        l.first[i] = (int)total, l.m[i].pieces = (int)n;
         total += eighths ? (n + 7) / 8 : n;
     }
-    void *args[] = {(void *)&l, (void *)&p, (void *)&extra};
+    for (int i = l.count; i < NS_MOST; i++) l.first[i] = INT_MAX;
+    void *args[] = {(void *)&l.count, (void *)&extra, (void *)&l, (void *)&p};
     return (int)hipLaunchKernel(kernel, dim3((unsigned)(eighths ? total * 8 : total)), dim3(threads), args, 0, st);
 }
 
