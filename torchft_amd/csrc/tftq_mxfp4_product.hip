@@ -25,7 +25,7 @@ struct MxOut {
 
 template <class T, int DTYPE>
 __global__ __launch_bounds__(T::THREADS) void k_mx_product(TileOperand a, TileOperand b, int panels, uint8_t *out, int64_t ld,
-                                                           int whole, int tiles_m, int tiles_n)
+                                                           int tiles_m, int tiles_n)
 {
     __shared__ __attribute__((aligned(128))) uint8_t lds[T::LDS_PIECES];
     using O = MxOut<DTYPE>;
@@ -41,8 +41,8 @@ __global__ __launch_bounds__(T::THREADS) void k_mx_product(TileOperand a, TileOp
         t.template store_pieces<O::SIZE>(row0, col0, lds + T::PIECES_AT, O::two, [&](tile_i4 v, int row, int col) {
             if (row >= a.rows) return;
             uint8_t *at = out + ((int64_t)row * ld + col) * O::SIZE;
-            if (whole) {
-                if (col < b.rows) *(tile_i4 *)at = v;
+            if (col + O::V <= b.rows) {  // at any element's address
+                *(mx_u4_any *)at = __builtin_bit_cast(mx_u4, v);
                 return;
             }
 #pragma unroll
@@ -192,11 +192,9 @@ static int few(const uint8_t *x, int64_t ld, const uint8_t *x_scales, int rows, 
 template <class T>
 static int product(int dtype, const TileOperand &a, const TileOperand &b, int panels, uint8_t *out, int64_t ld, hipStream_t st)
 {
-    const int size = dtype == TFTQ_F32 ? 4 : 2;
     int tiles_m = (a.rows + T::ROWS - 1) / T::ROWS, tiles_n = (b.rows + T::COLS - 1) / T::COLS;
     if ((int64_t)tiles_m * tiles_n > (1 << 22)) return TFTQ_E_SHAPE;
-    int whole = ld * size % 16 == 0 && b.rows * size % 16 == 0 && (uintptr_t)out % 16 == 0;
-    void *args[] = {(void *)&a, (void *)&b, (void *)&panels, (void *)&out, (void *)&ld, (void *)&whole, (void *)&tiles_m, (void *)&tiles_n};
+    void *args[] = {(void *)&a, (void *)&b, (void *)&panels, (void *)&out, (void *)&ld, (void *)&tiles_m, (void *)&tiles_n};
     const void *k = dtype == TFTQ_F32 ? (const void *)k_mx_product<T, TFTQ_F32>
                     : dtype == TFTQ_F16 ? (const void *)k_mx_product<T, TFTQ_F16>
                                         : (const void *)k_mx_product<T, TFTQ_BF16>;
