@@ -63,3 +63,36 @@ def test_gradient_of_zero_keeps_a_weight(ta):
     m = torch.zeros_like(w)
     ta.muon_([w], [torch.zeros_like(w)], [m], lr=0.1, weight_decay=0.5)
     assert (w - want).abs().le(want.abs() * 2.0 ** -22).all() and not m.any()
+
+
+# few tiles and long sums: workgroups share a tile
+WIDE = [[(64, 4096)], [(1, 5000)], [(9000, 40)], [(70, 20000)], [(600, 5000)], [(1030, 9000)], [(256, 16384), (33, 900), (700, 1000)],
+        [(64, 1024), (2000, 65), (128, 128), (300, 3000)]]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shapes", WIDE)
+def test_long_and_narrow(ta, shapes, dtype):
+    xs = [gradient(*s, dtype, 70 + i, device="cuda") for i, s in enumerate(shapes)]
+    got = ta.orthogonalize(xs)
+    for x, y in zip(xs, got):
+        check(y, reference(x), bound(dtype, dtype == torch.float32 or min(x.shape) < 64))
+    for _ in range(3):  # whichever workgroup is the last one
+        assert all(torch.equal(a, b) for a, b in zip(got, ta.orthogonalize(xs)))
+
+
+def test_graph_of_shared_tiles(ta):
+    x = gradient(80, 6000, torch.bfloat16, 80).cuda()
+    other = gradient(80, 6000, torch.bfloat16, 81).cuda()
+    want = ta.orthogonalize(x), ta.orthogonalize(other)
+    static = x.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ta.orthogonalize(static)
+    for i in (0, 1, 1, 0, 1):
+        static.copy_((x, other)[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[i])
+        assert torch.equal(ta.orthogonalize((x, other)[i]), want[i])

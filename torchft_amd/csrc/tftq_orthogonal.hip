@@ -64,6 +64,7 @@ struct NsMatrix {
     int flip;        // X is the transpose of the matrix as it lies
     float step;      // out = keep * out - step * X with NsParams::update, else out = X
     int pieces;      // the launch's workgroups of this matrix
+    int splits;      // of them share a tile, each a part of its panels (NsSplit)
 };
 struct NsLaunch {
     int count;
@@ -86,9 +87,12 @@ struct NsWork {
     float *d, *f;           // the diagonals
     float *scale;           // of X: SCALE_X, or more
     double *squares;        // of the parts of u
-    int64_t bytes;
+    int *tickets;           // of every tile that workgroups share: how many of them are done
+    float *sums;            // theirs
+    int64_t bytes;          // without `sums`
 };
-__host__ __device__ static inline NsWork ns_work(uint8_t *base, int64_t r, int64_t k, int flip, bool precise)
+constexpr int NS_SHARED = 512;  // workgroups of a launch with shared tiles, at most (2 to a compute unit)
+__host__ __device__ static __forceinline__ NsWork ns_work(uint8_t *base, int64_t r, int64_t k, int flip, bool precise)
 {
     const int64_t rp = (r + 63) / 64, kp = (k + 63) / 64, x = kp * r * PANEL_BYTES, t = rp * k * PANEL_BYTES, a = rp * r * PANEL_BYTES;
     const int64_t high = flip ? k : r, wide = flip ? r : k;
@@ -102,7 +106,9 @@ __host__ __device__ static inline NsWork ns_work(uint8_t *base, int64_t r, int64
     w.d = (float *)(w.gl + (precise ? a : 0)), w.f = w.d + ((r + 63) & ~63ll);
     w.scale = w.f + ((r + 63) & ~63ll);
     w.squares = (double *)(w.scale + 32);
-    w.bytes = (uint8_t *)(w.squares + ((parts + 15) & ~15ll)) - base;
+    w.tickets = (int *)(w.squares + ((parts + 15) & ~15ll));
+    w.sums = (float *)(w.tickets + NS_SHARED / 2);
+    w.bytes = (uint8_t *)w.sums - base;
     return w;
 }
 
@@ -143,7 +149,7 @@ __device__ static inline tile_f4 ns_read(const uint8_t *from, int64_t at, int dt
 // neighbouring ones (workgroups go to the 8 XCDs in turn), so that the matrices with most panels are
 // shared by all (one run of the whole list's tiles each: A of 3 matrices of 88 panels and 4 of 32, 161 us).
 // False for a workgroup that fills up a matrix's last eight.
-__device__ static inline bool ns_tile(const NsLaunch &l, int matrices, int id, int *matrix, int *piece)
+__device__ static __forceinline__ bool ns_tile(const NsLaunch &l, int matrices, int id, int *matrix, int *piece)
 {
     int n;
     *matrix = ns_find(l, matrices, id >> 3, &n);
@@ -246,6 +252,8 @@ __global__ __launch_bounds__(256) void k_ns_start(int count, int precise, const 
     const double by = 1.0 / (norm <= (double)p.eps ? (double)p.eps : norm);  // a NaN stays one
     const float scale = ns_scale(norm, p);
     if (piece == 0 && threadIdx.x == 0) *w.scale = scale;
+    if (piece == 0)
+        for (int i = threadIdx.x; i < NS_SHARED / 2; i += 256) w.tickets[i] = 0;
 
     // read along the rows of the matrix as it lies
     const int at_row = m.flip ? col0 : row0, at_col = m.flip ? row0 : col0;
@@ -297,32 +305,39 @@ __global__ __launch_bounds__(256) void k_ns_start(int count, int precise, const 
     }
 }
 
+// Where the results go: out = keep out - step X with `update`, else out = X.
+struct NsOut {
+    uint8_t *out;
+    int64_t ld;
+    float keep, step;
+    int update, dtype;
+};
 // 8 neighbouring results to the list's matrix: the row, the first column and how many of them exist.
-__device__ static inline void ns_put(const NsMatrix m, const NsParams p, int64_t row, int64_t col, int n, const float *v)
+__device__ static __forceinline__ void ns_put(const NsOut &into, int64_t row, int64_t col, int n, const float *v)
 {
-    const int64_t at = row * m.ld_out + col;
-    const int size = p.out_dtype == TFTQ_F32 ? 4 : 2;
+    const int64_t at = row * into.ld + col;
+    const int size = into.dtype == TFTQ_F32 ? 4 : 2;
 #pragma unroll
     for (int h = 0; h < 8; h += 4) {
-        uint8_t *to = m.out + (at + h) * size;
+        uint8_t *to = into.out + (at + h) * size;
         tile_f4 o = {v[h], v[h + 1], v[h + 2], v[h + 3]};
         if (n - h <= 0) return;
-        if (p.update) {
-            const tile_f4 old = ns_read(to, 0, p.out_dtype, n - h);
+        if (into.update) {
+            const tile_f4 old = ns_read(to, 0, into.dtype, n - h);
 #pragma unroll
-            for (int i = 0; i < 4; i++) o[i] = p.keep * old[i] - m.step * o[i];
+            for (int i = 0; i < 4; i++) o[i] = into.keep * old[i] - into.step * o[i];
         }
         if (n - h >= 4) {
-            if (p.out_dtype == TFTQ_F32) *(ns_f4_any *)to = o;
-            else if (p.out_dtype == TFTQ_F16) *(ns_h4_any *)to = __builtin_convertvector(o, ns_h4_any);
+            if (into.dtype == TFTQ_F32) *(ns_f4_any *)to = o;
+            else if (into.dtype == TFTQ_F16) *(ns_h4_any *)to = __builtin_convertvector(o, ns_h4_any);
             else *(ns_b4_any *)to = __builtin_convertvector(o, ns_b4_any);
             continue;
         }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             if (i >= n - h) continue;
-            if (p.out_dtype == TFTQ_F32) ((float *)to)[i] = o[i];
-            else if (p.out_dtype == TFTQ_F16) ((_Float16 *)to)[i] = (_Float16)o[i];
+            if (into.dtype == TFTQ_F32) ((float *)to)[i] = o[i];
+            else if (into.dtype == TFTQ_F16) ((_Float16 *)to)[i] = (_Float16)o[i];
             else ((__bf16 *)to)[i] = (__bf16)o[i];
         }
     }
@@ -337,22 +352,26 @@ enum { NS_A, NS_B, NS_X };
 template <int WHAT, bool PRECISE>
 struct NsFinish {
     static constexpr bool LOW = PRECISE || WHAT == NS_X;  // the result's rows have a remainder
-    NsMatrix m;
-    NsParams p;
-    NsWork w;
+    // only what it needs of the matrix, the workspace and the parameters: all of it stays in registers
+    NsOut into;
+    const uint8_t *old_high, *old_low;
+    float *d, *f;
     uint8_t *out, *out_l, *turned, *turned_l;  // panels along the result's rows, and along its columns
     float per_x;                               // one over X's scale, a power of two
-    int r, cols, padded;
+    float a, b, c;
+    int r, cols, padded, last, next_last, flip;
     bool mirror;
 
-    __device__ NsFinish(const NsMatrix &matrix, const NsParams &params, const NsWork &work, int turn, bool diagonal)
-        : m(matrix), p(params), w(work)
+    __device__ __forceinline__ NsFinish(const NsMatrix &m, const NsParams &p, const NsWork &w, int turn, bool diagonal)
     {
+        into.out = m.out, into.ld = m.ld_out, into.keep = p.keep, into.step = m.step, into.update = p.update, into.dtype = p.out_dtype;
+        old_high = WHAT == NS_B ? w.e : w.x, old_low = WHAT == NS_B ? w.el : w.xl;
+        d = w.d, f = w.f, a = p.a, b = p.b, c = p.c, last = p.last, next_last = p.next_last, flip = m.flip;
         out = WHAT == NS_A ? w.e : WHAT == NS_B ? w.g : w.x, out_l = WHAT == NS_A ? w.el : WHAT == NS_B ? w.gl : w.xl;
         turned = WHAT != NS_X ? out : turn ? w.t : w.t2, turned_l = WHAT != NS_X ? out_l : turn ? w.tl : w.tl2;
         per_x = 1.f / *w.scale;
         r = m.rows, cols = WHAT == NS_X ? m.cols : m.rows, padded = (cols + 63) & ~63;
-        mirror = WHAT == NS_X ? !p.last || m.flip : !diagonal;
+        mirror = WHAT == NS_X ? !last || flip : !diagonal;
     }
     __device__ int64_t at(int i, int j) const { return ((int64_t)(j >> 6) * r + i) * PANEL_BYTES + (j & 63) * 2; }
 
@@ -365,9 +384,9 @@ struct NsFinish {
     {
         Old o = {};
         if (WHAT == NS_A || i >= r || j >= padded) return o;
-        o.high = *(const ns_h8 *)((WHAT == NS_B ? w.e : w.x) + at(i, j));
-        if (PRECISE || (LOW && !p.last)) o.low = *(const ns_h8 *)((WHAT == NS_B ? w.el : w.xl) + at(i, j));
-        o.di = WHAT == NS_B ? w.d[i] : p.a + w.f[i];
+        o.high = *(const ns_h8 *)(old_high + at(i, j));
+        if (PRECISE || (LOW && !last)) o.low = *(const ns_h8 *)(old_low + at(i, j));
+        o.di = WHAT == NS_B ? d[i] : a + f[i];
         return o;
     }
     // v: the sums of row i, columns j to j + 7, and then their values as numbers (of the last iteration)
@@ -379,24 +398,24 @@ struct NsFinish {
             if ((unsigned)(i - j) < 8u && i < r) {
 #pragma unroll
                 for (int n = 0; n < 8; n++)
-                    if (i == j + n) w.d[i] = v[n] * per_x * per_x;
+                    if (i == j + n) d[i] = v[n] * per_x * per_x;
             }
             const float by = per_x * per_x * SCALE_E;
 #pragma unroll
             for (int n = 0; n < 8; n++) v[n] *= by;
         } else if (WHAT == NS_B) {
-            const float by = p.c * (SCALE_G / (SCALE_E * SCALE_E)), c = p.c * (SCALE_G / SCALE_E), b = p.b * (SCALE_G / SCALE_E);
+            const float by = c * (SCALE_G / (SCALE_E * SCALE_E)), ce = c * (SCALE_G / SCALE_E), be = b * (SCALE_G / SCALE_E);
             if ((unsigned)(i - j) < 8u && i < r) {
 #pragma unroll
                 for (int n = 0; n < 8; n++)
-                    if (i == j + n) w.f[i] = p.b * was.di + p.c * (v[n] * (1.f / (SCALE_E * SCALE_E)) + was.di * was.di);
+                    if (i == j + n) f[i] = b * was.di + c * (v[n] * (1.f / (SCALE_E * SCALE_E)) + was.di * was.di);
             }
-            tile_f4 d[2] = {};
-            if (inside) d[0] = *(const tile_f4 *)(w.d + j), d[1] = *(const tile_f4 *)(w.d + j + 4);
+            tile_f4 dj[2] = {};
+            if (inside) dj[0] = *(const tile_f4 *)(d + j), dj[1] = *(const tile_f4 *)(d + j + 4);
 #pragma unroll
             for (int n = 0; n < 8; n++) {
                 const float x = PRECISE ? (float)was.high[n] + (float)was.low[n] : (float)was.high[n];
-                v[n] = fmaf(x, fmaf(c, was.di + d[n / 4][n % 4], b), v[n] * by);
+                v[n] = fmaf(x, fmaf(ce, was.di + dj[n / 4][n % 4], be), v[n] * by);
             }
         } else {
 #pragma unroll
@@ -410,16 +429,16 @@ struct NsFinish {
 #pragma unroll
             for (int n = 0; n < 8; n++) v[n] = i == j + n ? 0.f : v[n];
         }
-        if (WHAT == NS_X && p.last) {
+        if (WHAT == NS_X && last) {
 #pragma unroll
             for (int n = 0; n < 8; n++) v[n] *= per_x;
-            if (inside && !m.flip) ns_put(m, p, i, j, cols - j, v);
+            if (inside && !flip) ns_put(into, i, j, cols - j, v);
             return;
         }
         split(v, high, low);
         if (!inside) return;
         *(ns_h8 *)(out + at(i, j)) = *high;
-        if (PRECISE || (LOW && !p.next_last)) *(ns_h8 *)(out_l + at(i, j)) = *low;
+        if (PRECISE || (LOW && !next_last)) *(ns_h8 *)(out_l + at(i, j)) = *low;
     }
     __device__ __forceinline__ static void split(const float *v, ns_h8 *high, ns_h8 *low)
     {
@@ -443,7 +462,7 @@ struct NsFinish {
     // The last one's values of column j, rows i to i + 7.
     __device__ __forceinline__ void column_out(int i, int j, const float *v) const
     {
-        if (j < cols && i < r) ns_put(m, p, j, i, r - i, v);
+        if (j < cols && i < r) ns_put(into, j, i, r - i, v);
     }
 };
 
@@ -455,14 +474,21 @@ template <int WHAT>
 struct NsProduct {
     const uint8_t *ah, *al, *bh, *bl;
     int a_rows, b_rows, panels;
-    __device__ NsProduct(const NsMatrix &m, const NsWork &w, int turn)
+    // part `split` of `splits` of the panels
+    __device__ __forceinline__ NsProduct(const NsMatrix &m, const NsWork &w, int turn, int split, int splits)
     {
         ah = WHAT == NS_A ? w.x : WHAT == NS_B ? w.e : w.g, al = WHAT == NS_A ? w.xl : WHAT == NS_B ? w.el : w.gl;
         bh = WHAT == NS_A ? w.x : WHAT == NS_B ? w.e : turn ? w.t2 : w.t, bl = WHAT == NS_A ? w.xl : WHAT == NS_B ? w.el : turn ? w.tl2 : w.tl;
         a_rows = m.rows, b_rows = WHAT == NS_X ? m.cols : m.rows;
         panels = ((WHAT == NS_A ? m.cols : m.rows) + 63) >> 6;
+        if (splits > 1) {
+            const int first = panels * split / splits;
+            panels = panels * (split + 1) / splits - first;
+            const int64_t a = (int64_t)first * a_rows * PANEL_BYTES, b = (int64_t)first * b_rows * PANEL_BYTES;
+            ah += a, al += a, bh += b, bl += b;
+        }
     }
-    __device__ void tile(int piece, int high, int wide, int *tm, int *tn) const
+    __device__ __forceinline__ void tile(int piece, int high, int wide, int *tm, int *tn) const
     {
         if (WHAT == NS_X) {
             tile_place(piece, ns_tiles(a_rows, high), ns_tiles(b_rows, wide), tm, tn);
@@ -487,6 +513,61 @@ __device__ static inline ns_h8 ns_down(const _Float16 *from, int pitch, int lane
     return ns_h8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
 
+// Where tiles are fewer than compute units, workgroups share one, each a part of its panels: every one
+// stores its sums, and the last one to be done adds all of them up, in their order, and goes on alone.
+// take(i): the i-th vector of the thread's sums, put(i, v): it becomes v.
+struct NsSplit {
+    int tile, split, splits;
+    __device__ __forceinline__ NsSplit(const NsMatrix &m, int piece, bool shared)
+    {
+        tile = piece, split = 0, splits = 1;
+        if (!shared || m.splits == 1) return;
+        const int tiles = m.pieces / m.splits;  // a part of all tiles, then the next part
+        split = piece / tiles, tile = piece - split * tiles, splits = m.splits;
+    }
+    // The sums are stored and loaded at the device's scope, past the caches of one XCD, and a workgroup takes
+    // its ticket when all of its stores are done: no cache has to be written back or emptied (with
+    // fences that do so, 70 us a launch of 500 workgroups).
+    template <int VECTORS, int THREADS, class A, class B>
+    __device__ __forceinline__ bool join(const NsWork &w, int *last, A take, B put) const
+    {
+        uint64_t *sums = (uint64_t *)w.sums + (int64_t)tile * splits * VECTORS * THREADS * 2 + threadIdx.x;
+        if (threadIdx.x < THREADS) {
+#pragma unroll
+            for (int i = 0; i < VECTORS; i++) {
+                const tile_f4 v = take(i);
+                uint64_t *at = sums + (split * VECTORS + i) * THREADS * 2;
+                __hip_atomic_store(at, pair(v[0], v[1]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_store(at + THREADS, pair(v[2], v[3]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            *last = __hip_atomic_fetch_add(w.tickets + tile, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == splits - 1;
+            if (*last) __hip_atomic_store(w.tickets + tile, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next launch
+        }
+        __syncthreads();
+        if (!*last) return false;
+        if (threadIdx.x < THREADS) {
+            tile_f4 v[VECTORS] = {};
+            for (int n = 0; n < splits; n++) {
+#pragma unroll
+                for (int i = 0; i < VECTORS; i++) {
+                    const uint64_t *at = sums + (n * VECTORS + i) * THREADS * 2;
+                    const uint64_t x = __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    const uint64_t y = __hip_atomic_load(at + THREADS, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    v[i] += tile_f4{__uint_as_float((uint32_t)x), __uint_as_float((uint32_t)(x >> 32)), __uint_as_float((uint32_t)y), __uint_as_float((uint32_t)(y >> 32))};
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < VECTORS; i++) put(i, v[i]);
+        }
+        return true;
+    }
+    __device__ __forceinline__ static uint64_t pair(float a, float b) { return __float_as_uint(a) | (uint64_t)__float_as_uint(b) << 32; }
+};
+
 // LDS of a product's workgroup: the tile's buffers, and when they are done with its strips as sums and as
 // two fp16 numbers each.
 template <class T>
@@ -495,7 +576,7 @@ struct NsLds {
     static constexpr int BYTES = T::LDS > STRIPS ? T::LDS : STRIPS;
 };
 
-template <class T, int WHAT, bool PRECISE>
+template <class T, int WHAT, bool PRECISE, bool SHARED>
 __global__ __launch_bounds__(T::THREADS) void k_ns_product(int count, int turn, const NsLaunch l, const NsParams p)
 {
     __shared__ __attribute__((aligned(128))) uint8_t lds[NsLds<T>::BYTES];
@@ -503,14 +584,28 @@ __global__ __launch_bounds__(T::THREADS) void k_ns_product(int count, int turn, 
     if (!ns_tile(l, count, blockIdx.x, &matrix, &piece)) return;
     const NsMatrix m = l.m[matrix];
     const NsWork w = ns_work(m.work, m.rows, m.cols, m.flip, PRECISE);
-    const NsProduct<WHAT> o(m, w, turn);
-    o.tile(piece, T::ROWS, T::COLS, &tm, &tn);
+    const NsSplit mine(m, piece, SHARED);
+    const NsProduct<WHAT> o(m, w, turn, mine.split, mine.splits);
+    o.tile(mine.tile, T::ROWS, T::COLS, &tm, &tn);
     const int row0 = tm * T::ROWS, col0 = tn * T::COLS;
     T t;
     auto place = [&](int, int *r0, int *c0) { *r0 = row0, *c0 = col0; };
     auto done = [](int, int) {};
     if constexpr (PRECISE) t.multiply(TileTriple{{o.ah, o.al, o.bh, o.bl, o.a_rows, o.b_rows, o.panels}}, 3 * o.panels, 1, place, lds, done);
     else t.multiply(TilePair{{o.ah, nullptr, o.a_rows}, {o.bh, nullptr, o.b_rows}}, o.panels, 1, place, lds, done);
+    if constexpr (SHARED) {
+        if (mine.splits > 1) {
+            static_assert(T::TM == 1 && T::TN == 1, "");
+            if (!mine.template join<4, T::THREADS>(w, (int *)lds, [&](int i) {
+                    return tile_f4{t.acc[0][0][4 * i], t.acc[0][0][4 * i + 1], t.acc[0][0][4 * i + 2], t.acc[0][0][4 * i + 3]};
+                }, [&](int i, tile_f4 v) {
+#pragma unroll
+                    for (int n = 0; n < 4; n++) t.acc[0][0][4 * i + n] = v[n];
+                }))
+                return;
+            __syncthreads();  // `last` has been read: the strips may take its place
+        }
+    }
 
     const NsFinish<WHAT, PRECISE> finish(m, p, w, turn, tm == tn);
     constexpr int ACROSS = T::WN / 8, PASSES = 32 * ACROSS / 64;  // 8 neighbours of a row per lane
@@ -521,27 +616,28 @@ __global__ __launch_bounds__(T::THREADS) void k_ns_product(int count, int turn, 
     const int lane = threadIdx.x & 63;
     _Float16 *halves = (_Float16 *)(lds + T::WAVES * 32 * T::PITCH * 4) + tile_wave() * 2 * HALF;
     typename NsFinish<WHAT, PRECISE>::Old was[2][PASSES];  // of the next strip while one is finished
-    t.store_strips(row0, col0, lds, [&](int i, int row, int col) __attribute__((always_inline)) {
-#pragma unroll
-        for (int q = 0; q < PASSES; q++) was[i & 1][q] = finish.old(row + (lane + 64 * q) / ACROSS, col + (lane + 64 * q) % ACROSS * 8);
-    }, [&](int i, float *strip, int row, int col) __attribute__((always_inline)) {
-        const bool last = WHAT == NS_X && p.last;
-#pragma unroll
-        for (int q = 0; q < PASSES; q++) {
+    const std::make_integer_sequence<int, PASSES> passes;
+    t.store_strips(row0, col0, lds, [&](auto i, int row, int col) __attribute__((always_inline)) {
+        tile_each(passes, [&](auto q) __attribute__((always_inline)) {
+            was[i & 1][q] = finish.old(row + (lane + 64 * q) / ACROSS, col + (lane + 64 * q) % ACROSS * 8);
+        });
+    }, [&](auto i, float *strip, int row, int col) __attribute__((always_inline)) {
+        const bool last = WHAT == NS_X && finish.last;
+        tile_each(passes, [&](auto q) __attribute__((always_inline)) {
             const int at = (lane + 64 * q) / ACROSS, c = (lane + 64 * q) % ACROSS * 8;
             float v[8];
             tile_f4 *from = (tile_f4 *)__builtin_assume_aligned(strip + at * T::PITCH + c, 16);
             *(tile_f4 *)v = from[0], *(tile_f4 *)(v + 4) = from[1];
             ns_h8 high, low;
             finish.row(row + at, col + c, v, was[i & 1][q], &high, &low);
-            if (!finish.mirror) continue;
+            if (!finish.mirror) return;
             if (last) {
                 from[0] = *(tile_f4 *)v, from[1] = *(tile_f4 *)(v + 4);
             } else {
                 *(ns_h8 *)__builtin_assume_aligned(halves + at * PITCH16 + c, 16) = high;
                 if (PRECISE) *(ns_h8 *)__builtin_assume_aligned(halves + HALF + at * PITCH16 + c, 16) = low;
             }
-        }
+        });
         T::wave_fence();
         if (!finish.mirror) return;
         if (last) {
@@ -566,17 +662,19 @@ __global__ __launch_bounds__(T::THREADS) void k_ns_product(int count, int turn, 
 // The same for matrices of few tiles, where a kernel's time is that of the loads it waits for: a tile of
 // 32 x 32 per workgroup, whose 8 wavefronts share the panels between them, take their operands straight
 // from memory with all of a panel's loads in flight, and add up in LDS.
-template <int WHAT, bool PRECISE>
+template <int WHAT, bool PRECISE, bool SHARED>
 __global__ __launch_bounds__(512) void k_ns_small(int count, int turn, const NsLaunch l, const NsParams p)
 {
     constexpr int WAVES = 8, PITCH = 36;
     __shared__ __attribute__((aligned(128))) float sums[WAVES][32 * PITCH];
+    __shared__ int last;
     int matrix, piece, tm, tn;
     if (!ns_tile(l, count, blockIdx.x, &matrix, &piece)) return;
     const NsMatrix m = l.m[matrix];
     const NsWork w = ns_work(m.work, m.rows, m.cols, m.flip, PRECISE);
-    const NsProduct<WHAT> o(m, w, turn);
-    o.tile(piece, 32, 32, &tm, &tn);
+    const NsSplit mine(m, piece, SHARED);
+    const NsProduct<WHAT> o(m, w, turn, mine.split, mine.splits);
+    o.tile(mine.tile, 32, 32, &tm, &tn);
     const int lane = threadIdx.x & 63, wave = tile_wave(), half = lane >> 5;
     const int64_t a_at = (int64_t)min(tm * 32 + (lane & 31), o.a_rows - 1) * PANEL_BYTES + half * 16;
     const int64_t b_at = (int64_t)min(tn * 32 + (lane & 31), o.b_rows - 1) * PANEL_BYTES + half * 16;
@@ -607,14 +705,19 @@ __global__ __launch_bounds__(512) void k_ns_small(int count, int turn, const NsL
     typename NsFinish<WHAT, PRECISE>::Old was = {};
     if (id < 128) was = finish.old(tm * 32 + at, tn * 32 + c);
     __syncthreads();
+    float v[8];
     if (id < 128) {
-        float v[8];
 #pragma unroll
         for (int n = 0; n < 8; n++) {
             v[n] = sums[0][at * PITCH + c + n];
 #pragma unroll
             for (int k = 1; k < WAVES; k++) v[n] += sums[k][at * PITCH + c + n];
         }
+    }
+    if (SHARED && mine.splits > 1 && !mine.template join<2, 128>(w, &last, [&](int i) { return tile_f4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]}; },
+                                                    [&](int i, tile_f4 to) { v[4 * i] = to[0], v[4 * i + 1] = to[1], v[4 * i + 2] = to[2], v[4 * i + 3] = to[3]; }))
+        return;
+    if (id < 128) {
         ns_h8 high, low;
         finish.row(tm * 32 + at, tn * 32 + c, v, was, &high, &low);
 #pragma unroll
@@ -627,7 +730,7 @@ __global__ __launch_bounds__(512) void k_ns_small(int count, int turn, const NsL
         float v[8];
 #pragma unroll
         for (int n = 0; n < 8; n++) v[n] = sums[0][(i + n) * PITCH + j];
-        if (WHAT == NS_X && p.last) {
+        if (WHAT == NS_X && finish.last) {
             finish.column_out(tm * 32 + i, tn * 32 + j, v);
         } else {
             ns_h8 high, low;
@@ -645,7 +748,7 @@ static int launch_over(NsLaunch &l, F workgroups, bool eighths, const void *kern
 {
     int64_t total = 0;
     for (int i = 0; i < l.count; i++) {
-        const int64_t n = workgroups(l.m[i]);
+        const int64_t n = workgroups(l.m[i]) * l.m[i].splits;
         l.first[i] = (int)total, l.m[i].pieces = (int)n;
         total += eighths ? (n + 7) / 8 : n;
     }
@@ -660,23 +763,52 @@ static int64_t tiles(const NsMatrix &m, int what, int high, int wide)
     return what == NS_X ? r * k : r * (r + 1) / 2;
 }
 
+static bool ns_shared(const NsLaunch &l)
+{
+    return std::any_of(l.m, l.m + l.count, [](const NsMatrix &m) { return m.splits > 1; });
+}
+
 template <class T, int WHAT>
 static int launch_tiles(NsLaunch &l, bool precise, const NsParams &p, int turn, hipStream_t st)
 {
-    const void *k = precise ? (const void *)k_ns_product<T, WHAT, true> : (const void *)k_ns_product<T, WHAT, false>;
+    const void *k = precise ? (const void *)k_ns_product<T, WHAT, true, false> : (const void *)k_ns_product<T, WHAT, false, false>;
+    if constexpr (T::ROWS == 64) {
+        if (ns_shared(l)) k = precise ? (const void *)k_ns_product<T, WHAT, true, true> : (const void *)k_ns_product<T, WHAT, false, true>;
+    }
     return launch_over(l, [](const NsMatrix &m) { return tiles(m, WHAT, T::ROWS, T::COLS); }, true, k, T::THREADS, p, turn, st);
 }
 
-// About how long a product of the matrices of a launch takes in tiles of a size.
-static double ns_time(const NsLaunch &l, int what, const TileShape &t)
+// How many workgroups share a tile of `all` in a launch, each at least `least` of its panels: a panel for every
+// wavefront of k_ns_small; what outweighs the sums' way through memory, 3 us, in tiles of 64 x 64.  No more
+// than 16, whose sums one workgroup adds up.  Graph replays of the whole orthogonalisation, us, with a
+// workgroup to a tile and so: fp32 64x3584 188, 99; 64x16384 661, 145; 256x16384 734, 282; 1024x16384 1714,
+// 1162; 1024x1024 286, 276; bf16 64x16384 352, 119; 1024x16384 670, 532 (from 8 panels on 1024x1024 bf16 is
+// shared too: 151, 192).
+static int ns_splits(int64_t all, int64_t panels, int least)
 {
-    double work = 0, longest = 0, count = 0;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({NS_SHARED / std::max<int64_t>(all, 1), panels / least, 16}));
+}
+static int64_t ns_panels(const NsMatrix &m, int what) { return ((what == NS_A ? m.cols : m.rows) + 63) / 64; }
+static int ns_least(int size, bool precise) { return size == 32 ? 8 : precise ? 6 : 16; }
+static int64_t ns_all(const NsLaunch &l, int what, int high, int wide)
+{
+    int64_t all = 0;
+    for (int i = 0; i < l.count; i++) all += tiles(l.m[i], what, high, wide);
+    return all;
+}
+
+// About how long a product of the matrices of a launch takes in tiles of a size.
+static double ns_time(const NsLaunch &l, int what, const TileShape &t, bool precise)
+{
+    double work = 0, longest = 0, count = 0, more = 0;
+    const int64_t all = ns_all(l, what, t.high, t.wide);
     for (int i = 0; i < l.count; i++) {
-        const double n = (double)tiles(l.m[i], what, t.high, t.wide);
-        const double panels = ((what == NS_A ? l.m[i].cols : l.m[i].rows) + 63) / 64;
-        count += n, work += n * panels, longest = std::max(longest, panels);
+        const double n = (double)tiles(l.m[i], what, t.high, t.wide), panels = (double)ns_panels(l.m[i], what) * (precise ? 3 : 1);
+        const int splits = t.high == 64 ? ns_splits(all, ns_panels(l.m[i], what), ns_least(64, precise)) : 1;
+        count += n * splits, work += n * panels, longest = std::max(longest, panels / splits);
+        if (splits > 1) more = 8 * t.one;  // the sums' way through memory
     }
-    return tile_time(t, count, work, longest);
+    return tile_time(t, count, work, longest) + more;
 }
 
 // One of the three products for all matrices of a launch.  Up to 512 tiles of 32 x 32 (256 where a product
@@ -687,17 +819,22 @@ template <int WHAT>
 static int product(NsLaunch &l, bool precise, const NsParams &p, int turn, hipStream_t st)
 {
     // the matrices with most panels first: the last workgroups are then short ones
-    std::stable_sort(l.m, l.m + l.count, [](const NsMatrix &x, const NsMatrix &y) { return WHAT == NS_A ? x.cols > y.cols : x.rows > y.rows; });
-    int64_t small = 0;
-    for (int i = 0; i < l.count; i++) small += tiles(l.m[i], WHAT, 32, 32);
-    if (small <= (precise ? 512 : 256)) {
-        const void *k = precise ? (const void *)k_ns_small<WHAT, true> : (const void *)k_ns_small<WHAT, false>;
+    std::stable_sort(l.m, l.m + l.count, [](const NsMatrix &x, const NsMatrix &y) { return ns_panels(x, WHAT) > ns_panels(y, WHAT); });
+    auto share = [&](int size) {
+        const int64_t all = ns_all(l, WHAT, size, size);
+        for (int i = 0; i < l.count; i++) l.m[i].splits = size > 64 ? 1 : ns_splits(all, ns_panels(l.m[i], WHAT), ns_least(size, precise));
+    };
+    if (ns_all(l, WHAT, 32, 32) <= (precise ? 512 : 256)) {
+        share(32);
+        const void *k = ns_shared(l) ? precise ? (const void *)k_ns_small<WHAT, true, true> : (const void *)k_ns_small<WHAT, false, true>
+                        : precise ? (const void *)k_ns_small<WHAT, true, false> : (const void *)k_ns_small<WHAT, false, false>;
         return launch_over(l, [](const NsMatrix &m) { return tiles(m, WHAT, 32, 32); }, true, k, 512, p, turn, st);
     }
     const TileShape choice[] = {TILES_256, WHAT == NS_X ? TILES_192X256 : TILES_192, TILES_128, TILES_64};
     int best = 0;
     for (int i = 1; i < 4; i++)
-        if (ns_time(l, WHAT, choice[i]) < ns_time(l, WHAT, choice[best])) best = i;
+        if (ns_time(l, WHAT, choice[i], precise) < ns_time(l, WHAT, choice[best], precise)) best = i;
+    share(choice[best].high);
     switch (best) {
     case 0: return launch_tiles<Tile<256, 256, 2, 4, false>, WHAT>(l, precise, p, turn, st);
     case 1:
@@ -706,6 +843,22 @@ static int product(NsLaunch &l, bool precise, const NsParams &p, int turn, hipSt
     case 2: return launch_tiles<Tile<128, 128, 2, 2, false>, WHAT>(l, precise, p, turn, st);
     default: return launch_tiles<Tile<64, 64, 2, 2, false, 3>, WHAT>(l, precise, p, turn, st);
     }
+}
+
+// Bytes of workspace of a matrix: its parts and, for the most workgroups that may ever share its tiles (those
+// of a launch of its own), their sums.
+static int64_t ns_bytes(int64_t r, int64_t k, bool flip, bool precise)
+{
+    NsMatrix m = {};
+    m.rows = (int)r, m.cols = (int)k;
+    int64_t sums = 0;
+    for (int what = NS_A; what <= NS_X; what++)
+        for (int size = 32; size <= 64; size += 32) {
+            const int64_t all = tiles(m, what, size, size);
+            const int splits = ns_splits(all, ns_panels(m, what), ns_least(size, precise));
+            if (splits > 1) sums = std::max(sums, all * splits * size * size * 4);
+        }
+    return ns_work(nullptr, r, k, flip, precise).bytes + sums;
 }
 
 static bool ns_shapes_ok(int n, const int64_t *shapes)
@@ -741,7 +894,7 @@ static int ns_parts(int n, const int64_t *shapes, int precise, F f)
                 if (const int rc = f(at, count, kind != 0, bytes)) return rc;
                 count = 0, bytes = 0, squares = 0;
             }
-            bytes += ns_work(nullptr, r, a < b ? b : a, a > b, kind != 0).bytes;
+            bytes += ns_bytes(r, a < b ? b : a, a > b, kind != 0);
             squares += more;
             at[count++] = i;
         }
@@ -802,7 +955,8 @@ extern "C" int tftq_newton_schulz(const tftq_ns *what, void *workspace, int64_t 
             m.rows = (int)std::min(rows, cols), m.cols = (int)std::max(rows, cols);
             m.step = s.steps ? s.steps[i] : 0.f;
             m.work = work;
-            work += ns_work(nullptr, m.rows, m.cols, m.flip, precise).bytes;
+            m.splits = 1;
+            work += ns_bytes(m.rows, m.cols, m.flip, precise);
         }
         float growth = 1.f;
         for (int it = 0; it < s.iterations; it++) growth *= fmaxf(1.f, fabsf(s.coefficients[3 * it]));

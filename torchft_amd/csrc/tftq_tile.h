@@ -23,6 +23,8 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
+#include <utility>
 
 typedef int tile_i4 __attribute__((ext_vector_type(4)));
 typedef uint32_t tile_u2 __attribute__((ext_vector_type(2)));
@@ -84,6 +86,14 @@ __device__ static inline __amdgpu_buffer_rsrc_t tile_buffer(const uint8_t *from,
 __device__ static inline void tile_load16(__amdgpu_buffer_rsrc_t from, int at, int more, uint8_t *lds)
 {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void *)lds, 16, at, more, 0, 0);
+}
+
+// f(0), f(1) and so on, constants: arrays that f indexes with them stay in registers, whatever f's size
+// (loops of large bodies are unrolled too late for that).
+template <class F, int... I>
+__device__ static __forceinline__ void tile_each(std::integer_sequence<int, I...>, F f)
+{
+    (f(std::integral_constant<int, I>()), ...);
 }
 
 // The wavefront's number in its workgroup, in a scalar register.
@@ -313,19 +323,20 @@ struct Tile {
     }
 
     // f(i, strip, row, col) for every 32 x WN values of the wavefront, strip[r * PITCH + c] in LDS being
-    // C[row + r][col + c]; before(i, row, col) is called a strip ahead, to load what f needs.  A lane's
-    // accumulators hold 4 neighbouring values of one row, 8 columns apart (b is the instruction's first
-    // operand); from the strip it takes what makes whole 16 bytes of the result.
+    // C[row + r][col + c]; before(i, row, col) is called a strip ahead, to load what f needs (i: a constant,
+    // so that what they keep from strip to strip stays in registers).  A lane's accumulators hold 4
+    // neighbouring values of one row, 8 columns apart (b is the instruction's first operand); from the strip
+    // it takes what makes whole 16 bytes of the result.
     template <class B, class F>
     __device__ __forceinline__ void store_strips(int row0, int col0, uint8_t *lds, B before, F f)
     {
-        const int lane = threadIdx.x & 63, wave = tile_wave();
-        const int wm = wave / WGN * WM, wn = wave % WGN * WN;
+        const int wave = tile_wave();
+        const int row = row0 + wave / WGN * WM, col = col0 + wave % WGN * WN;
         float *strip = (float *)lds + wave * 32 * PITCH;
-        before(0, row0 + wm, col0 + wn);
-#pragma unroll
-        for (int i = 0; i < TM; i++) {
-            if (i + 1 < TM) before(i + 1, row0 + wm + 32 * (i + 1), col0 + wn);
+        const int lane = threadIdx.x & 63;
+        before(std::integral_constant<int, 0>(), row, col);
+        tile_each(std::make_integer_sequence<int, TM>(), [&](auto i) __attribute__((always_inline)) {
+            if constexpr (i + 1 < TM) before(std::integral_constant<int, i + 1>(), row + 32 * (i + 1), col);
 #pragma unroll
             for (int j = 0; j < TN; j++)
 #pragma unroll
@@ -333,9 +344,9 @@ struct Tile {
                     *(tile_f4 *)(strip + (lane & 31) * PITCH + 32 * j + 8 * g + 4 * (lane >> 5)) =
                         tile_f4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
             wave_fence();
-            f(i, strip, row0 + wm + 32 * i, col0 + wn);
+            f(i, strip, row + 32 * i, col);
             wave_fence();
-        }
+        });
     }
     // f(the lane's 16 bytes, row, column) of the results, as elements of SIZE bytes; `to` makes a word of two
     // sums of those of 2.  By way of 2048 bytes of LDS per wavefront beside the buffers: 64 bytes of 32
