@@ -806,15 +806,31 @@ static double ns_time(const NsLaunch &l, int what, const TileShape &t, bool prec
         const double n = (double)tiles(l.m[i], what, t.high, t.wide), panels = (double)ns_panels(l.m[i], what) * (precise ? 3 : 1);
         const int splits = t.high == 64 ? ns_splits(all, ns_panels(l.m[i], what), ns_least(64, precise)) : 1;
         count += n * splits, work += n * panels, longest = std::max(longest, panels / splits);
-        if (splits > 1) more = 8 * t.one;  // the sums' way through memory
+        if (splits > 1) more = 12 * t.one;  // the sums' way through memory
     }
     return tile_time(t, count, work, longest) + more;
 }
 
-// One of the three products for all matrices of a launch.  Up to 512 tiles of 32 x 32 (256 where a product
-// is one, not three) take k_ns_small.  Graph replays of the whole orthogonalisation, us, so and with tiles of
-// 64 x 64: fp32 512x512 127, 182; 512x768 159, 164; 768x1024 264, 263; 1024x1024 432, 292.  bf16 512x512
-// 90, 102; 512x768 105, 104; 640x640 117, 112; 768x1024 162, 140.
+// The same for k_ns_small, to which one panel of its 8 wavefronts after the other comes from memory, on every
+// unit that has a workgroup at once, and beside whose launch that of a tile kernel takes 0.5 more.  Nothing
+// is faster where there is one such panel.  From (us) fp32 256x512, A (1 panel, 36 tiles) 7.4; 870x6665, A (14 panels, 406 tiles) 108, B (2, 406) 17.
+static double ns_small_time(const NsLaunch &l, int what, bool precise)
+{
+    const int64_t all = ns_all(l, what, 32, 32);
+    int64_t count = 0, panels = 0;
+    double more = -0.5;
+    for (int i = 0; i < l.count; i++) {
+        const int splits = ns_splits(all, ns_panels(l.m[i], what), ns_least(32, precise));
+        count += tiles(l.m[i], what, 32, 32) * splits, panels = std::max(panels, (ns_panels(l.m[i], what) + 8 * splits - 1) / (8 * splits));
+        if (splits > 1) more = 0.7;
+    }
+    panels *= (count + 255) / 256;
+    return panels <= 1 ? 0 : 2.2 + (precise ? 2.1 : 0.9) * (double)panels + more;
+}
+
+// One of the three products for all matrices of a launch.  k_ns_small and tiles of 64 x 64, graph replays of the
+// whole orthogonalisation, us: fp32 512x512 127, 182; 512x768 159, 164; 768x1024 264, 263; 1024x1024 432,
+// 292.  bf16 512x512 90, 102; 512x768 105, 104; 640x640 117, 112; 768x1024 162, 140.
 template <int WHAT>
 static int product(NsLaunch &l, bool precise, const NsParams &p, int turn, hipStream_t st)
 {
@@ -824,16 +840,16 @@ static int product(NsLaunch &l, bool precise, const NsParams &p, int turn, hipSt
         const int64_t all = ns_all(l, WHAT, size, size);
         for (int i = 0; i < l.count; i++) l.m[i].splits = size > 64 ? 1 : ns_splits(all, ns_panels(l.m[i], WHAT), ns_least(size, precise));
     };
-    if (ns_all(l, WHAT, 32, 32) <= (precise ? 512 : 256)) {
+    const TileShape choice[] = {TILES_256, WHAT == NS_X ? TILES_192X256 : TILES_192, TILES_128, TILES_64};
+    int best = 0;
+    for (int i = 1; i < 4; i++)
+        if (ns_time(l, WHAT, choice[i], precise) < ns_time(l, WHAT, choice[best], precise)) best = i;
+    if (ns_small_time(l, WHAT, precise) < ns_time(l, WHAT, choice[best], precise)) {
         share(32);
         const void *k = ns_shared(l) ? precise ? (const void *)k_ns_small<WHAT, true, true> : (const void *)k_ns_small<WHAT, false, true>
                         : precise ? (const void *)k_ns_small<WHAT, true, false> : (const void *)k_ns_small<WHAT, false, false>;
         return launch_over(l, [](const NsMatrix &m) { return tiles(m, WHAT, 32, 32); }, true, k, 512, p, turn, st);
     }
-    const TileShape choice[] = {TILES_256, WHAT == NS_X ? TILES_192X256 : TILES_192, TILES_128, TILES_64};
-    int best = 0;
-    for (int i = 1; i < 4; i++)
-        if (ns_time(l, WHAT, choice[i], precise) < ns_time(l, WHAT, choice[best], precise)) best = i;
     share(choice[best].high);
     switch (best) {
     case 0: return launch_tiles<Tile<256, 256, 2, 4, false>, WHAT>(l, precise, p, turn, st);
