@@ -890,6 +890,21 @@ static bool ns_shapes_ok(int n, const int64_t *shapes)
 // one tile high, and its products wait for memory, not for the matrix cores.
 static bool ns_precise(int64_t r, int precise) { return precise || r < 64; }
 
+// Whether the matrices of one product are so few and small that they join those of three in their launches: two
+// times their work more, but no 17 launches of their own (bf16, us, together and apart: 322x322 with 1x322 and
+// 322x1 111, 147; ten of up to 844x211 with two of 211x1 169, 193; 640x640 with 512x1 181, 178).
+static bool ns_together(int n, const int64_t *shapes)
+{
+    double work = 0;
+    bool narrow = false;
+    for (int i = 0; i < n; i++) {
+        const double a = (double)shapes[2 * i], b = (double)shapes[2 * i + 1], r = std::min(a, b);
+        if (r > 0 && ns_precise((int64_t)r, 0)) narrow = true;
+        else work += r * a * b;
+    }
+    return narrow && n <= NS_MOST && work <= 2.5e8;
+}
+
 // Squares of 64 of a launch's matrices: no kernel has more workgroups of 256 threads, or half as many of
 // 512, and a launch has fewer than 2^32 threads.
 constexpr int64_t NS_SQUARES = 1 << 23;
@@ -898,6 +913,7 @@ constexpr int64_t NS_SQUARES = 1 << 23;
 template <class F>
 static int ns_parts(int n, const int64_t *shapes, int precise, F f)
 {
+    if (!precise && ns_together(n, shapes)) precise = 1;
     for (int kind = 0; kind < 2; kind++) {
         int at[NS_MOST], count = 0;
         int64_t bytes = 0, squares = 0;
