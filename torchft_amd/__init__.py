@@ -1,5 +1,6 @@
 """MI355X-native FP8 quantized-collective kernels, a drop-in for torchft's
-``torchft.quantization`` (and its callers in ``torchft.collectives``)."""
+``torchft.quantization`` (and its callers in ``torchft.collectives``); and, with no counterpart there,
+operators of the training step around them: 4-bit matrices and linear layers on them, Muon's update."""
 
 from .quantization import (  # noqa: F401
     PreparedBucket,

