@@ -234,7 +234,7 @@ extern "C" int tftq_mx_product(int dtype, const void *a, int64_t m, const void *
         default: return few<MxQuantized, TFTQ_BF16>(ta.panels, 0, ta.scales, (int)m, tb, (int)k, (uint8_t *)out, row_stride, st);
         }
     }
-    const TileShape choice[] = {TILES_256, TILES_192X256_FP4, TILES_128, TILES_64_FP4};
+    const TileShape choice[] = {TILES_256, TILES_192X256, TILES_128, TILES_64_FP4};
     int best = 0;
     double least = 0;
     for (int i = 0; i < 4; i++) {

@@ -580,7 +580,7 @@ struct NsLds {
 };
 
 // One of the products, a tile per workgroup.  4096x14336 with one product each (us, and the rate of the
-// work that symmetry leaves): A 255 (0.94 PFLOP/s), B 82 (0.84), X 573 (0.84; a loop without an end
+// work that symmetry leaves): A 255 (0.94 PFLOP/s), B 82 (0.84), X 552 (0.87; a loop without an end
 // 1.23): X moves 10 bytes an element besides, with nothing to multiply meanwhile.  SHARED: some tiles have
 // several workgroups (NsSplit).
 template <class T, int WHAT, bool PRECISE, bool SHARED>

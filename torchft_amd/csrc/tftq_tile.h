@@ -429,15 +429,15 @@ __device__ static inline void tile_place(int piece, int tiles_m, int tiles_n, in
 // 1000, 64x64 760; 4-bit, 256x256 4300, 128x128 3500) and from short ones (4-bit, us, tiles of 256, 128,
 // 64: 256x4096x4096 23.5, 13.4, 10.8; 256x14336x4096 26.6, 17.9, 24.7; 2048x5632x2048 22.1, 22.6, 35.5).
 // 128x128 is 0.61 by its rate, but 3 to a unit take 1.02 (a list of products of depth 2048 in 696 tiles
-// 79 us, in 216 of 256x256 71).  4-bit 192x256: 6144x6144x6144 113, 256x256 123; 14336x4096x8192 230, 222.
+// 79 us, in 216 of 256x256 71), and 192x256 0.775, but with a round more than 256x256 it loses (4-bit
+// 14336x4096x8192 230 us, 222; X of 4096x14336 572, 552; with fewer, 4-bit 6144x6144x6144, 113, 123).
 struct TileShape {
     int high, wide, at_once;
     double one, cost;
 };
-constexpr TileShape TILES_256 = {256, 256, 1, 1.0, 1.0}, TILES_192X256 = {192, 256, 1, 0.775, 0.775},
+constexpr TileShape TILES_256 = {256, 256, 1, 1.0, 1.0}, TILES_192X256 = {192, 256, 1, 0.82, 0.82},
                     TILES_192 = {192, 192, 1, 0.665, 0.665}, TILES_128 = {128, 128, 2, 0.41, 0.68},
-                    TILES_64 = {64, 64, 3, 0.22, 0.30}, TILES_64_FP4 = {64, 64, 2, 0.26, 0.31},
-                    TILES_192X256_FP4 = {192, 256, 1, 0.82, 0.82};
+                    TILES_64 = {64, 64, 3, 0.22, 0.30}, TILES_64_FP4 = {64, 64, 2, 0.26, 0.31};
 
 // About how many panels of a 256 x 256 tile `count` tiles of that size take together: `work` panels in
 // all, `longest` the longest of them.  Storing a tile's values and waiting for its first operands takes
