@@ -73,7 +73,7 @@ struct NsLaunch {
 };
 struct NsParams {
     float momentum, keep, a, b, c, eps, growth;
-    int nesterov, in_dtype, out_dtype, update;
+    int nesterov, out_dtype, update;
     int last, next_last;  // the last iteration, the one before it
 };
 static_assert(sizeof(NsLaunch) + sizeof(NsParams) <= 3800, "kernel arguments");
@@ -145,6 +145,14 @@ __device__ static inline tile_f4 ns_read(const uint8_t *from, int64_t at, int dt
         if (i < n) v[i] = dtype == TFTQ_F32 ? ((const float *)from)[at + i] : dtype == TFTQ_F16 ? (float)((const _Float16 *)from)[at + i] : (float)((const __bf16 *)from)[at + i];
     return v;
 }
+// The same of one type, 4 elements that all exist: loads of several of them, without a branch between, go out together.
+template <int DTYPE>
+__device__ static inline tile_f4 ns_read4(const uint8_t *from, int64_t at)
+{
+    if constexpr (DTYPE == TFTQ_F32) return *(const ns_f4_any *)(from + at * 4);
+    else if constexpr (DTYPE == TFTQ_F16) return __builtin_convertvector(*(const ns_h4_any *)(from + at * 2), tile_f4);
+    else return __builtin_convertvector(*(const ns_b4_any *)(from + at * 2), tile_f4);
+}
 // The matrix and the tile of a product's workgroup: every XCD takes an eighth of every matrix's tiles,
 // neighbouring ones (workgroups go to the 8 XCDs in turn), so that the matrices with most panels are
 // shared by all (one run of the whole list's tiles each: A of 3 matrices of 88 panels and 4 of 32, 161 us).
@@ -165,9 +173,10 @@ __device__ static inline float ns_momentum(float m, float g, const NsParams &p) 
 __device__ static inline float ns_update(float m, float g, const NsParams &p) { return p.nesterov ? m * p.momentum + (1.f - p.momentum) * g : m; }
 
 // momentum <- its next value; the sums of the squares of u, one for 8 or 64 rows of 1024, in 64 bits: no
-// gradient's norm leaves their range, and the order of the additions is always the same.  4096x14336 bf16 55 us
-// (2.1 TB/s), 44 M elements with momentum 152 us (440 MB, 2.9 TB/s): bound by the arithmetic, not the
-// loads (with 16 rows in flight 92 us).
+// gradient's norm leaves their range, and the order of the additions is always the same.  Bound by memory:
+// 4096x14336 bf16 36 us (117 MB, 3.2 TB/s), 44 M elements with momentum 84 us (440 MB, 5.2 TB/s).  A branch on
+// the type or the row's end at every load makes each wait for the one before (55 and 154 us).
+template <int DTYPE, bool MOMENTUM>
 __global__ __launch_bounds__(256) void k_ns_squares(int count, int precise, const NsLaunch l, const NsParams p)
 {
     __shared__ double sums[4];
@@ -183,24 +192,26 @@ __global__ __launch_bounds__(256) void k_ns_squares(int count, int precise, cons
     const int c = col0 + (int)threadIdx.x % groups * 4, n = wide - c;
     double sum = 0;
     constexpr int AT_ONCE = 8;  // rows whose loads are in flight together
-    if ((int)threadIdx.x < groups * apart)
+    auto add = [&](auto whole) {
         for (int r0 = row0 + (int)threadIdx.x / groups; r0 < row0 + rows; r0 += AT_ONCE * apart) {
             tile_f4 u[AT_ONCE], next[AT_ONCE];
 #pragma unroll
             for (int q = 0; q < AT_ONCE; q++) {
                 const int64_t r = min(r0 + q * apart, row0 + rows - 1);
-                u[q] = ns_read(m.in, r * m.ld_in + c, p.in_dtype, n);
-                if (m.momentum) next[q] = ns_read((const uint8_t *)m.momentum, r * m.ld_momentum + c, TFTQ_F32, n);
+                u[q] = whole ? ns_read4<DTYPE>(m.in, r * m.ld_in + c) : ns_read(m.in, r * m.ld_in + c, DTYPE, n);
+                if (MOMENTUM)
+                    next[q] = whole ? ns_read4<TFTQ_F32>((const uint8_t *)m.momentum, r * m.ld_momentum + c)
+                                    : ns_read((const uint8_t *)m.momentum, r * m.ld_momentum + c, TFTQ_F32, n);
             }
 #pragma unroll
             for (int q = 0; q < AT_ONCE; q++) {
                 const int64_t r = r0 + q * apart;
                 if (r >= row0 + rows) continue;
-                if (m.momentum) {
+                if (MOMENTUM) {
                     float *at = m.momentum + r * m.ld_momentum + c;
 #pragma unroll
                     for (int i = 0; i < 4; i++) next[q][i] = ns_momentum(next[q][i], u[q][i], p), u[q][i] = ns_update(next[q][i], u[q][i], p);
-                    if (n >= 4) {
+                    if (whole) {
                         *(ns_f4_any *)at = next[q];
                     } else {
 #pragma unroll
@@ -212,6 +223,11 @@ __global__ __launch_bounds__(256) void k_ns_squares(int count, int precise, cons
                 for (int i = 0; i < 4; i++) sum += (double)u[q][i] * (double)u[q][i];
             }
         }
+    };
+    if ((int)threadIdx.x < groups * apart) {
+        if (n >= 4) add(std::true_type());
+        else add(std::false_type());
+    }
     for (int s = 32; s; s >>= 1) sum += __shfl_xor(sum, s);
     if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum;
     __syncthreads();
@@ -234,7 +250,8 @@ __device__ static inline void ns_split(float v, float scale, _Float16 *high, _Fl
 }
 
 // X and X^T in panels from u / |u|, a square of 64 per workgroup, turned in LDS.  Bound by memory: 4096x14336 bf16
-// 107 us (470 MB, 4.4 TB/s).
+// 100 us (470 MB, 4.7 TB/s).
+template <int DTYPE, bool MOMENTUM>
 __global__ __launch_bounds__(256) void k_ns_start(int count, int precise, const NsLaunch l, const NsParams p)
 {
     __shared__ float tile[64][65];
@@ -245,6 +262,28 @@ __global__ __launch_bounds__(256) void k_ns_start(int count, int precise, const 
     const int across = (m.cols + 63) / 64;
     const int row0 = piece / across * 64, col0 = piece % across * 64;
     const int high = m.flip ? m.cols : m.rows, wide = m.flip ? m.rows : m.cols;
+    // read along the rows of the matrix as it lies, on the way while the norm is added up
+    const int at_row = m.flip ? col0 : row0, at_col = m.flip ? row0 : col0;
+    const bool inside = at_row + 64 <= high && at_col + 64 <= wide;
+    tile_f4 v[4] = {}, old[4] = {};
+    if (inside) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int64_t row = at_row + ((int)threadIdx.x >> 4) + 16 * k;
+            const int col = at_col + ((int)threadIdx.x & 15) * 4;
+            v[k] = ns_read4<DTYPE>(m.in, row * m.ld_in + col);
+            if (MOMENTUM) old[k] = ns_read4<TFTQ_F32>((const uint8_t *)m.momentum, row * m.ld_momentum + col);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int64_t row = at_row + ((int)threadIdx.x >> 4) + 16 * k;
+            const int col = at_col + ((int)threadIdx.x & 15) * 4;
+            if (row >= high || col >= wide) continue;
+            v[k] = ns_read(m.in, row * m.ld_in + col, DTYPE, wide - col);
+            if (MOMENTUM) old[k] = ns_read((const uint8_t *)m.momentum, row * m.ld_momentum + col, TFTQ_F32, wide - col);
+        }
+    }
     const int parts = (int)ns_parts_of(high, wide);
     double sum = 0;
     for (int i = threadIdx.x; i < parts; i += 256) sum += w.squares[i];
@@ -258,23 +297,13 @@ __global__ __launch_bounds__(256) void k_ns_start(int count, int precise, const 
     if (piece == 0)
         for (int i = threadIdx.x; i < NS_SHARED / 2; i += 256) w.tickets[i] = 0;
 
-    // read along the rows of the matrix as it lies
-    const int at_row = m.flip ? col0 : row0, at_col = m.flip ? row0 : col0;
-    for (int q = threadIdx.x; q < 64 * 16; q += 256) {
-        const int r = q >> 4, c = (q & 15) * 4, n = wide - at_col - c;
-        tile_f4 v = {0.f, 0.f, 0.f, 0.f};
-        if (at_row + r < high && n > 0) {
-            const int64_t row = at_row + r;
-            v = ns_read(m.in, row * m.ld_in + at_col + c, p.in_dtype, n);
-            if (m.momentum) {
-                const tile_f4 old = ns_read((const uint8_t *)m.momentum, row * m.ld_momentum + at_col + c, TFTQ_F32, n);
 #pragma unroll
-                for (int i = 0; i < 4; i++) v[i] = ns_update(old[i], v[i], p);
-            }
-        }
+    for (int k = 0; k < 4; k++) {
+        const int r = ((int)threadIdx.x >> 4) + 16 * k, c = ((int)threadIdx.x & 15) * 4;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float x = i < n ? (float)(v[i] * by) : 0.f;
+            const float u = MOMENTUM ? ns_update(old[k][i], v[k][i], p) : v[k][i];
+            const float x = inside || (at_row + r < high && at_col + c + i < wide) ? (float)(u * by) : 0.f;
             if (m.flip) tile[c + i][r] = x;
             else tile[r][c + i] = x;
         }
@@ -956,6 +985,11 @@ extern "C" int64_t tftq_newton_schulz_workspace(int n, const int64_t *shapes, in
     return rc ? rc : most;
 }
 
+template <int DTYPE>
+static const void *ns_first(bool momentum) { return momentum ? (const void *)k_ns_squares<DTYPE, true> : (const void *)k_ns_squares<DTYPE, false>; }
+template <int DTYPE>
+static const void *ns_second(bool momentum) { return momentum ? (const void *)k_ns_start<DTYPE, true> : (const void *)k_ns_start<DTYPE, false>; }
+
 static bool ns_dtype_ok(int d) { return d == TFTQ_F32 || d == TFTQ_F16 || d == TFTQ_BF16; }
 
 extern "C" int tftq_newton_schulz(const tftq_ns *what, void *workspace, int64_t workspace_bytes, int device, void *stream)
@@ -1000,14 +1034,21 @@ extern "C" int tftq_newton_schulz(const tftq_ns *what, void *workspace, int64_t 
         }
         float growth = 1.f;
         for (int it = 0; it < s.iterations; it++) growth *= fmaxf(1.f, fabsf(s.coefficients[3 * it]));
-        NsParams p = {s.momentum, s.keep, 0, 0, 0, s.eps, growth, s.nesterov, s.in_dtype, s.out_dtype, s.steps != nullptr, 0, 0};
+        NsParams p = {s.momentum, s.keep, 0, 0, 0, s.eps, growth, s.nesterov, s.out_dtype, s.steps != nullptr, 0, 0};
+        const bool with = s.momenta != nullptr;
+        const void *squares, *start;
+        switch (s.in_dtype) {
+        case TFTQ_F32: squares = ns_first<TFTQ_F32>(with), start = ns_second<TFTQ_F32>(with); break;
+        case TFTQ_F16: squares = ns_first<TFTQ_F16>(with), start = ns_second<TFTQ_F16>(with); break;
+        default: squares = ns_first<TFTQ_BF16>(with), start = ns_second<TFTQ_BF16>(with); break;
+        }
         int rc = launch_over(l, [](const NsMatrix &m) {
             const int64_t high = m.flip ? m.cols : m.rows, wide = m.flip ? m.rows : m.cols;
             return ns_parts_of(high, wide);
-        }, false, (const void *)k_ns_squares, 256, p, precise, st);
+        }, false, squares, 256, p, precise, st);
         if (rc) return rc;
-        rc = launch_over(l, [](const NsMatrix &m) { return (int64_t)((m.rows + 63) / 64) * ((m.cols + 63) / 64); }, false,
-                         (const void *)k_ns_start, 256, p, precise, st);
+        rc = launch_over(l, [](const NsMatrix &m) { return (int64_t)((m.rows + 63) / 64) * ((m.cols + 63) / 64); }, false, start, 256,
+                         p, precise, st);
         if (rc) return rc;
         for (int it = 0; it < s.iterations; it++) {
             p.a = s.coefficients[3 * it], p.b = s.coefficients[3 * it + 1], p.c = s.coefficients[3 * it + 2];
