@@ -173,6 +173,28 @@ class Muon(torch.optim.Optimizer):
         for group in self.param_groups:
             assert all(p.dim() == 2 for p in group["params"]), "Only 2D tensors are supported"
 
+    def load_state_dict(self, state_dict) -> None:
+        """As ``torch.optim.Optimizer.load_state_dict``, which brings floating-point state to the type of its
+        weight; the momenta stay the float32 numbers that were saved."""
+        saved: dict = {}
+
+        def before(_, state):  # after the caller's own hooks, which may have replaced the state
+            saved.update(state)
+
+        def after(_):  # before the caller's own
+            ids = (i for group in saved["param_groups"] for i in group["params"])
+            params = (p for group in self.param_groups for p in group["params"])
+            for i, p in zip(ids, params):
+                if "momentum" in saved["state"].get(i, ()):
+                    self.state[p]["momentum"] = saved["state"][i]["momentum"].to(device=p.device, dtype=torch.float32)
+
+        hooks = self.register_load_state_dict_pre_hook(before), self.register_load_state_dict_post_hook(after, prepend=True)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
