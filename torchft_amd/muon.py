@@ -65,6 +65,10 @@ def _check_list(name: str, tensors: list, device: torch.device, dtype: torch.dty
         assert [tuple(t.shape) for t in tensors] == shapes, f"The {name} have other shapes than the first list"
 
 
+def _check_options(lr: float, weight_decay: float, momentum: float) -> None:
+    assert lr >= 0 and weight_decay >= 0 and 0 <= momentum < 1, "lr, weight_decay or momentum is out of range"
+
+
 def _run(outs: list, ins: list, momenta: "list | None", steps_sizes: "list | None", keep: float, momentum: float,
          nesterov: bool, iterations: int, coefficients, eps: float, precise: "bool | None") -> None:
     """out = X, or keep * out - step * X, for every matrix; all lists checked."""
@@ -146,7 +150,7 @@ def muon_(weights: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], moment
     :func:`orthogonalize`, by the type of the weights."""
     weights, grads, momenta = list(weights), list(grads), list(momenta)
     assert len(weights) == len(grads) == len(momenta), "The lists are of different lengths"
-    assert lr >= 0 and weight_decay >= 0 and 0 <= momentum < 1, "lr, weight_decay or momentum is out of range"
+    _check_options(lr, weight_decay, momentum)
     if not weights:
         return
     first = weights[0]
@@ -167,11 +171,19 @@ class Muon(torch.optim.Optimizer):
     def __init__(self, params: Iterable, lr: float = 0.02, weight_decay: float = 0.0, momentum: float = 0.95,
                  nesterov: bool = True, steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-7,
                  precise: "bool | None" = None) -> None:
-        assert lr >= 0 and weight_decay >= 0 and 0 <= momentum < 1, "lr, weight_decay or momentum is out of range"
+        _check_options(lr, weight_decay, momentum)
         super().__init__(params, dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=nesterov, steps=steps,
                                       coefficients=coefficients, eps=eps, precise=precise))
-        for group in self.param_groups:
+
+    def add_param_group(self, param_group) -> None:
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        try:
             assert all(p.dim() == 2 for p in group["params"]), "Only 2D tensors are supported"
+            _check_options(group["lr"], group["weight_decay"], group["momentum"])
+        except AssertionError:
+            self.param_groups.pop()
+            raise
 
     def load_state_dict(self, state_dict) -> None:
         """As ``torch.optim.Optimizer.load_state_dict``, which brings floating-point state to the type of its
