@@ -473,7 +473,8 @@ struct Matrix {
         if (!THPVariable_CheckExact(o)) return false;  // a tensor or a parameter
         const at::Tensor &t = THPVariable_Unpack(o);
         if (!t.defined() || t.key_set().has_any(WRAPPERS) ||
-            t.layout() != at::kStrided || !t.device().is_cuda() || t.dim() != 2 || t.is_neg())
+            t.layout() != at::kStrided || !t.device().is_cuda() || t.dim() != 2 || t.is_neg() ||
+            t._fw_grad(0).defined())  // a tangent goes along with it: Python says no
             return false;
         type = t.scalar_type();
         dtype = type == at::kFloat ? 0 : type == at::kHalf ? 1 : type == at::kBFloat16 ? 2 : -1;

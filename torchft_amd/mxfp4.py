@@ -22,6 +22,7 @@ import ctypes
 import threading
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -304,7 +305,7 @@ def linear_mxfp4(x: torch.Tensor, weight: "torch.Tensor | MXFP4Tensor") -> torch
     With a weight that is a tensor both gradients are available:
     ``dx = dy @ weight`` and ``dw = dy.T @ x`` with every operand quantised along the contracted axis.
     A weight that is kept in 4 bits along ``k`` cannot be contracted along ``n``: gradients through it are
-    refused."""
+    refused.  So are tangents (forward mode), whatever the weight."""
     if _native is not None and type(weight) is MXFP4Tensor and not (x.requires_grad and torch.is_grad_enabled()):
         out = _native.mx_linear(x, weight.buffer, *weight.shape)
         if out is not None:
@@ -315,7 +316,8 @@ def linear_mxfp4(x: torch.Tensor, weight: "torch.Tensor | MXFP4Tensor") -> torch
     assert x.device == weight.device, "All inputs must be on the same device"
     flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1]) if x.numel() else x.new_empty(x.shape[:-1].numel(), x.shape[-1])
     if isinstance(weight, MXFP4Tensor):
-        assert not (torch.is_grad_enabled() and x.requires_grad), "A weight in 4 bits has no gradient product"
+        assert not (torch.is_grad_enabled() and x.requires_grad or forward_ad.unpack_dual(x).tangent is not None), \
+            "A weight in 4 bits has no gradient product"
         y = _linear_rows(flat.detach(), weight, x.dtype)
     else:
         assert weight.dtype in _DTYPE_CODE, "Only fp32, fp16 and bf16 are supported"
