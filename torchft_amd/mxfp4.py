@@ -272,6 +272,11 @@ def _linear_rows(x: torch.Tensor, weight: MXFP4Tensor, dtype: torch.dtype) -> to
     return out
 
 
+def _has_tangent(t: torch.Tensor) -> bool:
+    """Whether forward-mode differentiation follows ``t``, with grad mode or without."""
+    return forward_ad.unpack_dual(t).tangent is not None
+
+
 class _Linear(torch.autograd.Function):
     """``x @ w.T`` of matrices; what the backward pass contracts along other axes is quantised along
     them while the forward pass reads x and w, and kept in place of x and w: 4.25 bits an element."""
@@ -316,10 +321,13 @@ def linear_mxfp4(x: torch.Tensor, weight: "torch.Tensor | MXFP4Tensor") -> torch
     assert x.device == weight.device, "All inputs must be on the same device"
     flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1]) if x.numel() else x.new_empty(x.shape[:-1].numel(), x.shape[-1])
     if isinstance(weight, MXFP4Tensor):
-        assert not (torch.is_grad_enabled() and x.requires_grad or forward_ad.unpack_dual(x).tangent is not None), \
+        assert not (torch.is_grad_enabled() and x.requires_grad or _has_tangent(x)), \
             "A weight in 4 bits has no gradient product"
         y = _linear_rows(flat.detach(), weight, x.dtype)
     else:
         assert weight.dtype in _DTYPE_CODE, "Only fp32, fp16 and bf16 are supported"
-        y = _Linear.apply(flat, weight)
+        if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad) or _has_tangent(x) or _has_tangent(weight):
+            y = _Linear.apply(flat, weight)
+        else:
+            y = _linear_rows(flat.detach(), _quantize(weight, True, False)[0], x.dtype)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], weight.shape[0])
