@@ -279,23 +279,22 @@ def _has_tangent(t: torch.Tensor) -> bool:
 
 class _Linear(torch.autograd.Function):
     """``x @ w.T`` of matrices; what the backward pass contracts along other axes is quantised along
-    them while the forward pass reads x and w, and kept in place of x and w: 4.25 bits an element."""
+    them while the forward pass reads x and w, and saved in place of x and w: 4.25 bits an element."""
 
     @staticmethod
     def forward(ctx, x, w):
-        for_dw, for_dx = ctx.needs_input_grad[1], ctx.needs_input_grad[0]
-        ctx.dtypes = x.dtype, w.dtype
-        ctx.x_columns = None
-        w_rows, ctx.w_columns = _quantize(w, True, for_dx)
-        if not for_dw:
-            return _linear_rows(x.detach(), w_rows, x.dtype)
-        x_rows, ctx.x_columns = _quantize(x, True, True)
-        return matmul_mxfp4(x_rows, w_rows, x.dtype)
+        for_dx, for_dw = ctx.needs_input_grad
+        ctx.dtypes, ctx.shapes = (x.dtype, w.dtype), (x.shape, w.shape)
+        w_rows, w_columns = _quantize(w, True, for_dx)
+        x_rows, x_columns = _quantize(x, True, True) if for_dw else (None, None)
+        ctx.save_for_backward(x_columns.buffer if for_dw else None, w_columns.buffer if for_dx else None)
+        return matmul_mxfp4(x_rows, w_rows, x.dtype) if for_dw else _linear_rows(x.detach(), w_rows, x.dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x_columns, w_columns = ctx.x_columns, ctx.w_columns
+        x_columns, w_columns = (buffer if buffer is None else MXFP4Tensor(buffer, (shape[1], shape[0]), dtype)
+                                for buffer, shape, dtype in zip(ctx.saved_tensors, ctx.shapes, ctx.dtypes))
         dy_rows, dy_columns = _quantize(dy, w_columns is not None, x_columns is not None)
         dx = matmul_mxfp4(dy_rows, w_columns, ctx.dtypes[0]) if w_columns is not None else None
         dw = matmul_mxfp4(dy_columns, x_columns, ctx.dtypes[1]) if x_columns is not None else None
