@@ -220,7 +220,8 @@ int tftq_reduce_static(const tftq_plan *plan, void *packed, int64_t packed_bytes
  *    codes   [P][rows][128]            columns 256 p to 256 p + 255 of every row, zero past the last one
  *    scales  [P][rows rounded up to an even number][8]   of those columns' blocks
  */
-/* bytes of a matrix, or TFTQ_E_SHAPE */
+/* bytes of a matrix, or TFTQ_E_SHAPE: rows and columns are at most 2^31 - 1024, here and below, and
+ * nothing else but memory bounds a matrix */
 int64_t tftq_mx_bytes(int64_t rows, int64_t cols);
 
 /*
@@ -260,7 +261,7 @@ int tftq_mx_linear(int dtype, const void *x, int64_t m, int64_t row_stride, cons
  */
 typedef struct tftq_ns {
     int n;                          /* matrices; empty ones are left alone */
-    const int64_t *shapes;          /* [n][2] rows, columns: at most 2^24 each, 2^35 elements */
+    const int64_t *shapes;          /* [n][2] rows, columns: at most 2^24 each, 2^35 elements with either rounded up to 64 */
     const void *const *in;          /* gradients; columns contiguous */
     const int64_t *in_stride;       /* [n] elements from row to row */
     int in_dtype;

@@ -32,14 +32,14 @@ __device__ static inline uint32_t mx_over_block(uint32_t m)
 // wavefronts to a SIMD.
 template <class T, bool BY_ROWS, bool BY_COLS, int P>
 __global__ __launch_bounds__(64, 2) void k_mx_quantize(const uint8_t *x, int64_t ld, int rows, int cols, int tiles_c,
-                                                       MxMatrix by_rows, MxMatrix by_cols)
+                                                       int row0, MxMatrix by_rows, MxMatrix by_cols)
 {
     constexpr int V = T::V, ACROSS = 128 / V, GROUPS = 64 / ACROSS;
     static_assert(!BY_COLS || P == 32, "");
     const int piece = tile_piece(blockIdx.x, gridDim.x);
     const int lane = threadIdx.x;
     const int col = piece % tiles_c * 128 + lane % ACROSS * V;
-    const int row = (piece / tiles_c * GROUPS + lane / ACROSS) * P;
+    const int row = row0 + (piece / tiles_c * GROUPS + lane / ACROSS) * P;
 
     mx_u4 raw[P];
     const uint8_t *at = x + ((int64_t)row * ld + col) * T::SIZE;
@@ -128,11 +128,11 @@ __global__ __launch_bounds__(64, 2) void k_mx_quantize(const uint8_t *x, int64_t
 // A lane turns V neighbouring codes into a vector of 16 bytes; codes are read in the order in which they lie.
 // Bound by its stores: 14336x4096 to bf16 24 us (149 MB, 6.2 TB/s).
 template <int DTYPE>
-__global__ __launch_bounds__(256) void k_mx_dequantize(MxMatrix m, int rows, int cols, uint8_t *out, int64_t ld)
+__global__ __launch_bounds__(256) void k_mx_dequantize(MxMatrix m, int rows, int cols, uint8_t *out, int64_t ld, int64_t first_group)
 {
     constexpr int SIZE = DTYPE == TFTQ_F32 ? 4 : 2, V = 16 / SIZE, PER_ROW = 256 / V;
     const int64_t pieces = (int64_t)((cols + 255) >> 8) * rows * PER_ROW;
-    const int64_t first = (int64_t)blockIdx.x * 1024 + threadIdx.x;
+    const int64_t first = (first_group + blockIdx.x) * 1024 + threadIdx.x;
 #pragma unroll
     for (int q = 0; q < 4; q++) {
         const int64_t piece = first + 256 * q;
@@ -185,18 +185,21 @@ static int quantize(const void *x, int64_t ld, int rows, int cols, const MxMatri
     constexpr int GROUPS = 64 / (128 / T::V);
     const int per_lane = c.panels ? 32 : 4;
     // every column of the last panel, and with columns every row of their last panel, is written
-    const int64_t tiles_c = mx_panels(cols) * 2;
-    const int64_t high = c.panels ? mx_panels(rows) * 256 : rows;
-    const int64_t tiles = tiles_c * ((high + GROUPS * per_lane - 1) / (GROUPS * per_lane));
-    if (tiles > (1 << 25)) return TFTQ_E_SHAPE;
-    const dim3 grid((unsigned)tiles), block(64);
+    int tc = (int)(mx_panels(cols) * 2);
+    const int64_t high = c.panels ? mx_panels(rows) * 256 : rows, each = GROUPS * per_lane, tiles_r = (high + each - 1) / each;
     const uint8_t *px = (const uint8_t *)x;
-    int tc = (int)tiles_c;
-    void *args[] = {(void *)&px, (void *)&ld, (void *)&rows, (void *)&cols, (void *)&tc, (void *)&r, (void *)&c};
     const void *k = !c.panels ? (const void *)k_mx_quantize<T, true, false, 4>
                     : r.panels ? (const void *)k_mx_quantize<T, true, true, 32>
                                : (const void *)k_mx_quantize<T, false, true, 32>;
-    return (int)hipLaunchKernel(k, grid, block, args, 0, st);
+    // 2^31 threads of a launch at most; a row has fewer than 2^24 tiles
+    const int64_t at_once = (1 << 25) / tc;
+    for (int64_t t = 0; t < tiles_r; t += at_once) {
+        int row0 = (int)(t * each);
+        void *args[] = {(void *)&px, (void *)&ld, (void *)&rows, (void *)&cols, (void *)&tc, (void *)&row0, (void *)&r, (void *)&c};
+        const dim3 grid((unsigned)(std::min(at_once, tiles_r - t) * tc)), block(64);
+        if (const int rc = (int)hipLaunchKernel(k, grid, block, args, 0, st)) return rc;
+    }
+    return 0;
 }
 
 extern "C" int tftq_mx_quantize(int dtype, const void *x, int64_t rows, int64_t cols, int64_t row_stride, void *by_rows,
@@ -227,14 +230,18 @@ extern "C" int tftq_mx_dequantize(int dtype, const void *matrix, int64_t rows, i
     if (rows == 0 || cols == 0) return 0;
     if (!matrix || !out || ((uintptr_t)matrix & 15) || row_stride < (rows > 1 ? cols : 0)) return TFTQ_E_ARG;
     const int64_t groups = (mx_panels(cols) * rows * (dtype == TFTQ_F32 ? 64 : 32) + 1023) / 1024;
-    if (groups > (1 << 23)) return TFTQ_E_SHAPE;
     DeviceScope scope(device);
     if (scope.err != hipSuccess) return (int)scope.err;
     MxMatrix m = mx_matrix((void *)matrix, rows, cols);
     int r = (int)rows, c = (int)cols;
-    void *args[] = {(void *)&m, (void *)&r, (void *)&c, (void *)&out, (void *)&row_stride};
+    constexpr int64_t AT_ONCE = 1 << 23;  // 2^31 threads
+    int64_t first = 0;
+    void *args[] = {(void *)&m, (void *)&r, (void *)&c, (void *)&out, (void *)&row_stride, (void *)&first};
     const void *k = dtype == TFTQ_F32 ? (const void *)k_mx_dequantize<TFTQ_F32>
                     : dtype == TFTQ_F16 ? (const void *)k_mx_dequantize<TFTQ_F16>
                                         : (const void *)k_mx_dequantize<TFTQ_BF16>;
-    return (int)hipLaunchKernel(k, dim3((unsigned)groups), dim3(256), args, 0, (hipStream_t)stream);
+    for (; first < groups; first += AT_ONCE)
+        if (const int rc = (int)hipLaunchKernel(k, dim3((unsigned)std::min(AT_ONCE, groups - first)), dim3(256), args, 0, (hipStream_t)stream))
+            return rc;
+    return 0;
 }

@@ -1,5 +1,6 @@
 // The product of two 4-bit microscaled matrices, c[i][j] = sum_k a[i][k] b[j][k], and its C entry.
 #include <hip/hip_runtime.h>
+#include <limits.h>
 #include <stdint.h>
 
 #include "tftq_mxfp4.h"
@@ -199,7 +200,7 @@ template <class T>
 static int product(int dtype, const TileOperand &a, const TileOperand &b, int panels, uint8_t *out, int64_t ld, hipStream_t st)
 {
     int tiles_m = (a.rows + T::ROWS - 1) / T::ROWS, tiles_n = (b.rows + T::COLS - 1) / T::COLS;
-    if ((int64_t)tiles_m * tiles_n > (1 << 22)) return TFTQ_E_SHAPE;
+    if ((int64_t)tiles_m * tiles_n > INT_MAX) return TFTQ_E_SHAPE;  // 8.8e12 results or more
     void *args[] = {(void *)&a, (void *)&b, (void *)&panels, (void *)&out, (void *)&ld, (void *)&tiles_m, (void *)&tiles_n};
     const void *k = dtype == TFTQ_F32 ? (const void *)k_mx_product<T, TFTQ_F32>
                     : dtype == TFTQ_F16 ? (const void *)k_mx_product<T, TFTQ_F16>
