@@ -280,7 +280,8 @@ typedef struct tftq_ns {
     int precise;
 } tftq_ns;
 
-/* bytes that tftq_newton_schulz needs for these matrices, or TFTQ_E_ARG / TFTQ_E_SHAPE */
+/* bytes that tftq_newton_schulz needs for these matrices, or TFTQ_E_ARG / TFTQ_E_SHAPE: those of the up to 24 that
+ * are worked on at once (8 to 12 bytes an element, 12 to 20 with `precise`; a caller who has less passes a shorter list) */
 int64_t tftq_newton_schulz_workspace(int n, const int64_t *shapes, int precise);
 
 /*

@@ -14,10 +14,11 @@ and takes that as the step:
 
 Products run on the 16-bit matrix cores with float32 sums.  bfloat16 results take one product each,
 with the diagonals and the remainders of the iterates kept apart, so that the result is off by less than
-its own rounding; float32 and float16 results, and matrices with a side of fewer than 64, take three, of
-high and low parts, with the accuracy of float32 products.
+its own rounding; float32 and float16 results, and matrices with a side of fewer than 64 (with the
+small ones beside them in a list), take three, of high and low parts, with the accuracy of float32 products.
 The whole list is worked on at once, 24 matrices to a launch: about 17 launches whatever their number.
-The workspace comes from torch's allocator for the length of the call.
+The workspace comes from torch's allocator for the length of the call: 8 to 12 bytes an element, 12 to 20 with
+three products, and 8 GiB at most for matrices that do not need more each (larger lists are taken in runs).
 """
 
 from __future__ import annotations
@@ -69,6 +70,33 @@ def _check_options(lr: float, weight_decay: float, momentum: float) -> None:
     assert lr >= 0 and weight_decay >= 0 and 0 <= momentum < 1, "lr, weight_decay or momentum is out of range"
 
 
+# Bytes of workspace that a call takes for several matrices together; what needs more by itself is taken alone.
+# So many fill the GPU many times over: 24 of 4096x14336 in bf16, 12.9 GB in one call, take 94.8 ms so, 94.7 in runs of
+# 8 GiB, 96.0 of 4, 102.6 of 1; 48 of 2048x5632 24.0, 24.0, 24.0, 27.0.
+_WORKSPACE = 8 << 30
+
+
+def _parts(lib, n: int, shapes, precise: bool) -> "list[tuple[int, int]]":
+    """The list in runs of matrices whose workspaces, one beside the other, stay within ``_WORKSPACE``."""
+    parts, first, held = [], 0, 0
+    for i in range(n):
+        size = lib.tftq_newton_schulz_workspace(1, _from(shapes, 2 * i), precise)
+        if size < 0:
+            _check(size, "tftq_newton_schulz_workspace")
+        if i > first and held + size > _WORKSPACE:
+            parts.append((first, i))
+            first, held = i, 0
+        held += size
+    return parts + [(first, n)]
+
+
+def _from(array, first: int):
+    """A C array from its element ``first`` on."""
+    if first == 0:
+        return array
+    return ctypes.cast(ctypes.addressof(array) + first * ctypes.sizeof(array._type_), ctypes.POINTER(array._type_))
+
+
 def _run(outs: list, ins: list, momenta: "list | None", steps_sizes: "list | None", keep: float, momentum: float,
          nesterov: bool, iterations: int, coefficients, eps: float, precise: "bool | None") -> None:
     """out = X, or keep * out - step * X, for every matrix; all lists checked."""
@@ -102,17 +130,23 @@ def _run(outs: list, ins: list, momenta: "list | None", steps_sizes: "list | Non
             strides[k][i] = t.stride(0) if t.shape[0] > 1 else t.shape[1]
     lib = _lib.load()
     size = lib.tftq_newton_schulz_workspace(n, shapes, precise)
-    if size < 0:
-        _check(size, "tftq_newton_schulz_workspace")
-    workspace = torch.empty(size, dtype=torch.uint8, device=device)
-    what = _lib.NewtonSchulz(
-        n=n, shapes=shapes, inputs=pointers[1], in_stride=strides[1], in_dtype=_DTYPE_CODE[ins[0].dtype],
-        momenta=pointers[2] if momenta is not None else None, momenta_stride=strides[2] if momenta is not None else None,
-        momentum=momentum, nesterov=nesterov, out=pointers[0], out_stride=strides[0], out_dtype=_DTYPE_CODE[out_dtype],
-        steps=(ctypes.c_float * n)(*steps_sizes) if steps_sizes is not None else None, keep=keep,
-        iterations=iterations, coefficients=coefficients, eps=eps, precise=precise)
-    _check(lib.tftq_newton_schulz(ctypes.byref(what), workspace.data_ptr(), size, device.index, _stream_of(device)),
-           "tftq_newton_schulz")
+    parts = [(0, n)] if size <= _WORKSPACE else _parts(lib, n, shapes, precise)
+    for first, last in parts:
+        if len(parts) > 1:
+            size = lib.tftq_newton_schulz_workspace(last - first, _from(shapes, 2 * first), precise)
+        if size < 0:
+            _check(size, "tftq_newton_schulz_workspace")
+        workspace = torch.empty(size, dtype=torch.uint8, device=device)
+        what = _lib.NewtonSchulz(
+            n=last - first, shapes=_from(shapes, 2 * first), inputs=_from(pointers[1], first), in_stride=_from(strides[1], first),
+            in_dtype=_DTYPE_CODE[ins[0].dtype], momenta=_from(pointers[2], first) if momenta is not None else None,
+            momenta_stride=_from(strides[2], first) if momenta is not None else None, momentum=momentum, nesterov=nesterov,
+            out=_from(pointers[0], first), out_stride=_from(strides[0], first), out_dtype=_DTYPE_CODE[out_dtype],
+            steps=(ctypes.c_float * (last - first))(*steps_sizes[first:last]) if steps_sizes is not None else None, keep=keep,
+            iterations=iterations, coefficients=coefficients, eps=eps, precise=precise)
+        _check(lib.tftq_newton_schulz(ctypes.byref(what), workspace.data_ptr(), size, device.index, _stream_of(device)),
+               "tftq_newton_schulz")
+        del workspace  # the next part's may take its place: the stream runs them one after the other
     for t, copy in after:
         t.copy_(copy)
 
