@@ -30,6 +30,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <initializer_list>
 
 #include "tftq_device.h"
 #include "tftq_tile.h"
@@ -38,7 +39,8 @@ typedef _Float16 ns_h8 __attribute__((ext_vector_type(8)));
 
 constexpr int NS_MOST = 24;            // matrices of a launch: their descriptors travel in its arguments
 constexpr int64_t NS_LONGEST = 1 << 24;  // rows or columns
-// |X| <= ~1.2, |A| <= ~1.5, |B| <= ~3 with the usual coefficients; others may pass these a few times over.
+// What X, E and G are scaled by at most: |X| <= ~1.2, |A| <= ~1.5, |B| <= ~3 with the usual coefficients, and fp16
+// ends at 65504.  Of others the bounds of every iteration say how much less (NsScales).
 // X of a gradient so small that eps divides it stays small: its scale is larger by a power of two (ns_scale).
 constexpr float SCALE_X = 16384.f, SCALE_E = 4096.f, SCALE_G = 2048.f;
 constexpr int NORM_COLS = 1024;
@@ -75,6 +77,9 @@ struct NsParams {
     float momentum, keep, a, b, c, eps, growth;
     int nesterov, out_dtype, update;
     int last, next_last;  // the last iteration, the one before it
+    // of this iteration (NsScales): X's scale in that of the first one, the next one's in this one's; E's; and
+    // what the sums of A A, E and the sums of G X are multiplied by for G and X
+    float x, x_next, e, per_ee, aa_to_g, c_to_g, b_to_g, gx_to_x;
 };
 static_assert(sizeof(NsLaunch) + sizeof(NsParams) <= 3800, "kernel arguments");
 
@@ -390,7 +395,7 @@ struct NsFinish {
     float *d, *f;
     uint8_t *out, *out_l, *turned, *turned_l;  // panels along the result's rows, and along its columns
     float per_x;                               // one over X's scale, a power of two
-    float a, b, c;
+    float a, b, c, e, per_ee, aa_to_g, c_to_g, b_to_g, gx_to_x, x_next;
     int r, cols, padded, last, next_last, flip;
     bool mirror;
 
@@ -401,7 +406,8 @@ struct NsFinish {
         d = w.d, f = w.f, a = p.a, b = p.b, c = p.c, last = p.last, next_last = p.next_last, flip = m.flip;
         out = WHAT == NS_A ? w.e : WHAT == NS_B ? w.g : w.x, out_l = WHAT == NS_A ? w.el : WHAT == NS_B ? w.gl : w.xl;
         turned = WHAT != NS_X ? out : turn ? w.t : w.t2, turned_l = WHAT != NS_X ? out_l : turn ? w.tl : w.tl2;
-        per_x = 1.f / *w.scale;
+        per_x = 1.f / (*w.scale * p.x);
+        e = p.e, per_ee = p.per_ee, aa_to_g = p.aa_to_g, c_to_g = p.c_to_g, b_to_g = p.b_to_g, gx_to_x = p.gx_to_x, x_next = p.x_next;
         r = m.rows, cols = WHAT == NS_X ? m.cols : m.rows, padded = (cols + 63) & ~63;
         mirror = WHAT == NS_X ? !last || flip : !diagonal;
     }
@@ -418,7 +424,7 @@ struct NsFinish {
         if (WHAT == NS_A || i >= r || j >= padded) return o;
         o.high = *(const ns_h8 *)(old_high + at(i, j));
         if (PRECISE || (LOW && !last)) o.low = *(const ns_h8 *)(old_low + at(i, j));
-        o.di = WHAT == NS_B ? d[i] : a + f[i];
+        o.di = WHAT == NS_B ? d[i] : (a + f[i]) * x_next;
         return o;
     }
     // v: the sums of row i, columns j to j + 7, and then their values as numbers (of the last iteration)
@@ -432,26 +438,25 @@ struct NsFinish {
                 for (int n = 0; n < 8; n++)
                     if (i == j + n) d[i] = v[n] * per_x * per_x;
             }
-            const float by = per_x * per_x * SCALE_E;
+            const float by = per_x * per_x * e;
 #pragma unroll
             for (int n = 0; n < 8; n++) v[n] *= by;
         } else if (WHAT == NS_B) {
-            const float by = c * (SCALE_G / (SCALE_E * SCALE_E)), ce = c * (SCALE_G / SCALE_E), be = b * (SCALE_G / SCALE_E);
             if ((unsigned)(i - j) < 8u && i < r) {
 #pragma unroll
                 for (int n = 0; n < 8; n++)
-                    if (i == j + n) f[i] = b * was.di + c * (v[n] * (1.f / (SCALE_E * SCALE_E)) + was.di * was.di);
+                    if (i == j + n) f[i] = b * was.di + c * (v[n] * per_ee + was.di * was.di);
             }
             tile_f4 dj[2] = {};
             if (inside) dj[0] = *(const tile_f4 *)(d + j), dj[1] = *(const tile_f4 *)(d + j + 4);
 #pragma unroll
             for (int n = 0; n < 8; n++) {
                 const float x = PRECISE ? (float)was.high[n] + (float)was.low[n] : (float)was.high[n];
-                v[n] = fmaf(x, fmaf(ce, was.di + dj[n / 4][n % 4], be), v[n] * by);
+                v[n] = fmaf(x, fmaf(c_to_g, was.di + dj[n / 4][n % 4], b_to_g), v[n] * aa_to_g);
             }
         } else {
 #pragma unroll
-            for (int n = 0; n < 8; n++) v[n] = fmaf(was.di, (float)was.high[n], fmaf(was.di, (float)was.low[n], v[n] * (1.f / SCALE_G)));
+            for (int n = 0; n < 8; n++) v[n] = fmaf(was.di, (float)was.high[n], fmaf(was.di, (float)was.low[n], v[n] * gx_to_x));
         }
         if (!(i < r && j + 8 <= cols)) {  // zeros past the last row and column
 #pragma unroll
@@ -990,6 +995,43 @@ static const void *ns_first(bool momentum) { return momentum ? (const void *)k_n
 template <int DTYPE>
 static const void *ns_second(bool momentum) { return momentum ? (const void *)k_ns_start<DTYPE, true> : (const void *)k_ns_start<DTYPE, false>; }
 
+// The scales of every iteration, powers of two.  X starts with singular values of at most 1 (its norm); an iteration
+// takes each of them, x, to a x + b x^3 + c x^5, and A and B have eigenvalues x^2 and b x^2 + c x^4: what these
+// are at most over all x up to the last bound is the next one, and bounds the matrices' elements.  Half of fp16's range
+// is left for rounding.  The scales end at 2^-50, for X of 4e9.
+struct NsScales {
+    double bound = 1;
+    static float fit(float most, double bound)
+    {
+        while (bound * 2 * most > 65504. && most > 0x1p-50f) most *= 0.5f;
+        return most;
+    }
+    // the largest of |f| at 0, at `end` and at the given ones of its extrema that lie between
+    template <class F>
+    static double largest(F f, double end, std::initializer_list<double> extrema)
+    {
+        double most = fabs(f(end));
+        for (double at : extrema)
+            if (at > 0 && at < end) most = std::max(most, fabs(f(at)));
+        return most;
+    }
+    // p's scales for its coefficients
+    void next(NsParams &p)
+    {
+        const double a = p.a, b = p.b, c = p.c, square = bound * bound;
+        const float x = fit(SCALE_X, bound), e = fit(SCALE_E, square);
+        const float g = fit(SCALE_G, largest([&](double y) { return b * y + c * y * y; }, square, {-b / (2 * c)}));
+        // extrema of a x + b x^3 + c x^5: a + 3 b y + 5 c y^2 = 0 with y = x^2
+        const double root = sqrt(9 * b * b - 20 * a * c);
+        bound = largest([&](double x) { return x * (a + x * x * (b + c * x * x)); }, bound,
+                        {sqrt((-3 * b + root) / (10 * c)), sqrt((-3 * b - root) / (10 * c)), sqrt(-a / (3 * b))});
+        p.x = x / SCALE_X, p.x_next = p.last ? 1.f : fit(SCALE_X, bound) / x;
+        p.e = e, p.per_ee = 1.f / (e * e);
+        p.aa_to_g = p.c * (g / (e * e)), p.c_to_g = p.c * (g / e), p.b_to_g = p.b * (g / e);
+        p.gx_to_x = p.x_next / g;
+    }
+};
+
 static bool ns_dtype_ok(int d) { return d == TFTQ_F32 || d == TFTQ_F16 || d == TFTQ_BF16; }
 
 extern "C" int tftq_newton_schulz(const tftq_ns *what, void *workspace, int64_t workspace_bytes, int device, void *stream)
@@ -1034,7 +1076,8 @@ extern "C" int tftq_newton_schulz(const tftq_ns *what, void *workspace, int64_t 
         }
         float growth = 1.f;
         for (int it = 0; it < s.iterations; it++) growth *= fmaxf(1.f, fabsf(s.coefficients[3 * it]));
-        NsParams p = {s.momentum, s.keep, 0, 0, 0, s.eps, growth, s.nesterov, s.out_dtype, s.steps != nullptr, 0, 0};
+        NsParams p = {s.momentum, s.keep, 0, 0, 0, s.eps, growth, s.nesterov, s.out_dtype, s.steps != nullptr};
+        NsScales scales;
         const bool with = s.momenta != nullptr;
         const void *squares, *start;
         switch (s.in_dtype) {
@@ -1053,6 +1096,7 @@ extern "C" int tftq_newton_schulz(const tftq_ns *what, void *workspace, int64_t 
         for (int it = 0; it < s.iterations; it++) {
             p.a = s.coefficients[3 * it], p.b = s.coefficients[3 * it + 1], p.c = s.coefficients[3 * it + 2];
             p.last = it + 1 == s.iterations, p.next_last = it + 2 == s.iterations;
+            scales.next(p);
             if ((rc = product<NS_A>(l, precise, p, it & 1, st)) || (rc = product<NS_B>(l, precise, p, it & 1, st)) ||
                 (rc = product<NS_X>(l, precise, p, it & 1, st)))
                 return rc;

@@ -156,7 +156,8 @@ def orthogonalize(matrices: "torch.Tensor | Sequence[torch.Tensor]", steps: int 
                   eps: float = 1e-7, out_dtype: "torch.dtype | None" = None, precise: "bool | None" = None):
     """The Newton-Schulz orthogonalisation of a matrix, or a list with that of each.
 
-    ``coefficients``: ``(a, b, c)``, or one such triple for every one of the ``steps`` iterations.
+    ``coefficients``: ``(a, b, c)``, or one such triple for every one of the ``steps`` iterations; the numbers
+    that they make of X are held in 16 bits, scaled by what they can be at most (up to 4e9).
     ``out_dtype``: of the results, the input's by default.  ``precise``: whether products are exact to
     22 bits and not to 11; by default only bfloat16 results do without."""
     single = isinstance(matrices, torch.Tensor)
