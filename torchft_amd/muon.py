@@ -45,7 +45,7 @@ def _coefficients(coefficients, steps: int):
 
 
 def _by_rows(t: torch.Tensor) -> bool:
-    return (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= max(1, t.shape[1]))
+    return (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= max(1, t.shape[1])) and not t.is_neg()
 
 
 def _same_order(tensors: tuple) -> "tuple | None":
@@ -110,7 +110,7 @@ def _run(outs: list, ins: list, momenta: "list | None", steps_sizes: "list | Non
     after = []  # (the caller's tensor, the one that took its place)
 
     def in_place(t):
-        copy = t.contiguous() if steps_sizes is not None or momenta is not None else torch.empty_like(t, memory_format=torch.contiguous_format)
+        copy = t.resolve_neg().contiguous() if steps_sizes is not None or momenta is not None else torch.empty_like(t, memory_format=torch.contiguous_format)
         after.append((t, copy))
         return copy
 
@@ -122,7 +122,7 @@ def _run(outs: list, ins: list, momenta: "list | None", steps_sizes: "list | Non
         group = (outs[i], ins[i]) if momenta is None else (outs[i], ins[i], momenta[i])
         ordered = _same_order(group)
         if ordered is None:
-            ordered = tuple(t if _by_rows(t) else t.contiguous() if k == 1 else in_place(t) for k, t in enumerate(group))
+            ordered = tuple(t if _by_rows(t) else t.resolve_neg().contiguous() if k == 1 else in_place(t) for k, t in enumerate(group))
         held.append(ordered)
         shapes[2 * i], shapes[2 * i + 1] = ordered[0].shape
         for k, t in enumerate(ordered):

@@ -204,7 +204,7 @@ def _quantize(x: torch.Tensor, by_rows: bool, by_columns: bool):
                     MXFP4Tensor(c, (shape[1], shape[0]), dtype) if by_columns else None)
     assert x.dim() == 2, "Only 2D tensors are supported"
     assert x.dtype in _DTYPE_CODE, "Only fp32, fp16 and bf16 are supported"
-    x = x.detach()
+    x = x.detach().resolve_neg()
     rows, columns = x.shape
     if columns > 1 and x.stride(1) != 1 or rows > 1 and x.stride(0) < columns:
         if x.stride(0) == 1 and x.stride(1) >= rows:  # stored column by column: its transpose is stored by rows
@@ -258,6 +258,7 @@ def _linear_rows(x: torch.Tensor, weight: MXFP4Tensor, dtype: torch.dtype) -> to
         out = _native.mx_linear(x, weight.buffer, n, k)
         if out is not None:
             return _result(out, "tftq_mx_linear")
+    x = x.resolve_neg()
     if k > 1 and x.stride(1) != 1 or m > 1 and x.stride(0) < k:
         x = x.contiguous()
     lib = _lib.load()
