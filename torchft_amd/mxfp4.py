@@ -104,9 +104,9 @@ class MXFP4Tensor:
             codes[:, -1, (past + 1) // 2:] = 0
         more = panels * _PANEL_BLOCKS - blocks
         by_panel = self._panel_views()
-        by_panel[0].copy_(torch.nn.functional.pad(codes, (0, 0, 0, more)).view(rows, panels, _PANEL_BYTES).transpose(0, 1))
+        by_panel[0].copy_(torch.nn.functional.pad(codes, (0, 0, 0, more)).reshape(rows, panels, _PANEL_BYTES).transpose(0, 1))
         by_panel[1].zero_()
-        by_panel[1][:, :rows].copy_(torch.nn.functional.pad(scales, (0, more)).view(rows, panels, _PANEL_BLOCKS).transpose(0, 1))
+        by_panel[1][:, :rows].copy_(torch.nn.functional.pad(scales, (0, more)).reshape(rows, panels, _PANEL_BLOCKS).transpose(0, 1))
         return self
 
     def _data(self) -> int:
