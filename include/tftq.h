@@ -257,7 +257,7 @@ int tftq_mx_linear(int dtype, const void *x, int64_t m, int64_t row_stride, cons
  *    X = u / max(|u|_F, eps);  iterations times:  X = a X + (b (X X^T) + c (X X^T)^2) X
  * (of u^T where rows > cols).  Products run on the 16-bit matrix cores with fp32 sums; with `precise`
  * set every one is three, of high and low parts, and the result has the accuracy of fp32 products
- * (as has, in any case, that of a matrix with fewer than 64 rows or columns).
+ * (as has, in any case, that of a matrix with fewer than 192 rows or columns).
  */
 typedef struct tftq_ns {
     int n;                          /* matrices; empty ones are left alone */

@@ -927,10 +927,13 @@ static bool ns_shapes_ok(int n, const int64_t *shapes)
 }
 
 // Whether a matrix of r rows (columns, if these are fewer) takes three products.  The errors of the one of 11
-// bits are those of many roundings, and average: 2e-3 at most in 20 draws of each spectrum from 32 rows
-// on, but 8e-3 for a 3x5 matrix with singular values of 1 and 0.02.  A matrix of fewer than 64 rows is
-// one tile high, and its products wait for memory, not for the matrix cores.
-static bool ns_precise(int64_t r, int precise) { return precise || r < 64; }
+// bits are those of many roundings, and average, the better the larger r is.  They are largest where one direction
+// holds the norm: what rounds off it is multiplied by up to 480 in the others.  Rank one with noise of 0 to 1e-3, bf16
+// results, worst of 24 (the same rounded once 1.7e-3, at most 3.9e-3): r = 64 1.1e-2, 96 7.8e-3, 128 6.7e-3, 160 5.0e-3,
+// 192 3.6e-3, 256 3.0e-3, 512 2.3e-3.  A matrix of fewer than 192 rows is at most three tiles high, and its products
+// wait for memory more than for the matrix cores: one and three products, us, 64x512 69, 82; 128x1024 82, 100;
+// 160x5120 115, 140 (256x2048 102, 131; 512x4096 153, 235).
+static bool ns_precise(int64_t r, int precise) { return precise || r < 192; }
 
 // Whether the matrices of one product are so few and small that they join those of three in their launches: two
 // times their work more, but no 17 launches of their own (bf16, us, together and apart: 322x322 with 1x322 and

@@ -14,7 +14,7 @@ and takes that as the step:
 
 Products run on the 16-bit matrix cores with float32 sums.  bfloat16 results take one product each,
 with the diagonals and the remainders of the iterates kept apart, so that the result is off by less than
-its own rounding; float32 and float16 results, and matrices with a side of fewer than 64 (with the
+its own rounding; float32 and float16 results, and matrices with a side of fewer than 192 (with the
 small ones beside them in a list), take three, of high and low parts, with the accuracy of float32 products.
 The whole list is worked on at once, 24 matrices to a launch: about 17 launches whatever their number.
 The workspace comes from torch's allocator for the length of the call: 8 to 12 bytes an element, 12 to 20 with
