@@ -18,8 +18,9 @@
 // one rounding of the result would leave: errors 0 to 10 % larger, and 4 of 46 bytes an element less.)
 // Relative error of the result against 64 bits, one product each, matrices of 64x64 to 1024x1024 with even, low-rank and 1/i spectra: 2.4e-4 to 1.3e-3
 // (bf16 results are rounded by 1.7e-3; A, B and X in plain bf16: 1.3e-2 to 7.7e-2, in plain fp16 up to
-// 9e-3).  `precise`: A, B and X^T have second numbers too and every product is three, high x high +
-// low x high + high x low: 5e-7 to 5e-6, where fp32 products give 1e-6 to 6e-6, at three times the work
+// 9e-3; matrices of nearly rank one: ns_precise).  `precise`: A, B and X^T have second numbers too and every product is
+// three, high x high + low x high + high x low: 5e-7 to 5e-6, where fp32 products give 1e-6 to 6e-6 (nearly rank one 5e-5
+// to 3.4e-4, where they give 7e-5 to 3.8e-4), at three times the work
 // of the 16-bit cores, which is a fifth of what the fp32 ones would take.
 //
 // A and A A are symmetric: only tiles on and above the diagonal are computed, and stored twice.
@@ -823,9 +824,9 @@ static int launch_tiles(NsLaunch &l, bool precise, const NsParams &p, int turn, 
 // How many workgroups share a tile of `all` in a launch, each at least `least` of its panels: a panel for every
 // wavefront of k_ns_small; what outweighs the sums' way through memory, 3 us, in tiles of 64 x 64.  No more
 // than 16, whose sums one workgroup adds up.  Graph replays of the whole orthogonalisation, us, with a
-// workgroup to a tile and so: fp32 64x3584 188, 99; 64x16384 661, 145; 256x16384 734, 282; 1024x16384 1714,
-// 1162; 1024x1024 286, 276; bf16 64x16384 352, 119; 1024x16384 670, 532 (from 8 panels on 1024x1024 bf16 is
-// shared too: 151, 192).
+// workgroup to a tile and so: fp32 64x3584 195, 102; 64x16384 666, 148; 256x16384 740, 283; 1024x16384 1840,
+// 1261; 768x1024 262, 239; 1024x1024 287, 291; bf16 256x16384 403, 194; 1024x16384 710, 547 (from 8 panels on
+// 1024x1024 bf16 is shared too: 151, 192).
 static int ns_splits(int64_t all, int64_t panels, int least)
 {
     return (int)std::max<int64_t>(1, std::min<int64_t>({NS_SHARED / std::max<int64_t>(all, 1), panels / least, 16}));
@@ -871,8 +872,8 @@ static double ns_small_time(const NsLaunch &l, int what, bool precise)
 }
 
 // One of the three products for all matrices of a launch.  k_ns_small and tiles of 64 x 64, graph replays of the
-// whole orthogonalisation, us: fp32 512x512 127, 182; 512x768 159, 164; 768x1024 264, 263; 1024x1024 432,
-// 292.  bf16 512x512 90, 102; 512x768 105, 104; 640x640 117, 112; 768x1024 162, 140.
+// whole orthogonalisation, us: fp32 512x512 130, 183; 512x768 159, 191; 768x1024 282, 239; 1024x1024 432,
+// 291.  bf16 512x512 92, 105; 512x768 107, 112; 640x640 119, 121; 768x1024 181, 142.
 template <int WHAT>
 static int product(NsLaunch &l, bool precise, const NsParams &p, int turn, hipStream_t st)
 {
@@ -931,13 +932,16 @@ static bool ns_shapes_ok(int n, const int64_t *shapes)
 // holds the norm: what rounds off it is multiplied by up to 480 in the others.  Rank one with noise of 0 to 1e-3, bf16
 // results, worst of 24 (the same rounded once 1.7e-3, at most 3.9e-3): r = 64 1.1e-2, 96 7.8e-3, 128 6.7e-3, 160 5.0e-3,
 // 192 3.6e-3, 256 3.0e-3, 512 2.3e-3.  A matrix of fewer than 192 rows is at most three tiles high, and its products
-// wait for memory more than for the matrix cores: one and three products, us, 64x512 69, 82; 128x1024 82, 100;
-// 160x5120 115, 140 (256x2048 102, 131; 512x4096 153, 235).
+// wait for memory more than for the matrix cores: one and three products, us, 64x512 67, 84; 128x1024 83, 100;
+// 160x5120 115, 141; 24 of 128x256 108, 141; 24 of 128x2048 217, 258 (256x2048 102, 131; 512x4096 153, 235).
 static bool ns_precise(int64_t r, int precise) { return precise || r < 192; }
 
 // Whether the matrices of one product are so few and small that they join those of three in their launches: two
 // times their work more, but no 17 launches of their own (bf16, us, together and apart: 322x322 with 1x322 and
-// 322x1 111, 147; ten of up to 844x211 with two of 211x1 169, 193; 640x640 with 512x1 181, 178).
+// 322x1 112, 148; 640x640 with 512x1 184, 183; four of 256x1024 with 128x1024 175, 213; ten of 844x211 with two of
+// 211x1 218, 226; three of 512x512 with three of 128x512 201, 232; four of 300x1200 with 1x300 187, 202; 768x768
+// with four of 96x768 237, 253; above the limit 1024x1024 with 1024x1 286, 230, two of 1024x1024 with two of
+// 128x1024 379, 293).
 static bool ns_together(int n, const int64_t *shapes)
 {
     double work = 0;
@@ -947,7 +951,7 @@ static bool ns_together(int n, const int64_t *shapes)
         if (r > 0 && ns_precise((int64_t)r, 0)) narrow = true;
         else work += r * a * b;
     }
-    return narrow && n <= NS_MOST && work <= 2.5e8;
+    return narrow && n <= NS_MOST && work <= 5e8;
 }
 
 // Squares of 64 of a launch's matrices: no kernel has more workgroups of 256 threads, or half as many of
