@@ -226,8 +226,8 @@ extern "C" int tftq_mx_product(int dtype, const void *a, int64_t m, const void *
     hipStream_t st = (hipStream_t)stream;
     // Up to 64 rows: by 16 rows of b and all of a (k_mx_few) up to 16 rows of a, and beyond that where tiles
     // of 64 x 64 are too few for the units: with the quantisation of a before it, n 14336, k 4096,
-    // 24 rows 15.8 us (tiles 14.6), 64 rows 30.9 (14.8); n 4096, k 14336, 24 rows 15.0 (36.8), 64 rows
-    // 23.8 (37.2); n 1024, k 4096, 64 rows 10.0 (11.7).
+    // 24 rows 15.6 us (tiles 12.6), 64 rows 30.6 (12.9); n 4096, k 14336, 24 rows 14.8 (29.2), 64 rows
+    // 23.6 (29.5); n 1024, k 4096, 64 rows 10.0 (11.6).
     if ((m <= 16 && n <= FEW_WIDEST) || (m <= FEW_MOST && (n + 63) / 64 < 160)) {
         switch (dtype) {
         case TFTQ_F32: return few<MxQuantized, TFTQ_F32>(ta.panels, 0, ta.scales, (int)m, tb, (int)k, (uint8_t *)out, row_stride, st);
@@ -253,9 +253,9 @@ extern "C" int tftq_mx_product(int dtype, const void *a, int64_t m, const void *
 
 // Whether x [m, k] is quantised by the workgroups of the product with n rows.  That saves a launch and the
 // wait for it, 2 to 3 us, and costs every workgroup time that grows with m k, which those that find no
-// room at first add to: n 14336, k 4096, aligned rows: 1 row 7.6 us (two launches 11.0), 4 rows 9.1
-// (11.4), 8 rows 12.4 (12.2); n 1024: 1 row 3.4 (5.2), 16 rows 5.7 (6.2), 24 rows 7.4 (7.1).  Rows at
-// other addresses take two and a half times as long to read: n 1024, 4 rows 5.0 (5.7), 8 rows 6.8 (5.9).
+// room at first add to: n 14336, k 4096, aligned rows: 1 row 6.9 us (two launches 10.1), 4 rows 8.4
+// (10.8), 8 rows 11.0 (11.5), 16 rows 15.3 (12.6); n 1024: 1 row 3.4 (5.4), 16 rows 5.7 (6.3), 24 rows 7.3
+// (7.2).  Rows at other addresses take longer to read: n 1024, 4 rows 4.4 (5.6), 8 rows 5.5 (5.8).
 static bool few_rows(int dtype, const void *x, int64_t m, int64_t row_stride, int64_t n, int64_t k)
 {
     const int64_t panels = (k + 255) / 256, size = dtype == TFTQ_F32 ? 4 : 2;

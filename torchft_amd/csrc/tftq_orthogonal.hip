@@ -931,7 +931,7 @@ static bool ns_shapes_ok(int n, const int64_t *shapes)
 // bits are those of many roundings, and average, the better the larger r is.  They are largest where one direction
 // holds the norm: what rounds off it is multiplied by up to 480 in the others.  Rank one with noise of 0 to 1e-3, bf16
 // results, worst of 24 (the same rounded once 1.7e-3, at most 3.9e-3): r = 64 1.1e-2, 96 7.8e-3, 128 6.7e-3, 160 5.0e-3,
-// 192 3.6e-3, 256 3.0e-3, 512 2.3e-3.  A matrix of fewer than 192 rows is at most three tiles high, and its products
+// 192 3.6e-3, 224 4.1e-3, 256 3.0e-3, 512 2.3e-3.  A matrix of fewer than 192 rows is at most three tiles high, and its products
 // wait for memory more than for the matrix cores: one and three products, us, 64x512 67, 84; 128x1024 83, 100;
 // 160x5120 115, 141; 24 of 128x256 108, 141; 24 of 128x2048 217, 258 (256x2048 102, 131; 512x4096 153, 235).
 static bool ns_precise(int64_t r, int precise) { return precise || r < 192; }

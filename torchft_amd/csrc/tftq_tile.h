@@ -77,8 +77,10 @@ struct TileTriple {  // three
 };
 
 // A buffer of `bytes` bytes (what lies past them reads as zero), and a load of 16 bytes per lane from it
-// into LDS, in lane order from `lds` on.  (The global instruction that does the same makes the compiler
-// wait for every LDS read in flight at the next use of one.)
+// into LDS, in lane order from `lds` on.  `more`, in a scalar register, counts in the check of the end as `at` does
+// (1024 bytes, at < 1024: all zeros from more = 1024 on, and half of the lanes at 512), also where it alone
+// passes the end.  (The global instruction that does the same makes the compiler wait for every LDS read in flight at the
+// next use of one.)
 __device__ static inline __amdgpu_buffer_rsrc_t tile_buffer(const uint8_t *from, int bytes)
 {
     return __builtin_amdgcn_make_buffer_rsrc((void *)from, 0, bytes, 0x00020000);
@@ -426,11 +428,11 @@ __device__ static inline void tile_place(int piece, int tiles_m, int tiles_n, in
 // A size of tiles.  `at_once`: the tiles that a compute unit runs at once; `cost`: what a panel of them all
 // takes then, `one` with one tile to a unit, a panel of one tile of 256 x 256 on every unit being 1.  From
 // launches that fill all units (8192^3, fp16, TFLOP/s: 256x256 1230, 192x256 1190, 192x192 1040, 128x128
-// 1000, 64x64 760; 4-bit, 256x256 4300, 128x128 3500) and from short ones (4-bit, us, tiles of 256, 128,
-// 64: 256x4096x4096 23.5, 13.4, 10.8; 256x14336x4096 26.6, 17.9, 24.7; 2048x5632x2048 22.1, 22.6, 35.5).
+// 1000, 64x64 760; 4-bit, 256x256 4600, 192x256 4100, 128x128 3580, 64x64 1870) and from short ones (4-bit, us, tiles
+// of 256, 128, 64: 256x4096x4096 22.8, 12.4, 9.6; 256x14336x4096 24.8, 16.5, 22.5; 2048x5632x2048 18.7, 21.0, 31.4).
 // 128x128 is 0.61 by its rate, but 3 to a unit take 1.02 (a list of products of depth 2048 in 696 tiles
 // 79 us, in 216 of 256x256 71), and 192x256 0.775, but with a round more than 256x256 it loses (4-bit
-// 14336x4096x8192 230 us, 222; X of 4096x14336 572, 552; with fewer, 4-bit 6144x6144x6144, 113, 123).
+// 14336x4096x8192 230 us, 221; X of 4096x14336 572, 552; with fewer, 4-bit 6144x6144x6144, 112, 122).
 struct TileShape {
     int high, wide, at_once;
     double one, cost;

@@ -38,8 +38,9 @@ _PANEL_BLOCKS = _PANEL // _BLOCK
 # The module that makes whole calls with plain arguments (_pylist.mx_quantize and the like: checks,
 # allocations and launch in one step), once it knows the library and a device that can run it.  It answers
 # None to anything else, and the functions below then go their own way.  Host time on small matrices, us, in
-# Python and so: quantisation 7.7, 4.3; along both axes 10, 5.5; product 6.0, 4.3; linear with a kept weight
-# 12, 7.8; linear with its gradients 147, 107 (torch's own linear: 115; most of it is autograd's).
+# Python and so: quantisation 8.1, 5.1; along both axes 9.9, 6.1; product 8.4, 5.2; linear with a kept weight
+# 10.1, 5.0; with an ordinary one and no gradients 19.5, 12.6, with its gradients 154, 113 (torch's own linear: 115; most
+# of it is autograd's, and in some processes all of these take half as long: 89, 62, 86).
 _native = None
 _bind_lock = threading.Lock()
 
