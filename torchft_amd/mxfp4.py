@@ -148,12 +148,13 @@ class MXFP4Tensor:
             return self.buffer.new_empty(rows, blocks)
         if panels == 1:
             return self._panel_views()[1][0, :rows, :blocks]
-        split = panels * rows * _PANEL_BYTES
-        scales = self.buffer[split:split + panels * even * _PANEL_BLOCKS]
-        if scales.storage_offset() % 8 == 0:  # a row's 8 scales of a panel are moved as one number
-            scales = scales.view(torch.int64).as_strided((rows, panels), (1, even)).contiguous().view(torch.uint8)
+        split, size = panels * rows * _PANEL_BYTES, panels * even * _PANEL_BLOCKS
+        buffer = self.buffer if self.buffer.numel() % 8 == 0 else self.buffer[:split + size]
+        start = buffer.storage_offset()
+        if start % 8 == 0:  # a row's 8 scales of a panel are moved as one number
+            scales = buffer.view(torch.int64).as_strided((rows, panels), (1, even), (start + split) // 8).contiguous().view(torch.uint8)
         else:
-            scales = scales.view(panels, even, _PANEL_BLOCKS)[:, :rows].transpose(0, 1).reshape(rows, panels * _PANEL_BLOCKS)
+            scales = buffer[split:split + size].view(panels, even, _PANEL_BLOCKS)[:, :rows].transpose(0, 1).reshape(rows, panels * _PANEL_BLOCKS)
         return scales if blocks == panels * _PANEL_BLOCKS else scales[:, :blocks]
 
     def dequantize(self, dtype: torch.dtype | None = None) -> torch.Tensor:
