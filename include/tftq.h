@@ -291,6 +291,84 @@ int64_t tftq_newton_schulz_workspace(int n, const int64_t *shapes, int precise);
  */
 int tftq_newton_schulz(const tftq_ns *what, void *workspace, int64_t workspace_bytes, int device, void *stream);
 
+/*
+ * Row operators of a training step (no counterpart in the reference).  Rows are contiguous runs of `cols` elements of
+ * TFTQ_F32, TFTQ_F16 or TFTQ_BF16 at any address that is a multiple of the element's size; strides are elements from
+ * row to row, and where none is given rows follow each other.  Rows, columns, tokens and choices are at most 2^31 - 65536
+ * (TFTQ_E_SHAPE).  Sums are fp32 in an order that the arguments alone decide; results are rounded once.  Workspaces
+ * are device memory, 16-byte aligned, at least as many bytes as the function beside says (TFTQ_E_SIZE), and hold
+ * nothing between calls.
+ *
+ * Root-mean-square norm:  h = x + residual, rounded to the rows' type;  y = h w / sqrt(mean(h^2) + eps).
+ *   residual  NULL for none; then h is x and the argument h has to be NULL
+ *   weight    [cols] of weight_dtype (dtype or TFTQ_F32); NULL for ones
+ *   y         [rows, cols]; or NULL, with codes [rows, cols] and scales [rows]: y in e4m3 codes that scales multiply,
+ *             a row's largest magnitude / 448 (1 where that is below 2^-126)
+ * The sum of squares is fp32: rows of magnitudes beyond 1e18 pass its range.
+ */
+int tftq_rms_norm(int dtype, int weight_dtype, const void *x, int64_t x_stride, const void *residual, int64_t residual_stride,
+                  const void *weight, int64_t rows, int64_t cols, float eps, void *h, void *y, void *codes, float *scales,
+                  int device, void *stream);
+/*
+ * Its gradients, from the h that was kept (x where there was no residual):
+ * dx = d/dx of <dy, y> + dh (dh may be NULL), also the residual's; dweight [cols] of weight_dtype (a weight is needed then).  Either may be NULL.
+ */
+int64_t tftq_rms_norm_backward_workspace(int dtype, int64_t rows, int64_t cols);
+int tftq_rms_norm_backward(int dtype, int weight_dtype, const void *dy, const void *dh, const void *h, int64_t h_stride,
+                           const void *weight, int64_t rows, int64_t cols, float eps, void *dx, void *dweight,
+                           void *workspace, int64_t workspace_bytes, int device, void *stream);
+
+/*
+ * Dropout:  out = residual + x keep / (1 - q) for n elements, q = round(p 65536) / 65536; residual may be NULL.  Element i
+ * is kept if its 16-bit number is at least q 65536: number i % 8 (low half of the first word first) of the block that
+ * the Philox generator of four 32-bit words and ten rounds makes of the counter (i / 8, offset) and the key seed,
+ * all 64-bit numbers with the low word first.  seed_at: NULL, or a device address to read the seed from.
+ */
+int tftq_dropout(int dtype, const void *x, const void *residual, int64_t n, double p, int64_t seed, const int64_t *seed_at,
+                 int64_t offset, void *out, int device, void *stream);
+
+/*
+ * Embedding:  out[t] = scale table[ids[t]], zeros where ids[t] is not in [0, vocab).  ids: signed, id_bytes 4 or 8 each.
+ * Gradient:  dtable[v] = scale sum of dy[t] over ids[t] = v, every row of dtable written; tokens with ids[t] = skip have none
+ * (skip outside [0, vocab): no such).
+ */
+int tftq_embedding(int dtype, int id_bytes, const void *ids, int64_t n, const void *table, int64_t vocab, int64_t cols,
+                   int64_t row_stride, float scale, void *out, int device, void *stream);
+int64_t tftq_embedding_backward_workspace(int64_t n, int64_t vocab, int64_t cols);
+int tftq_embedding_backward(int dtype, int id_bytes, const void *ids, int64_t n, int64_t skip, const void *dy, int64_t vocab,
+                            int64_t cols, float scale, void *dtable, void *workspace, int64_t workspace_bytes, int device,
+                            void *stream);
+
+/*
+ * Tokens by expert: `choices` numbers of experts, signed, id_bytes 4 or 8 each; what is not in [0, experts) names none.
+ *   position  [choices] the place of a choice: by expert, then in order; those of no expert behind all others
+ *   order     [choices] the choice at a place
+ *   offsets   [experts + 1] the first place of every expert; the last: how many places have an expert
+ */
+int64_t tftq_expert_sort_workspace(int64_t choices, int64_t experts);
+int tftq_expert_sort(int id_bytes, const void *chosen, int64_t choices, int64_t experts, int32_t *order, int32_t *position,
+                     int32_t *offsets, void *workspace, int64_t workspace_bytes, int device, void *stream);
+/*
+ * Rows to the places of their tokens' k choices each, and back.  position: [tokens][k] from the sort, `used` the address
+ * of the last of its offsets.
+ *   dispatch  out[position[t, s]] = x[t], elements of 1, 2 or 4 bytes; zeros in places of no expert
+ *   combine   out[t] = sum over s of weights[t, s] rows[position[t, s]], without choices of no expert.
+ *             weights of weight_dtype (dtype or TFTQ_F32), NULL for ones: the gradient of dispatch
+ *   combine_backward  drows[position[t, s]] = weights[t, s] dy[t], zeros in places of no expert;
+ *             dweights[t, s] = <dy[t], rows[position[t, s]]>, 0 for choices of no expert.  Either may be NULL
+ */
+int tftq_dispatch(int element_bytes, const void *x, int64_t x_stride, int64_t tokens, int64_t k, int64_t cols,
+                  const int32_t *position, const int32_t *used, void *out, int device, void *stream);
+int tftq_combine(int dtype, int weight_dtype, const void *rows, int64_t rows_stride, const void *weights, int64_t tokens,
+                 int64_t k, int64_t cols, const int32_t *position, const int32_t *used, void *out, int device, void *stream);
+int tftq_combine_backward(int dtype, int weight_dtype, const void *dy, int64_t dy_stride, const void *rows,
+                          int64_t rows_stride, const void *weights, int64_t tokens, int64_t k, int64_t cols,
+                          const int32_t *position, const int32_t *used, void *drows, void *dweights, int device, void *stream);
+
+/* Values of 8-bit rows: out[r, c] = codes[r, c] scales[r], e4m3 codes, rounded once to dtype. */
+int tftq_fp8_rows_dequantize(int dtype, const void *codes, const float *scales, int64_t rows, int64_t cols, void *out,
+                             int device, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,6 +1,7 @@
 """MI355X-native FP8 quantized-collective kernels, a drop-in for torchft's
 ``torchft.quantization`` (and its callers in ``torchft.collectives``); and, with no counterpart there,
-operators of the training step around them: 4-bit matrices and linear layers on them, Muon's update."""
+operators of the training step around them: 4-bit matrices and linear layers on them, Muon's update, and the row
+operators between the layers (norm, dropout, embedding, tokens to experts and back)."""
 
 from .quantization import (  # noqa: F401
     PreparedBucket,
@@ -19,6 +20,18 @@ from .mxfp4 import (  # noqa: F401
 )
 
 from .muon import Muon, muon_, orthogonalize  # noqa: F401
+
+from .rows import (  # noqa: F401
+    ExpertOrder,
+    FP8Rows,
+    combine,
+    dispatch,
+    dropout,
+    embedding,
+    rms_norm,
+    rms_norm_fp8,
+    sort_by_expert,
+)
 
 from .collectives import (  # noqa: F401
     allocate_reduce_scatter_output,
@@ -45,4 +58,13 @@ __all__ = [
     "Muon",
     "muon_",
     "orthogonalize",
+    "rms_norm",
+    "rms_norm_fp8",
+    "FP8Rows",
+    "dropout",
+    "embedding",
+    "sort_by_expert",
+    "ExpertOrder",
+    "dispatch",
+    "combine",
 ]

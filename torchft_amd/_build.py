@@ -14,7 +14,7 @@ CSRC = os.path.join(_HERE, "csrc")
 LIB_PATH = os.path.join(_HERE, "libtftq.so")
 SOURCES = ["tftq_quantize.hip", "tftq_dequantize.hip", "tftq_reduce.hip", "tftq_reduce_all.hip", "tftq_reduce_wide.hip",
            "tftq_reduce_long.hip", "tftq_reduce_one.hip", "tftq_runtime.hip", "tftq_mxfp4.hip", "tftq_mxfp4_product.hip", "tftq_orthogonal.hip",
-           "tftq_plan.cpp"]
+           "tftq_norm.hip", "tftq_dropout.hip", "tftq_sort.hip", "tftq_embedding.hip", "tftq_experts.hip", "tftq_plan.cpp"]
 # Streaming kernels without arithmetic that bench.py times beside the product kernels
 # (benchmark infrastructure; torchft_amd never loads this library).
 CEILING_LIB_PATH = os.path.join(_HERE, "libtftq_ceiling.so")
@@ -22,6 +22,8 @@ CEILING_SOURCE = "tftq_ceiling.hip"
 # The C++ walk over lists of tensors: a CPython extension module built with the host compiler
 # against the Python and libtorch headers.  Host code only; not part of libtftq.so.
 PYLIST_SOURCE = "tftq_pylist.cpp"
+# The calls of the row operators and their autograd nodes, built and kept apart in the same way.
+ROWS_SOURCE = "tftq_rows.cpp"
 
 # -ffp-contract=off: the arithmetic contract is separate IEEE multiply, divide
 # and add; fused multiply-adds are written out where they are wanted.
@@ -42,7 +44,7 @@ def source_hash() -> str:
     built with as tftq_build_id()."""
     h = hashlib.sha256()
     files = [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC))
-             if f.endswith((".hip", ".h", ".cpp")) and f not in (CEILING_SOURCE, PYLIST_SOURCE)]
+             if f.endswith((".hip", ".h", ".cpp")) and f not in (CEILING_SOURCE, PYLIST_SOURCE, ROWS_SOURCE)]
     files.append(os.path.join(os.path.dirname(_HERE), "include", "tftq.h"))
     for path in files:
         h.update(os.path.basename(path).encode() + b"\0")
@@ -63,37 +65,77 @@ def hipcc_path() -> str:
 
 
 
-def pylist_path() -> str:
+def _extension_path(name: str) -> str:
     import sysconfig
-    return os.path.join(_HERE, "_pylist" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
+    return os.path.join(_HERE, name + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
 
-def pylist_hash() -> str:
-    with open(os.path.join(CSRC, PYLIST_SOURCE), "rb") as fh:
+def _file_hash(source: str) -> str:
+    with open(os.path.join(CSRC, source), "rb") as fh:
         return hashlib.sha256(fh.read()).hexdigest()[:16]
 
 
-def pylist_command() -> list[str]:
+def _extension_command(source: str, path: str, flags: list[str], libraries: list[str]) -> list[str]:
+    """The host compiler's line for a CPython module against libtorch."""
     import sysconfig
 
     import torch
     from torch.utils import cpp_extension
     cxx = os.environ.get("CXX") or shutil.which("g++") or shutil.which("c++")
     if not cxx:
-        raise RuntimeError("no C++ compiler found; _pylist cannot be built")
+        raise RuntimeError(f"no C++ compiler found; {os.path.basename(path)} cannot be built")
     libdir = os.path.join(os.path.dirname(torch.__file__), "lib")
     cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           f'-DTFTQ_PYLIST_ID="{pylist_hash()}"']
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *flags]
     cmd += ["-I" + d for d in cpp_extension.include_paths()]
-    cmd += ["-I" + sysconfig.get_paths()["include"], "-o", pylist_path(), os.path.join(CSRC, PYLIST_SOURCE),
-            "-L" + libdir, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-Wl,-rpath," + libdir]
+    cmd += ["-I" + sysconfig.get_paths()["include"], "-o", path, os.path.join(CSRC, source),
+            "-L" + libdir, "-ltorch_python", "-ltorch", "-ltorch_cpu", *libraries, "-lc10", "-Wl,-rpath," + libdir]
     return cmd
+
+
+def pylist_path() -> str:
+    return _extension_path("_pylist")
+
+
+def pylist_hash() -> str:
+    return _file_hash(PYLIST_SOURCE)
+
+
+def pylist_command() -> list[str]:
+    return _extension_command(PYLIST_SOURCE, pylist_path(), [f'-DTFTQ_PYLIST_ID="{pylist_hash()}"'], [])
 
 
 def build_pylist() -> str:
     _run(pylist_command())
     return pylist_path()
+
+
+def rows_path() -> str:
+    return _extension_path("_rows")
+
+
+def rows_command() -> list[str]:
+    hip = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(hipcc_path()))), "include")
+    return _extension_command(ROWS_SOURCE, rows_path(), [f'-DTFTQ_ROWS_ID="{_file_hash(ROWS_SOURCE)}"', "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", "-I" + hip],
+                              ["-lc10_hip"])
+
+
+def build_rows() -> str:
+    _run(rows_command())
+    return rows_path()
+
+
+def load_rows():
+    """The _rows module, built first if there is no build.  Raises if it can be neither loaded nor built, or if the
+    build is of another source (TFTQ_ALLOW_STALE=1 loads it anyway): no other code makes these calls."""
+    import importlib
+    if not os.path.exists(rows_path()):
+        build_rows()
+    mod = importlib.import_module("torchft_amd._rows")
+    if mod.BUILD_ID != _file_hash(ROWS_SOURCE) and not os.environ.get("TFTQ_ALLOW_STALE"):
+        raise RuntimeError(f"{rows_path()} was built from another source; rebuild it with `python -m torchft_amd._build` "
+                           "(TFTQ_ALLOW_STALE=1 loads it anyway)")
+    return mod
 
 
 def load_pylist():
@@ -138,7 +180,7 @@ def build_library(verbose: bool = False) -> str:
         build_id = f'-DTFTQ_BUILD_ID="{source_hash()}"'
         cmds = [[hipcc, *HIPCC_FLAGS, build_id, "-c", "-o", o, os.path.join(CSRC, s)] for s, o in zip(SOURCES, objs)]
         cmds.append([hipcc, *HIPCC_FLAGS, "-shared", "-o", CEILING_LIB_PATH, os.path.join(CSRC, CEILING_SOURCE)])
-        cmds.append(pylist_command())
+        cmds += [pylist_command(), rows_command()]
         with ThreadPoolExecutor(max_workers=len(cmds)) as pool:
             outs = list(pool.map(_run, cmds))
         outs.append(_run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB_PATH, *objs]))

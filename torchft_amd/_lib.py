@@ -75,6 +75,33 @@ SYMBOLS = [
     ("tftq_newton_schulz", _c.c_int, [_c.POINTER(NewtonSchulz), _P, _c.c_int64, _c.c_int, _P]),
     # dtype, a, m, b, n, k, out, row_stride, device, stream
     ("tftq_mx_product", _c.c_int, [_c.c_int, _P, _c.c_int64, _P, _c.c_int64, _c.c_int64, _P, _c.c_int64, _c.c_int, _P]),
+    # dtype, weight_dtype, x, x_stride, residual, residual_stride, weight, rows, cols, eps, h, y, codes, scales, device, stream
+    ("tftq_rms_norm", _c.c_int, [_c.c_int, _c.c_int, _P, _c.c_int64, _P, _c.c_int64, _P, _c.c_int64, _c.c_int64, _c.c_float, _P, _P, _P, _P,
+                                 _c.c_int, _P]),
+    ("tftq_rms_norm_backward_workspace", _c.c_int64, [_c.c_int, _c.c_int64, _c.c_int64]),
+    # dtype, weight_dtype, dy, dh, h, h_stride, weight, rows, cols, eps, dx, dweight, workspace, workspace_bytes, device, stream
+    ("tftq_rms_norm_backward", _c.c_int, [_c.c_int, _c.c_int, _P, _P, _P, _c.c_int64, _P, _c.c_int64, _c.c_int64, _c.c_float, _P, _P, _P,
+                                          _c.c_int64, _c.c_int, _P]),
+    # dtype, x, residual, n, p, seed, seed_at, offset, out, device, stream
+    ("tftq_dropout", _c.c_int, [_c.c_int, _P, _P, _c.c_int64, _c.c_double, _c.c_int64, _P, _c.c_int64, _P, _c.c_int, _P]),
+    # dtype, id_bytes, ids, n, table, vocab, cols, row_stride, scale, out, device, stream
+    ("tftq_embedding", _c.c_int, [_c.c_int, _c.c_int, _P, _c.c_int64, _P, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_float, _P, _c.c_int, _P]),
+    ("tftq_embedding_backward_workspace", _c.c_int64, [_c.c_int64, _c.c_int64, _c.c_int64]),
+    # dtype, id_bytes, ids, n, skip, dy, vocab, cols, scale, dtable, workspace, workspace_bytes, device, stream
+    ("tftq_embedding_backward", _c.c_int, [_c.c_int, _c.c_int, _P, _c.c_int64, _c.c_int64, _P, _c.c_int64, _c.c_int64, _c.c_float, _P, _P,
+                                           _c.c_int64, _c.c_int, _P]),
+    ("tftq_expert_sort_workspace", _c.c_int64, [_c.c_int64, _c.c_int64]),
+    # id_bytes, chosen, choices, experts, order, position, offsets, workspace, workspace_bytes, device, stream
+    ("tftq_expert_sort", _c.c_int, [_c.c_int, _P, _c.c_int64, _c.c_int64, _P, _P, _P, _P, _c.c_int64, _c.c_int, _P]),
+    # element_bytes, x, x_stride, tokens, k, cols, position, used, out, device, stream
+    ("tftq_dispatch", _c.c_int, [_c.c_int, _P, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int64, _P, _P, _P, _c.c_int, _P]),
+    # dtype, weight_dtype, rows, rows_stride, weights, tokens, k, cols, position, used, out, device, stream
+    ("tftq_combine", _c.c_int, [_c.c_int, _c.c_int, _P, _c.c_int64, _P, _c.c_int64, _c.c_int64, _c.c_int64, _P, _P, _P, _c.c_int, _P]),
+    # dtype, weight_dtype, dy, dy_stride, rows, rows_stride, weights, tokens, k, cols, position, used, drows, dweights, device, stream
+    ("tftq_combine_backward", _c.c_int, [_c.c_int, _c.c_int, _P, _c.c_int64, _P, _c.c_int64, _P, _c.c_int64, _c.c_int64, _c.c_int64, _P, _P, _P,
+                                         _P, _c.c_int, _P]),
+    # dtype, codes, scales, rows, cols, out, device, stream
+    ("tftq_fp8_rows_dequantize", _c.c_int, [_c.c_int, _P, _P, _c.c_int64, _c.c_int64, _P, _c.c_int, _P]),
 ]
 ABI_VERSION = 2
 
