@@ -110,7 +110,7 @@ def test_c_entries_check_before_they_launch():
     assert emb(bytes=8) == -4 and emb(ws=None) == -1 and emb(dt=None) == -1 and emb(cols=-1) == -3 and emb(size=1) == -1 and emb(vocab=0) == 0
     sort = lambda **k: lib.tftq_expert_sort(*{**dict(size=8, chosen=p, n=3, experts=4, order=p, position=p, offsets=p, ws=p, bytes=1 << 20, device=-1,  # noqa: E731
                                                        stream=None), **k}.values())
-    assert sort(size=3) == -1 and sort(n=-1) == -3 and sort(offsets=None) == -1 and sort(bytes=0) == -4 and sort(ws=p + 4) == -1
+    assert sort(size=3) == -1 and sort(n=-1) == -3 and sort(offsets=None) == -1 and sort(n=100000, bytes=0) == -4 and sort(n=100000, ws=p + 4) == -1
     send = lambda **k: lib.tftq_dispatch(*{**dict(size=2, x=p, xs=8, tokens=3, k=2, cols=8, position=p, used=p, out=p, device=-1, stream=None), **k}.values())  # noqa: E731
     assert send(size=8) == -2 and send(xs=7) == -1 and send(tokens=2 ** 30, k=4) == -3 and send(used=None) == -1 and send(k=0) == 0
     back = lambda **k: lib.tftq_combine(*{**dict(dtype=2, wdtype=0, rows=p, rs=8, w=p, tokens=3, k=2, cols=8, position=p, used=p, out=p, device=-1,  # noqa: E731
@@ -124,9 +124,9 @@ def test_c_entries_check_before_they_launch():
 
 def test_workspaces_grow_with_their_sizes():
     lib = _lib.load()
-    assert lib.tftq_expert_sort_workspace(100, 8) == 400 and lib.tftq_expert_sort_workspace(0, 8) == 0
+    assert lib.tftq_expert_sort_workspace(100, 8) >= 0 and lib.tftq_expert_sort_workspace(0, 8) == 0
     n = 100000
-    assert lib.tftq_embedding_backward_workspace(n, 128256, 64) >= 8 * n + 2 * 8 * n and lib.tftq_expert_sort_workspace(n, 8) >= 4 * n
+    assert lib.tftq_embedding_backward_workspace(n, 128256, 64) >= 8 * n + 2 * 8 * n and lib.tftq_expert_sort_workspace(n, 1000) >= 12 * n
     assert lib.tftq_expert_sort_workspace(2 ** 31, 8) == -3
     assert lib.tftq_rms_norm_backward_workspace(2, 4, 100) >= 4 * 100
 

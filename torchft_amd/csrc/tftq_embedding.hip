@@ -8,9 +8,9 @@
 // The gradient is a sum over sorted tokens (tftq_sort.h), fp32, in an order that ids alone decide.  The sorted
 // tokens are cut into chunks of equal size, so that a token that half of the text consists of is no longer to work on
 // than any other: a team sums a chunk's runs, writes the table's row where a run begins and ends inside the
-// chunk, and leaves fp32 sums where it goes on outside (at most one of each end).  A second launch goes over
-// the table: rows of no token are filled with zeros, rows of several chunks add up their sums.  Every row is
-// written once, whatever was there.
+// chunk, and leaves fp32 sums where it goes on outside (at most one at each end).  The same launch fills the rows of no
+// token with zeros, which is most of the memory that it writes.  A second one adds up the sums of runs over several
+// chunks.  Every row is written once, whatever was there.
 #include "tftq_sort.h"
 
 struct EmbeddingArgs {
@@ -35,11 +35,11 @@ __global__ __launch_bounds__(256) void k_embedding(const EmbeddingArgs a)
     for (int col = lane * EPV; col < a.cols; col += U * TEAM * EPV) {
         u32x4 raw[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) raw[u] = inside ? load_row<ESZ, false>(from, col + u * TEAM * EPV, a.cols) : u32x4{0, 0, 0, 0};
+        for (int u = 0; u < U; u++) raw[u] = fetch_row<ESZ, false>(from, col + u * TEAM * EPV, inside ? a.cols : 0);
 #pragma unroll
         for (int u = 0; u < U; u++) {
             float f[EPV];
-            Elem<T>::unpack(raw[u], f);
+            Elem<T>::unpack(settle_row<ESZ>(raw[u], col + u * TEAM * EPV, a.cols), f);
 #pragma unroll
             for (int i = 0; i < EPV; i++) f[i] *= a.scale;
             store_row<ESZ>(to, col + u * TEAM * EPV, a.cols, Elem<T>::pack(f));
@@ -49,30 +49,90 @@ __global__ __launch_bounds__(256) void k_embedding(const EmbeddingArgs a)
 
 struct TableArgs {
     uint64_t dy, keys, order, heads, tails, dtable;  // heads, tails: fp32 [chunks][cols]
-    int64_t n, chunks, chunk0, vocab, row0;
-    int cols, chunk, rows, across;  // tokens of a chunk, rows of the table for a workgroup, teams across the columns
+    int64_t n, chunks, vocab, group0, chunk_groups;  // the launch's first workgroup; the workgroups of chunks, before those of zeros
+    int cols, chunk, rows, across;                   // tokens of a chunk, rows of the table for a workgroup, teams across the columns
     float scale;
 };
 
-// A lane sums the columns of one vector over a chunk; neighbouring workgroups are `across` parts of the same chunks.
-template <class T, int TEAM>
-__global__ __launch_bounds__(256) void k_embedding_chunks(const TableArgs a)
+// The first of the sorted keys that is not below k, by a wavefront: 64 probes at once, three steps for 262144 keys.
+DEV int64_t first_by_wave(const GLOBAL u32 *keys, int64_t n, int64_t k)
 {
-    constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, TEAMS = 256 / TEAM, U = 8;
-    int64_t chunk = a.chunk0 + (int64_t)(blockIdx.x / (u32)a.across) * TEAMS + (TEAM < 256 ? threadIdx.x / TEAM : 0);
-    if (TEAM == 64) chunk = __builtin_amdgcn_readfirstlane((int)chunk);  // a wavefront's: keys and places in scalar registers
-    if (chunk >= a.chunks) return;
-    const int col = (int)(blockIdx.x % (u32)a.across * TEAM + threadIdx.x % TEAM) * EPV;
-    if (col >= a.cols) return;
-    const GLOBAL u32 *keys = as_global<const u32>(a.keys), *order = as_global<const u32>(a.order);
-    const int64_t begin = chunk * a.chunk, end = begin + a.chunk < a.n ? begin + a.chunk : a.n;
-    const u32 none = 0xFFFFFFFFu;
-    const u32 previous = begin > 0 ? keys[begin - 1] : none, next = end < a.n ? keys[end] : none;
+    const int lane = threadIdx.x & 63;
+    int64_t lo = 0;
+    while (n > 0) {  // the answer is in lo to lo + n
+        const int64_t step = (n + 63) >> 6, at = (int64_t)lane * step + step - 1;
+        const bool below = at < n && keys[lo + at] < k;  // a run of lanes from the first on
+        const int count = __builtin_popcountll(__ballot(below));
+        lo += count * step;
+        n -= count * step;
+        if (n > step - 1) n = step - 1;
+    }
+    return lo;
+}
+
+// Zeros in those of up to 64 rows of the table that no token has, each run of them as one piece of memory.
+template <int ESZ>
+DEV void fill_empty(const TableArgs &a, int64_t group, int64_t *starts, int64_t *ends)
+{
+    const int64_t first = group * a.rows;
+    const GLOBAL u32 *keys = as_global<const u32>(a.keys);
+    if (threadIdx.x < 128) {
+        const int end = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
+        const int64_t at = first_by_wave(keys, a.n, end ? first + a.rows : first);
+        if ((threadIdx.x & 63) == 0) ends[end] = at;
+    }
+    __syncthreads();
+    if ((int)threadIdx.x <= a.rows) starts[threadIdx.x] = ends[0] + first_at(keys + ends[0], ends[1] - ends[0], first + threadIdx.x);
+    __syncthreads();
+    const int lane = threadIdx.x & 63;
+    uint64_t empty = __ballot(lane < a.rows && first + lane < a.vocab && starts[lane] == starts[lane + 1]);
+    while (empty) {
+        const int from = __builtin_ctzll(empty);
+        const uint64_t filled = ~(empty >> from);
+        const int count = filled ? __builtin_ctzll(filled) : 64;
+        empty = from + count >= 64 ? 0 : empty & (~(uint64_t)0 << (from + count));
+        const int64_t bytes = (int64_t)count * a.cols * ESZ;
+        const uint64_t to = a.dtable + (uint64_t)(first + from) * (uint64_t)a.cols * ESZ;
+        for (int64_t at = (int64_t)threadIdx.x * 16; at < bytes; at += 4096) {
+            if (at + 16 <= bytes) *as_global<u32x4_a1>(to + (uint64_t)at) = u32x4{0, 0, 0, 0};
+            else store_row<ESZ, false>(to + (uint64_t)at, 0, (int)((bytes - at) / ESZ), u32x4{0, 0, 0, 0});
+        }
+    }
+}
+
+// A lane sums the columns of one vector over a chunk of CHUNK tokens; neighbouring workgroups are `across` parts of the
+// same chunks.  The chunk's tokens are read into LDS first: then every row's address is known, and U rows are on their way at once.
+template <class T, int TEAM, int CHUNK>
+__global__ __launch_bounds__(256) void k_embedding_backward(const TableArgs a)
+{
+    constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, TEAMS = 256 / TEAM, U = 16;
+    constexpr u32 NONE = 0xFFFFFFFFu;
+    __shared__ u32 keys[TEAMS * CHUNK + 2], order[TEAMS * CHUNK];  // and the neighbours' keys
+    __shared__ int64_t starts[65], ends[2];
+    const int64_t group = a.group0 + blockIdx.x;
+    if (group >= a.chunk_groups) {
+        fill_empty<ESZ>(a, group - a.chunk_groups, starts, ends);
+        return;
+    }
+    const int64_t chunk0 = group / a.across * TEAMS, first = chunk0 * CHUNK;
+    for (int i = threadIdx.x; i < TEAMS * CHUNK + 2; i += 256) {
+        const int64_t at = first + i - 1;
+        keys[i] = at >= 0 && at < a.n ? as_global<const u32>(a.keys)[at] : NONE;
+    }
+    for (int i = threadIdx.x; i < TEAMS * CHUNK; i += 256)
+        if (first + i < a.n) order[i] = as_global<const u32>(a.order)[first + i];
+    __syncthreads();
+    const int team = TEAM == 64 ? __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64) : (int)threadIdx.x / TEAM;
+    const int64_t chunk = chunk0 + team;
+    const int col = ((int)(group % a.across) * TEAM + (int)threadIdx.x % TEAM) * EPV;
+    if (chunk >= a.chunks || col >= a.cols) return;
+    const u32 *key = keys + 1 + team * CHUNK, *from = order + team * CHUNK;
+    const u32 previous = key[-1], next = key[CHUNK];
     float acc[EPV] = {};
-    u32 current = none;
+    u32 current = NONE;
 
     auto leave = [&](bool last) {  // the run of `current` ends, or the chunk does
-        if (current == none || current >= (u32)a.vocab) return;
+        if (current >= (u32)a.vocab) return;
         const bool goes_on = last && next == current;
         if (current != previous && !goes_on) {
             float f[EPV];
@@ -86,26 +146,23 @@ __global__ __launch_bounds__(256) void k_embedding_chunks(const TableArgs a)
         for (int i = 0; i < EPV; i += 4)
             store_row<4, false>(sums, col + i, a.cols, u32x4{as_u(acc[i]), as_u(acc[i + 1]), as_u(acc[i + 2]), as_u(acc[i + 3])});
     };
-    for (int64_t at = begin; at < end; at += U) {
+    for (int at = 0; at < CHUNK; at += U) {
         u32x4 raw[U];
-        u32 key[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            key[u] = at + u < end ? keys[at + u] : none;
-            raw[u] = u32x4{0, 0, 0, 0};
-            if (key[u] < (u32)a.vocab) raw[u] = load_row<ESZ>(a.dy + (uint64_t)order[at + u] * (uint64_t)a.cols * ESZ, col, a.cols);
+            raw[u] = fetch_row<ESZ>(a.dy + (uint64_t)from[at + u] * (uint64_t)a.cols * ESZ, col, key[at + u] < (u32)a.vocab ? a.cols : 0);
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            if (key[u] == none) continue;
-            if (key[u] != current) {
+            const u32 k = key[at + u];
+            if (k != current) {
                 leave(false);
-                current = key[u];
+                current = k;
 #pragma unroll
                 for (int i = 0; i < EPV; i++) acc[i] = 0.0f;
             }
             float f[EPV];
-            Elem<T>::unpack(raw[u], f);
+            Elem<T>::unpack(settle_row<ESZ>(raw[u], col, a.cols), f);
 #pragma unroll
             for (int i = 0; i < EPV; i++) acc[i] += f[i];
         }
@@ -113,44 +170,42 @@ __global__ __launch_bounds__(256) void k_embedding_chunks(const TableArgs a)
     leave(true);
 }
 
-// The table's rows: zeros where no token is, the chunks' sums where there are several.
-template <class T, int TEAM>
-__global__ __launch_bounds__(256) void k_embedding_table(const TableArgs a)
+// The runs of several chunks: a workgroup to the chunk where one begins and 64 vectors of columns; its four wavefronts
+// share the chunks, and add up in their order.
+template <class T>
+__global__ __launch_bounds__(256) void k_embedding_join(const TableArgs a)
 {
-    constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, TEAMS = 256 / TEAM;
-    __shared__ int64_t starts[256];
-    const int64_t first = a.row0 + (int64_t)blockIdx.x * a.rows;
-    if ((int)threadIdx.x <= a.rows) starts[threadIdx.x] = first_at(as_global<const u32>(a.keys), a.n, first + threadIdx.x);
-    __syncthreads();
-    const int lane = threadIdx.x % TEAM;
-    for (int r = threadIdx.x / TEAM; r < a.rows && first + r < a.vocab; r += TEAMS) {
-        const int64_t s = starts[r], e = starts[r + 1];
-        const uint64_t to = a.dtable + (uint64_t)(first + r) * (uint64_t)a.cols * ESZ;
-        if (s == e) {
-            for (int col = lane * EPV; col < a.cols; col += TEAM * EPV) store_row<ESZ>(to, col, a.cols, u32x4{0, 0, 0, 0});
-            continue;
-        }
-        const int64_t c0 = s / a.chunk, c1 = (e - 1) / a.chunk;
-        if (c0 == c1) continue;  // written with its chunk
-        for (int col = lane * EPV; col < a.cols; col += TEAM * EPV) {
-            float acc[EPV];
+    constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV;
+    __shared__ float add[3][64][EPV + 1];
+    const int64_t group = a.group0 + blockIdx.x, chunk = group / a.across, begin = chunk * a.chunk, end = begin + a.chunk;
+    const GLOBAL u32 *keys = as_global<const u32>(a.keys);
+    if (end >= a.n) return;
+    const u32 key = keys[end - 1];
+    if (key >= (u32)a.vocab || keys[end] != key) return;                      // no run goes on
+    if (begin > 0 && keys[begin] == key && keys[begin - 1] == key) return;  // it began before
+    const int64_t last = (first_by_wave(keys, a.n, (int64_t)key + 1) - 1) / a.chunk, count = last - chunk + 1;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64, col = ((int)(group % a.across) * 64 + lane) * EPV;
+    const int64_t from = chunk + count * wave / 4, to = chunk + count * (wave + 1) / 4;
+    float acc[EPV] = {};
+#pragma unroll 8
+    for (int64_t c = from; c < to; c++) {
+        const uint64_t sums = (c == chunk ? a.tails : a.heads) + (uint64_t)(c * a.cols) * 4;
 #pragma unroll
-            for (int i = 0; i < EPV; i++) acc[i] = 0.0f;
-#pragma unroll 4
-            for (int64_t c = c0; c <= c1; c++) {
-                const uint64_t sums = (c == c0 ? a.tails : a.heads) + (uint64_t)(c * a.cols) * 4;
+        for (int i = 0; i < EPV; i += 4) {
+            const u32x4 v = load_row<4, false>(sums, col + i, a.cols);
 #pragma unroll
-                for (int i = 0; i < EPV; i += 4) {
-                    const u32x4 v = load_row<4, false>(sums, col + i, a.cols);
-#pragma unroll
-                    for (int j = 0; j < 4; j++) acc[i + j] += as_f(v[j]);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < EPV; i++) acc[i] *= a.scale;
-            store_row<ESZ>(to, col, a.cols, Elem<T>::pack(acc));
+            for (int j = 0; j < 4; j++) acc[i + j] += as_f(v[j]);
         }
     }
+    if (wave > 0) {
+#pragma unroll
+        for (int i = 0; i < EPV; i++) add[wave - 1][lane][i] = acc[i];
+    }
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int i = 0; i < EPV; i++) acc[i] = (((acc[i] + add[0][lane][i]) + add[1][lane][i]) + add[2][lane][i]) * a.scale;
+    store_row<ESZ>(a.dtable + (uint64_t)key * (uint64_t)a.cols * ESZ, col, a.cols, Elem<T>::pack(acc));
 }
 
 // ---------------------------------------------------------------------------
@@ -158,10 +213,13 @@ __global__ __launch_bounds__(256) void k_embedding_table(const TableArgs a)
 // ---------------------------------------------------------------------------
 static int embedding_team(int64_t vectors) { return vectors <= 8 ? 8 : vectors <= 64 ? 64 : 256; }
 
-#define EMBEDDING_KERNEL(K, dtype, team)                                                                                  \
-    (dtype == TFTQ_F32   ? team == 8 ? (const void *)K<float, 8> : team == 64 ? (const void *)K<float, 64> : (const void *)K<float, 256>            \
-     : dtype == TFTQ_F16 ? team == 8 ? (const void *)K<f16_tag, 8> : team == 64 ? (const void *)K<f16_tag, 64> : (const void *)K<f16_tag, 256>      \
-                         : team == 8 ? (const void *)K<bf16_tag, 8> : team == 64 ? (const void *)K<bf16_tag, 64> : (const void *)K<bf16_tag, 256>)
+#define EMBEDDING_TEAMS(K, T, ...) \
+    (team == 8 ? (const void *)K<T, 8 __VA_ARGS__> : team == 64 ? (const void *)K<T, 64 __VA_ARGS__> : (const void *)K<T, 256 __VA_ARGS__>)
+#define EMBEDDING_KERNEL(K, ...)                                \
+    (dtype == TFTQ_F32   ? EMBEDDING_TEAMS(K, float, __VA_ARGS__)   \
+     : dtype == TFTQ_F16 ? EMBEDDING_TEAMS(K, f16_tag, __VA_ARGS__) \
+                         : EMBEDDING_TEAMS(K, bf16_tag, __VA_ARGS__))
+#define EMBEDDING_COMMA ,
 
 extern "C" int tftq_embedding(int dtype, int id_bytes, const void *ids, int64_t n, const void *table, int64_t vocab, int64_t cols,
                               int64_t row_stride, float scale, void *out, int device, void *stream)
@@ -175,7 +233,7 @@ extern "C" int tftq_embedding(int dtype, int id_bytes, const void *ids, int64_t 
     if (scope.err != hipSuccess) return (int)scope.err;
     const int size = dtype_size(dtype), team = embedding_team((cols * size + 15) / 16), teams = 256 / team;
     EmbeddingArgs a = {(uint64_t)ids, (uint64_t)table, (uint64_t)out, row_stride * size, 0, n, vocab, (int)cols, id_bytes == 8, scale};
-    const void *k = EMBEDDING_KERNEL(k_embedding, dtype, team);
+    const void *k = EMBEDDING_KERNEL(k_embedding, );
     const int64_t at_once = ROWS_THREADS / team;
     for (; a.row0 < n; a.row0 += at_once) {
         void *args[] = {(void *)&a};
@@ -184,14 +242,9 @@ extern "C" int tftq_embedding(int dtype, int id_bytes, const void *ids, int64_t 
     return 0;
 }
 
-// Tokens of a chunk: 32, and with more than 8192 tokens as many as there are chunks for every eight, so that neither a
-// chunk nor the sums of one row are long.
-static int embedding_chunk(int64_t n)
-{
-    int chunk = 32;
-    while ((int64_t)chunk * chunk * 8 < n) chunk *= 2;
-    return chunk;
-}
+// Tokens of a chunk: neither a chunk nor the sums of one row of the table are to be long, and there are as many chunks of
+// one token as a chunk has tokens when it has the root of all.
+static int embedding_chunk(int64_t n) { return n <= 8192 ? 16 : n <= 131072 ? 64 : 256; }
 
 extern "C" int64_t tftq_embedding_backward_workspace(int64_t n, int64_t vocab, int64_t cols)
 {
@@ -230,25 +283,25 @@ extern "C" int tftq_embedding_backward(int dtype, int id_bytes, const void *ids,
     a.cols = (int)cols;
     a.across = (int)across;
     a.scale = scale;
-    void *args[] = {(void *)&a};
+    const int64_t row_bytes = cols * size, groups_at_once = ROWS_THREADS / 256;
+    a.rows = (int)std::min<int64_t>(64, std::max<int64_t>(1, 65536 / row_bytes));
+    a.chunk_groups = (a.chunks + teams - 1) / teams * across;
     if (n) {
         const SortArgs s = {(uint64_t)ids, id_bytes == 8, n, (u32)vocab, skip >= 0 && skip < vocab ? (u32)skip : (u32)vocab, keys, order, 0, 0};
         if (const int rc = sort_numbers(s, workspace, st)) return rc;
-        const void *k = EMBEDDING_KERNEL(k_embedding_chunks, dtype, team);
-        const int64_t at_once = std::max<int64_t>(1, ROWS_THREADS / 256 / across) * teams;
-        for (; a.chunk0 < a.chunks; a.chunk0 += at_once)
-            if (const int rc = (int)hipLaunchKernel(k, dim3((unsigned)((std::min(at_once, a.chunks - a.chunk0) + teams - 1) / teams * across)),
-                                                    dim3(256), args, 0, st))
-                return rc;
     }
-    // 64 KB of the table to a workgroup, 255 rows at most: the search for where its rows' tokens begin is one for all
-    const int64_t row_bytes = cols * size;
-    a.rows = (int)std::min<int64_t>(255, std::max<int64_t>(teams, 65536 / row_bytes));
-    const void *k = EMBEDDING_KERNEL(k_embedding_table, dtype, team);
-    const int64_t groups = (vocab + a.rows - 1) / a.rows, at_once = ROWS_THREADS / 256;
-    for (int64_t done = 0; done < groups; done += at_once) {
-        a.row0 = done * a.rows;
-        if (const int rc = (int)hipLaunchKernel(k, dim3((unsigned)std::min(at_once, groups - done)), dim3(256), args, 0, st)) return rc;
-    }
-    return 0;
+    auto launch = [&](const void *k, int64_t groups) {
+        void *args[] = {(void *)&a};
+        for (a.group0 = 0; a.group0 < groups; a.group0 += groups_at_once)
+            if (const int rc = (int)hipLaunchKernel(k, dim3((unsigned)std::min(groups_at_once, groups - a.group0)), dim3(256), args, 0, st)) return rc;
+        return 0;
+    };
+    const void *k = a.chunk == 16   ? EMBEDDING_KERNEL(k_embedding_backward, EMBEDDING_COMMA 16)
+                    : a.chunk == 64 ? EMBEDDING_KERNEL(k_embedding_backward, EMBEDDING_COMMA 64)
+                                    : EMBEDDING_KERNEL(k_embedding_backward, EMBEDDING_COMMA 256);
+    if (const int rc = launch(k, a.chunk_groups + (vocab + a.rows - 1) / a.rows)) return rc;
+    if (a.chunks < 2) return 0;
+    a.across = (int)((vectors + 63) / 64);
+    k = dtype == TFTQ_F32 ? (const void *)k_embedding_join<float> : dtype == TFTQ_F16 ? (const void *)k_embedding_join<f16_tag> : (const void *)k_embedding_join<bf16_tag>;
+    return launch(k, (a.chunks - 1) * a.across);
 }

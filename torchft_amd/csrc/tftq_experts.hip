@@ -23,10 +23,10 @@ struct ExpertArgs {
 };
 
 // x [tokens] -> y [tokens k] by places; elements of ESZ bytes.
-template <int ESZ, int TEAM>
+template <int ESZ, int TEAM, int U>
 __global__ __launch_bounds__(256) void k_dispatch(const ExpertArgs a)
 {
-    constexpr int EPV = 16 / ESZ, TEAMS = 256 / TEAM, U = 4;
+    constexpr int EPV = 16 / ESZ, TEAMS = 256 / TEAM;
     const int lane = threadIdx.x % TEAM;
     const int64_t token = a.token0 + (int64_t)blockIdx.x * TEAMS + threadIdx.x / TEAM;
     if (token >= a.tokens) return;
@@ -36,12 +36,14 @@ __global__ __launch_bounds__(256) void k_dispatch(const ExpertArgs a)
     for (int col = lane * EPV; col < a.cols; col += U * TEAM * EPV) {
         u32x4 raw[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) raw[u] = load_row<ESZ>(from, col + u * TEAM * EPV, a.cols);
+        for (int u = 0; u < U; u++) raw[u] = fetch_row<ESZ>(from, col + u * TEAM * EPV, a.cols);
+#pragma unroll
+        for (int u = 0; u < U; u++) raw[u] = settle_row<ESZ>(raw[u], col + u * TEAM * EPV, a.cols);
         for (int s = 0; s < a.k; s++) {
             const u32 place = position[s];
             const uint64_t to = a.y + (uint64_t)place * (uint64_t)a.cols * ESZ;
 #pragma unroll
-            for (int u = 0; u < U; u++) store_row<ESZ>(to, col + u * TEAM * EPV, a.cols, place < used ? raw[u] : u32x4{0, 0, 0, 0});
+            for (int u = 0; u < U; u++) store_row<ESZ, false>(to, col + u * TEAM * EPV, a.cols, place < used ? raw[u] : u32x4{0, 0, 0, 0});
         }
     }
 }
@@ -53,84 +55,118 @@ DEV float expert_weight(const ExpertArgs &a, int64_t choice)
     return a.wide ? as_global<const float>(a.weights)[choice] : Elem<T>::load(a.weights, choice);
 }
 
-template <class T, int TEAM>
+// Four choices at a time are on their way.
+template <class T, int TEAM, int U>
 __global__ __launch_bounds__(256) void k_combine(const ExpertArgs a)
 {
-    constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, TEAMS = 256 / TEAM, U = 2;
+    constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, TEAMS = 256 / TEAM, S = 4;
     const int lane = threadIdx.x % TEAM;
     const int64_t token = a.token0 + (int64_t)blockIdx.x * TEAMS + threadIdx.x / TEAM;
     if (token >= a.tokens) return;
     const u32 used = *as_global<const u32>(a.used);
-    const GLOBAL u32 *position = as_global<const u32>(a.position) + token * a.k;
+    const int64_t choice = token * a.k;
     const uint64_t to = a.y + (uint64_t)(token * a.cols) * ESZ;
     for (int col = lane * EPV; col < a.cols; col += U * TEAM * EPV) {
         float acc[U][EPV] = {};
-#pragma unroll 2
-        for (int s = 0; s < a.k; s++) {
-            const u32 place = position[s];
-            if (place >= used) continue;
-            const uint64_t from = a.rows + (uint64_t)place * (uint64_t)a.rows_stride;
-            const float w = expert_weight<T>(a, token * a.k + s);
-            u32x4 raw[U];
+        for (int s0 = 0; s0 < a.k; s0 += S) {
+            u32 place[S];
+            float w[S];
+            u32x4 raw[S][U];
 #pragma unroll
-            for (int u = 0; u < U; u++) raw[u] = load_row<ESZ>(from, col + u * TEAM * EPV, a.cols);
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                float f[EPV];
-                Elem<T>::unpack(raw[u], f);
-#pragma unroll
-                for (int i = 0; i < EPV; i++) acc[u][i] = __builtin_fmaf(w, f[i], acc[u][i]);
+            for (int s = 0; s < S; s++) {
+                const bool there = s0 + s < a.k;
+                place[s] = there ? as_global<const u32>(a.position)[choice + s0 + s] : used;
+                w[s] = there ? expert_weight<T>(a, choice + s0 + s) : 0.0f;
             }
+#pragma unroll
+            for (int s = 0; s < S; s++) {
+                // a choice without an expert: no elements, and a weight that leaves them at nothing
+                const int cols = place[s] < used ? a.cols : 0;
+                if (cols == 0) w[s] = 0.0f;
+#pragma unroll
+                for (int u = 0; u < U; u++)
+                    raw[s][u] = fetch_row<ESZ>(a.rows + (uint64_t)place[s] * (uint64_t)a.rows_stride, col + u * TEAM * EPV, cols);
+            }
+#pragma unroll
+            for (int s = 0; s < S; s++)
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    float f[EPV];
+                    Elem<T>::unpack(settle_row<ESZ>(raw[s][u], col + u * TEAM * EPV, a.cols), f);
+#pragma unroll
+                    for (int i = 0; i < EPV; i++) acc[u][i] = __builtin_fmaf(w[s], f[i], acc[u][i]);
+                }
         }
 #pragma unroll
         for (int u = 0; u < U; u++) store_row<ESZ>(to, col + u * TEAM * EPV, a.cols, Elem<T>::pack(acc[u]));
     }
 }
 
-// x is dy.  NV: vectors of dy that a lane keeps for all choices; 0: read again for every one.
-template <class T, int TEAM, int NV>
+// x is dy.  NV: vectors of dy that a lane keeps for all choices, and of the rows of two choices that are on their way; MORE:
+// the row is longer, and read again for every choice.
+template <class T, int TEAM, int NV, bool MORE>
 __global__ __launch_bounds__(256) void k_combine_backward(const ExpertArgs a)
 {
-    constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, TEAMS = 256 / TEAM;
-    __shared__ float lds[TEAM > 64 ? TEAM / 64 : 1];
+    constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, TEAMS = 256 / TEAM, S = 2;
+    __shared__ float lds[TEAM > 64 ? 2 * (TEAM / 64) : 1];
     const int lane = threadIdx.x % TEAM;
     const int64_t token = a.token0 + (int64_t)blockIdx.x * TEAMS + threadIdx.x / TEAM;
     if (token >= a.tokens) return;
     const u32 used = *as_global<const u32>(a.used);
     const uint64_t from = a.x + (uint64_t)(token * a.x_stride);
-    u32x4 dy[NV > 0 ? NV : 1];
+    u32x4 dy[NV];
 #pragma unroll
-    for (int v = 0; v < NV; v++) dy[v] = load_row<ESZ>(from, (v * TEAM + lane) * EPV, a.cols);
-    for (int s = 0; s < a.k; s++) {
-        const int64_t choice = token * a.k + s;
-        const u32 place = as_global<const u32>(a.position)[choice];
-        const bool live = place < used;
-        const float w = live ? expert_weight<T>(a, choice) : 0.0f;
-        const uint64_t row = a.rows + (uint64_t)place * (uint64_t)a.rows_stride, to = a.drows + (uint64_t)place * (uint64_t)a.cols * ESZ;
-        float dot = 0.0f;
-        auto step = [&](const u32x4 g, int col) {
-            u32x4 r = {0, 0, 0, 0};
-            if (live && a.dweights) r = load_row<ESZ>(row, col, a.cols);
-            float f[EPV], d[EPV];
-            Elem<T>::unpack(r, f);
-            Elem<T>::unpack(g, d);
+    for (int v = 0; v < NV; v++) dy[v] = fetch_row<ESZ, !MORE>(from, (v * TEAM + lane) * EPV, a.cols);
+    for (int s0 = 0; s0 < a.k; s0 += S) {
+        u32 place[S];
+        float w[S], dot[S];
+        bool live[S];
 #pragma unroll
-            for (int i = 0; i < EPV; i++) {
-                dot = __builtin_fmaf(d[i], f[i], dot);
-                d[i] = live ? d[i] * w : 0.0f;
+        for (int s = 0; s < S; s++) {
+            const int64_t choice = token * a.k + s0 + s;
+            const bool there = s0 + s < a.k;
+            place[s] = there ? as_global<const u32>(a.position)[choice] : used;
+            live[s] = place[s] < used;
+            w[s] = live[s] ? expert_weight<T>(a, choice) : 0.0f;
+            dot[s] = 0.0f;
+        }
+        for (int base = 0; base < (MORE ? a.cols : 1); base += NV * TEAM * EPV) {
+            u32x4 raw[S][NV];
+#pragma unroll
+            for (int s = 0; s < S; s++)
+#pragma unroll
+                for (int v = 0; v < NV; v++)
+                    raw[s][v] = fetch_row<ESZ>(a.rows + (uint64_t)place[s] * (uint64_t)a.rows_stride, base + (v * TEAM + lane) * EPV,
+                                               live[s] && a.dweights ? a.cols : 0);
+            if (MORE && (base > 0 || s0 > 0)) {
+#pragma unroll
+                for (int v = 0; v < NV; v++) dy[v] = fetch_row<ESZ, false>(from, base + (v * TEAM + lane) * EPV, a.cols);
             }
-            if (a.drows) store_row<ESZ>(to, col, a.cols, Elem<T>::pack(d));
-        };
-        if (NV > 0) {
 #pragma unroll
-            for (int v = 0; v < NV; v++) step(dy[v], (v * TEAM + lane) * EPV);
-        } else {
-            for (int col = lane * EPV; col < a.cols; col += TEAM * EPV) step(load_row<ESZ, false>(from, col, a.cols), col);
+            for (int v = 0; v < NV; v++) {
+                const int col = base + (v * TEAM + lane) * EPV;
+                float d[EPV];
+                Elem<T>::unpack(settle_row<ESZ>(dy[v], col, a.cols), d);
+#pragma unroll
+                for (int s = 0; s < S; s++) {
+                    if (s0 + s >= a.k) continue;
+                    float f[EPV], out[EPV];
+                    Elem<T>::unpack(settle_row<ESZ>(raw[s][v], col, a.cols), f);
+#pragma unroll
+                    for (int i = 0; i < EPV; i++) {
+                        dot[s] = __builtin_fmaf(d[i], f[i], dot[s]);
+                        out[i] = live[s] ? d[i] * w[s] : 0.0f;
+                    }
+                    if (a.drows) store_row<ESZ, false>(a.drows + (uint64_t)place[s] * (uint64_t)a.cols * ESZ, col, a.cols, Elem<T>::pack(out));
+                }
+            }
         }
         if (!a.dweights) continue;
-        dot = team_sum<TEAM>(dot, lds);
-        if (lane == 0) {
-            const float dw = live ? dot : 0.0f;
+        team_sum2<TEAM>(dot[0], dot[1], lds);
+        if (lane < S && s0 + lane < a.k) {
+            const int64_t choice = token * a.k + s0 + lane;
+            const bool taken = lane ? live[1] : live[0];
+            const float dw = taken ? lane ? dot[1] : dot[0] : 0.0f;
             if (a.wide) as_global<float>(a.dweights)[choice] = dw;
             else Elem<T>::store(a.dweights, choice, dw);
         }
@@ -144,7 +180,25 @@ static bool experts_ok(int64_t tokens, int64_t k, int64_t cols)
 {
     return rows_ok(tokens, cols) && k >= 0 && k <= ROWS_MOST && (k == 0 || tokens <= ROWS_MOST / k);
 }
-static int expert_team(int64_t vectors) { return vectors <= 8 ? 8 : vectors <= 128 ? 64 : 256; }
+// Lanes and vectors of a row that is taken in one go; longer ones take several.  Four vectors a lane, unless they are fewer.
+static RowShape expert_shape(int64_t vectors)
+{
+    if (vectors <= 8) return {8, 1};
+    if (vectors <= 16) return {8, 2};
+    if (vectors <= 32) return {8, 4};
+    if (vectors <= 64) return {16, 4};
+    if (vectors <= 128) return {64, 2};
+    if (vectors <= 256) return {64, 4};
+    return {256, 2};
+}
+#define EXPERT_SHAPES(K, X)                                           \
+    (shape.team == 8     ? shape.nv == 1   ? (const void *)K<X, 8, 1>     \
+                           : shape.nv == 2 ? (const void *)K<X, 8, 2>     \
+                                           : (const void *)K<X, 8, 4>     \
+     : shape.team == 16  ? (const void *)K<X, 16, 4>                      \
+     : shape.team == 256 ? (const void *)K<X, 256, 2>                     \
+     : shape.nv == 2     ? (const void *)K<X, 64, 2>                      \
+                         : (const void *)K<X, 64, 4>)
 
 static int expert_launch(const void *kernel, ExpertArgs a, int team, hipStream_t st)
 {
@@ -161,7 +215,7 @@ static int expert_launch(const void *kernel, ExpertArgs a, int team, hipStream_t
 extern "C" int64_t tftq_expert_sort_workspace(int64_t choices, int64_t experts)
 {
     if (!rows_ok(choices, experts)) return TFTQ_E_SHAPE;
-    return sort_workspace(choices, experts) + ((choices * 4 + 15) & ~(int64_t)15);
+    return sort_workspace(choices, experts) + (sort_needs_keys(choices, experts) ? (choices * 4 + 15) & ~(int64_t)15 : 0);
 }
 
 extern "C" int tftq_expert_sort(int id_bytes, const void *chosen, int64_t choices, int64_t experts, int32_t *order, int32_t *position,
@@ -170,12 +224,12 @@ extern "C" int tftq_expert_sort(int id_bytes, const void *chosen, int64_t choice
     const int64_t bytes = tftq_expert_sort_workspace(choices, experts);
     if (bytes < 0) return (int)bytes;
     if (id_bytes != 4 && id_bytes != 8) return TFTQ_E_ARG;
-    if (!offsets || (choices && (!chosen || !order || !position || !workspace || ((uintptr_t)workspace & 15)))) return TFTQ_E_ARG;
+    if (!offsets || (choices && (!chosen || !order || !position)) || (bytes && (!workspace || ((uintptr_t)workspace & 15)))) return TFTQ_E_ARG;
     if (workspace_bytes < bytes) return TFTQ_E_SIZE;
     DeviceScope scope(device);
     if (scope.err != hipSuccess) return (int)scope.err;
     const SortArgs a = {(uint64_t)chosen, id_bytes == 8, choices, (u32)experts, (u32)experts,
-                        choices ? (uint64_t)workspace + (uint64_t)sort_workspace(choices, experts) : 0, (uint64_t)order, (uint64_t)position, (uint64_t)offsets};
+                        sort_needs_keys(choices, experts) ? (uint64_t)workspace + (uint64_t)sort_workspace(choices, experts) : 0, (uint64_t)order, (uint64_t)position, (uint64_t)offsets};
     return sort_numbers(a, workspace, (hipStream_t)stream);
 }
 
@@ -188,7 +242,7 @@ extern "C" int tftq_dispatch(int element_bytes, const void *x, int64_t x_stride,
     if (!x || !position || !used || !out || x_stride < (tokens > 1 ? cols : 0)) return TFTQ_E_ARG;
     DeviceScope scope(device);
     if (scope.err != hipSuccess) return (int)scope.err;
-    const int team = expert_team((cols * element_bytes + 15) / 16);
+    const RowShape shape = expert_shape((cols * element_bytes + 15) / 16);
     ExpertArgs a = {};
     a.x = (uint64_t)x;
     a.x_stride = x_stride * element_bytes;
@@ -198,8 +252,8 @@ extern "C" int tftq_dispatch(int element_bytes, const void *x, int64_t x_stride,
     a.tokens = tokens;
     a.cols = (int)cols;
     a.k = (int)k;
-#define K(ESZ) (team == 8 ? (const void *)k_dispatch<ESZ, 8> : team == 64 ? (const void *)k_dispatch<ESZ, 64> : (const void *)k_dispatch<ESZ, 256>)
-    return expert_launch(element_bytes == 1 ? K(1) : element_bytes == 2 ? K(2) : K(4), a, team, (hipStream_t)stream);
+#define K(ESZ) EXPERT_SHAPES(k_dispatch, ESZ)
+    return expert_launch(element_bytes == 1 ? K(1) : element_bytes == 2 ? K(2) : K(4), a, shape.team, (hipStream_t)stream);
 #undef K
 }
 
@@ -212,7 +266,8 @@ extern "C" int tftq_combine(int dtype, int weight_dtype, const void *rows, int64
     if ((k && (!rows || !position || !used)) || !out || rows_stride < (tokens * k > 1 ? cols : 0)) return TFTQ_E_ARG;
     DeviceScope scope(device);
     if (scope.err != hipSuccess) return (int)scope.err;
-    const int size = dtype_size(dtype), team = expert_team((cols * size + 15) / 16);
+    const int size = dtype_size(dtype);
+    const RowShape shape = expert_shape((cols * size + 15) / 16);
     ExpertArgs a = {};
     a.rows = (uint64_t)rows;
     a.rows_stride = rows_stride * size;
@@ -224,8 +279,8 @@ extern "C" int tftq_combine(int dtype, int weight_dtype, const void *rows, int64
     a.tokens = tokens;
     a.cols = (int)cols;
     a.k = (int)k;
-#define K(T) (team == 8 ? (const void *)k_combine<T, 8> : team == 64 ? (const void *)k_combine<T, 64> : (const void *)k_combine<T, 256>)
-    return expert_launch(dtype == TFTQ_F32 ? K(float) : dtype == TFTQ_F16 ? K(f16_tag) : K(bf16_tag), a, team, (hipStream_t)stream);
+#define K(T) EXPERT_SHAPES(k_combine, T)
+    return expert_launch(dtype == TFTQ_F32 ? K(float) : dtype == TFTQ_F16 ? K(f16_tag) : K(bf16_tag), a, shape.team, (hipStream_t)stream);
 #undef K
 }
 
@@ -242,7 +297,8 @@ extern "C" int tftq_combine_backward(int dtype, int weight_dtype, const void *dy
     if (scope.err != hipSuccess) return (int)scope.err;
     const int size = dtype_size(dtype);
     const int64_t vectors = (cols * size + 15) / 16;
-    const int team = expert_team(vectors), nv = vectors <= team ? 1 : vectors <= 2 * team ? 2 : vectors <= 4 * team ? 4 : 0;
+    const RowShape shape = expert_shape(vectors);
+    const int per_lane = (int)std::min<int64_t>(5, (vectors + shape.team - 1) / shape.team);
     ExpertArgs a = {};
     a.x = (uint64_t)dy;
     a.x_stride = dy_stride * size;
@@ -257,13 +313,16 @@ extern "C" int tftq_combine_backward(int dtype, int weight_dtype, const void *dy
     a.tokens = tokens;
     a.cols = (int)cols;
     a.k = (int)k;
-#define K(T)                                                                                                          \
-    (team == 8    ? (const void *)k_combine_backward<T, 8, 1>                                                         \
-     : team == 64 ? nv == 1 ? (const void *)k_combine_backward<T, 64, 1> : (const void *)k_combine_backward<T, 64, 2> \
-     : nv == 1    ? (const void *)k_combine_backward<T, 256, 1>                                                       \
-     : nv == 2    ? (const void *)k_combine_backward<T, 256, 2>                                                       \
-     : nv == 4    ? (const void *)k_combine_backward<T, 256, 4>                                                       \
-                  : (const void *)k_combine_backward<T, 256, 0>)
-    return expert_launch(dtype == TFTQ_F32 ? K(float) : dtype == TFTQ_F16 ? K(f16_tag) : K(bf16_tag), a, team, (hipStream_t)stream);
+#define K(T)                                                                      \
+    (shape.team == 8     ? shape.nv == 1   ? (const void *)k_combine_backward<T, 8, 1, false>  \
+                           : shape.nv == 2 ? (const void *)k_combine_backward<T, 8, 2, false>  \
+                                           : (const void *)k_combine_backward<T, 8, 4, false>  \
+     : shape.team == 16  ? (const void *)k_combine_backward<T, 16, 4, false>                   \
+     : shape.team == 64  ? shape.nv == 2 ? (const void *)k_combine_backward<T, 64, 2, false>   \
+                                         : (const void *)k_combine_backward<T, 64, 4, false>   \
+     : per_lane <= 2     ? (const void *)k_combine_backward<T, 256, 2, false>                  \
+     : per_lane <= 4     ? (const void *)k_combine_backward<T, 256, 4, false>                  \
+                         : (const void *)k_combine_backward<T, 256, 4, true>)
+    return expert_launch(dtype == TFTQ_F32 ? K(float) : dtype == TFTQ_F16 ? K(f16_tag) : K(bf16_tag), a, shape.team, (hipStream_t)stream);
 #undef K
 }

@@ -23,15 +23,23 @@ struct NormArgs {
 template <class T>
 struct Weights {
     u32x4 raw, more;
-    DEV void load(uint64_t weight, int wide, int col, int cols)
+    DEV void fetch(uint64_t weight, int wide, int col, int cols)
     {
         constexpr int EPV = Elem<T>::EPV;
         more = u32x4{0, 0, 0, 0};
         if (!weight) return;
         if (EPV == 8 && wide) {
-            raw = load_row<4, false>(weight, col, cols);
-            more = load_row<4, false>(weight, col + 4, cols);
-        } else raw = load_row<Elem<T>::ESZ, false>(weight, col, cols);
+            raw = fetch_row<4, false>(weight, col, cols);
+            more = fetch_row<4, false>(weight, col + 4, cols);
+        } else raw = fetch_row<Elem<T>::ESZ, false>(weight, col, cols);
+    }
+    DEV void settle(uint64_t weight, int wide, int col, int cols)
+    {
+        if (!weight) return;
+        if (Elem<T>::EPV == 8 && wide) {
+            raw = settle_row<4>(raw, col, cols);
+            more = settle_row<4>(more, col + 4, cols);
+        } else raw = settle_row<Elem<T>::ESZ>(raw, col, cols);
     }
     DEV void unpack(uint64_t weight, int wide, float (&w)[Elem<T>::EPV]) const
     {
@@ -53,6 +61,8 @@ template <class T, int TEAM, int NV, bool FP8>
 __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void k_rms_norm(const NormArgs a)
 {
     constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, TEAMS = TEAM > 256 ? 1 : 256 / TEAM;
+    // weights in the registers of the residual, so that two workgroups of long rows run on a compute unit
+    constexpr bool LATE = TEAM * NV >= 2048;
     __shared__ float lds[TEAM > 64 ? TEAM / 64 : 1];
     const int lane = threadIdx.x % TEAM;
     const int64_t row = a.row0 + (int64_t)blockIdx.x * TEAMS + threadIdx.x / TEAM;
@@ -63,31 +73,39 @@ __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void k_rms_norm(const Norm
     u32x4 raw[NV], res[NV];
     Weights<T> weights[NV];
 #pragma unroll
-    for (int v = 0; v < NV; v++) raw[v] = load_row<ESZ>(px, (v * TEAM + lane) * EPV, a.cols);
+    for (int v = 0; v < NV; v++) raw[v] = fetch_row<ESZ>(px, (v * TEAM + lane) * EPV, a.cols);
     if (a.residual) {
 #pragma unroll
-        for (int v = 0; v < NV; v++) res[v] = load_row<ESZ>(pr, (v * TEAM + lane) * EPV, a.cols);
+        for (int v = 0; v < NV; v++) res[v] = fetch_row<ESZ>(pr, (v * TEAM + lane) * EPV, a.cols);
     }
+    auto fetch_weights = [&] {
 #pragma unroll
-    for (int v = 0; v < NV; v++) weights[v].load(a.weight, a.wide, (v * TEAM + lane) * EPV, a.cols);
+        for (int v = 0; v < NV; v++) weights[v].fetch(a.weight, a.wide, (v * TEAM + lane) * EPV, a.cols);
+    };
+    if (!LATE) fetch_weights();
     float sum = 0.0f;
 #pragma unroll
     for (int v = 0; v < NV; v++) {
+        const int col = (v * TEAM + lane) * EPV;
         float f[EPV];
+        raw[v] = settle_row<ESZ>(raw[v], col, a.cols);
         Elem<T>::unpack(raw[v], f);
         if (a.residual) {
             float r[EPV];
-            Elem<T>::unpack(res[v], r);
+            Elem<T>::unpack(settle_row<ESZ>(res[v], col, a.cols), r);
 #pragma unroll
             for (int i = 0; i < EPV; i++) f[i] += r[i];
             raw[v] = Elem<T>::pack(f);
-            store_row<ESZ>(a.h + at, (v * TEAM + lane) * EPV, a.cols, raw[v]);
+            store_row<ESZ>(a.h + at, col, a.cols, raw[v]);
             Elem<T>::unpack(raw[v], f);
         }
 #pragma unroll
         for (int i = 0; i < EPV; i++) sum = __builtin_fmaf(f[i], f[i], sum);
     }
+    if (LATE) fetch_weights();
     const float r = inverse_root(team_sum<TEAM>(sum, lds) * a.inv_cols, a.eps);
+#pragma unroll
+    for (int v = 0; v < NV; v++) weights[v].settle(a.weight, a.wide, (v * TEAM + lane) * EPV, a.cols);
     if constexpr (!FP8) {
 #pragma unroll
         for (int v = 0; v < NV; v++) {
@@ -170,7 +188,8 @@ __global__ __launch_bounds__(1024) void k_rms_norm_long(const NormArgs a)
             float f[EPV], w[EPV];
             Elem<T>::unpack(load_row<ESZ, false>(again, col, a.cols), f);
             Weights<T> weights;
-            weights.load(a.weight, a.wide, col, a.cols);
+            weights.fetch(a.weight, a.wide, col, a.cols);
+            weights.settle(a.weight, a.wide, col, a.cols);
             weights.unpack(a.weight, a.wide, w);
 #pragma unroll
             for (int i = 0; i < EPV; i++) f[i] = f[i] * r * w[i];
@@ -219,19 +238,40 @@ __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void k_rms_norm_backward(c
         for (int i = 0; i < EPV; i++) acc[v][i] = 0.0f;
     Weights<T> weights[NV];
 #pragma unroll
-    for (int v = 0; v < NV; v++) weights[v].load(a.weight, a.wide, (v * TEAM + lane) * EPV, a.cols);
+    for (int v = 0; v < NV; v++) weights[v].fetch(a.weight, a.wide, (v * TEAM + lane) * EPV, a.cols);
 
-    for (int64_t row = (int64_t)blockIdx.x * TEAMS + team; row < a.rows; row += (int64_t)gridDim.x * TEAMS) {
+    // the next row is on its way while this one is worked on, where there are registers for it
+    constexpr bool AHEAD = TEAM * NV * EPV <= 8192;
+    const int64_t step = (int64_t)gridDim.x * TEAMS;
+    u32x4 dy_next[NV], h_next[NV], dh_next[NV];
+    auto fetch = [&](int64_t row) {
+        const bool there = row < a.rows;
         const uint64_t at = (uint64_t)(row * a.cols) * ESZ, ph = a.h + (uint64_t)(row * a.h_stride);
-        u32x4 dy[NV], h[NV], dh[NV];
+        const int cols = there ? a.cols : 0;
 #pragma unroll
-        for (int v = 0; v < NV; v++) dy[v] = load_row<ESZ>(a.dy + at, (v * TEAM + lane) * EPV, a.cols);
+        for (int v = 0; v < NV; v++) dy_next[v] = fetch_row<ESZ>(a.dy + at, (v * TEAM + lane) * EPV, cols);
 #pragma unroll
-        for (int v = 0; v < NV; v++) h[v] = load_row<ESZ>(ph, (v * TEAM + lane) * EPV, a.cols);
+        for (int v = 0; v < NV; v++) h_next[v] = fetch_row<ESZ>(ph, (v * TEAM + lane) * EPV, cols);
         if (a.dh) {
 #pragma unroll
-            for (int v = 0; v < NV; v++) dh[v] = load_row<ESZ>(a.dh + at, (v * TEAM + lane) * EPV, a.cols);
+            for (int v = 0; v < NV; v++) dh_next[v] = fetch_row<ESZ>(a.dh + at, (v * TEAM + lane) * EPV, cols);
         }
+    };
+    int64_t row = (int64_t)blockIdx.x * TEAMS + team;
+    if (AHEAD) fetch(row);
+#pragma unroll
+    for (int v = 0; v < NV; v++) weights[v].settle(a.weight, a.wide, (v * TEAM + lane) * EPV, a.cols);
+    for (; row < a.rows; row += step) {
+        if (!AHEAD) fetch(row);
+        const uint64_t at = (uint64_t)(row * a.cols) * ESZ;
+        u32x4 dy[NV], h[NV], dh[NV];
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+            dy[v] = settle_row<ESZ>(dy_next[v], (v * TEAM + lane) * EPV, a.cols);
+            h[v] = settle_row<ESZ>(h_next[v], (v * TEAM + lane) * EPV, a.cols);
+            if (a.dh) dh[v] = settle_row<ESZ>(dh_next[v], (v * TEAM + lane) * EPV, a.cols);
+        }
+        if (AHEAD) fetch(row + step);
         float squares = 0.0f, along = 0.0f;
 #pragma unroll
         for (int v = 0; v < NV; v++) {
@@ -289,26 +329,36 @@ __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void k_rms_norm_backward(c
 }
 
 // Rows too long for that: first r and c of every row, then dx and the sums, a workgroup to 256 vectors of columns
-// and a share of the rows.
+// and a share of the rows, four rows at a time.
 template <class T>
 __global__ __launch_bounds__(1024) void k_rms_norm_backward_long(const NormBackwardArgs a, uint64_t factors)
 {
-    constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV;
+    constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, U = 2, STEP = 1024 * EPV;
     __shared__ float lds[32];
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const uint64_t at = (uint64_t)(row * a.cols) * ESZ, ph = a.h + (uint64_t)(row * a.h_stride);
         float squares = 0.0f, along = 0.0f;
-        for (int col = threadIdx.x * EPV; col < a.cols; col += 1024 * EPV) {
-            float f[EPV], g[EPV], w[EPV];
-            Weights<T> weights;
-            weights.load(a.weight, a.wide, col, a.cols);
-            Elem<T>::unpack(load_row<ESZ, false>(ph, col, a.cols), f);
-            Elem<T>::unpack(load_row<ESZ, false>(a.dy + at, col, a.cols), g);
-            weights.unpack(a.weight, a.wide, w);
+        for (int col = threadIdx.x * EPV; col < a.cols; col += U * STEP) {
+            Weights<T> weights[U];
+            u32x4 h[U], dy[U];
 #pragma unroll
-            for (int i = 0; i < EPV; i++) {
-                squares = __builtin_fmaf(f[i], f[i], squares);
-                along = __builtin_fmaf(g[i] * w[i], f[i], along);
+            for (int u = 0; u < U; u++) {
+                h[u] = fetch_row<ESZ, false>(ph, col + u * STEP, a.cols);
+                dy[u] = fetch_row<ESZ, false>(a.dy + at, col + u * STEP, a.cols);
+                weights[u].fetch(a.weight, a.wide, col + u * STEP, a.cols);
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                float f[EPV], g[EPV], w[EPV];
+                weights[u].settle(a.weight, a.wide, col + u * STEP, a.cols);
+                weights[u].unpack(a.weight, a.wide, w);
+                Elem<T>::unpack(settle_row<ESZ>(h[u], col + u * STEP, a.cols), f);
+                Elem<T>::unpack(settle_row<ESZ>(dy[u], col + u * STEP, a.cols), g);
+#pragma unroll
+                for (int i = 0; i < EPV; i++) {
+                    squares = __builtin_fmaf(f[i], f[i], squares);
+                    along = __builtin_fmaf(g[i] * w[i], f[i], along);
+                }
             }
         }
         team_sum2<1024>(squares, along, lds);
@@ -319,27 +369,42 @@ __global__ __launch_bounds__(1024) void k_rms_norm_backward_long(const NormBackw
 template <class T>
 __global__ __launch_bounds__(256) void k_rms_norm_backward_columns(const NormBackwardArgs a, uint64_t factors)
 {
-    constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV;
+    constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, U = 4;
     const int col = (int)(blockIdx.x * 256 + threadIdx.x) * EPV;
     if (col >= a.cols) return;
     float acc[EPV] = {}, w[EPV];
     Weights<T> weights;
-    weights.load(a.weight, a.wide, col, a.cols);
+    weights.fetch(a.weight, a.wide, col, a.cols);
+    weights.settle(a.weight, a.wide, col, a.cols);
     weights.unpack(a.weight, a.wide, w);
-    for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
-        const uint64_t at = (uint64_t)(row * a.cols) * ESZ;
-        float f[EPV], g[EPV], d[EPV];
-        Elem<T>::unpack(load_row<ESZ>(a.h + (uint64_t)(row * a.h_stride), col, a.cols), f);
-        Elem<T>::unpack(load_row<ESZ>(a.dy + at, col, a.cols), g);
-        if (a.dh) Elem<T>::unpack(load_row<ESZ>(a.dh + at, col, a.cols), d);
-        const float r = as_global<const float>(factors)[2 * row], c = as_global<const float>(factors)[2 * row + 1];
+    for (int64_t first = (int64_t)blockIdx.y * U; first < a.rows; first += (int64_t)gridDim.y * U) {
+        u32x4 h[U], dy[U], dh[U];
+        float r[U], c[U];
 #pragma unroll
-        for (int i = 0; i < EPV; i++) {
-            acc[i] = __builtin_fmaf(g[i], f[i] * r, acc[i]);
-            f[i] = r * (g[i] * w[i] - f[i] * c);
-            if (a.dh) f[i] += d[i];
+        for (int u = 0; u < U; u++) {
+            const int64_t row = first + u < a.rows ? first + u : a.rows - 1;
+            const uint64_t at = (uint64_t)(row * a.cols) * ESZ;
+            h[u] = fetch_row<ESZ>(a.h + (uint64_t)(row * a.h_stride), col, a.cols);
+            dy[u] = fetch_row<ESZ>(a.dy + at, col, a.cols);
+            if (a.dh) dh[u] = fetch_row<ESZ>(a.dh + at, col, a.cols);
+            r[u] = as_global<const float>(factors)[2 * row];
+            c[u] = as_global<const float>(factors)[2 * row + 1];
         }
-        if (a.dx) store_row<ESZ>(a.dx + at, col, a.cols, Elem<T>::pack(f));
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (first + u >= a.rows) continue;
+            float f[EPV], g[EPV], d[EPV];
+            Elem<T>::unpack(settle_row<ESZ>(h[u], col, a.cols), f);
+            Elem<T>::unpack(settle_row<ESZ>(dy[u], col, a.cols), g);
+            if (a.dh) Elem<T>::unpack(settle_row<ESZ>(dh[u], col, a.cols), d);
+#pragma unroll
+            for (int i = 0; i < EPV; i++) {
+                acc[i] = __builtin_fmaf(g[i], f[i] * r[u], acc[i]);
+                f[i] = r[u] * (g[i] * w[i] - f[i] * c[u]);
+                if (a.dh) f[i] += d[i];
+            }
+            if (a.dx) store_row<ESZ>(a.dx + (uint64_t)((first + u) * a.cols) * ESZ, col, a.cols, Elem<T>::pack(f));
+        }
     }
     if (!a.sums) return;
 #pragma unroll
@@ -348,15 +413,15 @@ __global__ __launch_bounds__(256) void k_rms_norm_backward_columns(const NormBac
                             u32x4{as_u(acc[i]), as_u(acc[i + 1]), as_u(acc[i + 2]), as_u(acc[i + 3])});
 }
 
-// out[c] = the sum of sums[p][c] over p, rounded once: 16 lanes to 64 columns, 16 of the parts side by side.
+// out[c] = the sum of sums[p][c] over p, rounded once: 4 lanes to 16 columns, 64 of the parts side by side.
 template <class T>
 __global__ __launch_bounds__(256) void k_column_sums(uint64_t sums, int64_t parts, int cols, uint64_t out)
 {
-    __shared__ float add[16][65];
-    const int lane = threadIdx.x & 15, group = threadIdx.x >> 4, col = (int)blockIdx.x * 64 + lane * 4;
+    __shared__ float add[64][17];
+    const int lane = threadIdx.x & 3, group = threadIdx.x >> 2, col = (int)blockIdx.x * 16 + lane * 4;
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int64_t p = group; p < parts; p += 16) {
+#pragma unroll 8
+    for (int64_t p = group; p < parts; p += 64) {
         const u32x4 v = load_row<4, false>(sums + (uint64_t)p * (uint64_t)cols * 4, col, cols);
 #pragma unroll
         for (int i = 0; i < 4; i++) s[i] += as_f(v[i]);
@@ -364,12 +429,18 @@ __global__ __launch_bounds__(256) void k_column_sums(uint64_t sums, int64_t part
 #pragma unroll
     for (int i = 0; i < 4; i++) add[group][lane * 4 + i] = s[i];
     __syncthreads();
-    if (threadIdx.x >= 64) return;
+    // 16 threads to a column, then one
+    const int c = threadIdx.x & 15, g = threadIdx.x >> 4;
+    const float part = (add[g][c] + add[g + 16][c]) + (add[g + 32][c] + add[g + 48][c]);
+    __syncthreads();
+    add[g][c] = part;
+    __syncthreads();
+    if (threadIdx.x >= 16) return;
     float total = 0.0f;
 #pragma unroll
-    for (int g = 0; g < 16; g++) total += add[g][threadIdx.x];
-    const int64_t c = (int64_t)blockIdx.x * 64 + threadIdx.x;
-    if (c < cols) Elem<T>::store(out, c, total);
+    for (int i = 0; i < 16; i++) total += add[i][c];
+    const int64_t at = (int64_t)blockIdx.x * 16 + c;
+    if (at < cols) Elem<T>::store(out, at, total);
 }
 
 // The values of 8-bit rows, a lane for EPV of them.
@@ -417,48 +488,58 @@ __global__ __launch_bounds__(256) void k_fp8_rows(uint64_t codes, uint64_t scale
 // ---------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------
-// Lanes and vectors to a row of `vectors`; {0, 0}: too long for registers.
-static RowShape norm_shape(int64_t vectors, bool backward)
+// Lanes and vectors to a row of `vectors`; {0, 0}: too long for registers.  Two vectors a lane hide more of memory's latency
+// than one, and lanes that a row leaves idle cost as much as others: rows of 16 vectors (163840 fp16) take 17.5 us with 8 lanes of
+// two, 18.4 with 16, 47 with 64; rows of 512 (8192 bf16 with a residual) 45.8 with 512 lanes, 47.5 with 256 of two, one
+// row 3.4 and 3.8.
+static RowShape norm_shape(int64_t vectors)
 {
     if (vectors <= 8) return {8, 1};
-    if (vectors <= 16) return {16, 1};
-    if (vectors <= 32) return {32, 1};
-    if (vectors <= 64) return {64, 1};
+    if (vectors <= 16) return {8, 2};
+    if (vectors <= 32) return {16, 2};
+    if (vectors <= 64) return {32, 2};
     if (vectors <= 128) return {64, 2};
     if (vectors <= 256) return {256, 1};
-    if (vectors <= 512) return {256, 2};
-    if (vectors <= 1024) return backward ? RowShape{1024, 1} : RowShape{256, 4};
+    if (vectors <= 512) return {512, 1};
+    if (vectors <= 1024) return {512, 2};
     if (vectors <= 2048) return {1024, 2};
-    if (vectors <= 4096 && !backward) return {1024, 4};
+    if (vectors <= 4096) return {1024, 4};
     return {0, 0};
 }
 
-// K(lanes, vectors) of the shapes that both directions have.
-#define NORM_CASES(K)                                        \
-    switch (shape.team * 16 + shape.nv) {                    \
-    case 8 * 16 + 1: K(8, 1); break;                         \
-    case 16 * 16 + 1: K(16, 1); break;                       \
-    case 32 * 16 + 1: K(32, 1); break;                       \
-    case 64 * 16 + 1: K(64, 1); break;                       \
-    case 64 * 16 + 2: K(64, 2); break;                       \
-    case 256 * 16 + 1: K(256, 1); break;                     \
-    case 256 * 16 + 2: K(256, 2); break;                     \
-    case 1024 * 16 + 2: K(1024, 2); break;                   \
-    }
+// The same for the backward pass, whose lanes keep a column's sum and the next row beside: us of rows of 42
+// vectors (65536 bf16) 42.3 with 16 lanes of three, 47.2 with 64 of one; of 251 (8192 fp32) 30.0 with 64 of four, 42.1 with
+// 256 of one; of 256 (16384 bf16, where four take all registers) 58.2 and 51.9; of 512 (8192 bf16) 49.9 with 512 of
+// one, 52.9 with 256 of two.
+static RowShape norm_backward_shape(int64_t vectors, int size)
+{
+    if (vectors <= 8) return {8, 1};
+    if (vectors <= 16) return {8, 2};
+    if (vectors <= 32) return {16, 2};
+    if (vectors <= 48) return {16, 3};
+    if (vectors <= 64) return {32, 2};
+    if (vectors <= 128) return {64, 2};
+    if (vectors <= 192) return {64, 3};
+    if (vectors <= 256) return size == 4 ? RowShape{64, 4} : RowShape{256, 1};
+    if (vectors <= 512) return {512, 1};
+    if (vectors <= 1024) return {512, 2};
+    if (vectors <= 2048) return {512, 4};
+    return {0, 0};
+}
+
+#define SHAPE(TEAM, NV) case TEAM * 16 + NV: K(TEAM, NV); break;
 
 template <class T, bool FP8>
 static int norm(NormArgs a, hipStream_t st)
 {
-    const RowShape shape = norm_shape((a.cols + Elem<T>::EPV - 1) / Elem<T>::EPV, false);
+    const RowShape shape = norm_shape((a.cols + Elem<T>::EPV - 1) / Elem<T>::EPV);
     const void *k = (const void *)k_rms_norm_long<T, FP8>;
 #define K(TEAM, NV) k = (const void *)k_rms_norm<T, TEAM, NV, FP8>
-    NORM_CASES(K)
-    if (shape.nv == 4) {
-        if (shape.team == 256) K(256, 4);
-        else K(1024, 4);
+    switch (shape.team * 16 + shape.nv) {
+        SHAPE(8, 1) SHAPE(8, 2) SHAPE(16, 2) SHAPE(32, 2) SHAPE(64, 2) SHAPE(256, 1) SHAPE(512, 1) SHAPE(512, 2) SHAPE(1024, 2) SHAPE(1024, 4)
     }
 #undef K
-    const int threads = shape.team == 0 || shape.team > 256 ? 1024 : 256, teams = shape.team == 0 ? 1 : threads / shape.team;
+    const int threads = shape.team == 0 ? 1024 : shape.team > 256 ? shape.team : 256, teams = shape.team == 0 ? 1 : threads / shape.team;
     const int64_t at_once = ROWS_THREADS / threads * teams;
     for (a.row0 = 0; a.row0 < a.rows; a.row0 += at_once) {
         const int64_t left = std::min(at_once, a.rows - a.row0);
@@ -468,22 +549,22 @@ static int norm(NormArgs a, hipStream_t st)
     return 0;
 }
 
-// Workgroups of the backward kernels, whose sums k_column_sums adds up.
-constexpr int64_t NORM_GROUPS = 1024;
+// Workgroups of the backward kernels, whose sums k_column_sums adds up: as many as run at once with their registers, so that
+// none starts when the others end, and no more sums than that (8192 rows of 4096 bf16 49.9 us with 256, 52.8 with 512, 58.2
+// with 1024).
 static int64_t norm_parts(int64_t rows, int64_t cols, int size)
 {
-    const RowShape shape = norm_shape((cols * size + 15) / 16, true);
+    const RowShape shape = norm_backward_shape((cols * size + 15) / 16, size);
     const int64_t teams = shape.team == 0 || shape.team > 256 ? 1 : 256 / shape.team;
-    int64_t most = NORM_GROUPS;
-    if (shape.team == 0) most = std::min<int64_t>(64, std::max<int64_t>(1, ROWS_THREADS / (cols + 4096)));
-    if (shape.team > 256) most = NORM_GROUPS / 2;
+    int64_t most = shape.team > 256 ? 256 : 512;
+    if (shape.team == 0) most = std::max<int64_t>(1, 1280 / ((cols * size + 4095) / 4096));  // five for every compute unit
     return std::min(most, (rows + teams - 1) / teams);
 }
 
 template <class T>
 static int norm_backward(NormBackwardArgs a, uint64_t factors, int64_t parts, hipStream_t st)
 {
-    const RowShape shape = norm_shape((a.cols + Elem<T>::EPV - 1) / Elem<T>::EPV, true);
+    const RowShape shape = norm_backward_shape((a.cols + Elem<T>::EPV - 1) / Elem<T>::EPV, Elem<T>::ESZ);
     if (shape.team == 0) {
         void *args[] = {(void *)&a, (void *)&factors};
         int rc = (int)hipLaunchKernel((const void *)k_rms_norm_backward_long<T>, dim3((unsigned)std::min<int64_t>(a.rows, 2048)), dim3(1024),
@@ -494,9 +575,14 @@ static int norm_backward(NormBackwardArgs a, uint64_t factors, int64_t parts, hi
     }
     const void *k = nullptr;
 #define K(TEAM, NV) k = (const void *)k_rms_norm_backward<T, TEAM, NV>
-    NORM_CASES(K)
-    if (shape.team == 1024 && shape.nv == 1) K(1024, 1);
+    if constexpr (Elem<T>::ESZ == 4) {
+        if (shape.team == 64 && shape.nv == 4) K(64, 4);
+    } else if (shape.team == 256) K(256, 1);
+    switch (shape.team * 16 + shape.nv) {
+        SHAPE(8, 1) SHAPE(8, 2) SHAPE(16, 2) SHAPE(16, 3) SHAPE(32, 2) SHAPE(64, 2) SHAPE(64, 3) SHAPE(512, 1) SHAPE(512, 2) SHAPE(512, 4)
+    }
 #undef K
+#undef SHAPE
     void *args[] = {(void *)&a};
     return (int)hipLaunchKernel(k, dim3((unsigned)parts), dim3(shape.team > 256 ? shape.team : 256), args, 0, st);
 }
@@ -560,7 +646,7 @@ extern "C" int tftq_rms_norm_backward(int dtype, int weight_dtype, const void *d
     const void *k = weight_dtype == TFTQ_F32   ? (const void *)k_column_sums<float>
                     : weight_dtype == TFTQ_F16 ? (const void *)k_column_sums<f16_tag>
                                                : (const void *)k_column_sums<bf16_tag>;
-    return (int)hipLaunchKernel(k, dim3((unsigned)((cols + 63) / 64)), dim3(256), args, 0, st);
+    return (int)hipLaunchKernel(k, dim3((unsigned)((cols + 15) / 16)), dim3(256), args, 0, st);
 }
 
 extern "C" int tftq_fp8_rows_dequantize(int dtype, const void *codes, const float *scales, int64_t rows, int64_t cols, void *out, int device,

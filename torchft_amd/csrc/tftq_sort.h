@@ -9,13 +9,15 @@ struct SortArgs {
     int64_t n;
     u32 classes;       // numbers outside [0, classes), and `skip`, count as `classes`, the last
     u32 skip;          // none: classes
-    uint64_t keys;     // u32 [n]: the numbers in order
+    uint64_t keys;     // u32 [n]: the numbers in order; 0: not wanted (sort_needs_keys)
     uint64_t order;    // u32 [n]: where they stood
     uint64_t position; // u32 [n]: where they went; 0: not wanted
     uint64_t offsets;  // u32 [classes + 1]: how many are below 0, 1, ... classes; 0: not wanted
 };
 
 __attribute__((visibility("hidden"))) int64_t sort_workspace(int64_t n, int64_t classes);  // bytes, a multiple of 16
+// Whether `keys` has to be there for `offsets`.
+__attribute__((visibility("hidden"))) bool sort_needs_keys(int64_t n, int64_t classes);
 __attribute__((visibility("hidden"))) int sort_numbers(const SortArgs &a, void *workspace, hipStream_t st);
 
 // The first of n ascending keys that is not below k.

@@ -1,12 +1,13 @@
-// Stable sort of n whole numbers below `classes`, least digit first, up to 8 bits a pass.
+// Stable sort of n whole numbers below `classes`, least digit first.
 //
 // A wavefront ranks 64 numbers at once: a ballot for each bit of the digit tells every lane who has the same
-// digit, the lanes below it among them are its rank, and a counter in LDS for each wavefront and digit goes on from one 64 to the
-// next.  The counters' prefix sums in the order (digit, wavefront) are the places.  Nothing is added with
-// atomics whose order could show: equal numbers keep their order.
+// digit, the lanes below it among them are its rank, and a counter in LDS for each wavefront and digit goes on from one
+// 64 to the next.  The counters' prefix sums in the order (digit, wavefront) are the places.  Nothing is added
+// with atomics whose order could show: equal numbers keep their order.
 //
-// Up to 16384 numbers stay in one workgroup's registers and LDS for all passes: one launch (times below).  More
-// go over two launches a pass, tiles of 8192: counts, then places.
+// Few numbers stay in one workgroup's registers and LDS for all passes of up to 9 bits: one launch, bound by the four
+// vector units of one compute unit (four instructions a bit and number).  More go over two launches a pass of up to 8
+// bits: counts of tiles of 2048, then places (three from 131072 on, where every tile would read too many counts).
 #include "tftq_sort.h"
 
 DEV u32 sort_key(const SortArgs &a, int64_t i)
@@ -15,196 +16,216 @@ DEV u32 sort_key(const SortArgs &a, int64_t i)
     return (uint64_t)id < a.classes && (u32)id != a.skip ? (u32)id : a.classes;
 }
 
-// The rank of every item among those of its digit in the wavefront's part, in the order of i, then lanes; `mine` ends
-// with how many of every digit there are.
+// The rank of every item among those of its digit in the wavefront's part, in the order of i, then lanes; `mine`, this
+// wavefront's counters, ends with how many of every digit there are.  Items from `items` on are not live.
 template <int ITEMS>
-DEV void sort_rank(const u32 (&digit)[ITEMS], const bool (&live)[ITEMS], int width, u32 *mine, u32 (&rank)[ITEMS])
+DEV void sort_rank(const u32 (&digit)[ITEMS], const bool (&live)[ITEMS], int items, int width, u32 *mine, u32 (&rank)[ITEMS])
 {
-    const uint64_t below = ((uint64_t)1 << (threadIdx.x & 63)) - 1;
+    u32 low[ITEMS], high[ITEMS];  // who has the same digit
 #pragma unroll
     for (int i = 0; i < ITEMS; i++) {
-        uint64_t same = __ballot(live[i]);
-        for (int b = 0; b < width; b++) {
-            const bool bit = digit[i] >> b & 1;
-            const uint64_t with = __ballot(bit);
-            same &= bit ? with : ~with;
+        const uint64_t all = __ballot(live[i]);
+        low[i] = (u32)all;
+        high[i] = (u32)(all >> 32);
+    }
+    for (int b = 0; b < width; b++) {
+#pragma unroll
+        for (int i = 0; i < ITEMS; i++) {
+            if (ITEMS > 4 && i >= items) continue;
+            const u32 mask = (u32)((int)(digit[i] << (31 - b)) >> 31);
+            const uint64_t with = __ballot(mask != 0);
+            low[i] &= ~((u32)with ^ mask);
+            high[i] &= ~((u32)(with >> 32) ^ mask);
         }
+    }
+#pragma unroll
+    for (int i = 0; i < ITEMS; i++) {
         rank[i] = 0;
         if (live[i]) {
-            const u32 before = __builtin_popcountll(same & below), base = mine[digit[i]];
+            const u32 before = __builtin_amdgcn_mbcnt_hi(high[i], __builtin_amdgcn_mbcnt_lo(low[i], 0)), base = mine[digit[i]];
             rank[i] = base + before;
             // every lane has read its counter before the first of its digit moves it on: one wavefront, in order
             __builtin_amdgcn_wave_barrier();
-            if (before == 0) mine[digit[i]] = base + (u32)__builtin_popcountll(same);
+            if (before == 0) mine[digit[i]] = base + (u32)(__builtin_popcount(low[i]) + __builtin_popcount(high[i]));
             __builtin_amdgcn_wave_barrier();
         }
     }
 }
 
-// Exclusive prefix sums of the counters in the order (digit, wavefront), in place; 256 digits.  sums: a u32 a wavefront.
-template <int THREADS>
-DEV void sort_scan(u32 (*counts)[256], u32 *sums)
+// The exclusive prefix sum of v over the workgroup's threads; sums: a u32 a wavefront, free again behind the next barrier.
+DEV u32 sort_prefix(u32 v, u32 *sums)
 {
-    constexpr int Q = THREADS / 256;  // threads a digit, four wavefronts' counters to each
-    const int digit = threadIdx.x / Q, q = threadIdx.x % Q * 4, lane = threadIdx.x & 63;
-    u32 c[4], s = 0;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        c[i] = counts[q + i][digit];
-        s += c[i];
-    }
-    u32 up = s;
+    u32 up = v;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
         const u32 from = (u32)__shfl_up((int)up, d);
-        if (lane >= d) up += from;
+        if ((int)(threadIdx.x & 63) >= d) up += from;
     }
-    if (lane == 63) sums[threadIdx.x / 64] = up;
+    if ((threadIdx.x & 63) == 63) sums[threadIdx.x / 64] = up;
     __syncthreads();
-    u32 base = up - s;
+    u32 base = up - v;
     for (int w = 0; w < (int)threadIdx.x / 64; w++) base += sums[w];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        counts[q + i][digit] = base;
-        base += c[i];
-    }
-    __syncthreads();
+    return base;
 }
 
-// n numbers in one workgroup, wavefront w the w-th share of 64 ITEMS.
+// n numbers in one workgroup, wavefront w the w-th share of them.
 template <int THREADS, int ITEMS>
 __global__ __launch_bounds__(THREADS) void k_sort_one(const SortArgs a, int passes, int width)
 {
-    constexpr int WAVES = THREADS / 64, MOST = THREADS * ITEMS;
-    __shared__ u32 counts[WAVES][256], sums[WAVES], keys[MOST];
+    constexpr int WAVES = THREADS / 64, MOST = THREADS * ITEMS, DIGITS = THREADS == 256 ? 256 : 512;
+    constexpr int Q = THREADS / DIGITS, EACH = WAVES / Q;  // threads to a digit, wavefronts' counters to a thread
+    __shared__ u32 counts[WAVES][DIGITS], sums[WAVES], keys[MOST];
     __shared__ uint16_t places[MOST];
-    const int n = (int)a.n, lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+    const int n = (int)a.n, lane = threadIdx.x & 63, items = (n + THREADS - 1) / THREADS, first = (int)(threadIdx.x / 64) * 64 * items + lane;
+    u32 *mine = counts[threadIdx.x / 64];
     u32 key[ITEMS], place[ITEMS], digit[ITEMS], rank[ITEMS];
     bool live[ITEMS];
 #pragma unroll
     for (int i = 0; i < ITEMS; i++) {
-        place[i] = (u32)(wave * 64 * ITEMS + i * 64 + lane);
-        live[i] = (int)place[i] < n;
+        place[i] = (u32)(first + i * 64);
+        live[i] = i < items && (int)place[i] < n;
         key[i] = live[i] ? sort_key(a, place[i]) : 0;
     }
     for (int pass = 0; pass < passes; pass++) {
-        for (int c = threadIdx.x; c < WAVES * 256; c += THREADS) (&counts[0][0])[c] = 0;
+        for (int c = threadIdx.x; c < WAVES * DIGITS; c += THREADS) (&counts[0][0])[c] = 0;
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < ITEMS; i++) digit[i] = key[i] >> (pass * width) & ((1u << width) - 1);
-        sort_rank<ITEMS>(digit, live, width, counts[wave], rank);
+        sort_rank<ITEMS>(digit, live, items, width, mine, rank);
         __syncthreads();
-        sort_scan<THREADS>(counts, sums);
+        {
+            const int d = threadIdx.x / Q, w = threadIdx.x % Q * EACH;
+            u32 c[EACH], s = 0;
+#pragma unroll
+            for (int i = 0; i < EACH; i++) {
+                c[i] = counts[w + i][d];
+                s += c[i];
+            }
+            u32 base = sort_prefix(s, sums);
+#pragma unroll
+            for (int i = 0; i < EACH; i++) {
+                counts[w + i][d] = base;
+                base += c[i];
+            }
+        }
+        __syncthreads();
 #pragma unroll
         for (int i = 0; i < ITEMS; i++)
             if (live[i]) {
-                const u32 to = counts[wave][digit[i]] + rank[i];
+                const u32 to = mine[digit[i]] + rank[i];
                 keys[to] = key[i];
                 places[to] = (uint16_t)place[i];
             }
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < ITEMS; i++) {
-            const int at = wave * 64 * ITEMS + i * 64 + lane;
+        for (int i = 0; i < ITEMS; i++)
             if (live[i]) {
-                key[i] = keys[at];
-                place[i] = places[at];
+                key[i] = keys[first + i * 64];
+                place[i] = places[first + i * 64];
             }
-        }
     }
 #pragma unroll
     for (int i = 0; i < ITEMS; i++) {
-        const int at = wave * 64 * ITEMS + i * 64 + lane;
         if (!live[i]) continue;
+        const int at = first + i * 64;
         if (a.keys) as_global<u32>(a.keys)[at] = key[i];
         as_global<u32>(a.order)[at] = place[i];
         if (a.position) as_global<u32>(a.position)[place[i]] = (u32)at;
     }
     if (a.offsets)
         for (int64_t c = threadIdx.x; c <= (int64_t)a.classes; c += THREADS)
-            as_global<u32>(a.offsets)[c] = (u32)first_at((const u32 *)keys, n, (u32)c);
+            as_global<u32>(a.offsets)[c] = (u32)first_at((const u32 *)keys, n, c);
 }
 
-constexpr int SORT_ITEMS = 8, SORT_TILE = 1024 * SORT_ITEMS, SORT_ONE = 16384;
+constexpr int SORT_ITEMS = 8, SORT_TILE = 256 * SORT_ITEMS;
+constexpr int SORT_DIRECT = 64;  // so many tiles read each other's counts themselves
 
 // A pass over many numbers: from ids (the first) or from keys and places.
 struct SortPass {
     uint64_t keys, places;  // 0: the ids themselves
-    uint64_t to_keys, to_places, position;
-    uint64_t counts;        // u32 [tiles][256]
-    int shift, width, tiles;
+    uint64_t to_keys, to_places, position, offsets;
+    uint64_t counts;        // u32 [256][pitch]: of a digit and a tile; with more than SORT_DIRECT tiles, then u32 [256] of all
+    int shift, width, tiles, pitch;
 };
 
 DEV u32 sort_read(const SortArgs &a, const SortPass &p, int64_t i) { return p.keys ? as_global<const u32>(p.keys)[i] : sort_key(a, i); }
 
-__global__ __launch_bounds__(1024) void k_sort_count(const SortArgs a, const SortPass p)
+__global__ __launch_bounds__(256) void k_sort_count(const SortArgs a, const SortPass p)
 {
     __shared__ u32 counts[256];
-    if (threadIdx.x < 256) counts[threadIdx.x] = 0;
+    counts[threadIdx.x] = 0;
     __syncthreads();
-    const int64_t first = (int64_t)blockIdx.x * SORT_TILE;
+    const int64_t first = (int64_t)blockIdx.x * SORT_TILE + threadIdx.x;
+    u32 key[SORT_ITEMS];
 #pragma unroll
-    for (int i = 0; i < SORT_ITEMS; i++) {
-        const int64_t at = first + i * 1024 + threadIdx.x;
-        if (at < a.n) atomicAdd(&counts[sort_read(a, p, at) >> p.shift & ((1u << p.width) - 1)], 1u);
-    }
+    for (int i = 0; i < SORT_ITEMS; i++) key[i] = first + i * 256 < a.n ? sort_read(a, p, first + i * 256) : 0;
+#pragma unroll
+    for (int i = 0; i < SORT_ITEMS; i++)
+        if (first + i * 256 < a.n) atomicAdd(&counts[key[i] >> p.shift & ((1u << p.width) - 1)], 1u);
     __syncthreads();
-    if (threadIdx.x < 256) as_global<u32>(p.counts)[(int64_t)blockIdx.x * 256 + threadIdx.x] = counts[threadIdx.x];
+    as_global<u32>(p.counts)[(int64_t)threadIdx.x * p.pitch + blockIdx.x] = counts[threadIdx.x];
 }
 
-__global__ __launch_bounds__(1024) void k_sort_place(const SortArgs a, const SortPass p)
+// A workgroup to a digit: its counts become how many there are in the tiles before.
+__global__ __launch_bounds__(256) void k_sort_before(const SortPass p)
 {
-    __shared__ u32 counts[16][256], sums[16], before[4][256], total[4][256], start[256];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64, d = threadIdx.x & 255, q = threadIdx.x >> 8;
-    for (int c = threadIdx.x; c < 16 * 256; c += 1024) (&counts[0][0])[c] = 0;
-    // of digit d: how many there are in all tiles, and in those before this one
-    u32 b = 0, t = 0;
-    for (int tile = q; tile < p.tiles; tile += 4) {
-        const u32 c = as_global<const u32>(p.counts)[(int64_t)tile * 256 + d];
-        t += c;
-        if (tile < (int)blockIdx.x) b += c;
+    __shared__ u32 sums[4];
+    GLOBAL u32 *row = as_global<u32>(p.counts) + (int64_t)blockIdx.x * p.pitch;
+    u32 base = 0;
+    for (int tile = 0; tile < p.tiles; tile += 256) {
+        const int at = tile + (int)threadIdx.x;
+        const u32 c = at < p.tiles ? row[at] : 0, before = sort_prefix(c, sums);
+        if (at < p.tiles) row[at] = base + before;
+        base += sums[0] + sums[1] + sums[2] + sums[3];
+        __syncthreads();
     }
-    before[q][d] = b;
-    total[q][d] = t;
-    __syncthreads();
-    u32 up = 0, own = 0;
-    if (threadIdx.x < 256) {
-        own = total[0][d] + total[1][d] + total[2][d] + total[3][d];
-        up = own;
-#pragma unroll
-        for (int s = 1; s < 64; s *= 2) {
-            const u32 from = (u32)__shfl_up((int)up, s);
-            if (lane >= s) up += from;
-        }
-        if (lane == 63) sums[wave] = up;
-    }
-    __syncthreads();
-    if (threadIdx.x < 256) {
-        u32 base = up - own;
-        for (int w = 0; w < wave; w++) base += sums[w];
-        start[d] = base + before[0][d] + before[1][d] + before[2][d] + before[3][d];
-    }
+    if (threadIdx.x == 0) as_global<u32>(p.counts)[(int64_t)256 * p.pitch + blockIdx.x] = base;
+}
+
+__global__ __launch_bounds__(256) void k_sort_place(const SortArgs a, const SortPass p)
+{
+    __shared__ u32 counts[4][256], sums[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64, d = threadIdx.x;
     u32 key[SORT_ITEMS], digit[SORT_ITEMS], rank[SORT_ITEMS], place[SORT_ITEMS];
     bool live[SORT_ITEMS];
-    const int64_t first = (int64_t)blockIdx.x * SORT_TILE + wave * 64 * SORT_ITEMS;
+    const int64_t first = (int64_t)blockIdx.x * SORT_TILE + wave * 64 * SORT_ITEMS + lane;
 #pragma unroll
     for (int i = 0; i < SORT_ITEMS; i++) {
-        const int64_t at = first + i * 64 + lane;
+        const int64_t at = first + i * 64;
         live[i] = at < a.n;
         key[i] = live[i] ? sort_read(a, p, at) : 0;
         place[i] = live[i] && p.keys ? as_global<const u32>(p.places)[at] : (u32)at;
-        digit[i] = key[i] >> p.shift & ((1u << p.width) - 1);
     }
-    sort_rank<SORT_ITEMS>(digit, live, p.width, counts[wave], rank);
-    __syncthreads();
-    // of every wavefront and digit: how many there are in the wavefronts before
-    if (threadIdx.x < 256) {
-        u32 s = start[d];
-        for (int w = 0; w < 16; w++) {
-            const u32 c = counts[w][d];
-            counts[w][d] = s;
-            s += c;
+    // of digit d: how many there are in all tiles, and in those before this one
+    u32 before = 0, total = 0;
+    if (p.tiles > SORT_DIRECT) {
+        before = as_global<const u32>(p.counts)[(int64_t)d * p.pitch + blockIdx.x];
+        total = as_global<const u32>(p.counts)[(int64_t)256 * p.pitch + d];
+    } else {
+        for (int tile = 0; tile < p.tiles; tile += 4) {
+            const u32x4 c = *(as_global<const u32x4>(p.counts + ((uint64_t)d * p.pitch + tile) * 4));
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (tile + i >= p.tiles) continue;
+                total += c[i];
+                if (tile + i < (int)blockIdx.x) before += c[i];
+            }
         }
+    }
+#pragma unroll
+    for (int w = 0; w < 4; w++) counts[w][d] = 0;
+    const u32 start = sort_prefix(total, sums);  // a barrier
+    if (p.offsets && blockIdx.x == 0 && d <= (int)a.classes) as_global<u32>(p.offsets)[d] = start;
+#pragma unroll
+    for (int i = 0; i < SORT_ITEMS; i++) digit[i] = key[i] >> p.shift & ((1u << p.width) - 1);
+    sort_rank<SORT_ITEMS>(digit, live, SORT_ITEMS, p.width, counts[wave], rank);
+    __syncthreads();
+    u32 s = start + before;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        const u32 c = counts[w][d];
+        counts[w][d] = s;
+        s += c;
     }
     __syncthreads();
 #pragma unroll
@@ -220,37 +241,67 @@ __global__ __launch_bounds__(1024) void k_sort_place(const SortArgs a, const Sor
 __global__ __launch_bounds__(256) void k_sort_offsets(const SortArgs a)
 {
     const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (c <= (int64_t)a.classes) as_global<u32>(a.offsets)[c] = (u32)first_at(as_global<const u32>(a.keys), a.n, (u32)c);
+    if (c <= (int64_t)a.classes) as_global<u32>(a.offsets)[c] = (u32)first_at(as_global<const u32>(a.keys), a.n, c);
 }
 
-static int sort_passes(int64_t classes)  // numbers from 0 to classes
+static int sort_bits(int64_t classes)  // numbers from 0 to classes
 {
     int bits = 1;
     while (classes >> bits) bits++;
     return bits;
 }
 
+// Whether one workgroup takes all.  Times of a sort with places and offsets, us, in one workgroup and in tiles:
+// 4096 numbers below 8 6.5, 8.7, below 255 7.7, 9.3, below 1000 11.0, 21.1; 8192 9.3, 8.8 / 12.9, 9.5 / 17.5, 21.9;
+// 16384 16.3, 9.2 / 23.7, 9.9 / 31.1, 22.9: one compute unit's scattered stores, and its ballots, against two launches a pass.
+static bool sort_one(int64_t n, int64_t classes) { return n <= (classes > 255 ? 8192 : 4096); }
+
+// Whether the offsets are a launch of their own, which searches the keys: a tile that knows all digits' places writes
+// them along with a sort of one pass, and one workgroup up to 2048.
+static bool sort_searches(int64_t n, int64_t classes) { return classes > (sort_one(n, classes) ? 2048 : 255); }
+
+static int64_t sort_pitch(int64_t n) { return ((n + SORT_TILE - 1) / SORT_TILE + 3) & ~(int64_t)3; }
+
 int64_t sort_workspace(int64_t n, int64_t classes)
 {
-    if (n <= SORT_ONE) return 0;
-    const int64_t tiles = (n + SORT_TILE - 1) / SORT_TILE, pairs = (sort_passes(classes) + 7) / 8 - 1;
-    return tiles * 1024 + std::min<int64_t>(pairs, 2) * ((n * 8 + 15) & ~(int64_t)15);
+    if (sort_one(n, classes)) return 0;
+    const int64_t pairs = (sort_bits(classes) + 7) / 8 - 1;
+    return (sort_pitch(n) + 1) * 1024 + std::min<int64_t>(pairs, 2) * ((n * 8 + 15) & ~(int64_t)15);
+}
+
+bool sort_needs_keys(int64_t n, int64_t classes) { return sort_searches(n, classes); }
+
+static int sort_offsets(SortArgs a, hipStream_t st)
+{
+    void *args[] = {(void *)&a};
+    return (int)hipLaunchKernel((const void *)k_sort_offsets, dim3((unsigned)(a.classes / 256 + 1)), dim3(256), args, 0, st);
 }
 
 int sort_numbers(const SortArgs &in, void *workspace, hipStream_t st)
 {
     SortArgs a = in;
-    const int bits = sort_passes(a.classes);
-    int passes = (bits + 7) / 8, width = (bits + passes - 1) / passes;
-    if (a.n <= SORT_ONE) {
+    const int bits = sort_bits(a.classes);
+    if (sort_one(a.n, a.classes)) {
+        const int most = a.n <= 256 ? 8 : 9;
+        int passes = (bits + most - 1) / most, width = (bits + passes - 1) / passes;
         void *args[] = {(void *)&a, (void *)&passes, (void *)&width};
-        const void *k = a.n <= 256 ? (const void *)k_sort_one<256, 1> : a.n <= 4096 ? (const void *)k_sort_one<1024, 4> : (const void *)k_sort_one<1024, 16>;
-        return (int)hipLaunchKernel(k, dim3(1), dim3(a.n <= 256 ? 256 : 1024), args, 0, st);
+        const void *k = a.n <= 256    ? (const void *)k_sort_one<256, 1>
+                        : a.n <= 4096 ? (const void *)k_sort_one<1024, 4>
+                                      : (const void *)k_sort_one<1024, 8>;
+        const uint64_t offsets = a.offsets;
+        if (sort_searches(a.n, a.classes)) a.offsets = 0;
+        const int rc = (int)hipLaunchKernel(k, dim3(1), dim3(a.n <= 256 ? 256 : 1024), args, 0, st);
+        if (rc || a.offsets == offsets) return rc;
+        a.offsets = offsets;
+        return sort_offsets(a, st);
     }
+    const int passes = (bits + 7) / 8, width = (bits + passes - 1) / passes;
     SortPass p = {};
     p.tiles = (int)((a.n + SORT_TILE - 1) / SORT_TILE);
+    p.pitch = (int)sort_pitch(a.n);
     p.counts = (uint64_t)workspace;
-    const uint64_t pairs = p.counts + (uint64_t)p.tiles * 1024, pair = ((uint64_t)a.n * 8 + 15) & ~(uint64_t)15;
+    p.width = width;
+    const uint64_t pairs = p.counts + (uint64_t)(p.pitch + 1) * 1024, pair = ((uint64_t)a.n * 8 + 15) & ~(uint64_t)15;
     for (int pass = 0; pass < passes; pass++) {
         const bool last = pass == passes - 1;
         p.keys = p.to_keys;
@@ -258,13 +309,13 @@ int sort_numbers(const SortArgs &in, void *workspace, hipStream_t st)
         p.to_keys = last ? a.keys : pairs + (uint64_t)(pass & 1) * pair;
         p.to_places = last ? a.order : p.to_keys + (uint64_t)a.n * 4;
         p.position = last ? a.position : 0;
+        p.offsets = passes == 1 ? a.offsets : 0;
         p.shift = pass * width;
-        p.width = width;
-        void *args[] = {(void *)&a, (void *)&p};
-        if (const int rc = (int)hipLaunchKernel((const void *)k_sort_count, dim3((unsigned)p.tiles), dim3(1024), args, 0, st)) return rc;
-        if (const int rc = (int)hipLaunchKernel((const void *)k_sort_place, dim3((unsigned)p.tiles), dim3(1024), args, 0, st)) return rc;
+        void *args[] = {(void *)&a, (void *)&p}, *before[] = {(void *)&p};
+        if (const int rc = (int)hipLaunchKernel((const void *)k_sort_count, dim3((unsigned)p.tiles), dim3(256), args, 0, st)) return rc;
+        if (p.tiles > SORT_DIRECT)
+            if (const int rc = (int)hipLaunchKernel((const void *)k_sort_before, dim3(256), dim3(256), before, 0, st)) return rc;
+        if (const int rc = (int)hipLaunchKernel((const void *)k_sort_place, dim3((unsigned)p.tiles), dim3(256), args, 0, st)) return rc;
     }
-    if (!a.offsets) return 0;
-    void *args[] = {(void *)&a};
-    return (int)hipLaunchKernel((const void *)k_sort_offsets, dim3((unsigned)(a.classes / 256 + 1)), dim3(256), args, 0, st);
+    return a.offsets && passes > 1 ? sort_offsets(a, st) : 0;
 }
