@@ -28,23 +28,30 @@ DEV u32x4 philox(u32x4 c, u32 k0, u32 k1)
     return c;
 }
 
-// A lane takes two blocks of eight elements.
+// A lane takes two blocks of eight elements; the last one may be shorter.
 template <class T>
 __global__ __launch_bounds__(256) void k_dropout(const DropoutArgs a)
 {
     constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, NV = 8 / EPV, U = 2;
     const uint64_t seed = a.seed_at ? *as_global<const uint64_t>(a.seed_at) : a.seed;
     u32x4 raw[U][NV], res[U][NV];
-    int left[U];
+    int left[U];  // bytes
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const int64_t block = a.first + (int64_t)blockIdx.x * (256 * U) + u * 256 + threadIdx.x, rest = a.n - block * 8;
-        left[u] = rest < 0 ? 0 : rest > 8 ? 8 : (int)rest;
+        left[u] = rest < 0 ? 0 : rest > 8 ? 8 * ESZ : (int)rest * ESZ;
 #pragma unroll
-        for (int v = 0; v < NV; v++) raw[u][v] = load_row<ESZ>(a.x + (uint64_t)(block * 8) * ESZ, v * EPV, left[u]);
-        if (a.residual) {
-#pragma unroll
-            for (int v = 0; v < NV; v++) res[u][v] = load_row<ESZ>(a.residual + (uint64_t)(block * 8) * ESZ, v * EPV, left[u]);
+        for (int v = 0; v < NV; v++) {
+            const uint64_t at = (uint64_t)(block * 8) * ESZ + v * 16;
+            const bool whole = left[u] >= (v + 1) * 16;
+            raw[u][v] = res[u][v] = u32x4{0, 0, 0, 0};
+            if (whole) {
+                raw[u][v] = LOAD_STREAM(as_global<const u32x4_a1>(a.x + at));
+                if (a.residual) res[u][v] = LOAD_STREAM(as_global<const u32x4_a1>(a.residual + at));
+            } else if (left[u] > v * 16) {
+                raw[u][v] = load_bytes(a.x + at, (u32)(left[u] - v * 16));
+                if (a.residual) res[u][v] = load_bytes(a.residual + at, (u32)(left[u] - v * 16));
+            }
         }
     }
 #pragma unroll
@@ -55,7 +62,7 @@ __global__ __launch_bounds__(256) void k_dropout(const DropoutArgs a)
         for (int v = 0; v < NV; v++) {
             float f[EPV], r[EPV];
             Elem<T>::unpack(raw[u][v], f);
-            if (a.residual) Elem<T>::unpack(res[u][v], r);
+            Elem<T>::unpack(res[u][v], r);
 #pragma unroll
             for (int i = 0; i < EPV; i++) {
                 const int e = v * EPV + i;
@@ -63,7 +70,10 @@ __global__ __launch_bounds__(256) void k_dropout(const DropoutArgs a)
                 f[i] = number >= a.threshold ? f[i] * a.factor : 0.0f;
                 if (a.residual) f[i] += r[i];
             }
-            store_row<ESZ>(a.out + (uint64_t)(block * 8) * ESZ, v * EPV, left[u], Elem<T>::pack(f));
+            const uint64_t to = a.out + (uint64_t)(block * 8) * ESZ + v * 16;
+            const u32x4 out = Elem<T>::pack(f);
+            if (left[u] >= (v + 1) * 16) STORE_STREAM(out, as_global<u32x4_a1>(to));
+            else if (left[u] > v * 16) store_bytes(to, (u32)(left[u] - v * 16), out);
         }
     }
 }

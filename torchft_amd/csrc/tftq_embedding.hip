@@ -8,9 +8,9 @@
 // The gradient is a sum over sorted tokens (tftq_sort.h), fp32, in an order that ids alone decide.  The sorted
 // tokens are cut into chunks of equal size, so that a token that half of the text consists of is no longer to work on
 // than any other: a team sums a chunk's runs, writes the table's row where a run begins and ends inside the
-// chunk, and leaves fp32 sums where it goes on outside (at most one at each end).  The same launch fills the rows of no
-// token with zeros, which is most of the memory that it writes.  A second one adds up the sums of runs over several
-// chunks.  Every row is written once, whatever was there.
+// chunk, and leaves fp32 sums where it goes on outside (at most one at each end).  A second launch adds up the sums of
+// runs over several chunks.  Rows of no token are filled with zeros on the side, most of the memory that is written: the last ones,
+// as many as it takes no time for, while the tokens are sorted, whether they have tokens or not; the others beside the chunks.
 #include "tftq_sort.h"
 
 struct EmbeddingArgs {
@@ -22,10 +22,10 @@ struct EmbeddingArgs {
     float scale;
 };
 
-template <class T, int TEAM>
+template <class T, int TEAM, bool NARROW>
 __global__ __launch_bounds__(256) void k_embedding(const EmbeddingArgs a)
 {
-    constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, TEAMS = 256 / TEAM, U = 4;
+    constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, TEAMS = 256 / TEAM, U = TEAM == 8 ? 1 : 4;
     const int lane = threadIdx.x % TEAM;
     const int64_t row = a.row0 + (int64_t)blockIdx.x * TEAMS + threadIdx.x / TEAM;
     if (row >= a.rows) return;
@@ -35,21 +35,26 @@ __global__ __launch_bounds__(256) void k_embedding(const EmbeddingArgs a)
     for (int col = lane * EPV; col < a.cols; col += U * TEAM * EPV) {
         u32x4 raw[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) raw[u] = fetch_row<ESZ, false>(from, col + u * TEAM * EPV, inside ? a.cols : 0);
+        for (int u = 0; u < U; u++) {
+            Piece p = piece_of<EPV, NARROW>(col + u * TEAM * EPV, a.cols);
+            p.in = p.in && inside;
+            raw[u] = load_row<ESZ, NARROW, false>(from, p, a.cols);
+        }
 #pragma unroll
         for (int u = 0; u < U; u++) {
             float f[EPV];
-            Elem<T>::unpack(settle_row<ESZ>(raw[u], col + u * TEAM * EPV, a.cols), f);
+            Elem<T>::unpack(raw[u], f);
 #pragma unroll
             for (int i = 0; i < EPV; i++) f[i] *= a.scale;
-            store_row<ESZ>(to, col + u * TEAM * EPV, a.cols, Elem<T>::pack(f));
+            store_row<ESZ, NARROW>(to, piece_of<EPV, NARROW>(col + u * TEAM * EPV, a.cols), a.cols, Elem<T>::pack(f));
         }
     }
 }
 
 struct TableArgs {
-    uint64_t dy, keys, order, heads, tails, dtable;  // heads, tails: fp32 [chunks][cols]
-    int64_t n, chunks, vocab, group0, chunk_groups;  // the launch's first workgroup; the workgroups of chunks, before those of zeros
+    uint64_t dy, keys, order, heads, tails, dtable;  // heads, tails: fp32 [chunks][sums_stride(cols)]
+    int64_t n, chunks, vocab, filled;  // from row `filled` on, rows without a token are zeros already
+    int64_t group0, chunk_groups;      // the launch's first workgroup; the workgroups of chunks, before those of zeros
     int cols, chunk, rows, across;                   // tokens of a chunk, rows of the table for a workgroup, teams across the columns
     float scale;
 };
@@ -85,7 +90,7 @@ DEV void fill_empty(const TableArgs &a, int64_t group, int64_t *starts, int64_t 
     if ((int)threadIdx.x <= a.rows) starts[threadIdx.x] = ends[0] + first_at(keys + ends[0], ends[1] - ends[0], first + threadIdx.x);
     __syncthreads();
     const int lane = threadIdx.x & 63;
-    uint64_t empty = __ballot(lane < a.rows && first + lane < a.vocab && starts[lane] == starts[lane + 1]);
+    uint64_t empty = __ballot(lane < a.rows && first + lane < a.filled && starts[lane] == starts[lane + 1]);
     while (empty) {
         const int from = __builtin_ctzll(empty);
         const uint64_t filled = ~(empty >> from);
@@ -93,16 +98,13 @@ DEV void fill_empty(const TableArgs &a, int64_t group, int64_t *starts, int64_t 
         empty = from + count >= 64 ? 0 : empty & (~(uint64_t)0 << (from + count));
         const int64_t bytes = (int64_t)count * a.cols * ESZ;
         const uint64_t to = a.dtable + (uint64_t)(first + from) * (uint64_t)a.cols * ESZ;
-        for (int64_t at = (int64_t)threadIdx.x * 16; at < bytes; at += 4096) {
-            if (at + 16 <= bytes) *as_global<u32x4_a1>(to + (uint64_t)at) = u32x4{0, 0, 0, 0};
-            else store_row<ESZ, false>(to + (uint64_t)at, 0, (int)((bytes - at) / ESZ), u32x4{0, 0, 0, 0});
-        }
+        fill_zeros<256>(to, bytes);
     }
 }
 
 // A lane sums the columns of one vector over a chunk of CHUNK tokens; neighbouring workgroups are `across` parts of the
 // same chunks.  The chunk's tokens are read into LDS first: then every row's address is known, and U rows are on their way at once.
-template <class T, int TEAM, int CHUNK>
+template <class T, int TEAM, int CHUNK, bool NARROW>
 __global__ __launch_bounds__(256) void k_embedding_backward(const TableArgs a)
 {
     constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, TEAMS = 256 / TEAM, U = 16;
@@ -124,8 +126,8 @@ __global__ __launch_bounds__(256) void k_embedding_backward(const TableArgs a)
     __syncthreads();
     const int team = TEAM == 64 ? __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64) : (int)threadIdx.x / TEAM;
     const int64_t chunk = chunk0 + team;
-    const int col = ((int)(group % a.across) * TEAM + (int)threadIdx.x % TEAM) * EPV;
-    if (chunk >= a.chunks || col >= a.cols) return;
+    const Piece piece = piece_of<EPV, NARROW>(((int)(group % a.across) * TEAM + (int)threadIdx.x % TEAM) * EPV, a.cols);
+    if (chunk >= a.chunks || !piece.in) return;
     const u32 *key = keys + 1 + team * CHUNK, *from = order + team * CHUNK;
     const u32 previous = key[-1], next = key[CHUNK];
     float acc[EPV] = {};
@@ -133,24 +135,22 @@ __global__ __launch_bounds__(256) void k_embedding_backward(const TableArgs a)
 
     auto leave = [&](bool last) {  // the run of `current` ends, or the chunk does
         if (current >= (u32)a.vocab) return;
-        const bool goes_on = last && next == current;
-        if (current != previous && !goes_on) {
-            float f[EPV];
-#pragma unroll
-            for (int i = 0; i < EPV; i++) f[i] = acc[i] * a.scale;
-            store_row<ESZ>(a.dtable + (uint64_t)current * (uint64_t)a.cols * ESZ, col, a.cols, Elem<T>::pack(f));
+        if (current == previous || (last && next == current)) {
+            store_sums((current == previous ? a.heads : a.tails) + (uint64_t)(chunk * sums_stride(a.cols)) * 4, piece, acc);
             return;
         }
-        const uint64_t sums = (current == previous ? a.heads : a.tails) + (uint64_t)(chunk * a.cols) * 4;
+        float f[EPV];
 #pragma unroll
-        for (int i = 0; i < EPV; i += 4)
-            store_row<4, false>(sums, col + i, a.cols, u32x4{as_u(acc[i]), as_u(acc[i + 1]), as_u(acc[i + 2]), as_u(acc[i + 3])});
+        for (int i = 0; i < EPV; i++) f[i] = acc[i] * a.scale;
+        store_row<ESZ, NARROW, false>(a.dtable + (uint64_t)current * (uint64_t)a.cols * ESZ, piece, a.cols, Elem<T>::pack(f));
     };
+#pragma unroll 1
     for (int at = 0; at < CHUNK; at += U) {
         u32x4 raw[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            raw[u] = fetch_row<ESZ>(a.dy + (uint64_t)from[at + u] * (uint64_t)a.cols * ESZ, col, key[at + u] < (u32)a.vocab ? a.cols : 0);
+            raw[u] = u32x4{0, 0, 0, 0};
+            if (key[at + u] < (u32)a.vocab) raw[u] = load_row<ESZ, NARROW>(a.dy + (uint64_t)from[at + u] * (uint64_t)a.cols * ESZ, piece, a.cols);
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
@@ -162,7 +162,7 @@ __global__ __launch_bounds__(256) void k_embedding_backward(const TableArgs a)
                 for (int i = 0; i < EPV; i++) acc[i] = 0.0f;
             }
             float f[EPV];
-            Elem<T>::unpack(settle_row<ESZ>(raw[u], col, a.cols), f);
+            Elem<T>::unpack(raw[u], f);
 #pragma unroll
             for (int i = 0; i < EPV; i++) acc[i] += f[i];
         }
@@ -172,29 +172,38 @@ __global__ __launch_bounds__(256) void k_embedding_backward(const TableArgs a)
 
 // The runs of several chunks: a workgroup to the chunk where one begins and 64 vectors of columns; its four wavefronts
 // share the chunks, and add up in their order.
-template <class T>
+template <class T, bool NARROW>
 __global__ __launch_bounds__(256) void k_embedding_join(const TableArgs a)
 {
     constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV;
     __shared__ float add[3][64][EPV + 1];
     const int64_t group = a.group0 + blockIdx.x, chunk = group / a.across, begin = chunk * a.chunk, end = begin + a.chunk;
-    const GLOBAL u32 *keys = as_global<const u32>(a.keys);
     if (end >= a.n) return;
-    const u32 key = keys[end - 1];
-    if (key >= (u32)a.vocab || keys[end] != key) return;                      // no run goes on
-    if (begin > 0 && keys[begin] == key && keys[begin - 1] == key) return;  // it began before
-    const int64_t last = (first_by_wave(keys, a.n, (int64_t)key + 1) - 1) / a.chunk, count = last - chunk + 1;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64, col = ((int)(group % a.across) * 64 + lane) * EPV;
+    const GLOBAL u32 *keys = as_global<const u32>(a.keys);
+    const u32 before = keys[begin > 0 ? begin - 1 : 0], first = keys[begin], key = keys[end - 1], next = keys[end];
+    if (key >= (u32)a.vocab || next != key) return;                   // no run goes on
+    if (begin > 0 && first == key && before == key) return;          // it began before
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+    int64_t count = 1;  // chunks
+    for (bool more = true; more;) {
+        const int64_t at = (chunk + count + lane) * a.chunk;
+        const uint64_t others = ~__ballot(at < a.n && keys[at] == key);
+        count += others ? __builtin_ctzll(others) : 64;
+        more = others == 0;
+    }
+    const Piece piece = piece_of<EPV, NARROW>(((int)(group % a.across) * 64 + lane) * EPV, a.cols);
     const int64_t from = chunk + count * wave / 4, to = chunk + count * (wave + 1) / 4;
     float acc[EPV] = {};
+    if (piece.in) {
 #pragma unroll 8
-    for (int64_t c = from; c < to; c++) {
-        const uint64_t sums = (c == chunk ? a.tails : a.heads) + (uint64_t)(c * a.cols) * 4;
+        for (int64_t c = from; c < to; c++) {
+            const uint64_t sums = (c == chunk ? a.tails : a.heads) + (uint64_t)(c * sums_stride(a.cols) + piece.at) * 4;
 #pragma unroll
-        for (int i = 0; i < EPV; i += 4) {
-            const u32x4 v = load_row<4, false>(sums, col + i, a.cols);
+            for (int i = 0; i < EPV; i += 4) {
+                const u32x4 v = *as_global<const u32x4_a4>(sums + i * 4);
 #pragma unroll
-            for (int j = 0; j < 4; j++) acc[i + j] += as_f(v[j]);
+                for (int j = 0; j < 4; j++) acc[i + j] += as_f(v[j]);
+            }
         }
     }
     if (wave > 0) {
@@ -205,21 +214,38 @@ __global__ __launch_bounds__(256) void k_embedding_join(const TableArgs a)
     if (wave > 0) return;
 #pragma unroll
     for (int i = 0; i < EPV; i++) acc[i] = (((acc[i] + add[0][lane][i]) + add[1][lane][i]) + add[2][lane][i]) * a.scale;
-    store_row<ESZ>(a.dtable + (uint64_t)key * (uint64_t)a.cols * ESZ, col, a.cols, Elem<T>::pack(acc));
+    store_row<ESZ, NARROW, false>(a.dtable + (uint64_t)key * (uint64_t)a.cols * ESZ, piece, a.cols, Elem<T>::pack(acc));
 }
 
 // ---------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------
-static int embedding_team(int64_t vectors) { return vectors <= 8 ? 8 : vectors <= 64 ? 64 : 256; }
+static bool narrow_row(int64_t cols, int size) { return cols * size < 16; }
 
-#define EMBEDDING_TEAMS(K, T, ...) \
-    (team == 8 ? (const void *)K<T, 8 __VA_ARGS__> : team == 64 ? (const void *)K<T, 64 __VA_ARGS__> : (const void *)K<T, 256 __VA_ARGS__>)
-#define EMBEDDING_KERNEL(K, ...)                                \
-    (dtype == TFTQ_F32   ? EMBEDDING_TEAMS(K, float, __VA_ARGS__)   \
-     : dtype == TFTQ_F16 ? EMBEDDING_TEAMS(K, f16_tag, __VA_ARGS__) \
-                         : EMBEDDING_TEAMS(K, bf16_tag, __VA_ARGS__))
-#define EMBEDDING_COMMA ,
+template <class T>
+static const void *embedding_kernel(int64_t cols, int team)
+{
+    if (narrow_row(cols, Elem<T>::ESZ)) return (const void *)k_embedding<T, 8, true>;
+    return team == 8 ? (const void *)k_embedding<T, 8, false> : team == 64 ? (const void *)k_embedding<T, 64, false> : (const void *)k_embedding<T, 256, false>;
+}
+template <class T, int TEAM, bool NARROW>
+static const void *backward_kernel(int chunk)
+{
+    return chunk == 16   ? (const void *)k_embedding_backward<T, TEAM, 16, NARROW>
+           : chunk == 64 ? (const void *)k_embedding_backward<T, TEAM, 64, NARROW>
+                         : (const void *)k_embedding_backward<T, TEAM, 256, NARROW>;
+}
+template <class T>
+static const void *backward_kernel(int64_t cols, int team, int chunk)
+{
+    if (narrow_row(cols, Elem<T>::ESZ)) return backward_kernel<T, 8, true>(chunk);
+    return team == 8 ? backward_kernel<T, 8, false>(chunk) : backward_kernel<T, 64, false>(chunk);
+}
+template <class T>
+static const void *join_kernel(int64_t cols)
+{
+    return narrow_row(cols, Elem<T>::ESZ) ? (const void *)k_embedding_join<T, true> : (const void *)k_embedding_join<T, false>;
+}
 
 extern "C" int tftq_embedding(int dtype, int id_bytes, const void *ids, int64_t n, const void *table, int64_t vocab, int64_t cols,
                               int64_t row_stride, float scale, void *out, int device, void *stream)
@@ -231,9 +257,11 @@ extern "C" int tftq_embedding(int dtype, int id_bytes, const void *ids, int64_t 
     if (!ids || (vocab && !table) || !out || row_stride < (vocab > 1 ? cols : 0)) return TFTQ_E_ARG;
     DeviceScope scope(device);
     if (scope.err != hipSuccess) return (int)scope.err;
-    const int size = dtype_size(dtype), team = embedding_team((cols * size + 15) / 16), teams = 256 / team;
+    const int size = dtype_size(dtype), team = cols * size <= 128 ? 8 : cols * size <= 4096 ? 64 : 256, teams = 256 / team;
     EmbeddingArgs a = {(uint64_t)ids, (uint64_t)table, (uint64_t)out, row_stride * size, 0, n, vocab, (int)cols, id_bytes == 8, scale};
-    const void *k = EMBEDDING_KERNEL(k_embedding, );
+    const void *k = dtype == TFTQ_F32   ? embedding_kernel<float>(cols, team)
+                    : dtype == TFTQ_F16 ? embedding_kernel<f16_tag>(cols, team)
+                                        : embedding_kernel<bf16_tag>(cols, team);
     const int64_t at_once = ROWS_THREADS / team;
     for (; a.row0 < n; a.row0 += at_once) {
         void *args[] = {(void *)&a};
@@ -244,13 +272,13 @@ extern "C" int tftq_embedding(int dtype, int id_bytes, const void *ids, int64_t 
 
 // Tokens of a chunk: neither a chunk nor the sums of one row of the table are to be long, and there are as many chunks of
 // one token as a chunk has tokens when it has the root of all.
-static int embedding_chunk(int64_t n) { return n <= 8192 ? 16 : n <= 131072 ? 64 : 256; }
+static int embedding_chunk(int64_t n) { return n <= 32768 ? 16 : n <= 524288 ? 64 : 256; }
 
 extern "C" int64_t tftq_embedding_backward_workspace(int64_t n, int64_t vocab, int64_t cols)
 {
     if (!rows_ok(n, cols) || !rows_ok(vocab, 0)) return TFTQ_E_SHAPE;
     const int64_t chunks = (n + embedding_chunk(n) - 1) / embedding_chunk(n), numbers = (n * 8 + 15) & ~(int64_t)15;
-    return sort_workspace(n, vocab) + numbers + chunks * cols * 8;
+    return sort_workspace(n, vocab) + numbers + chunks * sums_stride(cols) * 8;
 }
 
 extern "C" int tftq_embedding_backward(int dtype, int id_bytes, const void *ids, int64_t n, int64_t skip, const void *dy, int64_t vocab,
@@ -266,7 +294,7 @@ extern "C" int tftq_embedding_backward(int dtype, int id_bytes, const void *ids,
     DeviceScope scope(device);
     if (scope.err != hipSuccess) return (int)scope.err;
     hipStream_t st = (hipStream_t)stream;
-    const int size = dtype_size(dtype), team = embedding_team((cols * size + 15) / 16), teams = 256 / team;
+    const int size = dtype_size(dtype), team = cols * size <= 128 ? 8 : 64, teams = 256 / team;
     const int64_t vectors = (cols * size + 15) / 16, across = (vectors + team - 1) / team;
     const uint64_t keys = (uint64_t)workspace + (uint64_t)sort_workspace(n, vocab), order = keys + (uint64_t)n * 4;
     TableArgs a = {};
@@ -278,7 +306,7 @@ extern "C" int tftq_embedding_backward(int dtype, int id_bytes, const void *ids,
     a.chunk = embedding_chunk(n);
     a.chunks = (n + a.chunk - 1) / a.chunk;
     a.heads = (keys + (uint64_t)n * 8 + 15) & ~(uint64_t)15;
-    a.tails = a.heads + (uint64_t)(a.chunks * cols) * 4;
+    a.tails = a.heads + (uint64_t)(a.chunks * sums_stride(cols)) * 4;
     a.vocab = vocab;
     a.cols = (int)cols;
     a.across = (int)across;
@@ -286,8 +314,11 @@ extern "C" int tftq_embedding_backward(int dtype, int id_bytes, const void *ids,
     const int64_t row_bytes = cols * size, groups_at_once = ROWS_THREADS / 256;
     a.rows = (int)std::min<int64_t>(64, std::max<int64_t>(1, 65536 / row_bytes));
     a.chunk_groups = (a.chunks + teams - 1) / teams * across;
+    a.filled = vocab;
     if (n) {
-        const SortArgs s = {(uint64_t)ids, id_bytes == 8, n, (u32)vocab, skip >= 0 && skip < vocab ? (u32)skip : (u32)vocab, keys, order, 0, 0};
+        a.filled -= std::min(vocab, sort_fills(n, vocab) / row_bytes);
+        const SortArgs s = {(uint64_t)ids, id_bytes == 8, n, (u32)vocab, skip >= 0 && skip < vocab ? (u32)skip : (u32)vocab, keys, order, 0, 0,
+                            (uint64_t)dtable + (uint64_t)(a.filled * row_bytes), (vocab - a.filled) * row_bytes};
         if (const int rc = sort_numbers(s, workspace, st)) return rc;
     }
     auto launch = [&](const void *k, int64_t groups) {
@@ -296,12 +327,12 @@ extern "C" int tftq_embedding_backward(int dtype, int id_bytes, const void *ids,
             if (const int rc = (int)hipLaunchKernel(k, dim3((unsigned)std::min(groups_at_once, groups - a.group0)), dim3(256), args, 0, st)) return rc;
         return 0;
     };
-    const void *k = a.chunk == 16   ? EMBEDDING_KERNEL(k_embedding_backward, EMBEDDING_COMMA 16)
-                    : a.chunk == 64 ? EMBEDDING_KERNEL(k_embedding_backward, EMBEDDING_COMMA 64)
-                                    : EMBEDDING_KERNEL(k_embedding_backward, EMBEDDING_COMMA 256);
-    if (const int rc = launch(k, a.chunk_groups + (vocab + a.rows - 1) / a.rows)) return rc;
+    const void *k = dtype == TFTQ_F32   ? backward_kernel<float>(cols, team, a.chunk)
+                    : dtype == TFTQ_F16 ? backward_kernel<f16_tag>(cols, team, a.chunk)
+                                        : backward_kernel<bf16_tag>(cols, team, a.chunk);
+    if (const int rc = launch(k, a.chunk_groups + (a.filled + a.rows - 1) / a.rows)) return rc;
     if (a.chunks < 2) return 0;
     a.across = (int)((vectors + 63) / 64);
-    k = dtype == TFTQ_F32 ? (const void *)k_embedding_join<float> : dtype == TFTQ_F16 ? (const void *)k_embedding_join<f16_tag> : (const void *)k_embedding_join<bf16_tag>;
+    k = dtype == TFTQ_F32 ? join_kernel<float>(cols) : dtype == TFTQ_F16 ? join_kernel<f16_tag>(cols) : join_kernel<bf16_tag>(cols);
     return launch(k, (a.chunks - 1) * a.across);
 }

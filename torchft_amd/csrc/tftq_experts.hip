@@ -23,7 +23,7 @@ struct ExpertArgs {
 };
 
 // x [tokens] -> y [tokens k] by places; elements of ESZ bytes.
-template <int ESZ, int TEAM, int U>
+template <int ESZ, int TEAM, int U, bool NARROW>
 __global__ __launch_bounds__(256) void k_dispatch(const ExpertArgs a)
 {
     constexpr int EPV = 16 / ESZ, TEAMS = 256 / TEAM;
@@ -34,16 +34,18 @@ __global__ __launch_bounds__(256) void k_dispatch(const ExpertArgs a)
     const GLOBAL u32 *position = as_global<const u32>(a.position) + token * a.k;
     const uint64_t from = a.x + (uint64_t)(token * a.x_stride);
     for (int col = lane * EPV; col < a.cols; col += U * TEAM * EPV) {
+        Piece p[U];
         u32x4 raw[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) raw[u] = fetch_row<ESZ>(from, col + u * TEAM * EPV, a.cols);
-#pragma unroll
-        for (int u = 0; u < U; u++) raw[u] = settle_row<ESZ>(raw[u], col + u * TEAM * EPV, a.cols);
+        for (int u = 0; u < U; u++) {
+            p[u] = piece_of<EPV, NARROW>(col + u * TEAM * EPV, a.cols);
+            raw[u] = load_row<ESZ, NARROW>(from, p[u], a.cols);
+        }
         for (int s = 0; s < a.k; s++) {
             const u32 place = position[s];
             const uint64_t to = a.y + (uint64_t)place * (uint64_t)a.cols * ESZ;
 #pragma unroll
-            for (int u = 0; u < U; u++) store_row<ESZ, false>(to, col + u * TEAM * EPV, a.cols, place < used ? raw[u] : u32x4{0, 0, 0, 0});
+            for (int u = 0; u < U; u++) store_row<ESZ, NARROW, false>(to, p[u], a.cols, place < used ? raw[u] : u32x4{0, 0, 0, 0});
         }
     }
 }
@@ -56,7 +58,7 @@ DEV float expert_weight(const ExpertArgs &a, int64_t choice)
 }
 
 // Four choices at a time are on their way.
-template <class T, int TEAM, int U>
+template <class T, int TEAM, int U, bool NARROW>
 __global__ __launch_bounds__(256) void k_combine(const ExpertArgs a)
 {
     constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, TEAMS = 256 / TEAM, S = 4;
@@ -80,31 +82,34 @@ __global__ __launch_bounds__(256) void k_combine(const ExpertArgs a)
             }
 #pragma unroll
             for (int s = 0; s < S; s++) {
-                // a choice without an expert: no elements, and a weight that leaves them at nothing
-                const int cols = place[s] < used ? a.cols : 0;
-                if (cols == 0) w[s] = 0.0f;
+                // of a choice without an expert nothing is read, and its weight leaves it at nothing
+                const bool live = place[s] < used;
+                if (!live) w[s] = 0.0f;
 #pragma unroll
-                for (int u = 0; u < U; u++)
-                    raw[s][u] = fetch_row<ESZ>(a.rows + (uint64_t)place[s] * (uint64_t)a.rows_stride, col + u * TEAM * EPV, cols);
+                for (int u = 0; u < U; u++) {
+                    Piece p = piece_of<EPV, NARROW>(col + u * TEAM * EPV, a.cols);
+                    p.in = p.in && live;
+                    raw[s][u] = load_row<ESZ, NARROW>(a.rows + (uint64_t)place[s] * (uint64_t)a.rows_stride, p, a.cols);
+                }
             }
 #pragma unroll
             for (int s = 0; s < S; s++)
 #pragma unroll
                 for (int u = 0; u < U; u++) {
                     float f[EPV];
-                    Elem<T>::unpack(settle_row<ESZ>(raw[s][u], col + u * TEAM * EPV, a.cols), f);
+                    Elem<T>::unpack(raw[s][u], f);
 #pragma unroll
                     for (int i = 0; i < EPV; i++) acc[u][i] = __builtin_fmaf(w[s], f[i], acc[u][i]);
                 }
         }
 #pragma unroll
-        for (int u = 0; u < U; u++) store_row<ESZ>(to, col + u * TEAM * EPV, a.cols, Elem<T>::pack(acc[u]));
+        for (int u = 0; u < U; u++) store_row<ESZ, NARROW>(to, piece_of<EPV, NARROW>(col + u * TEAM * EPV, a.cols), a.cols, Elem<T>::pack(acc[u]));
     }
 }
 
 // x is dy.  NV: vectors of dy that a lane keeps for all choices, and of the rows of two choices that are on their way; MORE:
 // the row is longer, and read again for every choice.
-template <class T, int TEAM, int NV, bool MORE>
+template <class T, int TEAM, int NV, bool NARROW, bool MORE>
 __global__ __launch_bounds__(256) void k_combine_backward(const ExpertArgs a)
 {
     constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, TEAMS = 256 / TEAM, S = 2;
@@ -114,9 +119,13 @@ __global__ __launch_bounds__(256) void k_combine_backward(const ExpertArgs a)
     if (token >= a.tokens) return;
     const u32 used = *as_global<const u32>(a.used);
     const uint64_t from = a.x + (uint64_t)(token * a.x_stride);
+    Piece piece[NV];
     u32x4 dy[NV];
 #pragma unroll
-    for (int v = 0; v < NV; v++) dy[v] = fetch_row<ESZ, !MORE>(from, (v * TEAM + lane) * EPV, a.cols);
+    for (int v = 0; v < NV; v++) {
+        piece[v] = piece_of<EPV, NARROW>((v * TEAM + lane) * EPV, a.cols);
+        dy[v] = load_row<ESZ, NARROW, !MORE>(from, piece[v], a.cols);
+    }
     for (int s0 = 0; s0 < a.k; s0 += S) {
         u32 place[S];
         float w[S], dot[S];
@@ -131,33 +140,40 @@ __global__ __launch_bounds__(256) void k_combine_backward(const ExpertArgs a)
             dot[s] = 0.0f;
         }
         for (int base = 0; base < (MORE ? a.cols : 1); base += NV * TEAM * EPV) {
+            if (MORE && (base > 0 || s0 > 0)) {
+#pragma unroll
+                for (int v = 0; v < NV; v++) {
+                    piece[v] = piece_of<EPV, NARROW>(base + (v * TEAM + lane) * EPV, a.cols);
+                    dy[v] = load_row<ESZ, NARROW, false>(from, piece[v], a.cols);
+                }
+            }
             u32x4 raw[S][NV];
 #pragma unroll
             for (int s = 0; s < S; s++)
 #pragma unroll
-                for (int v = 0; v < NV; v++)
-                    raw[s][v] = fetch_row<ESZ>(a.rows + (uint64_t)place[s] * (uint64_t)a.rows_stride, base + (v * TEAM + lane) * EPV,
-                                               live[s] && a.dweights ? a.cols : 0);
-            if (MORE && (base > 0 || s0 > 0)) {
-#pragma unroll
-                for (int v = 0; v < NV; v++) dy[v] = fetch_row<ESZ, false>(from, base + (v * TEAM + lane) * EPV, a.cols);
-            }
+                for (int v = 0; v < NV; v++) {
+                    Piece p = piece[v];
+                    p.in = p.in && live[s] && a.dweights;
+                    raw[s][v] = load_row<ESZ, NARROW>(a.rows + (uint64_t)place[s] * (uint64_t)a.rows_stride, p, a.cols);
+                }
 #pragma unroll
             for (int v = 0; v < NV; v++) {
-                const int col = base + (v * TEAM + lane) * EPV;
-                float d[EPV];
-                Elem<T>::unpack(settle_row<ESZ>(dy[v], col, a.cols), d);
+                float d[EPV], once[EPV];
+                Elem<T>::unpack(dy[v], d);
+                Elem<T>::unpack(dy[v], once);
+                if (!NARROW) count_once(once, piece[v]);
 #pragma unroll
                 for (int s = 0; s < S; s++) {
                     if (s0 + s >= a.k) continue;
                     float f[EPV], out[EPV];
-                    Elem<T>::unpack(settle_row<ESZ>(raw[s][v], col, a.cols), f);
+                    Elem<T>::unpack(raw[s][v], f);
+                    if (!NARROW) count_once(f, piece[v]);  // no 0 times infinity
 #pragma unroll
                     for (int i = 0; i < EPV; i++) {
-                        dot[s] = __builtin_fmaf(d[i], f[i], dot[s]);
+                        dot[s] = __builtin_fmaf(once[i], f[i], dot[s]);
                         out[i] = live[s] ? d[i] * w[s] : 0.0f;
                     }
-                    if (a.drows) store_row<ESZ, false>(a.drows + (uint64_t)place[s] * (uint64_t)a.cols * ESZ, col, a.cols, Elem<T>::pack(out));
+                    if (a.drows) store_row<ESZ, NARROW, false>(a.drows + (uint64_t)place[s] * (uint64_t)a.cols * ESZ, piece[v], a.cols, Elem<T>::pack(out));
                 }
             }
         }
@@ -191,14 +207,15 @@ static RowShape expert_shape(int64_t vectors)
     if (vectors <= 256) return {64, 4};
     return {256, 2};
 }
-#define EXPERT_SHAPES(K, X)                                           \
-    (shape.team == 8     ? shape.nv == 1   ? (const void *)K<X, 8, 1>     \
-                           : shape.nv == 2 ? (const void *)K<X, 8, 2>     \
-                                           : (const void *)K<X, 8, 4>     \
-     : shape.team == 16  ? (const void *)K<X, 16, 4>                      \
-     : shape.team == 256 ? (const void *)K<X, 256, 2>                     \
-     : shape.nv == 2     ? (const void *)K<X, 64, 2>                      \
-                         : (const void *)K<X, 64, 4>)
+#define EXPERT_SHAPES(K, X, size)                                        \
+    (cols * size < 16    ? (const void *)K<X, 8, 1, true>                    \
+     : shape.team == 8   ? shape.nv == 1   ? (const void *)K<X, 8, 1, false> \
+                           : shape.nv == 2 ? (const void *)K<X, 8, 2, false> \
+                                           : (const void *)K<X, 8, 4, false> \
+     : shape.team == 16  ? (const void *)K<X, 16, 4, false>                  \
+     : shape.team == 256 ? (const void *)K<X, 256, 2, false>                 \
+     : shape.nv == 2     ? (const void *)K<X, 64, 2, false>                  \
+                         : (const void *)K<X, 64, 4, false>)
 
 static int expert_launch(const void *kernel, ExpertArgs a, int team, hipStream_t st)
 {
@@ -229,7 +246,7 @@ extern "C" int tftq_expert_sort(int id_bytes, const void *chosen, int64_t choice
     DeviceScope scope(device);
     if (scope.err != hipSuccess) return (int)scope.err;
     const SortArgs a = {(uint64_t)chosen, id_bytes == 8, choices, (u32)experts, (u32)experts,
-                        sort_needs_keys(choices, experts) ? (uint64_t)workspace + (uint64_t)sort_workspace(choices, experts) : 0, (uint64_t)order, (uint64_t)position, (uint64_t)offsets};
+                        sort_needs_keys(choices, experts) ? (uint64_t)workspace + (uint64_t)sort_workspace(choices, experts) : 0, (uint64_t)order, (uint64_t)position, (uint64_t)offsets, 0, 0};
     return sort_numbers(a, workspace, (hipStream_t)stream);
 }
 
@@ -252,7 +269,7 @@ extern "C" int tftq_dispatch(int element_bytes, const void *x, int64_t x_stride,
     a.tokens = tokens;
     a.cols = (int)cols;
     a.k = (int)k;
-#define K(ESZ) EXPERT_SHAPES(k_dispatch, ESZ)
+#define K(ESZ) EXPERT_SHAPES(k_dispatch, ESZ, ESZ)
     return expert_launch(element_bytes == 1 ? K(1) : element_bytes == 2 ? K(2) : K(4), a, shape.team, (hipStream_t)stream);
 #undef K
 }
@@ -279,7 +296,7 @@ extern "C" int tftq_combine(int dtype, int weight_dtype, const void *rows, int64
     a.tokens = tokens;
     a.cols = (int)cols;
     a.k = (int)k;
-#define K(T) EXPERT_SHAPES(k_combine, T)
+#define K(T) EXPERT_SHAPES(k_combine, T, size)
     return expert_launch(dtype == TFTQ_F32 ? K(float) : dtype == TFTQ_F16 ? K(f16_tag) : K(bf16_tag), a, shape.team, (hipStream_t)stream);
 #undef K
 }
@@ -313,16 +330,17 @@ extern "C" int tftq_combine_backward(int dtype, int weight_dtype, const void *dy
     a.tokens = tokens;
     a.cols = (int)cols;
     a.k = (int)k;
-#define K(T)                                                                      \
-    (shape.team == 8     ? shape.nv == 1   ? (const void *)k_combine_backward<T, 8, 1, false>  \
-                           : shape.nv == 2 ? (const void *)k_combine_backward<T, 8, 2, false>  \
-                                           : (const void *)k_combine_backward<T, 8, 4, false>  \
-     : shape.team == 16  ? (const void *)k_combine_backward<T, 16, 4, false>                   \
-     : shape.team == 64  ? shape.nv == 2 ? (const void *)k_combine_backward<T, 64, 2, false>   \
-                                         : (const void *)k_combine_backward<T, 64, 4, false>   \
-     : per_lane <= 2     ? (const void *)k_combine_backward<T, 256, 2, false>                  \
-     : per_lane <= 4     ? (const void *)k_combine_backward<T, 256, 4, false>                  \
-                         : (const void *)k_combine_backward<T, 256, 4, true>)
+#define K(T)                                                                                          \
+    (cols * size < 16    ? (const void *)k_combine_backward<T, 8, 1, true, false>                         \
+     : shape.team == 8   ? shape.nv == 1   ? (const void *)k_combine_backward<T, 8, 1, false, false>      \
+                           : shape.nv == 2 ? (const void *)k_combine_backward<T, 8, 2, false, false>      \
+                                           : (const void *)k_combine_backward<T, 8, 4, false, false>      \
+     : shape.team == 16  ? (const void *)k_combine_backward<T, 16, 4, false, false>                       \
+     : shape.team == 64  ? shape.nv == 2 ? (const void *)k_combine_backward<T, 64, 2, false, false>       \
+                                         : (const void *)k_combine_backward<T, 64, 4, false, false>       \
+     : per_lane <= 2     ? (const void *)k_combine_backward<T, 256, 2, false, false>                      \
+     : per_lane <= 4     ? (const void *)k_combine_backward<T, 256, 4, false, false>                      \
+                         : (const void *)k_combine_backward<T, 256, 4, false, true>)
     return expert_launch(dtype == TFTQ_F32 ? K(float) : dtype == TFTQ_F16 ? K(f16_tag) : K(bf16_tag), a, shape.team, (hipStream_t)stream);
 #undef K
 }

@@ -15,54 +15,69 @@ struct NormArgs {
     uint64_t x, residual, weight, y, h, codes, scales;  // residual, weight, h: 0 for none; codes and scales for 8 bits, else y
     int64_t x_stride, residual_stride;                  // bytes from row to row; all others are contiguous
     int64_t row0, rows;
-    int cols, wide;  // wide: the weight is fp32 and the rows are not
+    int cols;
     float eps, inv_cols;
 };
 
-// The weight's elements that belong to a vector: loaded early, widened late.
-template <class T>
+// The weight's elements that belong to a vector: loaded early, widened late.  WIDE: the weight is fp32 and the rows are not.
+template <class T, bool NARROW, bool WIDE>
 struct Weights {
-    u32x4 raw, more;
-    DEV void fetch(uint64_t weight, int wide, int col, int cols)
+    static_assert(!WIDE || Elem<T>::EPV == 8, "");
+    u32x4 raw[WIDE ? 2 : 1];
+    DEV void load(uint64_t weight, const Piece &p, int cols)
     {
-        constexpr int EPV = Elem<T>::EPV;
-        more = u32x4{0, 0, 0, 0};
-        if (!weight) return;
-        if (EPV == 8 && wide) {
-            raw = fetch_row<4, false>(weight, col, cols);
-            more = fetch_row<4, false>(weight, col + 4, cols);
-        } else raw = fetch_row<Elem<T>::ESZ, false>(weight, col, cols);
+#pragma unroll
+        for (int i = 0; i < (WIDE ? 2 : 1); i++) raw[i] = u32x4{0, 0, 0, 0};
+        if (!weight || !p.in) return;
+        if constexpr (!WIDE) raw[0] = load_row<Elem<T>::ESZ, NARROW, false>(weight, p, cols);
+        else {
+            const uint64_t at = weight + (uint64_t)(u32)p.at * 4;
+            if (NARROW) {
+                raw[0] = load_bytes(at, min(16u, (u32)cols * 4));
+                if (cols > 4) raw[1] = load_bytes(at + 16, (u32)(cols - 4) * 4);
+            } else {
+                raw[0] = *as_global<const u32x4_a4>(at);
+                raw[1] = *as_global<const u32x4_a4>(at + 16);
+            }
+        }
     }
-    DEV void settle(uint64_t weight, int wide, int col, int cols)
-    {
-        if (!weight) return;
-        if (Elem<T>::EPV == 8 && wide) {
-            raw = settle_row<4>(raw, col, cols);
-            more = settle_row<4>(more, col + 4, cols);
-        } else raw = settle_row<Elem<T>::ESZ>(raw, col, cols);
-    }
-    DEV void unpack(uint64_t weight, int wide, float (&w)[Elem<T>::EPV]) const
+    DEV void unpack(uint64_t weight, float (&w)[Elem<T>::EPV]) const
     {
         constexpr int EPV = Elem<T>::EPV;
         if (!weight) {
 #pragma unroll
             for (int i = 0; i < EPV; i++) w[i] = 1.0f;
-        } else if (EPV == 8 && wide) {
+        } else if constexpr (WIDE) {
 #pragma unroll
-            for (int i = 0; i < EPV; i++) w[i] = as_f(i < 4 ? raw[i & 3] : more[i & 3]);
-        } else Elem<T>::unpack(raw, w);
+            for (int i = 0; i < EPV; i++) w[i] = as_f(raw[i / 4][i % 4]);
+        } else Elem<T>::unpack(raw[0], w);
     }
 };
 
 DEV float inverse_root(float mean_square, float eps) { return 1.0f / __builtin_sqrtf(mean_square + eps); }
 
+DEV float fp8_scale(float amax)
+{
+    const float part = amax / 448.0f;
+    return part >= 0x1p-126f ? part : 1.0f;
+}
+// EPV codes of a vector.
+template <int EPV, bool NARROW>
+DEV void store_codes(uint64_t row, const Piece &p, int cols, const float (&f)[EPV])
+{
+    if (!p.in) return;
+    u32x4 c = {pack_fp8x4(f[0], f[1], f[2], f[3]), 0, 0, 0};
+    if constexpr (EPV == 8) c.y = pack_fp8x4(f[4], f[5], f[6], f[7]);
+    if (NARROW) store_bytes(row + (u32)p.at, (u32)cols, c);
+    else if constexpr (EPV == 8) *as_global<u32x2_a1>(row + (u32)p.at) = u32x2{c.x, c.y};
+    else *as_global<u32_a1>(row + (u32)p.at) = c.x;
+}
+
 // One team of TEAM lanes to a row, which stays in its registers: memory is read and written once.
-template <class T, int TEAM, int NV, bool FP8>
+template <class T, int TEAM, int NV, bool NARROW, bool WIDE, bool FP8>
 __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void k_rms_norm(const NormArgs a)
 {
     constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, TEAMS = TEAM > 256 ? 1 : 256 / TEAM;
-    // weights in the registers of the residual, so that two workgroups of long rows run on a compute unit
-    constexpr bool LATE = TEAM * NV >= 2048;
     __shared__ float lds[TEAM > 64 ? TEAM / 64 : 1];
     const int lane = threadIdx.x % TEAM;
     const int64_t row = a.row0 + (int64_t)blockIdx.x * TEAMS + threadIdx.x / TEAM;
@@ -70,51 +85,48 @@ __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void k_rms_norm(const Norm
     const uint64_t px = a.x + (uint64_t)(row * a.x_stride), pr = a.residual + (uint64_t)(row * a.residual_stride);
     const uint64_t at = (uint64_t)(row * a.cols) * ESZ;
 
+    Piece piece[NV];
     u32x4 raw[NV], res[NV];
-    Weights<T> weights[NV];
+    Weights<T, NARROW, WIDE> weights[NV];
 #pragma unroll
-    for (int v = 0; v < NV; v++) raw[v] = fetch_row<ESZ>(px, (v * TEAM + lane) * EPV, a.cols);
+    for (int v = 0; v < NV; v++) {
+        piece[v] = piece_of<EPV, NARROW>((v * TEAM + lane) * EPV, a.cols);
+        raw[v] = load_row<ESZ, NARROW>(px, piece[v], a.cols);
+    }
     if (a.residual) {
 #pragma unroll
-        for (int v = 0; v < NV; v++) res[v] = fetch_row<ESZ>(pr, (v * TEAM + lane) * EPV, a.cols);
+        for (int v = 0; v < NV; v++) res[v] = load_row<ESZ, NARROW>(pr, piece[v], a.cols);
     }
-    auto fetch_weights = [&] {
 #pragma unroll
-        for (int v = 0; v < NV; v++) weights[v].fetch(a.weight, a.wide, (v * TEAM + lane) * EPV, a.cols);
-    };
-    if (!LATE) fetch_weights();
+    for (int v = 0; v < NV; v++) weights[v].load(a.weight, piece[v], a.cols);
     float sum = 0.0f;
 #pragma unroll
     for (int v = 0; v < NV; v++) {
-        const int col = (v * TEAM + lane) * EPV;
         float f[EPV];
-        raw[v] = settle_row<ESZ>(raw[v], col, a.cols);
         Elem<T>::unpack(raw[v], f);
         if (a.residual) {
             float r[EPV];
-            Elem<T>::unpack(settle_row<ESZ>(res[v], col, a.cols), r);
+            Elem<T>::unpack(res[v], r);
 #pragma unroll
             for (int i = 0; i < EPV; i++) f[i] += r[i];
             raw[v] = Elem<T>::pack(f);
-            store_row<ESZ>(a.h + at, col, a.cols, raw[v]);
+            store_row<ESZ, NARROW>(a.h + at, piece[v], a.cols, raw[v]);
             Elem<T>::unpack(raw[v], f);
         }
+        if (!NARROW) count_once(f, piece[v]);
 #pragma unroll
         for (int i = 0; i < EPV; i++) sum = __builtin_fmaf(f[i], f[i], sum);
     }
-    if (LATE) fetch_weights();
     const float r = inverse_root(team_sum<TEAM>(sum, lds) * a.inv_cols, a.eps);
-#pragma unroll
-    for (int v = 0; v < NV; v++) weights[v].settle(a.weight, a.wide, (v * TEAM + lane) * EPV, a.cols);
     if constexpr (!FP8) {
 #pragma unroll
         for (int v = 0; v < NV; v++) {
             float f[EPV], w[EPV];
             Elem<T>::unpack(raw[v], f);
-            weights[v].unpack(a.weight, a.wide, w);
+            weights[v].unpack(a.weight, w);
 #pragma unroll
             for (int i = 0; i < EPV; i++) f[i] = f[i] * r * w[i];
-            store_row<ESZ>(a.y + at, (v * TEAM + lane) * EPV, a.cols, Elem<T>::pack(f));
+            store_row<ESZ, NARROW>(a.y + at, piece[v], a.cols, Elem<T>::pack(f));
         }
     } else {
         float amax = 0.0f;
@@ -122,39 +134,27 @@ __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void k_rms_norm(const Norm
         for (int v = 0; v < NV; v++) {
             float f[EPV], w[EPV];
             Elem<T>::unpack(raw[v], f);
-            weights[v].unpack(a.weight, a.wide, w);
+            weights[v].unpack(a.weight, w);
 #pragma unroll
             for (int i = 0; i < EPV; i++) amax = fmaxf(amax, __builtin_fabsf(f[i] * r * w[i]));
         }
-        amax = team_largest<TEAM>(amax, lds);
-        const float part = amax / 448.0f, scale = part >= 0x1p-126f ? part : 1.0f, inverse = 1.0f / scale;
+        const float scale = fp8_scale(team_largest<TEAM>(amax, lds)), inverse = 1.0f / scale;
         if (lane == 0) as_global<float>(a.scales)[row] = scale;
-        const uint64_t codes = a.codes + (uint64_t)(row * a.cols);
 #pragma unroll
         for (int v = 0; v < NV; v++) {
-            const int col = (v * TEAM + lane) * EPV;
             float f[EPV], w[EPV];
             Elem<T>::unpack(raw[v], f);
-            weights[v].unpack(a.weight, a.wide, w);
+            weights[v].unpack(a.weight, w);
 #pragma unroll
             for (int i = 0; i < EPV; i++) f[i] = f[i] * r * w[i] * inverse;
-            u32 c[2] = {pack_fp8x4(f[0], f[1], f[2], f[3]), 0};
-            if constexpr (EPV == 8) c[1] = pack_fp8x4(f[4], f[5], f[6], f[7]);
-            if (col + EPV <= a.cols) {
-                if constexpr (EPV == 8) *as_global<u32x2_a1>(codes + (u32)col) = u32x2{c[0], c[1]};
-                else *as_global<u32_a1>(codes + (u32)col) = c[0];
-            } else {
-#pragma unroll
-                for (int i = 0; i < EPV; i++)
-                    if (col + i < a.cols) as_global<uint8_t>(codes + (u32)col)[i] = (uint8_t)(c[i / 4] >> (i % 4 * 8));
-            }
+            store_codes<EPV, NARROW>(a.codes + (uint64_t)(row * a.cols), piece[v], a.cols, f);
         }
     }
 }
 
 // Rows too long for the registers of a workgroup: its 1024 lanes go over the row two or three times, behind the
 // first time in h (or x), which the caches may still have.
-template <class T, bool FP8>
+template <class T, bool WIDE, bool FP8>
 __global__ __launch_bounds__(1024) void k_rms_norm_long(const NormArgs a)
 {
     constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, STEP = 1024 * EPV;
@@ -164,50 +164,51 @@ __global__ __launch_bounds__(1024) void k_rms_norm_long(const NormArgs a)
     const uint64_t at = (uint64_t)(row * a.cols) * ESZ, again = a.residual ? a.h + at : px;
     float sum = 0.0f;
     for (int col = threadIdx.x * EPV; col < a.cols; col += STEP) {
-        u32x4 raw = load_row<ESZ, false>(px, col, a.cols);
+        const Piece p = piece_of<EPV, false>(col, a.cols);
+        u32x4 raw = load_row<ESZ, false, false>(px, p, a.cols), res = {0, 0, 0, 0};
+        if (a.residual) res = load_row<ESZ, false>(pr, p, a.cols);
         float f[EPV];
         Elem<T>::unpack(raw, f);
         if (a.residual) {
             float r[EPV];
-            Elem<T>::unpack(load_row<ESZ>(pr, col, a.cols), r);
+            Elem<T>::unpack(res, r);
 #pragma unroll
             for (int i = 0; i < EPV; i++) f[i] += r[i];
             raw = Elem<T>::pack(f);
-            store_row<ESZ, false>(a.h + at, col, a.cols, raw);
+            store_row<ESZ, false, false>(a.h + at, p, a.cols, raw);
             Elem<T>::unpack(raw, f);
         }
+        count_once(f, p);
 #pragma unroll
         for (int i = 0; i < EPV; i++) sum = __builtin_fmaf(f[i], f[i], sum);
     }
     const float r = inverse_root(team_sum<1024>(sum, lds) * a.inv_cols, a.eps);
-    // every lane reads back what it wrote itself: its own stores come before its own loads
-    float inverse = 1.0f;
+    // every lane reads back the vectors that it wrote itself: its own stores come before its own loads
+    float scale = 1.0f, inverse = 1.0f;
     for (int pass = FP8 ? 0 : 1; pass < 2; pass++) {
         float amax = 0.0f;
         for (int col = threadIdx.x * EPV; col < a.cols; col += STEP) {
+            const Piece p = piece_of<EPV, false>(col, a.cols);
             float f[EPV], w[EPV];
-            Elem<T>::unpack(load_row<ESZ, false>(again, col, a.cols), f);
-            Weights<T> weights;
-            weights.fetch(a.weight, a.wide, col, a.cols);
-            weights.settle(a.weight, a.wide, col, a.cols);
-            weights.unpack(a.weight, a.wide, w);
+            const u32x4 raw = load_row<ESZ, false, false>(again, p, a.cols);
+            Weights<T, false, WIDE> weights;
+            weights.load(a.weight, p, a.cols);
+            weights.unpack(a.weight, w);
+            Elem<T>::unpack(raw, f);
 #pragma unroll
             for (int i = 0; i < EPV; i++) f[i] = f[i] * r * w[i];
-            if (!FP8) store_row<ESZ>(a.y + at, col, a.cols, Elem<T>::pack(f));
+            if (!FP8) store_row<ESZ, false>(a.y + at, p, a.cols, Elem<T>::pack(f));
             else if (pass == 0) {
 #pragma unroll
                 for (int i = 0; i < EPV; i++) amax = fmaxf(amax, __builtin_fabsf(f[i]));
             } else {
-                const uint64_t codes = a.codes + (uint64_t)(row * a.cols);
 #pragma unroll
-                for (int i = 0; i < EPV; i++)
-                    if (col + i < a.cols)
-                        as_global<uint8_t>(codes + (u32)col)[i] = (uint8_t)pack_fp8x4(f[i] * inverse, 0.0f, 0.0f, 0.0f);
+                for (int i = 0; i < EPV; i++) f[i] *= inverse;
+                store_codes<EPV, false>(a.codes + (uint64_t)(row * a.cols), p, a.cols, f);
             }
         }
         if (FP8 && pass == 0) {
-            amax = team_largest<1024>(amax, lds);
-            const float part = amax / 448.0f, scale = part >= 0x1p-126f ? part : 1.0f;
+            scale = fp8_scale(team_largest<1024>(amax, lds));
             inverse = 1.0f / scale;
             if (threadIdx.x == 0) as_global<float>(a.scales)[row] = scale;
         }
@@ -215,16 +216,16 @@ __global__ __launch_bounds__(1024) void k_rms_norm_long(const NormArgs a)
 }
 
 struct NormBackwardArgs {
-    uint64_t dy, dh, h, weight, dx, sums;  // dh, weight, sums: 0 for none
+    uint64_t dy, dh, h, weight, dx, sums;  // dh, weight, dx, sums: 0 for none.  sums: fp32 [workgroups][sums_stride(cols)]
     int64_t h_stride;                      // bytes; all others are contiguous
     int64_t rows;
-    int cols, wide;
+    int cols;
     float eps, inv_cols;
 };
 
 // A team goes over every (teams in the grid)-th row, one after the other, and keeps its part of dw in registers;
 // a workgroup's teams add theirs up in LDS and leave a row of fp32 sums, which k_column_sums adds up.
-template <class T, int TEAM, int NV>
+template <class T, int TEAM, int NV, bool NARROW, bool WIDE>
 __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void k_rms_norm_backward(const NormBackwardArgs a)
 {
     constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, TEAMS = TEAM > 256 ? 1 : 256 / TEAM;
@@ -232,44 +233,43 @@ __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void k_rms_norm_backward(c
     __shared__ float add[TEAMS > 1 ? 256 * NV * EPV : 1];
     const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
     float acc[NV][EPV];
+    Piece piece[NV];
+    Weights<T, NARROW, WIDE> weights[NV];
 #pragma unroll
-    for (int v = 0; v < NV; v++)
+    for (int v = 0; v < NV; v++) {
+        piece[v] = piece_of<EPV, NARROW>((v * TEAM + lane) * EPV, a.cols);
+        weights[v].load(a.weight, piece[v], a.cols);
 #pragma unroll
         for (int i = 0; i < EPV; i++) acc[v][i] = 0.0f;
-    Weights<T> weights[NV];
-#pragma unroll
-    for (int v = 0; v < NV; v++) weights[v].fetch(a.weight, a.wide, (v * TEAM + lane) * EPV, a.cols);
+    }
 
     // the next row is on its way while this one is worked on, where there are registers for it
     constexpr bool AHEAD = TEAM * NV * EPV <= 8192;
     const int64_t step = (int64_t)gridDim.x * TEAMS;
     u32x4 dy_next[NV], h_next[NV], dh_next[NV];
     auto fetch = [&](int64_t row) {
-        const bool there = row < a.rows;
+        if (AHEAD && row >= a.rows) return;
         const uint64_t at = (uint64_t)(row * a.cols) * ESZ, ph = a.h + (uint64_t)(row * a.h_stride);
-        const int cols = there ? a.cols : 0;
 #pragma unroll
-        for (int v = 0; v < NV; v++) dy_next[v] = fetch_row<ESZ>(a.dy + at, (v * TEAM + lane) * EPV, cols);
+        for (int v = 0; v < NV; v++) dy_next[v] = load_row<ESZ, NARROW>(a.dy + at, piece[v], a.cols);
 #pragma unroll
-        for (int v = 0; v < NV; v++) h_next[v] = fetch_row<ESZ>(ph, (v * TEAM + lane) * EPV, cols);
+        for (int v = 0; v < NV; v++) h_next[v] = load_row<ESZ, NARROW>(ph, piece[v], a.cols);
         if (a.dh) {
 #pragma unroll
-            for (int v = 0; v < NV; v++) dh_next[v] = fetch_row<ESZ>(a.dh + at, (v * TEAM + lane) * EPV, cols);
+            for (int v = 0; v < NV; v++) dh_next[v] = load_row<ESZ, NARROW>(a.dh + at, piece[v], a.cols);
         }
     };
     int64_t row = (int64_t)blockIdx.x * TEAMS + team;
     if (AHEAD) fetch(row);
-#pragma unroll
-    for (int v = 0; v < NV; v++) weights[v].settle(a.weight, a.wide, (v * TEAM + lane) * EPV, a.cols);
     for (; row < a.rows; row += step) {
         if (!AHEAD) fetch(row);
         const uint64_t at = (uint64_t)(row * a.cols) * ESZ;
         u32x4 dy[NV], h[NV], dh[NV];
 #pragma unroll
         for (int v = 0; v < NV; v++) {
-            dy[v] = settle_row<ESZ>(dy_next[v], (v * TEAM + lane) * EPV, a.cols);
-            h[v] = settle_row<ESZ>(h_next[v], (v * TEAM + lane) * EPV, a.cols);
-            if (a.dh) dh[v] = settle_row<ESZ>(dh_next[v], (v * TEAM + lane) * EPV, a.cols);
+            dy[v] = dy_next[v];
+            h[v] = h_next[v];
+            dh[v] = dh_next[v];
         }
         if (AHEAD) fetch(row + step);
         float squares = 0.0f, along = 0.0f;
@@ -278,7 +278,11 @@ __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void k_rms_norm_backward(c
             float f[EPV], g[EPV], w[EPV];
             Elem<T>::unpack(h[v], f);
             Elem<T>::unpack(dy[v], g);
-            weights[v].unpack(a.weight, a.wide, w);
+            weights[v].unpack(a.weight, w);
+            if (!NARROW) {
+                count_once(f, piece[v]);
+                count_once(g, piece[v]);
+            }
 #pragma unroll
             for (int i = 0; i < EPV; i++) {
                 squares = __builtin_fmaf(f[i], f[i], squares);
@@ -292,7 +296,7 @@ __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void k_rms_norm_backward(c
             float f[EPV], g[EPV], w[EPV], d[EPV];
             Elem<T>::unpack(h[v], f);
             Elem<T>::unpack(dy[v], g);
-            weights[v].unpack(a.weight, a.wide, w);
+            weights[v].unpack(a.weight, w);
             if (a.dh) Elem<T>::unpack(dh[v], d);
 #pragma unroll
             for (int i = 0; i < EPV; i++) {
@@ -300,37 +304,35 @@ __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void k_rms_norm_backward(c
                 f[i] = r * (g[i] * w[i] - f[i] * c);
                 if (a.dh) f[i] += d[i];
             }
-            if (a.dx) store_row<ESZ>(a.dx + at, (v * TEAM + lane) * EPV, a.cols, Elem<T>::pack(f));
+            if (a.dx) store_row<ESZ, NARROW>(a.dx + at, piece[v], a.cols, Elem<T>::pack(f));
         }
     }
     if (!a.sums) return;
-    const uint64_t sums = a.sums + (uint64_t)blockIdx.x * (uint64_t)a.cols * 4;
+    const uint64_t sums = a.sums + (uint64_t)blockIdx.x * (uint64_t)sums_stride(a.cols) * 4;
     if constexpr (TEAMS > 1) {
-        constexpr int WIDTH = TEAM * EPV;
+        constexpr int WIDTH = NV * TEAM * EPV;  // [team][vector][element][lane]
 #pragma unroll
         for (int v = 0; v < NV; v++)
 #pragma unroll
-            for (int i = 0; i < EPV; i++) add[(team * NV + v) * WIDTH + i * TEAM + lane] = acc[v][i];
+            for (int i = 0; i < EPV; i++) add[team * WIDTH + (v * EPV + i) * TEAM + lane] = acc[v][i];
         __syncthreads();
-        for (int c = threadIdx.x; c < NV * WIDTH; c += 256) {
+        for (int c = threadIdx.x; c < WIDTH; c += 256) {
             float s = 0.0f;
-            for (int t = 0; t < TEAMS; t++) s += add[t * NV * WIDTH + c];
-            const int v = c / WIDTH, i = c % WIDTH / TEAM, l = c % TEAM, col = (v * TEAM + l) * EPV + i;
-            if (col < a.cols) as_global<float>(sums)[col] = s;
+#pragma unroll 4
+            for (int t = 0; t < TEAMS; t++) s += add[t * WIDTH + c];
+            const int v = c / (EPV * TEAM), e = c / TEAM % EPV, l = c % TEAM;
+            const Piece p = piece_of<EPV, NARROW>((v * TEAM + l) * EPV, a.cols);
+            if (p.in) as_global<float>(sums)[p.at + e] = s;
         }
     } else {
 #pragma unroll
-        for (int v = 0; v < NV; v++)
-#pragma unroll
-            for (int i = 0; i < EPV; i += 4)
-                store_row<4, false>(sums, (v * TEAM + lane) * EPV + i, a.cols,
-                                    u32x4{as_u(acc[v][i]), as_u(acc[v][i + 1]), as_u(acc[v][i + 2]), as_u(acc[v][i + 3])});
+        for (int v = 0; v < NV; v++) store_sums(sums, piece[v], acc[v]);
     }
 }
 
 // Rows too long for that: first r and c of every row, then dx and the sums, a workgroup to 256 vectors of columns
 // and a share of the rows, four rows at a time.
-template <class T>
+template <class T, bool WIDE>
 __global__ __launch_bounds__(1024) void k_rms_norm_backward_long(const NormBackwardArgs a, uint64_t factors)
 {
     constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, U = 2, STEP = 1024 * EPV;
@@ -339,21 +341,24 @@ __global__ __launch_bounds__(1024) void k_rms_norm_backward_long(const NormBackw
         const uint64_t at = (uint64_t)(row * a.cols) * ESZ, ph = a.h + (uint64_t)(row * a.h_stride);
         float squares = 0.0f, along = 0.0f;
         for (int col = threadIdx.x * EPV; col < a.cols; col += U * STEP) {
-            Weights<T> weights[U];
+            Weights<T, false, WIDE> weights[U];
+            Piece p[U];
             u32x4 h[U], dy[U];
 #pragma unroll
             for (int u = 0; u < U; u++) {
-                h[u] = fetch_row<ESZ, false>(ph, col + u * STEP, a.cols);
-                dy[u] = fetch_row<ESZ, false>(a.dy + at, col + u * STEP, a.cols);
-                weights[u].fetch(a.weight, a.wide, col + u * STEP, a.cols);
+                p[u] = piece_of<EPV, false>(col + u * STEP, a.cols);
+                h[u] = load_row<ESZ, false, false>(ph, p[u], a.cols);
+                dy[u] = load_row<ESZ, false, false>(a.dy + at, p[u], a.cols);
+                weights[u].load(a.weight, p[u], a.cols);
             }
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 float f[EPV], g[EPV], w[EPV];
-                weights[u].settle(a.weight, a.wide, col + u * STEP, a.cols);
-                weights[u].unpack(a.weight, a.wide, w);
-                Elem<T>::unpack(settle_row<ESZ>(h[u], col + u * STEP, a.cols), f);
-                Elem<T>::unpack(settle_row<ESZ>(dy[u], col + u * STEP, a.cols), g);
+                weights[u].unpack(a.weight, w);
+                Elem<T>::unpack(h[u], f);
+                Elem<T>::unpack(dy[u], g);
+                count_once(f, p[u]);
+                count_once(g, p[u]);
 #pragma unroll
                 for (int i = 0; i < EPV; i++) {
                     squares = __builtin_fmaf(f[i], f[i], squares);
@@ -366,17 +371,16 @@ __global__ __launch_bounds__(1024) void k_rms_norm_backward_long(const NormBackw
         if (threadIdx.x < 2) as_global<float>(factors)[2 * row + threadIdx.x] = threadIdx.x ? r * r * (along * a.inv_cols) : r;
     }
 }
-template <class T>
+template <class T, bool WIDE>
 __global__ __launch_bounds__(256) void k_rms_norm_backward_columns(const NormBackwardArgs a, uint64_t factors)
 {
     constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, U = 4;
-    const int col = (int)(blockIdx.x * 256 + threadIdx.x) * EPV;
-    if (col >= a.cols) return;
+    const Piece p = piece_of<EPV, false>((int)(blockIdx.x * 256 + threadIdx.x) * EPV, a.cols);
+    if (!p.in) return;
     float acc[EPV] = {}, w[EPV];
-    Weights<T> weights;
-    weights.fetch(a.weight, a.wide, col, a.cols);
-    weights.settle(a.weight, a.wide, col, a.cols);
-    weights.unpack(a.weight, a.wide, w);
+    Weights<T, false, WIDE> weights;
+    weights.load(a.weight, p, a.cols);
+    weights.unpack(a.weight, w);
     for (int64_t first = (int64_t)blockIdx.y * U; first < a.rows; first += (int64_t)gridDim.y * U) {
         u32x4 h[U], dy[U], dh[U];
         float r[U], c[U];
@@ -384,9 +388,9 @@ __global__ __launch_bounds__(256) void k_rms_norm_backward_columns(const NormBac
         for (int u = 0; u < U; u++) {
             const int64_t row = first + u < a.rows ? first + u : a.rows - 1;
             const uint64_t at = (uint64_t)(row * a.cols) * ESZ;
-            h[u] = fetch_row<ESZ>(a.h + (uint64_t)(row * a.h_stride), col, a.cols);
-            dy[u] = fetch_row<ESZ>(a.dy + at, col, a.cols);
-            if (a.dh) dh[u] = fetch_row<ESZ>(a.dh + at, col, a.cols);
+            h[u] = load_row<ESZ, false>(a.h + (uint64_t)(row * a.h_stride), p, a.cols);
+            dy[u] = load_row<ESZ, false>(a.dy + at, p, a.cols);
+            if (a.dh) dh[u] = load_row<ESZ, false>(a.dh + at, p, a.cols);
             r[u] = as_global<const float>(factors)[2 * row];
             c[u] = as_global<const float>(factors)[2 * row + 1];
         }
@@ -394,23 +398,19 @@ __global__ __launch_bounds__(256) void k_rms_norm_backward_columns(const NormBac
         for (int u = 0; u < U; u++) {
             if (first + u >= a.rows) continue;
             float f[EPV], g[EPV], d[EPV];
-            Elem<T>::unpack(settle_row<ESZ>(h[u], col, a.cols), f);
-            Elem<T>::unpack(settle_row<ESZ>(dy[u], col, a.cols), g);
-            if (a.dh) Elem<T>::unpack(settle_row<ESZ>(dh[u], col, a.cols), d);
+            Elem<T>::unpack(h[u], f);
+            Elem<T>::unpack(dy[u], g);
+            if (a.dh) Elem<T>::unpack(dh[u], d);
 #pragma unroll
             for (int i = 0; i < EPV; i++) {
                 acc[i] = __builtin_fmaf(g[i], f[i] * r[u], acc[i]);
                 f[i] = r[u] * (g[i] * w[i] - f[i] * c[u]);
                 if (a.dh) f[i] += d[i];
             }
-            if (a.dx) store_row<ESZ>(a.dx + (uint64_t)((first + u) * a.cols) * ESZ, col, a.cols, Elem<T>::pack(f));
+            if (a.dx) store_row<ESZ, false>(a.dx + (uint64_t)((first + u) * a.cols) * ESZ, p, a.cols, Elem<T>::pack(f));
         }
     }
-    if (!a.sums) return;
-#pragma unroll
-    for (int i = 0; i < EPV; i += 4)
-        store_row<4, false>(a.sums + (uint64_t)blockIdx.y * (uint64_t)a.cols * 4, col + i, a.cols,
-                            u32x4{as_u(acc[i]), as_u(acc[i + 1]), as_u(acc[i + 2]), as_u(acc[i + 3])});
+    if (a.sums) store_sums(a.sums + (uint64_t)blockIdx.y * (uint64_t)sums_stride(a.cols) * 4, p, acc);
 }
 
 // out[c] = the sum of sums[p][c] over p, rounded once: 4 lanes to 16 columns, 64 of the parts side by side.
@@ -418,13 +418,17 @@ template <class T>
 __global__ __launch_bounds__(256) void k_column_sums(uint64_t sums, int64_t parts, int cols, uint64_t out)
 {
     __shared__ float add[64][17];
-    const int lane = threadIdx.x & 3, group = threadIdx.x >> 2, col = (int)blockIdx.x * 16 + lane * 4;
+    const int64_t stride = sums_stride(cols);
+    const int lane = threadIdx.x & 3, group = threadIdx.x >> 2;
+    const int64_t col = (int64_t)blockIdx.x * 16 + lane * 4;
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (col < stride) {
 #pragma unroll 8
-    for (int64_t p = group; p < parts; p += 64) {
-        const u32x4 v = load_row<4, false>(sums + (uint64_t)p * (uint64_t)cols * 4, col, cols);
+        for (int64_t p = group; p < parts; p += 64) {
+            const u32x4 v = *as_global<const u32x4>(sums + (uint64_t)(p * stride + col) * 4);
 #pragma unroll
-        for (int i = 0; i < 4; i++) s[i] += as_f(v[i]);
+            for (int i = 0; i < 4; i++) s[i] += as_f(v[i]);
+        }
     }
 #pragma unroll
     for (int i = 0; i < 4; i++) add[group][lane * 4 + i] = s[i];
@@ -444,7 +448,7 @@ __global__ __launch_bounds__(256) void k_column_sums(uint64_t sums, int64_t part
 }
 
 // The values of 8-bit rows, a lane for EPV of them.
-template <class T, int TEAM>
+template <class T, int TEAM, bool NARROW>
 __global__ __launch_bounds__(256) void k_fp8_rows(uint64_t codes, uint64_t scales, int64_t row0, int64_t rows, int cols, uint64_t out)
 {
     constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, TEAMS = 256 / TEAM, U = 2;
@@ -453,22 +457,22 @@ __global__ __launch_bounds__(256) void k_fp8_rows(uint64_t codes, uint64_t scale
     const float scale = as_global<const float>(scales)[row];
     const uint64_t from = codes + (uint64_t)(row * cols), to = out + (uint64_t)(row * cols) * ESZ;
     for (int col = threadIdx.x % TEAM * EPV; col < cols; col += U * TEAM * EPV) {
-        u32 w[U][2];
+        u32 w[U][2] = {};
+        Piece p[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int at = col + u * TEAM * EPV;
-            w[u][0] = w[u][1] = 0;
-            if (at + EPV <= cols) {
-                if constexpr (EPV == 8) {
-                    const u32x2 v = LOAD_STREAM(as_global<const u32x2_a1>(from + (u32)at));
-                    w[u][0] = v.x;
-                    w[u][1] = v.y;
-                } else w[u][0] = LOAD_STREAM(as_global<const u32_a1>(from + (u32)at));
-            } else {
-#pragma unroll
-                for (int i = 0; i < EPV; i++)
-                    if (at + i < cols) w[u][i / 4] |= (u32)as_global<const uint8_t>(from + (u32)at)[i] << (i % 4 * 8);
-            }
+            p[u] = piece_of<EPV, NARROW>(col + u * TEAM * EPV, cols);
+            if (!p[u].in) continue;
+            const uint64_t at = from + (u32)p[u].at;
+            if (NARROW) {
+                const u32x4 v = load_bytes(at, (u32)cols);
+                w[u][0] = v.x;
+                w[u][1] = v.y;
+            } else if constexpr (EPV == 8) {
+                const u32x2 v = LOAD_STREAM(as_global<const u32x2_a1>(at));
+                w[u][0] = v.x;
+                w[u][1] = v.y;
+            } else w[u][0] = LOAD_STREAM(as_global<const u32_a1>(at));
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
@@ -480,7 +484,7 @@ __global__ __launch_bounds__(256) void k_fp8_rows(uint64_t codes, uint64_t scale
 #pragma unroll
                 for (int j = 0; j < 4; j++) f[i + j] = four[j] * scale;
             }
-            store_row<ESZ>(to, col + u * TEAM * EPV, cols, Elem<T>::pack(f));
+            store_row<ESZ, NARROW>(to, p[u], cols, Elem<T>::pack(f));
         }
     }
 }
@@ -489,9 +493,9 @@ __global__ __launch_bounds__(256) void k_fp8_rows(uint64_t codes, uint64_t scale
 // launches
 // ---------------------------------------------------------------------------
 // Lanes and vectors to a row of `vectors`; {0, 0}: too long for registers.  Two vectors a lane hide more of memory's latency
-// than one, and lanes that a row leaves idle cost as much as others: rows of 16 vectors (163840 fp16) take 17.5 us with 8 lanes of
+// than one, and lanes that a row leaves idle cost as much as others: rows of 16 vectors (163840 fp16) took 17.5 us with 8 lanes of
 // two, 18.4 with 16, 47 with 64; rows of 512 (8192 bf16 with a residual) 45.8 with 512 lanes, 47.5 with 256 of two, one
-// row 3.4 and 3.8.
+// row 3.4 and 3.8.  Now 15.5, 44.1 (6.1 TB/s) and 3.1.
 static RowShape norm_shape(int64_t vectors)
 {
     if (vectors <= 8) return {8, 1};
@@ -510,7 +514,8 @@ static RowShape norm_shape(int64_t vectors)
 // The same for the backward pass, whose lanes keep a column's sum and the next row beside: us of rows of 42
 // vectors (65536 bf16) 42.3 with 16 lanes of three, 47.2 with 64 of one; of 251 (8192 fp32) 30.0 with 64 of four, 42.1 with
 // 256 of one; of 256 (16384 bf16, where four take all registers) 58.2 and 51.9; of 512 (8192 bf16) 49.9 with 512 of
-// one, 52.9 with 256 of two.
+// one, 52.9 with 256 of two; of 2048 (2048 bf16) 71 with 1024 of two, 121 with 512 of four, which spill.  Now 43, 28, 49, 50
+// and 71: 4.0, 4.7, 5.5, 5.3 and 3.8 TB/s.
 static RowShape norm_backward_shape(int64_t vectors, int size)
 {
     if (vectors <= 8) return {8, 1};
@@ -523,21 +528,24 @@ static RowShape norm_backward_shape(int64_t vectors, int size)
     if (vectors <= 256) return size == 4 ? RowShape{64, 4} : RowShape{256, 1};
     if (vectors <= 512) return {512, 1};
     if (vectors <= 1024) return {512, 2};
-    if (vectors <= 2048) return {512, 4};
+    if (vectors <= 2048) return {1024, 2};
     return {0, 0};
 }
 
-#define SHAPE(TEAM, NV) case TEAM * 16 + NV: K(TEAM, NV); break;
+static bool narrow_row(int64_t cols, int size) { return cols * size < 16; }
 
-template <class T, bool FP8>
+#define SHAPE(TEAM, NV) case TEAM * 16 + NV: K(TEAM, NV, false); break;
+
+template <class T, bool WIDE, bool FP8>
 static int norm(NormArgs a, hipStream_t st)
 {
     const RowShape shape = norm_shape((a.cols + Elem<T>::EPV - 1) / Elem<T>::EPV);
-    const void *k = (const void *)k_rms_norm_long<T, FP8>;
-#define K(TEAM, NV) k = (const void *)k_rms_norm<T, TEAM, NV, FP8>
+    const void *k = (const void *)k_rms_norm_long<T, WIDE, FP8>;
+#define K(TEAM, NV, NARROW) k = (const void *)k_rms_norm<T, TEAM, NV, NARROW, WIDE, FP8>
     switch (shape.team * 16 + shape.nv) {
         SHAPE(8, 1) SHAPE(8, 2) SHAPE(16, 2) SHAPE(32, 2) SHAPE(64, 2) SHAPE(256, 1) SHAPE(512, 1) SHAPE(512, 2) SHAPE(1024, 2) SHAPE(1024, 4)
     }
+    if (narrow_row(a.cols, Elem<T>::ESZ)) K(8, 1, true);
 #undef K
     const int threads = shape.team == 0 ? 1024 : shape.team > 256 ? shape.team : 256, teams = shape.team == 0 ? 1 : threads / shape.team;
     const int64_t at_once = ROWS_THREADS / threads * teams;
@@ -561,26 +569,27 @@ static int64_t norm_parts(int64_t rows, int64_t cols, int size)
     return std::min(most, (rows + teams - 1) / teams);
 }
 
-template <class T>
+template <class T, bool WIDE>
 static int norm_backward(NormBackwardArgs a, uint64_t factors, int64_t parts, hipStream_t st)
 {
     const RowShape shape = norm_backward_shape((a.cols + Elem<T>::EPV - 1) / Elem<T>::EPV, Elem<T>::ESZ);
     if (shape.team == 0) {
         void *args[] = {(void *)&a, (void *)&factors};
-        int rc = (int)hipLaunchKernel((const void *)k_rms_norm_backward_long<T>, dim3((unsigned)std::min<int64_t>(a.rows, 2048)), dim3(1024),
+        int rc = (int)hipLaunchKernel((const void *)k_rms_norm_backward_long<T, WIDE>, dim3((unsigned)std::min<int64_t>(a.rows, 2048)), dim3(1024),
                                       args, 0, st);
         if (rc) return rc;
         const unsigned across = (unsigned)((a.cols + 256 * Elem<T>::EPV - 1) / (256 * Elem<T>::EPV));
-        return (int)hipLaunchKernel((const void *)k_rms_norm_backward_columns<T>, dim3(across, (unsigned)parts), dim3(256), args, 0, st);
+        return (int)hipLaunchKernel((const void *)k_rms_norm_backward_columns<T, WIDE>, dim3(across, (unsigned)parts), dim3(256), args, 0, st);
     }
     const void *k = nullptr;
-#define K(TEAM, NV) k = (const void *)k_rms_norm_backward<T, TEAM, NV>
+#define K(TEAM, NV, NARROW) k = (const void *)k_rms_norm_backward<T, TEAM, NV, NARROW, WIDE>
     if constexpr (Elem<T>::ESZ == 4) {
-        if (shape.team == 64 && shape.nv == 4) K(64, 4);
-    } else if (shape.team == 256) K(256, 1);
+        if (shape.team == 64 && shape.nv == 4) K(64, 4, false);
+    } else if (shape.team == 256) K(256, 1, false);
     switch (shape.team * 16 + shape.nv) {
-        SHAPE(8, 1) SHAPE(8, 2) SHAPE(16, 2) SHAPE(16, 3) SHAPE(32, 2) SHAPE(64, 2) SHAPE(64, 3) SHAPE(512, 1) SHAPE(512, 2) SHAPE(512, 4)
+        SHAPE(8, 1) SHAPE(8, 2) SHAPE(16, 2) SHAPE(16, 3) SHAPE(32, 2) SHAPE(64, 2) SHAPE(64, 3) SHAPE(512, 1) SHAPE(512, 2) SHAPE(1024, 2)
     }
+    if (narrow_row(a.cols, Elem<T>::ESZ)) K(8, 1, true);
 #undef K
 #undef SHAPE
     void *args[] = {(void *)&a};
@@ -601,10 +610,13 @@ extern "C" int tftq_rms_norm(int dtype, int weight_dtype, const void *x, int64_t
     if (scope.err != hipSuccess) return (int)scope.err;
     const int size = dtype_size(dtype);
     const NormArgs a = {(uint64_t)x, (uint64_t)residual, (uint64_t)weight, (uint64_t)y, (uint64_t)h, (uint64_t)codes, (uint64_t)scales,
-                        x_stride * size, residual_stride * size, 0, rows, (int)cols, weight && weight_dtype != dtype, eps, 1.0f / (float)cols};
+                        x_stride * size, residual_stride * size, 0, rows, (int)cols, eps, 1.0f / (float)cols};
     hipStream_t st = (hipStream_t)stream;
-    if (codes) return dtype == TFTQ_F32 ? norm<float, true>(a, st) : dtype == TFTQ_F16 ? norm<f16_tag, true>(a, st) : norm<bf16_tag, true>(a, st);
-    return dtype == TFTQ_F32 ? norm<float, false>(a, st) : dtype == TFTQ_F16 ? norm<f16_tag, false>(a, st) : norm<bf16_tag, false>(a, st);
+    const bool wide = weight && weight_dtype != dtype;
+#define NORM(T) (wide ? codes ? norm<T, true, true>(a, st) : norm<T, true, false>(a, st) : codes ? norm<T, false, true>(a, st) : norm<T, false, false>(a, st))
+    if (dtype == TFTQ_F32) return codes ? norm<float, false, true>(a, st) : norm<float, false, false>(a, st);
+    return dtype == TFTQ_F16 ? NORM(f16_tag) : NORM(bf16_tag);
+#undef NORM
 }
 
 extern "C" int64_t tftq_rms_norm_backward_workspace(int dtype, int64_t rows, int64_t cols)
@@ -612,7 +624,7 @@ extern "C" int64_t tftq_rms_norm_backward_workspace(int dtype, int64_t rows, int
     if (!dtype_ok(dtype)) return TFTQ_E_DTYPE;
     if (!rows_ok(rows, cols)) return TFTQ_E_SHAPE;
     if (rows == 0 || cols == 0) return 0;
-    return norm_parts(rows, cols, dtype_size(dtype)) * cols * 4 + rows * 8;
+    return norm_parts(rows, cols, dtype_size(dtype)) * sums_stride(cols) * 4 + rows * 8;
 }
 
 extern "C" int tftq_rms_norm_backward(int dtype, int weight_dtype, const void *dy, const void *dh, const void *h, int64_t h_stride,
@@ -625,18 +637,19 @@ extern "C" int tftq_rms_norm_backward(int dtype, int weight_dtype, const void *d
     if ((dweight && !weight) || (rows && (!dy || !h || !workspace || ((uintptr_t)workspace & 15))) || (!dx && !dweight) || !(eps >= 0.0f)) return TFTQ_E_ARG;
     if (rows && h_stride < (rows > 1 ? cols : 0)) return TFTQ_E_ARG;
     const int size = dtype_size(dtype);
-    const int64_t parts = rows ? norm_parts(rows, cols, size) : 0, sums = parts * cols * 4;
+    const int64_t parts = rows ? norm_parts(rows, cols, size) : 0, sums = parts * sums_stride(cols) * 4;
     if (rows && workspace_bytes < sums + rows * 8) return TFTQ_E_SIZE;
     DeviceScope scope(device);
     if (scope.err != hipSuccess) return (int)scope.err;
     hipStream_t st = (hipStream_t)stream;
     if (rows) {
         const NormBackwardArgs a = {(uint64_t)dy, (uint64_t)dh, (uint64_t)h, (uint64_t)weight, (uint64_t)dx, dweight ? (uint64_t)workspace : 0,
-                                    h_stride * size, rows, (int)cols, weight && weight_dtype != dtype, eps, 1.0f / (float)cols};
+                                    h_stride * size, rows, (int)cols, eps, 1.0f / (float)cols};
         const uint64_t factors = (uint64_t)workspace + (uint64_t)sums;
-        const int rc = dtype == TFTQ_F32   ? norm_backward<float>(a, factors, parts, st)
-                       : dtype == TFTQ_F16 ? norm_backward<f16_tag>(a, factors, parts, st)
-                                           : norm_backward<bf16_tag>(a, factors, parts, st);
+        const bool wide = weight && weight_dtype != dtype;
+#define NORM(T) (wide ? norm_backward<T, true>(a, factors, parts, st) : norm_backward<T, false>(a, factors, parts, st))
+        const int rc = dtype == TFTQ_F32 ? norm_backward<float, false>(a, factors, parts, st) : dtype == TFTQ_F16 ? NORM(f16_tag) : NORM(bf16_tag);
+#undef NORM
         if (rc || !dweight) return rc;
     }
     uint64_t from = (uint64_t)workspace, to = (uint64_t)dweight;
@@ -663,7 +676,11 @@ extern "C" int tftq_fp8_rows_dequantize(int dtype, const void *codes, const floa
     int64_t row0 = 0;
     int c = (int)cols;
     void *args[] = {(void *)&from, (void *)&by, (void *)&row0, (void *)&rows, (void *)&c, (void *)&to};
-#define K(T) (team == 8 ? (const void *)k_fp8_rows<T, 8> : team == 64 ? (const void *)k_fp8_rows<T, 64> : (const void *)k_fp8_rows<T, 256>)
+#define K(T)                                                                                  \
+    (narrow_row(cols, Elem<T>::ESZ) ? (const void *)k_fp8_rows<T, 8, true>                        \
+     : team == 8                    ? (const void *)k_fp8_rows<T, 8, false>                       \
+     : team == 64                   ? (const void *)k_fp8_rows<T, 64, false>                      \
+                                    : (const void *)k_fp8_rows<T, 256, false>)
     const void *k = dtype == TFTQ_F32 ? K(float) : dtype == TFTQ_F16 ? K(f16_tag) : K(bf16_tag);
 #undef K
     const int64_t at_once = ROWS_THREADS / team;

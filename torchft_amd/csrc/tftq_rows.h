@@ -1,8 +1,12 @@
 // What the kernels of row operators share (tftq_norm.hip, tftq_dropout.hip, tftq_embedding.hip, tftq_experts.hip).
 //
 // A row is a run of `cols` elements at any address that is a multiple of the element's size.  A team of
-// lanes takes it in vectors of 16 bytes: lane l of the team has the vectors l, l + TEAM, l + 2 TEAM, ...
-// The last vector may hold fewer elements; what lies past the row reads as zero and is not written.
+// lanes takes it in vectors of 16 bytes: lane l of the team has the vectors l, l + TEAM, l + 2 TEAM, ...  Where a row is
+// no whole number of vectors its last one is moved back to end with the row: the elements that two lanes
+// then have (Piece::over of the later one) are the same in both, are stored twice, and count in a sum once.  So every load and
+// store is a whole vector and no lane waits for one before it has asked for all (rows of 333 bf16 columns whose last
+// vector was read element by element took 2.6 TB/s, now 5).  Rows shorter than a vector have kernels of their own (NARROW), where the first
+// lane has all of the row and zeros behind it.
 #pragma once
 
 #include "tftq_device.h"
@@ -16,81 +20,116 @@ typedef uint16_t uint16_a1 __attribute__((aligned(1)));
 constexpr int64_t ROWS_THREADS = (int64_t)1 << 31;
 constexpr int64_t ROWS_MOST = ((int64_t)1 << 31) - 65536;  // rows, columns, tokens and choices are at most so many
 
-template <int ESZ> struct RowWord;
-template <> struct RowWord<1> { typedef uint8_t type; };
-template <> struct RowWord<2> { typedef uint16_t type; };
-template <> struct RowWord<4> { typedef uint32_t type; };
-
-// Elements col to col + 16 / ESZ - 1 of the row at `row` in two steps: fetch_row asks memory for them, settle_row puts
-// them in their places.  The last vector of a row is fetched further ahead, so that it ends with the row, and
-// moved down afterwards: no lane waits for memory before all it needs has been asked for (with the two in one, rows
-// of 333 bf16 columns took 2.6 TB/s).  A row of fewer elements than a vector is fetched one by one.
-template <int ESZ, bool STREAM = true>
-DEV u32x4 fetch_row(uint64_t row, int col, int cols)
+// The first n (0 to 16) bytes at an address, zeros behind, and back.
+DEV u32x4 load_bytes(uint64_t at, u32 n)
 {
-    constexpr int EPV = 16 / ESZ;
-    typedef typename RowWord<ESZ>::type Word;
+    if (n >= 16) return *as_global<const u32x4_a1>(at);
     u32x4 v = {0, 0, 0, 0};
-    if (cols >= EPV) {
-        if (col < cols) {
-            const GLOBAL u32x4_a1 *at = as_global<const u32x4_a1>(row + (uint64_t)(u32)min(col, cols - EPV) * ESZ);
-            if (STREAM) v = LOAD_STREAM(at);
-            else v = *at;
-        }
-    } else if (col == 0) {
-#pragma unroll
-        for (int i = 0; i < EPV - 1; i++)
-            if (i < cols) v[i * ESZ / 4] |= (u32)as_global<const Word>(row)[i] << (i * ESZ % 4 * 8);
+    u32 low = 0, high = 0;
+    if (n & 8) {
+        const u32x2 w = *as_global<const u32x2_a1>(at);
+        v.x = w.x;
+        v.y = w.y;
+        at += 8;
+    }
+    if (n & 4) {
+        low = *as_global<const u32_a1>(at);
+        at += 4;
+    }
+    if (n & 2) {
+        high = *as_global<const uint16_a1>(at);
+        at += 2;
+    }
+    if (n & 1) high |= (u32)*as_global<const uint8_t>(at) << (n & 2 ? 16 : 0);
+    if (!(n & 4)) {
+        low = high;
+        high = 0;
+    }
+    if (n & 8) return u32x4{v.x, v.y, low, high};
+    return u32x4{low, high, 0, 0};
+}
+DEV void store_bytes(uint64_t at, u32 n, u32x4 v)
+{
+    if (n >= 16) {
+        *as_global<u32x4_a1>(at) = v;
+        return;
+    }
+    if (n & 8) {
+        *as_global<u32x2_a1>(at) = u32x2{v.x, v.y};
+        v.x = v.z;
+        v.y = v.w;
+        at += 8;
+    }
+    if (n & 4) {
+        *as_global<u32_a1>(at) = v.x;
+        v.x = v.y;
+        at += 4;
+    }
+    if (n & 2) {
+        *as_global<uint16_a1>(at) = (uint16_t)v.x;
+        v.x >>= 16;
+        at += 2;
+    }
+    if (n & 1) *as_global<uint8_t>(at) = (uint8_t)v.x;
+}
+
+// Where a lane's vector of EPV elements is in a row, for the column at which it would begin if it were not moved.
+struct Piece {
+    bool in;   // there is one
+    int at;    // its first column
+    int over;  // so many of its first elements belong to the lane before
+};
+template <int EPV, bool NARROW>
+DEV Piece piece_of(int col, int cols)
+{
+    const int at = NARROW ? 0 : min(col, cols - EPV);
+    return {NARROW ? col == 0 : col < cols, at, col - at};
+}
+
+// The vector at a piece, zeros where there is none, and back.
+template <int ESZ, bool NARROW, bool STREAM = true>
+DEV u32x4 load_row(uint64_t row, const Piece &p, int cols)
+{
+    u32x4 v = {0, 0, 0, 0};
+    if (p.in) {
+        const uint64_t at = row + (uint64_t)(u32)p.at * ESZ;
+        if (NARROW) v = load_bytes(at, (u32)cols * ESZ);
+        else if (STREAM) v = LOAD_STREAM(as_global<const u32x4_a1>(at));
+        else v = *as_global<const u32x4_a1>(at);
     }
     return v;
 }
-template <int ESZ>
-DEV u32x4 settle_row(u32x4 w, int col, int cols)
+template <int ESZ, bool NARROW, bool STREAM = true>
+DEV void store_row(uint64_t row, const Piece &p, int cols, u32x4 v)
 {
-    constexpr int EPV = 16 / ESZ;
-    const int over = col + EPV - cols;  // elements past the row
-    if (cols >= EPV && over > 0 && over < EPV) {
-        const u32 n = (u32)over * ESZ >> 2, sh = ((u32)over * ESZ & 3) * 8;
-        const u32 a[5] = {n == 0 ? w.x : n == 1 ? w.y : n == 2 ? w.z : w.w, n == 0 ? w.y : n == 1 ? w.z : n == 2 ? w.w : 0u,
-                          n == 0 ? w.z : n == 1 ? w.w : 0u, n == 0 ? w.w : 0u, 0u};
-#pragma unroll
-        for (int i = 0; i < 4; i++) w[i] = ESZ == 4 ? a[i] : (u32)((((uint64_t)a[i + 1] << 32) | a[i]) >> sh);
-    }
-    return w;
+    if (!p.in) return;
+    const uint64_t at = row + (uint64_t)(u32)p.at * ESZ;
+    if (NARROW) store_bytes(at, (u32)cols * ESZ, v);
+    else if (STREAM) STORE_STREAM(v, as_global<u32x4_a1>(at));
+    else *as_global<u32x4_a1>(at) = v;
 }
-// Both at once, where nothing else is under way.
-template <int ESZ, bool STREAM = true>
-DEV u32x4 load_row(uint64_t row, int col, int cols) { return settle_row<ESZ>(fetch_row<ESZ, STREAM>(row, col, cols), col, cols); }
 
-template <int ESZ, bool STREAM = true>
-DEV void store_row(uint64_t row, int col, int cols, u32x4 v)
+// Zeros for the elements that the lane before has too: before a sum over the row.
+template <int EPV>
+DEV void count_once(float (&f)[EPV], const Piece &p)
 {
-    constexpr int EPV = 16 / ESZ;
-    uint64_t at = row + (uint64_t)(u32)col * ESZ;
-    const int left = cols - col;
-    if (left >= EPV) {
-        if (STREAM) STORE_STREAM(v, as_global<u32x4_a1>(at));
-        else *as_global<u32x4_a1>(at) = v;
-    } else if (left > 0) {  // 8, 4, 2 and 1 bytes
-        const u32 bytes = (u32)left * ESZ;
-        if (bytes & 8) {
-            *as_global<u32x2_a1>(at) = u32x2{v.x, v.y};
-            v.x = v.z;
-            v.y = v.w;
-            at += 8;
-        }
-        if (bytes & 4) {
-            *as_global<u32_a1>(at) = v.x;
-            v.x = v.y;
-            at += 4;
-        }
-        if (ESZ <= 2 && (bytes & 2)) {
-            *as_global<uint16_a1>(at) = (uint16_t)v.x;
-            v.x >>= 16;
-            at += 2;
-        }
-        if (ESZ == 1 && (bytes & 1)) *as_global<uint8_t>(at) = (uint8_t)v.x;
+    if (p.over > 0) {
+#pragma unroll
+        for (int i = 0; i < EPV - 1; i++)
+            if (i < p.over) f[i] = 0.0f;
     }
+}
+
+// fp32 sums of a row's columns, kept apart: EPV of them from a piece's first column on.  Their rows are
+// sums_stride(cols) long, so that a narrow row has room for a vector.
+static TFTQ_HD inline int64_t sums_stride(int64_t cols) { return cols < 8 ? 8 : (cols + 3) & ~(int64_t)3; }
+template <int EPV>
+DEV void store_sums(uint64_t row, const Piece &p, const float (&f)[EPV])
+{
+    if (!p.in) return;
+#pragma unroll
+    for (int i = 0; i < EPV; i += 4)
+        *as_global<u32x4_a4>(row + (uint64_t)(u32)(p.at + i) * 4) = u32x4{as_u(f[i]), as_u(f[i + 1]), as_u(f[i + 2]), as_u(f[i + 3])};
 }
 
 // The sum over the team's lanes, in an order that the team alone decides; every lane gets it.

@@ -68,6 +68,17 @@ DEV u32 sort_prefix(u32 v, u32 *sums)
     return base;
 }
 
+// Workgroups from `tiles` on write zeros, a piece each.
+constexpr int64_t SORT_PIECE = 65536;
+template <int THREADS>
+DEV bool sort_fill(const SortArgs &a, int tiles)
+{
+    if ((int)blockIdx.x < tiles) return false;
+    const int64_t at = ((int64_t)blockIdx.x - tiles) * SORT_PIECE;
+    fill_zeros<THREADS>(a.fill + (uint64_t)at, min(SORT_PIECE, a.fill_bytes - at));
+    return true;
+}
+
 // n numbers in one workgroup, wavefront w the w-th share of them.
 template <int THREADS, int ITEMS>
 __global__ __launch_bounds__(THREADS) void k_sort_one(const SortArgs a, int passes, int width)
@@ -76,6 +87,7 @@ __global__ __launch_bounds__(THREADS) void k_sort_one(const SortArgs a, int pass
     constexpr int Q = THREADS / DIGITS, EACH = WAVES / Q;  // threads to a digit, wavefronts' counters to a thread
     __shared__ u32 counts[WAVES][DIGITS], sums[WAVES], keys[MOST];
     __shared__ uint16_t places[MOST];
+    if (sort_fill<THREADS>(a, 1)) return;
     const int n = (int)a.n, lane = threadIdx.x & 63, items = (n + THREADS - 1) / THREADS, first = (int)(threadIdx.x / 64) * 64 * items + lane;
     u32 *mine = counts[threadIdx.x / 64];
     u32 key[ITEMS], place[ITEMS], digit[ITEMS], rank[ITEMS];
@@ -153,6 +165,7 @@ DEV u32 sort_read(const SortArgs &a, const SortPass &p, int64_t i) { return p.ke
 __global__ __launch_bounds__(256) void k_sort_count(const SortArgs a, const SortPass p)
 {
     __shared__ u32 counts[256];
+    if (sort_fill<256>(a, p.tiles)) return;
     counts[threadIdx.x] = 0;
     __syncthreads();
     const int64_t first = (int64_t)blockIdx.x * SORT_TILE + threadIdx.x;
@@ -185,6 +198,7 @@ __global__ __launch_bounds__(256) void k_sort_before(const SortPass p)
 __global__ __launch_bounds__(256) void k_sort_place(const SortArgs a, const SortPass p)
 {
     __shared__ u32 counts[4][256], sums[4];
+    if (sort_fill<256>(a, p.tiles)) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x / 64, d = threadIdx.x;
     u32 key[SORT_ITEMS], digit[SORT_ITEMS], rank[SORT_ITEMS], place[SORT_ITEMS];
     bool live[SORT_ITEMS];
@@ -271,6 +285,15 @@ int64_t sort_workspace(int64_t n, int64_t classes)
 
 bool sort_needs_keys(int64_t n, int64_t classes) { return sort_searches(n, classes); }
 
+// At 6.5 TB/s: one workgroup takes 3 us for up to 256 numbers and 6 to 18 for up to 8192, a pass over tiles 8.
+int64_t sort_fills(int64_t n, int64_t classes)
+{
+    if (sort_one(n, classes)) return n <= 256 ? 20000000 : 40000000 + n * 10000;
+    return (sort_bits(classes) + 7) / 8 * 52000000;
+}
+
+static unsigned sort_groups(const SortArgs &a, int tiles) { return (unsigned)(tiles + (a.fill_bytes + SORT_PIECE - 1) / SORT_PIECE); }
+
 static int sort_offsets(SortArgs a, hipStream_t st)
 {
     void *args[] = {(void *)&a};
@@ -290,7 +313,7 @@ int sort_numbers(const SortArgs &in, void *workspace, hipStream_t st)
                                       : (const void *)k_sort_one<1024, 8>;
         const uint64_t offsets = a.offsets;
         if (sort_searches(a.n, a.classes)) a.offsets = 0;
-        const int rc = (int)hipLaunchKernel(k, dim3(1), dim3(a.n <= 256 ? 256 : 1024), args, 0, st);
+        const int rc = (int)hipLaunchKernel(k, dim3(sort_groups(a, 1)), dim3(a.n <= 256 ? 256 : 1024), args, 0, st);
         if (rc || a.offsets == offsets) return rc;
         a.offsets = offsets;
         return sort_offsets(a, st);
@@ -302,6 +325,12 @@ int sort_numbers(const SortArgs &in, void *workspace, hipStream_t st)
     p.counts = (uint64_t)workspace;
     p.width = width;
     const uint64_t pairs = p.counts + (uint64_t)(p.pitch + 1) * 1024, pair = ((uint64_t)a.n * 8 + 15) & ~(uint64_t)15;
+    // the launches' shares of the zeros
+    const int64_t share = (in.fill_bytes / (2 * passes) + SORT_PIECE - 1) / SORT_PIECE * SORT_PIECE;
+    auto next_share = [&](bool first) {
+        if (!first) a.fill += (uint64_t)a.fill_bytes;
+        a.fill_bytes = std::min(share, in.fill_bytes - (int64_t)(a.fill - in.fill));
+    };
     for (int pass = 0; pass < passes; pass++) {
         const bool last = pass == passes - 1;
         p.keys = p.to_keys;
@@ -312,10 +341,12 @@ int sort_numbers(const SortArgs &in, void *workspace, hipStream_t st)
         p.offsets = passes == 1 ? a.offsets : 0;
         p.shift = pass * width;
         void *args[] = {(void *)&a, (void *)&p}, *before[] = {(void *)&p};
-        if (const int rc = (int)hipLaunchKernel((const void *)k_sort_count, dim3((unsigned)p.tiles), dim3(256), args, 0, st)) return rc;
+        next_share(pass == 0);
+        if (const int rc = (int)hipLaunchKernel((const void *)k_sort_count, dim3(sort_groups(a, p.tiles)), dim3(256), args, 0, st)) return rc;
         if (p.tiles > SORT_DIRECT)
             if (const int rc = (int)hipLaunchKernel((const void *)k_sort_before, dim3(256), dim3(256), before, 0, st)) return rc;
-        if (const int rc = (int)hipLaunchKernel((const void *)k_sort_place, dim3((unsigned)p.tiles), dim3(256), args, 0, st)) return rc;
+        next_share(false);
+        if (const int rc = (int)hipLaunchKernel((const void *)k_sort_place, dim3(sort_groups(a, p.tiles)), dim3(256), args, 0, st)) return rc;
     }
     return a.offsets && passes > 1 ? sort_offsets(a, st) : 0;
 }
