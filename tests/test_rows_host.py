@@ -115,7 +115,7 @@ def test_c_entries_check_before_they_launch():
     assert send(size=8) == -2 and send(xs=7) == -1 and send(tokens=2 ** 30, k=4) == -3 and send(used=None) == -1 and send(k=0) == 0
     back = lambda **k: lib.tftq_combine(*{**dict(dtype=2, wdtype=0, rows=p, rs=8, w=p, tokens=3, k=2, cols=8, position=p, used=p, out=p, device=-1,  # noqa: E731
                                                    stream=None), **k}.values())
-    assert back(wdtype=1) == -2 and back(rs=3) == -1 and back(rows=None) == -1 and back(tokens=0) == 0
+    assert back(wdtype=1) == -2 and back(rs=3) == -1 and back(rows=None) == -1 and back(tokens=0) == 0 and back(k=0, used=None) == -1
     back = lambda **k: lib.tftq_combine_backward(*{**dict(dtype=2, wdtype=0, dy=p, ds=8, rows=p, rs=8, w=p, tokens=3, k=2, cols=8, position=p, used=p,  # noqa: E731
                                                             dr=p, dw=p, device=-1, stream=None), **k}.values())
     assert back(w=None) == -1 and back(rows=None) == -1 and back(dr=None, dw=None) == -1 and back(ds=1) == -1 and back(wdtype=1) == -2

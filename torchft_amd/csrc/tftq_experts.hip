@@ -22,6 +22,9 @@ struct ExpertArgs {
     int cols, k, wide;  // wide: the weights are fp32 and the rows are not
 };
 
+// How many places have an expert: whatever memory says, no more than there are.
+DEV u32 places_used(const ExpertArgs &a) { return min(*as_global<const u32>(a.used), (u32)(a.tokens * a.k)); }
+
 // x [tokens] -> y [tokens k] by places; elements of ESZ bytes.
 template <int ESZ, int TEAM, int U, bool NARROW>
 __global__ __launch_bounds__(256) void k_dispatch(const ExpertArgs a)
@@ -30,7 +33,7 @@ __global__ __launch_bounds__(256) void k_dispatch(const ExpertArgs a)
     const int lane = threadIdx.x % TEAM;
     const int64_t token = a.token0 + (int64_t)blockIdx.x * TEAMS + threadIdx.x / TEAM;
     if (token >= a.tokens) return;
-    const u32 used = *as_global<const u32>(a.used);
+    const u32 used = places_used(a);
     const GLOBAL u32 *position = as_global<const u32>(a.position) + token * a.k;
     const uint64_t from = a.x + (uint64_t)(token * a.x_stride);
     for (int col = lane * EPV; col < a.cols; col += U * TEAM * EPV) {
@@ -43,6 +46,7 @@ __global__ __launch_bounds__(256) void k_dispatch(const ExpertArgs a)
         }
         for (int s = 0; s < a.k; s++) {
             const u32 place = position[s];
+            if (place >= (u32)(a.tokens * a.k)) continue;
             const uint64_t to = a.y + (uint64_t)place * (uint64_t)a.cols * ESZ;
 #pragma unroll
             for (int u = 0; u < U; u++) store_row<ESZ, NARROW, false>(to, p[u], a.cols, place < used ? raw[u] : u32x4{0, 0, 0, 0});
@@ -65,7 +69,7 @@ __global__ __launch_bounds__(256) void k_combine(const ExpertArgs a)
     const int lane = threadIdx.x % TEAM;
     const int64_t token = a.token0 + (int64_t)blockIdx.x * TEAMS + threadIdx.x / TEAM;
     if (token >= a.tokens) return;
-    const u32 used = *as_global<const u32>(a.used);
+    const u32 used = places_used(a);
     const int64_t choice = token * a.k;
     const uint64_t to = a.y + (uint64_t)(token * a.cols) * ESZ;
     for (int col = lane * EPV; col < a.cols; col += U * TEAM * EPV) {
@@ -117,7 +121,7 @@ __global__ __launch_bounds__(256) void k_combine_backward(const ExpertArgs a)
     const int lane = threadIdx.x % TEAM;
     const int64_t token = a.token0 + (int64_t)blockIdx.x * TEAMS + threadIdx.x / TEAM;
     if (token >= a.tokens) return;
-    const u32 used = *as_global<const u32>(a.used);
+    const u32 used = places_used(a);
     const uint64_t from = a.x + (uint64_t)(token * a.x_stride);
     Piece piece[NV];
     u32x4 dy[NV];
@@ -164,7 +168,7 @@ __global__ __launch_bounds__(256) void k_combine_backward(const ExpertArgs a)
                 if (!NARROW) count_once(once, piece[v]);
 #pragma unroll
                 for (int s = 0; s < S; s++) {
-                    if (s0 + s >= a.k) continue;
+                    if (s0 + s >= a.k || place[s] >= (u32)(a.tokens * a.k)) continue;
                     float f[EPV], out[EPV];
                     Elem<T>::unpack(raw[s][v], f);
                     if (!NARROW) count_once(f, piece[v]);  // no 0 times infinity
@@ -280,7 +284,7 @@ extern "C" int tftq_combine(int dtype, int weight_dtype, const void *rows, int64
     if (!dtype_ok(dtype) || (weights && weight_dtype != dtype && weight_dtype != TFTQ_F32)) return TFTQ_E_DTYPE;
     if (!experts_ok(tokens, k, cols)) return TFTQ_E_SHAPE;
     if (tokens == 0 || cols == 0) return 0;
-    if ((k && (!rows || !position || !used)) || !out || rows_stride < (tokens * k > 1 ? cols : 0)) return TFTQ_E_ARG;
+    if ((k && (!rows || !position)) || !used || !out || rows_stride < (tokens * k > 1 ? cols : 0)) return TFTQ_E_ARG;
     DeviceScope scope(device);
     if (scope.err != hipSuccess) return (int)scope.err;
     const int size = dtype_size(dtype);

@@ -69,12 +69,18 @@ struct {
     int (*fp8_rows_dequantize)(int, const void *, const float *, int64_t, int64_t, void *, int, void *) = nullptr;
 } lib;
 
-int64_t checked(int64_t code, const char *what)
+[[noreturn]] void failed(int code, const char *what)
 {
-    if (code < 0 || (code > 0 && !strstr(what, "workspace")))
-        throw std::runtime_error(std::string(what) + " failed: " +
-                                 (code > 0 ? "hipError_t " + std::to_string(code) : lib.strerror(static_cast<int>(code))));
-    return code;
+    throw std::runtime_error(std::string(what) + " failed: " + (code > 0 ? "hipError_t " + std::to_string(code) : lib.strerror(code)));
+}
+void checked(int code, const char *what)
+{
+    if (code) failed(code, what);
+}
+int64_t bytes_needed(int64_t size, const char *what)
+{
+    if (size < 0) failed(static_cast<int>(size), what);
+    return size;
 }
 
 // Tensors that stand for others.
@@ -99,9 +105,7 @@ void ready(const Tensor &t)
     require(t.device().is_cuda(), "A GPU tensor is required");
     const int i = t.device().index();
     if (i < 64 && (known.load() >> i & 1)) return;
-    if (const int rc = lib.check_device(i))
-        throw std::runtime_error("cuda:" + std::to_string(i) + " cannot run the tftq kernels: " +
-                                 (rc > 0 ? "hipError_t " + std::to_string(rc) : lib.strerror(rc)));
+    checked(lib.check_device(i), "tftq_check_device");
     if (i < 64) known |= 1ull << i;
 }
 
@@ -229,7 +233,7 @@ struct Norm : torch::autograd::Function<Norm> {
                          weight = weight_.defined() ? weight_.resolve_neg().contiguous() : weight_;
             if (for_x || for_r) dx = fresh(h_.sizes(), h_.scalar_type(), h_);
             if (for_w) dw = fresh(weight.sizes(), weight.scalar_type(), h_);
-            const int64_t size = checked(lib.rms_norm_backward_workspace(code_of(h_), h.rows, h.cols), "tftq_rms_norm_backward_workspace");
+            const int64_t size = bytes_needed(lib.rms_norm_backward_workspace(code_of(h_), h.rows, h.cols), "tftq_rms_norm_backward_workspace");
             const Tensor workspace = bytes_of(size, h_);
             if (dx.defined() || dw.defined())
                 checked(lib.rms_norm_backward(code_of(h_), weight.defined() ? code_of(weight) : 0, data_of(dy), data_of(dh), h.data(), h.stride,
@@ -316,7 +320,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
             const Tensor ids = ctx->get_saved_variables()[0].contiguous(), dy = dy_.resolve_neg().contiguous();
             const int64_t vocab = ctx->saved_data["vocab"].toInt(), cols = ctx->saved_data["cols"].toInt(), n = ids.numel();
             dtable = fresh({vocab, cols}, dy.scalar_type(), dy);
-            const int64_t size = checked(lib.embedding_backward_workspace(n, vocab, cols), "tftq_embedding_backward_workspace");
+            const int64_t size = bytes_needed(lib.embedding_backward_workspace(n, vocab, cols), "tftq_embedding_backward_workspace");
             const Tensor workspace = bytes_of(size, dy);
             checked(lib.embedding_backward(code_of(dy), static_cast<int>(ids.element_size()), data_of(ids), n, ctx->saved_data["skip"].toInt(),
                                            data_of(dy), vocab, cols, static_cast<float>(ctx->saved_data["scale"].toDouble()), data_of(dtable),
@@ -639,7 +643,7 @@ PyObject *sort_by_expert(PyObject *, PyObject *const *args, Py_ssize_t n)
             at::NoGradGuard guard;
             const Tensor chosen = chosen_.contiguous();
             const int64_t choices = chosen.numel();
-            const int64_t size = checked(lib.expert_sort_workspace(choices, experts), "tftq_expert_sort_workspace");
+            const int64_t size = bytes_needed(lib.expert_sort_workspace(choices, experts), "tftq_expert_sort_workspace");
             const Tensor workspace = bytes_of(size, chosen), order = fresh({choices}, at::kInt, chosen),
                          position = fresh({chosen.size(0), chosen.dim() == 2 ? chosen.size(1) : 1}, at::kInt, chosen),
                          offsets = fresh({experts + 1}, at::kInt, chosen);

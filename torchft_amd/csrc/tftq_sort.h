@@ -13,24 +13,14 @@ struct SortArgs {
     uint64_t order;    // u32 [n]: where they stood
     uint64_t position; // u32 [n]: where they went; 0: not wanted
     uint64_t offsets;  // u32 [classes + 1]: how many are below 0, 1, ... classes; 0: not wanted
-    uint64_t fill;     // fill_bytes, a multiple of 2, of zeros to write on the side: a sort leaves most of the machine idle
+    uint64_t fill;     // fill_bytes of zeros to write on the side: a sort leaves most of the machine idle
     int64_t fill_bytes;
 };
 
 __attribute__((visibility("hidden"))) int64_t sort_workspace(int64_t n, int64_t classes);  // bytes, a multiple of 16
 // Whether `keys` has to be there for `offsets`.
 __attribute__((visibility("hidden"))) bool sort_needs_keys(int64_t n, int64_t classes);
-// About how many bytes of zeros the machine can write while so many numbers are sorted.
-__attribute__((visibility("hidden"))) int64_t sort_fills(int64_t n, int64_t classes);
 __attribute__((visibility("hidden"))) int sort_numbers(const SortArgs &a, void *workspace, hipStream_t st);
-
-// The bytes from `to` on become zero, as many as the workgroup's THREADS threads write together.
-template <int THREADS>
-DEV void fill_zeros(uint64_t to, int64_t bytes)
-{
-    for (int64_t at = (int64_t)threadIdx.x * 16; at < bytes; at += THREADS * 16)
-        store_bytes(to + (uint64_t)at, (u32)min((int64_t)16, bytes - at), u32x4{0, 0, 0, 0});
-}
 
 // The first of n ascending keys that is not below k.
 template <class P>
