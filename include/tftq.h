@@ -300,23 +300,25 @@ int tftq_newton_schulz(const tftq_ns *what, void *workspace, int64_t workspace_b
  * nothing between calls.
  *
  * Root-mean-square norm:  h = x + residual, rounded to the rows' type;  y = h w / sqrt(mean(h^2) + eps).
+ *   x         x_group rows x_stride apart, and as many again x_group_stride behind their beginning, and so on (heads inside
+ *             wider rows); x_group = rows for rows that are one stride apart
  *   residual  NULL for none; then h is x and the argument h has to be NULL
  *   weight    [cols] of weight_dtype (dtype or TFTQ_F32); NULL for ones
  *   y         [rows, cols]; or NULL, with codes [rows, cols] and scales [rows]: y in e4m3 codes that scales multiply,
  *             a row's largest magnitude / 448 (1 where that is below 2^-126)
  * The sum of squares is fp32: rows of magnitudes beyond 1e18 pass its range.
  */
-int tftq_rms_norm(int dtype, int weight_dtype, const void *x, int64_t x_stride, const void *residual, int64_t residual_stride,
-                  const void *weight, int64_t rows, int64_t cols, float eps, void *h, void *y, void *codes, float *scales,
-                  int device, void *stream);
+int tftq_rms_norm(int dtype, int weight_dtype, const void *x, int64_t x_stride, int64_t x_group, int64_t x_group_stride,
+                  const void *residual, int64_t residual_stride, const void *weight, int64_t rows, int64_t cols, float eps,
+                  void *h, void *y, void *codes, float *scales, int device, void *stream);
 /*
  * Its gradients, from the h that was kept (x where there was no residual):
  * dx = d/dx of <dy, y> + dh (dh may be NULL), also the residual's; dweight [cols] of weight_dtype (a weight is needed then).  Either may be NULL.
  */
 int64_t tftq_rms_norm_backward_workspace(int dtype, int64_t rows, int64_t cols);
 int tftq_rms_norm_backward(int dtype, int weight_dtype, const void *dy, const void *dh, const void *h, int64_t h_stride,
-                           const void *weight, int64_t rows, int64_t cols, float eps, void *dx, void *dweight,
-                           void *workspace, int64_t workspace_bytes, int device, void *stream);
+                           int64_t h_group, int64_t h_group_stride, const void *weight, int64_t rows, int64_t cols, float eps,
+                           void *dx, void *dweight, void *workspace, int64_t workspace_bytes, int device, void *stream);
 
 /*
  * Dropout:  out = residual + x keep / (1 - q) for n elements, q = round(p 65536) / 65536; residual may be NULL.  Element i

@@ -124,6 +124,29 @@ def test_orders(t, dtype):
             assert torch.autograd.grad(got.sum(), leaf)[0].shape == leaf.shape
 
 
+@pytest.mark.parametrize("dtype", ref.DTYPES)
+def test_heads(t, dtype):
+    """Queries and keys inside wider rows, heads before tokens, groups of one row, rows long and short; without a copy of x."""
+    for heads, d in ((5, 64), (3, 33), (1, 128), (7, 4), (2, 1100), (2, 9000), (2, 40000)):
+        wide = values(6, 3 * heads * d, dtype, d).cuda().view(2, 3, 3, heads, d)
+        w = (1 + values(1, d, torch.float32, d)[0]).to(dtype)
+        for view in (wide[:, :, 1], wide[:, :, 2, :, : max(1, d - 1)], wide[:, :, 0].transpose(1, 2), wide[:, :, :2], wide[:, 1, 1:]):
+            n = view.shape[-1]
+            x = view.cpu()
+            leaf = view.detach().requires_grad_()
+            weight = w[:n].cuda().requires_grad_()
+            y = t.rms_norm(leaf, weight, None, EPS)
+            want, h, _ = ref.norm(x, w[:n], None, EPS)
+            ref.close(y, want, ref.norm_error(want, n), dtype)
+            dy = values(x.numel() // n, n, dtype, 5).view(x.shape)
+            dx, dw = torch.autograd.grad(y, (leaf, weight), dy.cuda())
+            want, dw_want, error, dw_error = ref.norm_backward(dy, None, x, w[:n], EPS)
+            ref.close(dx, want, error, dtype)
+            ref.close(dw, dw_want, dw_error, dtype)
+            y, h = t.rms_norm(view, weight.detach(), view, EPS)
+            assert torch.equal(h.cpu(), (x.float() + x.float()).to(dtype))
+
+
 def test_no_rows(t):
     """A batch without tokens: the weight's gradient is zeros."""
     x = torch.empty(0, 40, device="cuda", requires_grad=True)

@@ -90,14 +90,14 @@ def test_c_entries_check_before_they_launch():
     """Sizes, types, pointers, strides, workspaces: no device is touched."""
     lib = _lib.load()
     p = 4096  # an address that is never read
-    norm = lambda **k: lib.tftq_rms_norm(*{**dict(dtype=2, wdtype=2, x=p, xs=8, r=None, rs=0, w=p, rows=2, cols=8, eps=1e-6, h=None, y=p, c=None,  # noqa: E731
+    norm = lambda **k: lib.tftq_rms_norm(*{**dict(dtype=2, wdtype=2, x=p, xs=8, xg=2, xgs=0, r=None, rs=0, w=p, rows=2, cols=8, eps=1e-6, h=None, y=p, c=None,  # noqa: E731
                                                     s=None, device=-1, stream=None), **k}.values())
     assert norm(dtype=3) == -2 and norm(wdtype=1) == -2 and norm(rows=-1) == -3 and norm(cols=2 ** 31) == -3
-    assert norm(x=None) == -1 and norm(xs=7) == -1 and norm(h=p) == -1 and norm(r=p, h=p, rs=7) == -1 and norm(c=p) == -1 and norm(y=None) == -1
+    assert norm(x=None) == -1 and norm(xs=7) == -1 and norm(xg=0) == -1 and norm(xg=1) == -1 and norm(xg=1, xgs=7) == -1 and norm(h=p) == -1 and norm(r=p, h=p, rs=7) == -1 and norm(c=p) == -1 and norm(y=None) == -1
     assert norm(y=None, c=p) == -1 and norm(eps=-1.0) == -1 and norm(rows=0, x=None) == 0 and norm(cols=0) == 0
-    back = lambda **k: lib.tftq_rms_norm_backward(*{**dict(dtype=2, wdtype=2, dy=p, dh=None, h=p, hs=8, w=p, rows=2, cols=8, eps=1e-6, dx=p, dw=p, ws=p,  # noqa: E731
+    back = lambda **k: lib.tftq_rms_norm_backward(*{**dict(dtype=2, wdtype=2, dy=p, dh=None, h=p, hs=8, hg=2, hgs=0, w=p, rows=2, cols=8, eps=1e-6, dx=p, dw=p, ws=p,  # noqa: E731
                                                              n=1 << 20, device=-1, stream=None), **k}.values())
-    assert back(n=16) == -4 and back(ws=p + 8) == -1 and back(w=None) == -1 and back(dy=None) == -1 and back(dx=None, dw=None) == -1 and back(hs=3) == -1
+    assert back(n=16) == -4 and back(ws=p + 8) == -1 and back(w=None) == -1 and back(dy=None) == -1 and back(dx=None, dw=None) == -1 and back(hs=3) == -1 and back(hg=1) == -1
     assert lib.tftq_rms_norm_backward_workspace(2, -1, 3) == -3 and lib.tftq_rms_norm_backward_workspace(7, 1, 3) == -2
     drop = lambda **k: lib.tftq_dropout(*{**dict(dtype=0, x=p, r=None, n=8, p=0.5, seed=1, at=None, offset=0, out=p, device=-1, stream=None), **k}.values())  # noqa: E731
     assert drop(dtype=5) == -2 and drop(n=-1) == -3 and drop(p=1.01) == -1 and drop(p=float("nan")) == -1 and drop(out=None) == -1 and drop(at=p + 4) == -1

@@ -75,12 +75,12 @@ SYMBOLS = [
     ("tftq_newton_schulz", _c.c_int, [_c.POINTER(NewtonSchulz), _P, _c.c_int64, _c.c_int, _P]),
     # dtype, a, m, b, n, k, out, row_stride, device, stream
     ("tftq_mx_product", _c.c_int, [_c.c_int, _P, _c.c_int64, _P, _c.c_int64, _c.c_int64, _P, _c.c_int64, _c.c_int, _P]),
-    # dtype, weight_dtype, x, x_stride, residual, residual_stride, weight, rows, cols, eps, h, y, codes, scales, device, stream
-    ("tftq_rms_norm", _c.c_int, [_c.c_int, _c.c_int, _P, _c.c_int64, _P, _c.c_int64, _P, _c.c_int64, _c.c_int64, _c.c_float, _P, _P, _P, _P,
+    # dtype, weight_dtype, x, x_stride, x_group, x_group_stride, residual, residual_stride, weight, rows, cols, eps, h, y, codes, scales, device, stream
+    ("tftq_rms_norm", _c.c_int, [_c.c_int, _c.c_int, _P, _c.c_int64, _c.c_int64, _c.c_int64, _P, _c.c_int64, _P, _c.c_int64, _c.c_int64, _c.c_float, _P, _P, _P, _P,
                                  _c.c_int, _P]),
     ("tftq_rms_norm_backward_workspace", _c.c_int64, [_c.c_int, _c.c_int64, _c.c_int64]),
-    # dtype, weight_dtype, dy, dh, h, h_stride, weight, rows, cols, eps, dx, dweight, workspace, workspace_bytes, device, stream
-    ("tftq_rms_norm_backward", _c.c_int, [_c.c_int, _c.c_int, _P, _P, _P, _c.c_int64, _P, _c.c_int64, _c.c_int64, _c.c_float, _P, _P, _P,
+    # dtype, weight_dtype, dy, dh, h, h_stride, h_group, h_group_stride, weight, rows, cols, eps, dx, dweight, workspace, workspace_bytes, device, stream
+    ("tftq_rms_norm_backward", _c.c_int, [_c.c_int, _c.c_int, _P, _P, _P, _c.c_int64, _c.c_int64, _c.c_int64, _P, _c.c_int64, _c.c_int64, _c.c_float, _P, _P, _P,
                                           _c.c_int64, _c.c_int, _P]),
     # dtype, x, residual, n, p, seed, seed_at, offset, out, device, stream
     ("tftq_dropout", _c.c_int, [_c.c_int, _P, _P, _c.c_int64, _c.c_double, _c.c_int64, _P, _c.c_int64, _P, _c.c_int, _P]),

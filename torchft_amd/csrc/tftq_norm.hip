@@ -14,10 +14,19 @@
 struct NormArgs {
     uint64_t x, residual, weight, y, h, codes, scales;  // residual, weight, h: 0 for none; codes and scales for 8 bits, else y
     int64_t x_stride, residual_stride;                  // bytes from row to row; all others are contiguous
+    int64_t x_group_stride;                             // and from group to group of
+    u32 x_group;                                        // so many rows of x
     int64_t row0, rows;
     int cols;
     float eps, inv_cols;
 };
+
+// Where a row begins among rows in groups.
+DEV uint64_t row_at(uint64_t base, int64_t row, int64_t stride, u32 group, int64_t group_stride, int64_t rows)
+{
+    if (group >= rows) return base + (uint64_t)(row * stride);
+    return base + (uint64_t)((int64_t)((u32)row / group) * group_stride + (int64_t)((u32)row % group) * stride);
+}
 
 // The weight's elements that belong to a vector: loaded early, widened late.  WIDE: the weight is fp32 and the rows are not.
 template <class T, bool NARROW, bool WIDE>
@@ -82,7 +91,7 @@ __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void k_rms_norm(const Norm
     const int lane = threadIdx.x % TEAM;
     const int64_t row = a.row0 + (int64_t)blockIdx.x * TEAMS + threadIdx.x / TEAM;
     if (row >= a.rows) return;  // a whole team; teams of several wavefronts are whole workgroups
-    const uint64_t px = a.x + (uint64_t)(row * a.x_stride), pr = a.residual + (uint64_t)(row * a.residual_stride);
+    const uint64_t px = row_at(a.x, row, a.x_stride, a.x_group, a.x_group_stride, a.rows), pr = a.residual + (uint64_t)(row * a.residual_stride);
     const uint64_t at = (uint64_t)(row * a.cols) * ESZ;
 
     Piece piece[NV];
@@ -160,7 +169,7 @@ __global__ __launch_bounds__(1024) void k_rms_norm_long(const NormArgs a)
     constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, STEP = 1024 * EPV;
     __shared__ float lds[16];
     const int64_t row = a.row0 + blockIdx.x;
-    const uint64_t px = a.x + (uint64_t)(row * a.x_stride), pr = a.residual + (uint64_t)(row * a.residual_stride);
+    const uint64_t px = row_at(a.x, row, a.x_stride, a.x_group, a.x_group_stride, a.rows), pr = a.residual + (uint64_t)(row * a.residual_stride);
     const uint64_t at = (uint64_t)(row * a.cols) * ESZ, again = a.residual ? a.h + at : px;
     float sum = 0.0f;
     for (int col = threadIdx.x * EPV; col < a.cols; col += STEP) {
@@ -217,7 +226,8 @@ __global__ __launch_bounds__(1024) void k_rms_norm_long(const NormArgs a)
 
 struct NormBackwardArgs {
     uint64_t dy, dh, h, weight, dx, sums;  // dh, weight, dx, sums: 0 for none.  sums: fp32 [workgroups][sums_stride(cols)]
-    int64_t h_stride;                      // bytes; all others are contiguous
+    int64_t h_stride, h_group_stride;      // bytes; all others are contiguous
+    u32 h_group;
     int64_t rows;
     int cols;
     float eps, inv_cols;
@@ -249,7 +259,7 @@ __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void k_rms_norm_backward(c
     u32x4 dy_next[NV], h_next[NV], dh_next[NV];
     auto fetch = [&](int64_t row) {
         if (AHEAD && row >= a.rows) return;
-        const uint64_t at = (uint64_t)(row * a.cols) * ESZ, ph = a.h + (uint64_t)(row * a.h_stride);
+        const uint64_t at = (uint64_t)(row * a.cols) * ESZ, ph = row_at(a.h, row, a.h_stride, a.h_group, a.h_group_stride, a.rows);
 #pragma unroll
         for (int v = 0; v < NV; v++) dy_next[v] = load_row<ESZ, NARROW>(a.dy + at, piece[v], a.cols);
 #pragma unroll
@@ -338,7 +348,7 @@ __global__ __launch_bounds__(1024) void k_rms_norm_backward_long(const NormBackw
     constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, U = 2, STEP = 1024 * EPV;
     __shared__ float lds[32];
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const uint64_t at = (uint64_t)(row * a.cols) * ESZ, ph = a.h + (uint64_t)(row * a.h_stride);
+        const uint64_t at = (uint64_t)(row * a.cols) * ESZ, ph = row_at(a.h, row, a.h_stride, a.h_group, a.h_group_stride, a.rows);
         float squares = 0.0f, along = 0.0f;
         for (int col = threadIdx.x * EPV; col < a.cols; col += U * STEP) {
             Weights<T, false, WIDE> weights[U];
@@ -388,7 +398,7 @@ __global__ __launch_bounds__(256) void k_rms_norm_backward_columns(const NormBac
         for (int u = 0; u < U; u++) {
             const int64_t row = first + u < a.rows ? first + u : a.rows - 1;
             const uint64_t at = (uint64_t)(row * a.cols) * ESZ;
-            h[u] = load_row<ESZ, false>(a.h + (uint64_t)(row * a.h_stride), p, a.cols);
+            h[u] = load_row<ESZ, false>(row_at(a.h, row, a.h_stride, a.h_group, a.h_group_stride, a.rows), p, a.cols);
             dy[u] = load_row<ESZ, false>(a.dy + at, p, a.cols);
             if (a.dh) dh[u] = load_row<ESZ, false>(a.dh + at, p, a.cols);
             r[u] = as_global<const float>(factors)[2 * row];
@@ -596,21 +606,25 @@ static int norm_backward(NormBackwardArgs a, uint64_t factors, int64_t parts, hi
     return (int)hipLaunchKernel(k, dim3((unsigned)parts), dim3(shape.team > 256 ? shape.team : 256), args, 0, st);
 }
 
-extern "C" int tftq_rms_norm(int dtype, int weight_dtype, const void *x, int64_t x_stride, const void *residual, int64_t residual_stride,
-                             const void *weight, int64_t rows, int64_t cols, float eps, void *h, void *y, void *codes, float *scales,
+static bool groups_ok(int64_t rows, int64_t cols, int64_t stride, int64_t group, int64_t group_stride)
+{
+    return group >= 1 && group <= ROWS_MOST && stride >= (group > 1 && rows > 1 ? cols : 0) && group_stride >= (rows > group ? cols : 0);
+}
+
+extern "C" int tftq_rms_norm(int dtype, int weight_dtype, const void *x, int64_t x_stride, int64_t x_group, int64_t x_group_stride,
+                             const void *residual, int64_t residual_stride, const void *weight, int64_t rows, int64_t cols, float eps, void *h, void *y, void *codes, float *scales,
                              int device, void *stream)
 {
     if (!dtype_ok(dtype) || (weight && weight_dtype != dtype && weight_dtype != TFTQ_F32)) return TFTQ_E_DTYPE;
     if (!rows_ok(rows, cols)) return TFTQ_E_SHAPE;
     if (rows == 0 || cols == 0) return 0;
     if (!x || !residual != !h || !codes != !scales || !y == !codes || !(eps >= 0.0f)) return TFTQ_E_ARG;
-    const int64_t across = rows > 1 ? cols : 0;
-    if (x_stride < across || (residual && residual_stride < across)) return TFTQ_E_ARG;
+    if (!groups_ok(rows, cols, x_stride, x_group, x_group_stride) || (residual && residual_stride < (rows > 1 ? cols : 0))) return TFTQ_E_ARG;
     DeviceScope scope(device);
     if (scope.err != hipSuccess) return (int)scope.err;
     const int size = dtype_size(dtype);
     const NormArgs a = {(uint64_t)x, (uint64_t)residual, (uint64_t)weight, (uint64_t)y, (uint64_t)h, (uint64_t)codes, (uint64_t)scales,
-                        x_stride * size, residual_stride * size, 0, rows, (int)cols, eps, 1.0f / (float)cols};
+                        x_stride * size, residual_stride * size, x_group_stride * size, (u32)x_group, 0, rows, (int)cols, eps, 1.0f / (float)cols};
     hipStream_t st = (hipStream_t)stream;
     const bool wide = weight && weight_dtype != dtype;
 #define NORM(T) (wide ? codes ? norm<T, true, true>(a, st) : norm<T, true, false>(a, st) : codes ? norm<T, false, true>(a, st) : norm<T, false, false>(a, st))
@@ -628,14 +642,14 @@ extern "C" int64_t tftq_rms_norm_backward_workspace(int dtype, int64_t rows, int
 }
 
 extern "C" int tftq_rms_norm_backward(int dtype, int weight_dtype, const void *dy, const void *dh, const void *h, int64_t h_stride,
-                                      const void *weight, int64_t rows, int64_t cols, float eps, void *dx, void *dweight, void *workspace,
+                                      int64_t h_group, int64_t h_group_stride, const void *weight, int64_t rows, int64_t cols, float eps, void *dx, void *dweight, void *workspace,
                                       int64_t workspace_bytes, int device, void *stream)
 {
     if (!dtype_ok(dtype) || (weight && weight_dtype != dtype && weight_dtype != TFTQ_F32)) return TFTQ_E_DTYPE;
     if (!rows_ok(rows, cols)) return TFTQ_E_SHAPE;
     if (cols == 0 || (rows == 0 && !dweight)) return 0;
     if ((dweight && !weight) || (rows && (!dy || !h || !workspace || ((uintptr_t)workspace & 15))) || (!dx && !dweight) || !(eps >= 0.0f)) return TFTQ_E_ARG;
-    if (rows && h_stride < (rows > 1 ? cols : 0)) return TFTQ_E_ARG;
+    if (rows && !groups_ok(rows, cols, h_stride, h_group, h_group_stride)) return TFTQ_E_ARG;
     const int size = dtype_size(dtype);
     const int64_t parts = rows ? norm_parts(rows, cols, size) : 0, sums = parts * sums_stride(cols) * 4;
     if (rows && workspace_bytes < sums + rows * 8) return TFTQ_E_SIZE;
@@ -644,7 +658,7 @@ extern "C" int tftq_rms_norm_backward(int dtype, int weight_dtype, const void *d
     hipStream_t st = (hipStream_t)stream;
     if (rows) {
         const NormBackwardArgs a = {(uint64_t)dy, (uint64_t)dh, (uint64_t)h, (uint64_t)weight, (uint64_t)dx, dweight ? (uint64_t)workspace : 0,
-                                    h_stride * size, rows, (int)cols, eps, 1.0f / (float)cols};
+                                    h_stride * size, h_group_stride * size, (u32)h_group, rows, (int)cols, eps, 1.0f / (float)cols};
         const uint64_t factors = (uint64_t)workspace + (uint64_t)sums;
         const bool wide = weight && weight_dtype != dtype;
 #define NORM(T) (wide ? norm_backward<T, true>(a, factors, parts, st) : norm_backward<T, false>(a, factors, parts, st))

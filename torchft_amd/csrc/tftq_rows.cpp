@@ -49,11 +49,11 @@ void require(bool ok, const char *why)
 struct {
     const char *(*strerror)(int) = nullptr;
     int (*check_device)(int) = nullptr;
-    int (*rms_norm)(int, int, const void *, int64_t, const void *, int64_t, const void *, int64_t, int64_t, float, void *, void *, void *, float *, int,
-                    void *) = nullptr;
+    int (*rms_norm)(int, int, const void *, int64_t, int64_t, int64_t, const void *, int64_t, const void *, int64_t, int64_t, float, void *, void *, void *,
+                    float *, int, void *) = nullptr;
     int64_t (*rms_norm_backward_workspace)(int, int64_t, int64_t) = nullptr;
-    int (*rms_norm_backward)(int, int, const void *, const void *, const void *, int64_t, const void *, int64_t, int64_t, float, void *, void *, void *,
-                             int64_t, int, void *) = nullptr;
+    int (*rms_norm_backward)(int, int, const void *, const void *, const void *, int64_t, int64_t, int64_t, const void *, int64_t, int64_t, float, void *,
+                             void *, void *, int64_t, int, void *) = nullptr;
     int (*dropout)(int, const void *, const void *, int64_t, double, int64_t, const int64_t *, int64_t, void *, int, void *) = nullptr;
     int (*embedding)(int, int, const void *, int64_t, const void *, int64_t, int64_t, int64_t, float, void *, int, void *) = nullptr;
     int64_t (*embedding_backward_workspace)(int64_t, int64_t, int64_t) = nullptr;
@@ -118,33 +118,43 @@ Tensor fresh(c10::IntArrayRef sizes, at::ScalarType type, const Tensor &beside)
 Tensor bytes_of(int64_t n, const Tensor &beside) { return n ? fresh({n}, at::kByte, beside) : Tensor(); }
 void *data_of(const Tensor &t) { return t.defined() && t.numel() ? t.data_ptr() : nullptr; }
 
-// A tensor as rows: the last dimension in a piece, the others one stride apart; `held` is what the addresses are of.
+// A tensor as rows: the last dimension in a piece, the others one stride apart, or with `grouped` two (heads inside a wider
+// row, say: groups of rows one stride apart, the groups another); `held` is what the addresses are of.
 struct Rows {
     Tensor held;
-    int64_t rows = 1, cols = 0, stride = 0;
+    int64_t rows = 1, cols = 0, stride = 0, group = 1, group_stride = 0;
 
-    explicit Rows(const Tensor &t) : held(t.resolve_neg())
+    explicit Rows(const Tensor &t, bool grouped = false) : held(t.resolve_neg())
     {
         cols = t.size(-1);
         for (int64_t d = 0; d + 1 < t.dim(); d++) rows *= t.size(d);
-        stride = cols;
-        if (rows == 0 || cols == 0 || describe()) return;
-        held = held.contiguous();
-        stride = cols;
+        if (rows != 0 && cols != 0 && !describe(grouped)) {
+            held = held.contiguous();
+            group = 0;
+        }
+        if (rows == 0 || cols == 0 || group == 0) {
+            stride = cols;
+            group = rows;
+        }
     }
-    bool describe()
+    bool describe(bool grouped)
     {
         const c10::IntArrayRef size = held.sizes(), step = held.strides();
         const int64_t last = held.dim() - 1;
         if (cols > 1 && step[last] != 1) return false;
-        int64_t inner = 0, expect = 0;  // the innermost of the others that is longer than one
+        int levels = 0;  // 1: rows, 2: groups of them
+        int64_t expect = 0;
         for (int64_t d = last - 1; d >= 0; d--) {
             if (size[d] == 1) continue;
-            if (inner == 0) stride = step[d], inner = 1;
-            else if (step[d] != expect) return false;
+            if (levels == 0 || step[d] != expect) {
+                if (step[d] < cols || ++levels > (grouped ? 2 : 1)) return false;
+                (levels == 1 ? stride : group_stride) = step[d];
+            }
+            if (levels == 1) group *= size[d];
             expect = step[d] * size[d];
         }
-        return stride >= cols;
+        if (levels == 0) stride = cols;
+        return true;
     }
     void *data() const { return data_of(held); }
 };
@@ -180,7 +190,7 @@ variable_list once(variable_list grads, const variable_list &from, const char *n
 // (y, h), or (codes, h, scales)
 variable_list norm_forward(const Tensor &x_, const Tensor &weight_, const Tensor &residual_, double eps, bool fp8)
 {
-    const Rows x(x_);
+    const Rows x(x_, true);
     const Tensor weight = weight_.defined() ? weight_.resolve_neg().contiguous() : weight_;
     Tensor y = fresh(x_.sizes(), fp8 ? at::kFloat8_e4m3fn : x_.scalar_type(), x_), h, scales;
     if (fp8) {
@@ -189,16 +199,15 @@ variable_list norm_forward(const Tensor &x_, const Tensor &weight_, const Tensor
         scales = fresh(sizes, at::kFloat, x_);
         if (x.cols == 0) scales.fill_(1.0);
     }
+    std::optional<Rows> residual;
     if (residual_.defined()) {
-        const Rows residual(residual_);
+        residual.emplace(residual_);
         h = fresh(x_.sizes(), x_.scalar_type(), x_);
-        checked(lib.rms_norm(code_of(x_), weight.defined() ? code_of(weight) : 0, x.data(), x.stride, residual.data(), residual.stride, data_of(weight),
-                             x.rows, x.cols, static_cast<float>(eps), data_of(h), fp8 ? nullptr : data_of(y), fp8 ? data_of(y) : nullptr,
-                             static_cast<float *>(data_of(scales)), x_.device().index(), stream_of(x_)), "tftq_rms_norm");
-    } else
-        checked(lib.rms_norm(code_of(x_), weight.defined() ? code_of(weight) : 0, x.data(), x.stride, nullptr, 0, data_of(weight), x.rows, x.cols,
-                             static_cast<float>(eps), nullptr, fp8 ? nullptr : data_of(y), fp8 ? data_of(y) : nullptr,
-                             static_cast<float *>(data_of(scales)), x_.device().index(), stream_of(x_)), "tftq_rms_norm");
+    }
+    checked(lib.rms_norm(code_of(x_), weight.defined() ? code_of(weight) : 0, x.data(), x.stride, x.group, x.group_stride,
+                         residual ? residual->data() : nullptr, residual ? residual->stride : 0, data_of(weight), x.rows, x.cols,
+                         static_cast<float>(eps), data_of(h), fp8 ? nullptr : data_of(y), fp8 ? data_of(y) : nullptr,
+                         static_cast<float *>(data_of(scales)), x_.device().index(), stream_of(x_)), "tftq_rms_norm");
     return {y, h, scales};
 }
 
@@ -228,7 +237,7 @@ struct Norm : torch::autograd::Function<Norm> {
         if (!dy_.defined()) dx = dh_;
         else {
             at::NoGradGuard guard;
-            const Rows h(h_);
+            const Rows h(h_, true);
             const Tensor dy = dy_.resolve_neg().contiguous(), dh = dh_.defined() ? dh_.resolve_neg().contiguous() : dh_,
                          weight = weight_.defined() ? weight_.resolve_neg().contiguous() : weight_;
             if (for_x || for_r) dx = fresh(h_.sizes(), h_.scalar_type(), h_);
@@ -236,7 +245,7 @@ struct Norm : torch::autograd::Function<Norm> {
             const int64_t size = bytes_needed(lib.rms_norm_backward_workspace(code_of(h_), h.rows, h.cols), "tftq_rms_norm_backward_workspace");
             const Tensor workspace = bytes_of(size, h_);
             if (dx.defined() || dw.defined())
-                checked(lib.rms_norm_backward(code_of(h_), weight.defined() ? code_of(weight) : 0, data_of(dy), data_of(dh), h.data(), h.stride,
+                checked(lib.rms_norm_backward(code_of(h_), weight.defined() ? code_of(weight) : 0, data_of(dy), data_of(dh), h.data(), h.stride, h.group, h.group_stride,
                                               data_of(weight), h.rows, h.cols, static_cast<float>(ctx->saved_data["eps"].toDouble()), data_of(dx),
                                               data_of(dw), data_of(workspace), size, h_.device().index(), stream_of(h_)),
                         "tftq_rms_norm_backward");
