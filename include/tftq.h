@@ -336,7 +336,7 @@ int tftq_dropout(int dtype, const void *x, const void *residual, int64_t n, doub
  */
 int tftq_embedding(int dtype, int id_bytes, const void *ids, int64_t n, const void *table, int64_t vocab, int64_t cols,
                    int64_t row_stride, float scale, void *out, int device, void *stream);
-int64_t tftq_embedding_backward_workspace(int64_t n, int64_t vocab, int64_t cols);
+int64_t tftq_embedding_backward_workspace(int dtype, int64_t n, int64_t vocab, int64_t cols);
 int tftq_embedding_backward(int dtype, int id_bytes, const void *ids, int64_t n, int64_t skip, const void *dy, int64_t vocab,
                             int64_t cols, float scale, void *dtable, void *workspace, int64_t workspace_bytes, int device,
                             void *stream);

@@ -126,7 +126,7 @@ def test_workspaces_grow_with_their_sizes():
     lib = _lib.load()
     assert lib.tftq_expert_sort_workspace(100, 8) >= 0 and lib.tftq_expert_sort_workspace(0, 8) == 0
     n = 100000
-    assert lib.tftq_embedding_backward_workspace(n, 128256, 64) >= 8 * n + 2 * 8 * n and lib.tftq_expert_sort_workspace(n, 1000) >= 12 * n
+    assert lib.tftq_embedding_backward_workspace(0, n, 128256, 64) >= 8 * n + 2 * 8 * n and lib.tftq_expert_sort_workspace(n, 1000) >= 12 * n
     assert lib.tftq_expert_sort_workspace(2 ** 31, 8) == -3
     assert lib.tftq_rms_norm_backward_workspace(2, 4, 100) >= 4 * 100
 

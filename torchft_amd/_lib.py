@@ -86,7 +86,7 @@ SYMBOLS = [
     ("tftq_dropout", _c.c_int, [_c.c_int, _P, _P, _c.c_int64, _c.c_double, _c.c_int64, _P, _c.c_int64, _P, _c.c_int, _P]),
     # dtype, id_bytes, ids, n, table, vocab, cols, row_stride, scale, out, device, stream
     ("tftq_embedding", _c.c_int, [_c.c_int, _c.c_int, _P, _c.c_int64, _P, _c.c_int64, _c.c_int64, _c.c_int64, _c.c_float, _P, _c.c_int, _P]),
-    ("tftq_embedding_backward_workspace", _c.c_int64, [_c.c_int64, _c.c_int64, _c.c_int64]),
+    ("tftq_embedding_backward_workspace", _c.c_int64, [_c.c_int, _c.c_int64, _c.c_int64, _c.c_int64]),
     # dtype, id_bytes, ids, n, skip, dy, vocab, cols, scale, dtable, workspace, workspace_bytes, device, stream
     ("tftq_embedding_backward", _c.c_int, [_c.c_int, _c.c_int, _P, _c.c_int64, _c.c_int64, _P, _c.c_int64, _c.c_int64, _c.c_float, _P, _P,
                                            _c.c_int64, _c.c_int, _P]),

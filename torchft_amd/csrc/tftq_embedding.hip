@@ -23,10 +23,10 @@ struct EmbeddingArgs {
     float scale;
 };
 
-template <class T, int TEAM, bool NARROW>
+template <class T, int TEAM, int U, bool NARROW>
 __global__ __launch_bounds__(256) void k_embedding(const EmbeddingArgs a)
 {
-    constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, TEAMS = 256 / TEAM, U = TEAM == 8 ? 1 : 4;
+    constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, TEAMS = 256 / TEAM;
     const int lane = threadIdx.x % TEAM;
     const int64_t row = a.row0 + (int64_t)blockIdx.x * TEAMS + threadIdx.x / TEAM;
     if (row >= a.rows) return;
@@ -122,29 +122,41 @@ __global__ __launch_bounds__(256) void k_embedding_backward(const TableArgs a)
     leave(true);
 }
 
-// The runs of several chunks: a workgroup to the chunk where one begins and 64 vectors of columns; its four wavefronts
+// How many of n sorted keys are not above k, by a wavefront: 64 probes at once.
+DEV int64_t first_above(const GLOBAL u32 *keys, int64_t n, u32 k)
+{
+    const int lane = threadIdx.x & 63;
+    int64_t lo = 0;
+    while (n > 0) {  // the answer is in lo to lo + n
+        const int64_t step = (n + 63) >> 6, at = (int64_t)lane * step + step - 1;
+        const int count = __builtin_popcountll(__ballot(at < n && keys[lo + at] <= k));  // a run of lanes from the first on
+        lo += count * step;
+        n = min(n - count * step, step - 1);
+    }
+    return lo;
+}
+
+// The runs of several chunks: a workgroup to the chunk where one begins and TEAM vectors of columns; its teams
 // share the chunks, and add up in their order.
-template <class T, bool NARROW>
+template <class T, int TEAM, bool NARROW>
 __global__ __launch_bounds__(256) void k_embedding_join(const TableArgs a)
 {
-    constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV;
-    __shared__ float add[3][64][EPV + 1];
+    constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, TEAMS = 256 / TEAM;
+    __shared__ float add[TEAMS][TEAM][EPV + 1];
     const int64_t group = a.group0 + blockIdx.x, chunk = group / a.across, begin = chunk * a.chunk, end = begin + a.chunk;
     if (end >= a.n) return;
     const GLOBAL u32 *keys = as_global<const u32>(a.keys);
     const u32 before = keys[begin > 0 ? begin - 1 : 0], first = keys[begin], key = keys[end - 1], next = keys[end];
     if (key >= (u32)a.vocab || next != key) return;                   // no run goes on
     if (begin > 0 && first == key && before == key) return;          // it began before
-    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
-    int64_t count = 1;  // chunks
-    for (bool more = true; more;) {
-        const int64_t at = (chunk + count + lane) * a.chunk;
-        const uint64_t others = ~__ballot(at < a.n && keys[at] == key);
-        count += others ? __builtin_ctzll(others) : 64;
-        more = others == 0;
-    }
-    const Piece piece = piece_of<EPV, NARROW>(((int)(group % a.across) * 64 + lane) * EPV, a.cols);
-    const int64_t from = chunk + count * wave / 4, to = chunk + count * (wave + 1) / 4;
+    // the chunks that begin with the key: 64 looked at together, or else as the sorted numbers that they are
+    const int64_t ahead = (chunk + 1 + (threadIdx.x & 63)) * a.chunk;
+    const uint64_t others = ~__ballot(ahead < a.n && keys[ahead] == key);
+    int64_t count = 1 + (others ? __builtin_ctzll(others) : 64);
+    if (!others) count += (first_above(keys + (chunk + 65) * a.chunk, a.n - (chunk + 65) * a.chunk, key) + a.chunk - 1) / a.chunk;
+    const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+    const Piece piece = piece_of<EPV, NARROW>(((int)(group % a.across) * TEAM + lane) * EPV, a.cols);
+    const int64_t from = chunk + count * team / TEAMS, to = chunk + count * (team + 1) / TEAMS;
     float acc[EPV] = {};
     if (piece.in) {
 #pragma unroll 8
@@ -158,14 +170,16 @@ __global__ __launch_bounds__(256) void k_embedding_join(const TableArgs a)
             }
         }
     }
-    if (wave > 0) {
 #pragma unroll
-        for (int i = 0; i < EPV; i++) add[wave - 1][lane][i] = acc[i];
-    }
+    for (int i = 0; i < EPV; i++) add[team][lane][i] = acc[i];
     __syncthreads();
-    if (wave > 0) return;
+    if (team > 0) return;
+#pragma unroll 4
+    for (int t = 1; t < TEAMS; t++)
 #pragma unroll
-    for (int i = 0; i < EPV; i++) acc[i] = (((acc[i] + add[0][lane][i]) + add[1][lane][i]) + add[2][lane][i]) * a.scale;
+        for (int i = 0; i < EPV; i++) acc[i] += add[t][lane][i];
+#pragma unroll
+    for (int i = 0; i < EPV; i++) acc[i] *= a.scale;
     store_row<ESZ, NARROW, false>(a.dtable + (uint64_t)key * (uint64_t)a.cols * ESZ, piece, a.cols, Elem<T>::pack(acc));
 }
 
@@ -174,12 +188,29 @@ __global__ __launch_bounds__(256) void k_embedding_join(const TableArgs a)
 // ---------------------------------------------------------------------------
 static bool narrow_row(int64_t cols, int size) { return cols * size < 16; }
 
-template <class T>
-static const void *embedding_kernel(int64_t cols, int team)
+// Lanes and vectors of a row that is looked up in one go; longer ones take several.
+static RowShape embedding_shape(int64_t vectors)
 {
-    if (narrow_row(cols, Elem<T>::ESZ)) return (const void *)k_embedding<T, 8, true>;
-    return team == 8 ? (const void *)k_embedding<T, 8, false> : team == 64 ? (const void *)k_embedding<T, 64, false> : (const void *)k_embedding<T, 256, false>;
+    if (vectors <= 8) return {8, 1};
+    if (vectors <= 16) return {8, 2};
+    if (vectors <= 32) return {16, 2};
+    if (vectors <= 64) return {32, 2};
+    if (vectors <= 256) return {64, 4};
+    return {256, 2};
 }
+template <class T>
+static const void *embedding_kernel(int64_t cols, RowShape shape)
+{
+    if (narrow_row(cols, Elem<T>::ESZ)) return (const void *)k_embedding<T, 8, 1, true>;
+    return shape.team == 8    ? shape.nv == 1 ? (const void *)k_embedding<T, 8, 1, false> : (const void *)k_embedding<T, 8, 2, false>
+           : shape.team == 16 ? (const void *)k_embedding<T, 16, 2, false>
+           : shape.team == 32 ? (const void *)k_embedding<T, 32, 2, false>
+           : shape.team == 64 ? (const void *)k_embedding<T, 64, 4, false>
+                              : (const void *)k_embedding<T, 256, 2, false>;
+}
+
+// Lanes to a row of a chunk.
+static int backward_team(int64_t vectors) { return vectors <= 8 ? 8 : vectors <= 16 ? 16 : vectors <= 32 ? 32 : 64; }
 template <class T, int TEAM, bool NARROW>
 static const void *backward_kernel(int chunk)
 {
@@ -191,12 +222,19 @@ template <class T>
 static const void *backward_kernel(int64_t cols, int team, int chunk)
 {
     if (narrow_row(cols, Elem<T>::ESZ)) return backward_kernel<T, 8, true>(chunk);
-    return team == 8 ? backward_kernel<T, 8, false>(chunk) : backward_kernel<T, 64, false>(chunk);
+    return team == 8    ? backward_kernel<T, 8, false>(chunk)
+           : team == 16 ? backward_kernel<T, 16, false>(chunk)
+           : team == 32 ? backward_kernel<T, 32, false>(chunk)
+                        : backward_kernel<T, 64, false>(chunk);
 }
 template <class T>
-static const void *join_kernel(int64_t cols)
+static const void *join_kernel(int64_t cols, int team)
 {
-    return narrow_row(cols, Elem<T>::ESZ) ? (const void *)k_embedding_join<T, true> : (const void *)k_embedding_join<T, false>;
+    if (narrow_row(cols, Elem<T>::ESZ)) return (const void *)k_embedding_join<T, 8, true>;
+    return team == 8    ? (const void *)k_embedding_join<T, 8, false>
+           : team == 16 ? (const void *)k_embedding_join<T, 16, false>
+           : team == 32 ? (const void *)k_embedding_join<T, 32, false>
+                        : (const void *)k_embedding_join<T, 64, false>;
 }
 
 extern "C" int tftq_embedding(int dtype, int id_bytes, const void *ids, int64_t n, const void *table, int64_t vocab, int64_t cols,
@@ -209,12 +247,14 @@ extern "C" int tftq_embedding(int dtype, int id_bytes, const void *ids, int64_t 
     if (!ids || (vocab && !table) || !out || row_stride < (vocab > 1 ? cols : 0)) return TFTQ_E_ARG;
     DeviceScope scope(device);
     if (scope.err != hipSuccess) return (int)scope.err;
-    const int size = dtype_size(dtype), team = cols * size <= 128 ? 8 : cols * size <= 4096 ? 64 : 256, teams = 256 / team;
+    const int size = dtype_size(dtype);
+    const RowShape shape = embedding_shape((cols * size + 15) / 16);
+    const int teams = 256 / shape.team;
     EmbeddingArgs a = {(uint64_t)ids, (uint64_t)table, (uint64_t)out, row_stride * size, 0, n, vocab, (int)cols, id_bytes == 8, scale};
-    const void *k = dtype == TFTQ_F32   ? embedding_kernel<float>(cols, team)
-                    : dtype == TFTQ_F16 ? embedding_kernel<f16_tag>(cols, team)
-                                        : embedding_kernel<bf16_tag>(cols, team);
-    const int64_t at_once = ROWS_THREADS / team;
+    const void *k = dtype == TFTQ_F32   ? embedding_kernel<float>(cols, shape)
+                    : dtype == TFTQ_F16 ? embedding_kernel<f16_tag>(cols, shape)
+                                        : embedding_kernel<bf16_tag>(cols, shape);
+    const int64_t at_once = ROWS_THREADS / shape.team;
     for (; a.row0 < n; a.row0 += at_once) {
         void *args[] = {(void *)&a};
         if (const int rc = (int)hipLaunchKernel(k, dim3((unsigned)((std::min(at_once, n - a.row0) + teams - 1) / teams)), dim3(256), args, 0, (hipStream_t)stream)) return rc;
@@ -222,22 +262,22 @@ extern "C" int tftq_embedding(int dtype, int id_bytes, const void *ids, int64_t 
     return 0;
 }
 
-// Tokens of a chunk: neither a chunk nor the sums of one row of the table are to be long, and there are as many chunks of
-// one token as a chunk has tokens when it has the root of all.
-static int embedding_chunk(int64_t n) { return n <= 32768 ? 16 : n <= 524288 ? 64 : 256; }
+// Tokens of a chunk: as few as there are sums to spare (they are as many bytes as a quarter to a half of dy with 16), and
+// more where the machine is full without: 2^17 lanes are 8 wavefronts to a compute unit.
+static int embedding_chunk(int64_t n, int64_t vectors) { return n * vectors < 1 << 23 ? 16 : n * vectors < 1 << 25 ? 64 : 256; }
 
-extern "C" int64_t tftq_embedding_backward_workspace(int64_t n, int64_t vocab, int64_t cols)
+extern "C" int64_t tftq_embedding_backward_workspace(int dtype, int64_t n, int64_t vocab, int64_t cols)
 {
+    if (!dtype_ok(dtype)) return TFTQ_E_DTYPE;
     if (!rows_ok(n, cols) || !rows_ok(vocab, 0)) return TFTQ_E_SHAPE;
-    const int64_t chunks = (n + embedding_chunk(n) - 1) / embedding_chunk(n), numbers = (n * 8 + 15) & ~(int64_t)15;
+    const int64_t chunk = embedding_chunk(n, (cols * dtype_size(dtype) + 15) / 16), chunks = (n + chunk - 1) / chunk, numbers = (n * 8 + 15) & ~(int64_t)15;
     return sort_workspace(n, vocab) + numbers + chunks * sums_stride(cols) * 8;
 }
 
 extern "C" int tftq_embedding_backward(int dtype, int id_bytes, const void *ids, int64_t n, int64_t skip, const void *dy, int64_t vocab,
                                        int64_t cols, float scale, void *dtable, void *workspace, int64_t workspace_bytes, int device, void *stream)
 {
-    if (!dtype_ok(dtype)) return TFTQ_E_DTYPE;
-    const int64_t bytes = tftq_embedding_backward_workspace(n, vocab, cols);
+    const int64_t bytes = tftq_embedding_backward_workspace(dtype, n, vocab, cols);
     if (bytes < 0) return (int)bytes;
     if (id_bytes != 4 && id_bytes != 8) return TFTQ_E_ARG;
     if (vocab == 0 || cols == 0) return 0;
@@ -246,8 +286,10 @@ extern "C" int tftq_embedding_backward(int dtype, int id_bytes, const void *ids,
     DeviceScope scope(device);
     if (scope.err != hipSuccess) return (int)scope.err;
     hipStream_t st = (hipStream_t)stream;
-    const int size = dtype_size(dtype), team = cols * size <= 128 ? 8 : 64, teams = 256 / team;
-    const int64_t vectors = (cols * size + 15) / 16, across = (vectors + team - 1) / team;
+    const int size = dtype_size(dtype);
+    const int64_t vectors = (cols * size + 15) / 16;
+    const int team = backward_team(vectors), teams = 256 / team;
+    const int64_t across = (vectors + team - 1) / team;
     const uint64_t keys = (uint64_t)workspace + (uint64_t)sort_workspace(n, vocab), order = keys + (uint64_t)n * 4;
     TableArgs a = {};
     a.dy = (uint64_t)dy;
@@ -255,7 +297,7 @@ extern "C" int tftq_embedding_backward(int dtype, int id_bytes, const void *ids,
     a.order = order;
     a.dtable = (uint64_t)dtable;
     a.n = n;
-    a.chunk = embedding_chunk(n);
+    a.chunk = embedding_chunk(n, vectors);
     a.chunks = (n + a.chunk - 1) / a.chunk;
     a.heads = (keys + (uint64_t)n * 8 + 15) & ~(uint64_t)15;
     a.tails = a.heads + (uint64_t)(a.chunks * sums_stride(cols)) * 4;
@@ -279,7 +321,6 @@ extern "C" int tftq_embedding_backward(int dtype, int id_bytes, const void *ids,
                                         : backward_kernel<bf16_tag>(cols, team, a.chunk);
     if (const int rc = launch(k, (a.chunks + teams - 1) / teams * across)) return rc;
     if (a.chunks < 2) return 0;
-    a.across = (int)((vectors + 63) / 64);
-    k = dtype == TFTQ_F32 ? join_kernel<float>(cols) : dtype == TFTQ_F16 ? join_kernel<f16_tag>(cols) : join_kernel<bf16_tag>(cols);
+    k = dtype == TFTQ_F32 ? join_kernel<float>(cols, team) : dtype == TFTQ_F16 ? join_kernel<f16_tag>(cols, team) : join_kernel<bf16_tag>(cols, team);
     return launch(k, (a.chunks - 1) * a.across);
 }

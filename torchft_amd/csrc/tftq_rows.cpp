@@ -56,7 +56,7 @@ struct {
                              void *, void *, int64_t, int, void *) = nullptr;
     int (*dropout)(int, const void *, const void *, int64_t, double, int64_t, const int64_t *, int64_t, void *, int, void *) = nullptr;
     int (*embedding)(int, int, const void *, int64_t, const void *, int64_t, int64_t, int64_t, float, void *, int, void *) = nullptr;
-    int64_t (*embedding_backward_workspace)(int64_t, int64_t, int64_t) = nullptr;
+    int64_t (*embedding_backward_workspace)(int, int64_t, int64_t, int64_t) = nullptr;
     int (*embedding_backward)(int, int, const void *, int64_t, int64_t, const void *, int64_t, int64_t, float, void *, void *, int64_t, int,
                               void *) = nullptr;
     int64_t (*expert_sort_workspace)(int64_t, int64_t) = nullptr;
@@ -329,7 +329,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
             const Tensor ids = ctx->get_saved_variables()[0].contiguous(), dy = dy_.resolve_neg().contiguous();
             const int64_t vocab = ctx->saved_data["vocab"].toInt(), cols = ctx->saved_data["cols"].toInt(), n = ids.numel();
             dtable = fresh({vocab, cols}, dy.scalar_type(), dy);
-            const int64_t size = bytes_needed(lib.embedding_backward_workspace(n, vocab, cols), "tftq_embedding_backward_workspace");
+            const int64_t size = bytes_needed(lib.embedding_backward_workspace(code_of(dy), n, vocab, cols), "tftq_embedding_backward_workspace");
             const Tensor workspace = bytes_of(size, dy);
             checked(lib.embedding_backward(code_of(dy), static_cast<int>(ids.element_size()), data_of(ids), n, ctx->saved_data["skip"].toInt(),
                                            data_of(dy), vocab, cols, static_cast<float>(ctx->saved_data["scale"].toDouble()), data_of(dtable),

@@ -6,7 +6,7 @@
 // with atomics whose order could show: equal numbers keep their order.
 //
 // Few numbers stay in one workgroup's registers and LDS for all passes of up to 9 bits: one launch, bound by the four
-// vector units of one compute unit (four instructions a bit and number).  More go over two launches a pass of up to 8
+// vector units of one compute unit (four instructions a bit and number).  More go over two launches a pass of as many
 // bits: counts of tiles of 2048, then places (three from 131072 on, where every tile would read too many counts).
 #include "tftq_sort.h"
 
@@ -153,34 +153,34 @@ __global__ __launch_bounds__(THREADS) void k_sort_one(const SortArgs a, int pass
             as_global<u32>(a.offsets)[c] = (u32)first_at((const u32 *)keys, n, c);
 }
 
-constexpr int SORT_ITEMS = 8, SORT_TILE = 256 * SORT_ITEMS;
+constexpr int SORT_THREADS = 512, SORT_ITEMS = 4, SORT_TILE = SORT_THREADS * SORT_ITEMS, SORT_DIGITS = 512;
 constexpr int SORT_DIRECT = 64;  // so many tiles read each other's counts themselves
 
 // A pass over many numbers: from ids (the first) or from keys and places.
 struct SortPass {
     uint64_t keys, places;  // 0: the ids themselves
     uint64_t to_keys, to_places, position, offsets;
-    uint64_t counts;        // u32 [256][pitch]: of a digit and a tile; with more than SORT_DIRECT tiles, then u32 [256] of all
+    uint64_t counts;        // u32 [SORT_DIGITS][pitch]: of a digit and a tile; with more than SORT_DIRECT tiles, then u32 [SORT_DIGITS] of all
     int shift, width, tiles, pitch;
 };
 
 DEV u32 sort_read(const SortArgs &a, const SortPass &p, int64_t i) { return p.keys ? as_global<const u32>(p.keys)[i] : sort_key(a, i); }
 
-__global__ __launch_bounds__(256) void k_sort_count(const SortArgs a, const SortPass p)
+__global__ __launch_bounds__(SORT_THREADS) void k_sort_count(const SortArgs a, const SortPass p)
 {
-    __shared__ u32 counts[256];
-    if (sort_fill<256>(a, p.tiles)) return;
+    __shared__ u32 counts[SORT_DIGITS];
+    if (sort_fill<SORT_THREADS>(a, p.tiles)) return;
     counts[threadIdx.x] = 0;
     __syncthreads();
     const int64_t first = (int64_t)blockIdx.x * SORT_TILE + threadIdx.x;
     u32 key[SORT_ITEMS];
 #pragma unroll
-    for (int i = 0; i < SORT_ITEMS; i++) key[i] = first + i * 256 < a.n ? sort_read(a, p, first + i * 256) : 0;
+    for (int i = 0; i < SORT_ITEMS; i++) key[i] = first + i * SORT_THREADS < a.n ? sort_read(a, p, first + i * SORT_THREADS) : 0;
 #pragma unroll
     for (int i = 0; i < SORT_ITEMS; i++)
-        if (first + i * 256 < a.n) atomicAdd(&counts[key[i] >> p.shift & ((1u << p.width) - 1)], 1u);
+        if (first + i * SORT_THREADS < a.n) atomicAdd(&counts[key[i] >> p.shift & ((1u << p.width) - 1)], 1u);
     __syncthreads();
-    as_global<u32>(p.counts)[(int64_t)threadIdx.x * p.pitch + blockIdx.x] = counts[threadIdx.x];
+    if (threadIdx.x >> p.width == 0) as_global<u32>(p.counts)[(int64_t)threadIdx.x * p.pitch + blockIdx.x] = counts[threadIdx.x];
 }
 
 // A workgroup to a digit: its counts become how many there are in the tiles before.
@@ -196,13 +196,14 @@ __global__ __launch_bounds__(256) void k_sort_before(const SortPass p)
         base += sums[0] + sums[1] + sums[2] + sums[3];
         __syncthreads();
     }
-    if (threadIdx.x == 0) as_global<u32>(p.counts)[(int64_t)256 * p.pitch + blockIdx.x] = base;
+    if (threadIdx.x == 0) as_global<u32>(p.counts)[(int64_t)SORT_DIGITS * p.pitch + blockIdx.x] = base;
 }
 
-__global__ __launch_bounds__(256) void k_sort_place(const SortArgs a, const SortPass p)
+__global__ __launch_bounds__(SORT_THREADS) void k_sort_place(const SortArgs a, const SortPass p)
 {
-    __shared__ u32 counts[4][256], sums[4];
-    if (sort_fill<256>(a, p.tiles)) return;
+    constexpr int WAVES = SORT_THREADS / 64;
+    __shared__ u32 counts[WAVES][SORT_DIGITS], sums[WAVES];
+    if (sort_fill<SORT_THREADS>(a, p.tiles)) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x / 64, d = threadIdx.x;
     u32 key[SORT_ITEMS], digit[SORT_ITEMS], rank[SORT_ITEMS], place[SORT_ITEMS];
     bool live[SORT_ITEMS];
@@ -216,22 +217,24 @@ __global__ __launch_bounds__(256) void k_sort_place(const SortArgs a, const Sort
     }
     // of digit d: how many there are in all tiles, and in those before this one
     u32 before = 0, total = 0;
-    if (p.tiles > SORT_DIRECT) {
-        before = as_global<const u32>(p.counts)[(int64_t)d * p.pitch + blockIdx.x];
-        total = as_global<const u32>(p.counts)[(int64_t)256 * p.pitch + d];
-    } else {
-        for (int tile = 0; tile < p.tiles; tile += 4) {
-            const u32x4 c = *(as_global<const u32x4>(p.counts + ((uint64_t)d * p.pitch + tile) * 4));
+    if (d >> p.width == 0) {
+        if (p.tiles > SORT_DIRECT) {
+            before = as_global<const u32>(p.counts)[(int64_t)d * p.pitch + blockIdx.x];
+            total = as_global<const u32>(p.counts)[(int64_t)SORT_DIGITS * p.pitch + d];
+        } else {
+            for (int tile = 0; tile < p.tiles; tile += 4) {
+                const u32x4 c = *(as_global<const u32x4>(p.counts + ((uint64_t)d * p.pitch + tile) * 4));
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if (tile + i >= p.tiles) continue;
-                total += c[i];
-                if (tile + i < (int)blockIdx.x) before += c[i];
+                for (int i = 0; i < 4; i++) {
+                    if (tile + i >= p.tiles) continue;
+                    total += c[i];
+                    if (tile + i < (int)blockIdx.x) before += c[i];
+                }
             }
         }
     }
 #pragma unroll
-    for (int w = 0; w < 4; w++) counts[w][d] = 0;
+    for (int w = 0; w < WAVES; w++) counts[w][d] = 0;
     const u32 start = sort_prefix(total, sums);  // a barrier
     if (p.offsets && blockIdx.x == 0 && d <= (int)a.classes) as_global<u32>(p.offsets)[d] = start;
 #pragma unroll
@@ -240,7 +243,7 @@ __global__ __launch_bounds__(256) void k_sort_place(const SortArgs a, const Sort
     __syncthreads();
     u32 s = start + before;
 #pragma unroll
-    for (int w = 0; w < 4; w++) {
+    for (int w = 0; w < WAVES; w++) {
         const u32 c = counts[w][d];
         counts[w][d] = s;
         s += c;
@@ -270,21 +273,21 @@ static int sort_bits(int64_t classes)  // numbers from 0 to classes
 }
 
 // Whether one workgroup takes all.  Times of a sort with places and offsets, us, in one workgroup and in tiles:
-// 4096 numbers below 8 6.5, 8.7, below 255 7.7, 9.3, below 1000 11.0, 21.1; 8192 9.3, 8.8 / 12.9, 9.5 / 17.5, 21.9;
-// 16384 16.3, 9.2 / 23.7, 9.9 / 31.1, 22.9: one compute unit's scattered stores, and its ballots, against two launches a pass.
-static bool sort_one(int64_t n, int64_t classes) { return n <= (classes > 255 ? 8192 : 4096); }
+// 4096 numbers below 8 6.5, 7.2, below 255 7.7, 7.5, below 1000 11.1, 18.4; 8192 9.3, 7.3 / 13.0, 8.0 / 17.7, 19.4; 16384
+// 16.3, 7.6 / 23.7, 8.5 / 31.1, 20.6: one compute unit's scattered stores, and its ballots, against two launches a pass.
+static bool sort_one(int64_t n, int64_t classes) { return n <= (classes >= SORT_DIGITS ? 8192 : 4096); }
 
 // Whether the offsets are a launch of their own, which searches the keys: a tile that knows all digits' places writes
 // them along with a sort of one pass, and one workgroup up to 2048.
-static bool sort_searches(int64_t n, int64_t classes) { return classes > (sort_one(n, classes) ? 2048 : 255); }
+static bool sort_searches(int64_t n, int64_t classes) { return classes >= (sort_one(n, classes) ? 2049 : SORT_DIGITS); }
 
 static int64_t sort_pitch(int64_t n) { return ((n + SORT_TILE - 1) / SORT_TILE + 3) & ~(int64_t)3; }
 
 int64_t sort_workspace(int64_t n, int64_t classes)
 {
     if (sort_one(n, classes)) return 0;
-    const int64_t pairs = (sort_bits(classes) + 7) / 8 - 1;
-    return (sort_pitch(n) + 1) * 1024 + std::min<int64_t>(pairs, 2) * ((n * 8 + 15) & ~(int64_t)15);
+    const int64_t pairs = (sort_bits(classes) + 8) / 9 - 1;
+    return (sort_pitch(n) + 1) * SORT_DIGITS * 4 + std::min<int64_t>(pairs, 2) * ((n * 8 + 15) & ~(int64_t)15);
 }
 
 bool sort_needs_keys(int64_t n, int64_t classes) { return sort_searches(n, classes); }
@@ -320,13 +323,13 @@ int sort_numbers(const SortArgs &in, void *workspace, hipStream_t st)
         a.offsets = offsets;
         return sort_offsets(a, st);
     }
-    const int passes = (bits + 7) / 8, width = (bits + passes - 1) / passes;
+    const int passes = (bits + 8) / 9, width = (bits + passes - 1) / passes;
     SortPass p = {};
     p.tiles = (int)((a.n + SORT_TILE - 1) / SORT_TILE);
     p.pitch = (int)sort_pitch(a.n);
     p.counts = (uint64_t)workspace;
     p.width = width;
-    const uint64_t pairs = p.counts + (uint64_t)(p.pitch + 1) * 1024, pair = ((uint64_t)a.n * 8 + 15) & ~(uint64_t)15;
+    const uint64_t pairs = p.counts + (uint64_t)(p.pitch + 1) * SORT_DIGITS * 4, pair = ((uint64_t)a.n * 8 + 15) & ~(uint64_t)15;
     // the launches' shares of the zeros
     const int64_t share = (in.fill_bytes / (2 * passes) + 4095) & ~(int64_t)4095;
     auto next_share = [&](bool first) {
@@ -344,11 +347,11 @@ int sort_numbers(const SortArgs &in, void *workspace, hipStream_t st)
         p.shift = pass * width;
         void *args[] = {(void *)&a, (void *)&p}, *before[] = {(void *)&p};
         next_share(pass == 0);
-        if (const int rc = (int)hipLaunchKernel((const void *)k_sort_count, dim3(sort_groups(a, p.tiles, 256)), dim3(256), args, 0, st)) return rc;
+        if (const int rc = (int)hipLaunchKernel((const void *)k_sort_count, dim3(sort_groups(a, p.tiles, SORT_THREADS)), dim3(SORT_THREADS), args, 0, st)) return rc;
         if (p.tiles > SORT_DIRECT)
-            if (const int rc = (int)hipLaunchKernel((const void *)k_sort_before, dim3(256), dim3(256), before, 0, st)) return rc;
+            if (const int rc = (int)hipLaunchKernel((const void *)k_sort_before, dim3(1u << width), dim3(256), before, 0, st)) return rc;
         next_share(false);
-        if (const int rc = (int)hipLaunchKernel((const void *)k_sort_place, dim3(sort_groups(a, p.tiles, 256)), dim3(256), args, 0, st)) return rc;
+        if (const int rc = (int)hipLaunchKernel((const void *)k_sort_place, dim3(sort_groups(a, p.tiles, SORT_THREADS)), dim3(SORT_THREADS), args, 0, st)) return rc;
     }
     return a.offsets && passes > 1 ? sort_offsets(a, st) : 0;
 }
