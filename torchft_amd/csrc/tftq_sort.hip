@@ -16,6 +16,14 @@ DEV u32 sort_key(const SortArgs &a, int64_t i)
     return (uint64_t)id < a.classes && (u32)id != a.skip ? (u32)id : a.classes;
 }
 
+// What the wavefront's lanes wrote to LDS is there for all of them; nothing to wait for, as one wavefront's accesses stay in order.
+DEV void wave_sync()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // The rank of every item among those of its digit in the wavefront's part, in the order of i, then lanes; `mine`, this
 // wavefront's counters, ends with how many of every digit there are.  Items from `items` on are not live.
 template <int ITEMS>
@@ -44,10 +52,10 @@ DEV void sort_rank(const u32 (&digit)[ITEMS], const bool (&live)[ITEMS], int ite
         if (live[i]) {
             const u32 before = __builtin_amdgcn_mbcnt_hi(high[i], __builtin_amdgcn_mbcnt_lo(low[i], 0)), base = mine[digit[i]];
             rank[i] = base + before;
-            // every lane has read its counter before the first of its digit moves it on: one wavefront, in order
-            __builtin_amdgcn_wave_barrier();
+            // every lane has read its counter before the first of its digit moves it on, and the next item's read is behind that
+            wave_sync();
             if (before == 0) mine[digit[i]] = base + (u32)(__builtin_popcount(low[i]) + __builtin_popcount(high[i]));
-            __builtin_amdgcn_wave_barrier();
+            wave_sync();
         }
     }
 }
