@@ -99,6 +99,19 @@ def test_fp8(t, shape, dtype):
         assert rows.dequantize().dtype == dtype
 
 
+@pytest.mark.parametrize("shape", [(40000, 3), (3000, 64), (700, 333), (90, 2900), (60, 4480), (20, 8000), (6, 16390), (4, 40001)])
+def test_fp8_nearest(t, shape):
+    """Codes of fp32 rows are the nearest: two results of 64 bits lie on two sides of a border once in 10^14 codes."""
+    x, r, w = values(*shape, torch.float32, 1), values(*shape, torch.float32, 2), 1 + values(1, shape[1], torch.float32, 5)[0]
+    for residual in (None, r):
+        got = t.rms_norm_fp8(x.cuda(), w.cuda(), None if residual is None else residual.cuda(), EPS)
+        rows = got if residual is None else got[0]
+        y, _, _ = ref.norm(x, w, residual, EPS)
+        z = y / (y.abs().amax(1, keepdim=True) / 448)
+        step = torch.exp2(torch.frexp(z.abs().clamp(min=2.0 ** -6)).exponent.double() - 4)  # e4m3: 4 bits, 2^-9 at least
+        assert torch.equal(rows.codes.cpu().double(), (z / step).round() * step)
+
+
 @pytest.mark.parametrize("dtype", ref.DTYPES)
 def test_orders(t, dtype):
     """Slices, transposes, heads inside wider rows, expanded rows, more dimensions, empty ones."""
