@@ -270,7 +270,12 @@ extern "C" int tftq_embedding(int dtype, int id_bytes, const void *ids, int64_t 
 // their sums cost more than they hasten (with 16 these are a quarter of dy's bytes or half).  The gradient in us with 16, 64 and 256:
 // 65536 tokens of 64 bf16 37, 50, 110; 65536 of 256 56, 58, 106; 8192 of 4096 66, 66, 107; 300000 of 128 82, 70, 114; 131072 of
 // 1024 144, 111, 119; 300000 of 1024 278, 197, 199; 2000000 of 128 349, 216, 200, and where all tokens are one 2737, 822, 326.
-static int embedding_chunk(int64_t n, int64_t vectors) { return n * vectors < 1 << 22 ? 16 : n * vectors < 1 << 25 ? 64 : 256; }
+// Few tokens (up to 8192) have few sums to join, however long they are, and stay with 16 for twice the work: even numbers, 8192
+// tokens of 4096 67.5 and 72, 4096 of 8192 166 and 172; 65536 of 512, where half of the numbers are in a hundredth of the table, 70 and 59.
+static int embedding_chunk(int64_t n, int64_t vectors)
+{
+    return n * vectors < 1 << (n <= 8192 ? 23 : 22) ? 16 : n * vectors < 1 << 25 ? 64 : 256;
+}
 
 extern "C" int64_t tftq_embedding_backward_workspace(int dtype, int64_t n, int64_t vocab, int64_t cols)
 {
