@@ -120,6 +120,7 @@ def test_graph(t):
         return y.detach(), torch.autograd.grad(y, table, dy)[0]
 
     side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
         step()
     torch.cuda.synchronize()

@@ -149,6 +149,7 @@ def test_graph(t):
         return (order.position, order.offsets, y.detach(), *torch.autograd.grad(y, (x, w), dy))
 
     side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
         step()
     torch.cuda.synchronize()
