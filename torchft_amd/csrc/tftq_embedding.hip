@@ -76,7 +76,7 @@ __global__ __launch_bounds__(256) void k_embedding_backward(const TableArgs a)
         keys[i] = at >= 0 && at < a.n ? as_global<const u32>(a.keys)[at] : NONE;
     }
     for (int i = threadIdx.x; i < TEAMS * CHUNK; i += 256)
-        if (first + i < a.n) order[i] = as_global<const u32>(a.order)[first + i];
+        if (first + i < a.n) order[i] = min(as_global<const u32>(a.order)[first + i], (u32)a.n - 1);  // whatever memory says
     __syncthreads();
     const int team = TEAM == 64 ? __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64) : (int)threadIdx.x / TEAM;
     const int64_t chunk = chunk0 + team;

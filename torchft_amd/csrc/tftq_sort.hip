@@ -7,7 +7,8 @@
 //
 // Few numbers stay in one workgroup's registers and LDS for all passes of up to 9 bits: one launch, bound by the four
 // vector units of one compute unit (four instructions a bit and number).  More go over two launches a pass of as many
-// bits: counts of tiles of 2048, then places (three from 131072 on, where every tile would read too many counts).
+// bits: counts of tiles of 2048, then places (three from 131072 on, where every tile would read too many counts).  Numbers
+// that another stream changes between the two would not fit the counts; places are held below n, whatever memory says.
 #include "tftq_sort.h"
 
 DEV u32 sort_key(const SortArgs &a, int64_t i)
@@ -221,7 +222,7 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_place(const SortArgs a, c
         const int64_t at = first + i * 64;
         live[i] = at < a.n;
         key[i] = live[i] ? sort_read(a, p, at) : 0;
-        place[i] = live[i] && p.keys ? as_global<const u32>(p.places)[at] : (u32)at;
+        place[i] = live[i] && p.keys ? min(as_global<const u32>(p.places)[at], (u32)a.n - 1) : (u32)at;
     }
     // of digit d: how many there are in all tiles, and in those before this one
     u32 before = 0, total = 0;
@@ -260,7 +261,7 @@ __global__ __launch_bounds__(SORT_THREADS) void k_sort_place(const SortArgs a, c
 #pragma unroll
     for (int i = 0; i < SORT_ITEMS; i++) {
         if (!live[i]) continue;
-        const u32 to = counts[wave][digit[i]] + rank[i];
+        const u32 to = min(counts[wave][digit[i]] + rank[i], (u32)a.n - 1);
         if (p.to_keys) as_global<u32>(p.to_keys)[to] = key[i];
         as_global<u32>(p.to_places)[to] = place[i];
         if (p.position) as_global<u32>(p.position)[place[i]] = to;
