@@ -164,6 +164,22 @@ bool wants_grad(const Tensor &t) { return t.defined() && t.requires_grad(); }
 bool wants_grad(const Maybe &t) { return t && wants_grad(*t); }
 Tensor or_none(const Maybe &t) { return t ? *t : Tensor(); }
 
+// Begins a backward pass.  Under a stream capture no gradient may go to a node of the default stream (a leaf's, made with an eager
+// graph of the leaf that still lives): that stream would have to wait for the capture, which it cannot, and the capture breaks
+// off in ways that the process may not survive.  Refused here, where nothing has crossed yet.
+void begin_backward(const Tensor &beside)
+{
+    const c10::hip::HIPStream here = c10::hip::getCurrentHIPStream(beside.device().index());
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (here.id() == 0 || hipStreamIsCapturing(here.stream(), &status) != hipSuccess || status != hipStreamCaptureStatusActive) return;
+    const std::shared_ptr<torch::autograd::Node> node = torch::autograd::get_current_node();
+    if (!node) return;
+    for (const torch::autograd::Edge &edge : node->next_edges()) {
+        const auto there = edge.function ? edge.function->stream() : std::nullopt;
+        require(!there || there->id() != 0, "A backward pass cannot be captured while a graph of the same tensors lives that was made on the default stream");
+    }
+}
+
 // What a backward pass returns where second derivatives may be asked for: an error once they are.
 variable_list once(variable_list grads, const variable_list &from, const char *name)
 {
@@ -234,6 +250,7 @@ struct Norm : torch::autograd::Function<Norm> {
         const Tensor &dy_ = grads[0];
         const Tensor dh_ = with_residual ? grads[1] : Tensor();
         Tensor dx, dw;
+        if (dy_.defined() || dh_.defined()) begin_backward(h_);
         if (!dy_.defined()) dx = dh_;
         else {
             at::NoGradGuard guard;
@@ -283,6 +300,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
     {
         const Tensor &dy = grads[0], seed_at = ctx->get_saved_variables()[0];
         Tensor dx;
+        if (dy.defined()) begin_backward(dy);
         if (dy.defined() && ctx->needs_input_grad(0)) {
             at::NoGradGuard guard;
             dx = dropout_run(dy, Tensor(), ctx->saved_data["p"].toDouble(), ctx->saved_data["seed"].toInt(), seed_at, ctx->saved_data["offset"].toInt());
@@ -325,6 +343,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
         const Tensor &dy_ = grads[0];
         Tensor dtable;
         if (dy_.defined()) {
+            begin_backward(dy_);
             at::NoGradGuard guard;
             const Tensor ids = ctx->get_saved_variables()[0].contiguous(), dy = dy_.resolve_neg().contiguous();
             const int64_t vocab = ctx->saved_data["vocab"].toInt(), cols = ctx->saved_data["cols"].toInt(), n = ids.numel();
@@ -385,6 +404,7 @@ struct Dispatch : torch::autograd::Function<Dispatch> {
         const variable_list saved = ctx->get_saved_variables();
         Tensor dx;
         if (grads[0].defined()) {
+            begin_backward(grads[0]);
             at::NoGradGuard guard;
             dx = combine_run(grads[0], Places(saved[0], saved[1]), Tensor());
         }
@@ -409,6 +429,7 @@ struct Combine : torch::autograd::Function<Combine> {
         const bool for_rows = ctx->needs_input_grad(0), for_weights = rows_.defined() && ctx->needs_input_grad(1);
         Tensor drows, dweights;
         if (dy_.defined() && (for_rows || for_weights)) {
+            begin_backward(dy_);
             at::NoGradGuard guard;
             const Places places(saved[2], saved[3]);
             const Rows dy(dy_);
