@@ -297,7 +297,7 @@ int tftq_newton_schulz(const tftq_ns *what, void *workspace, int64_t workspace_b
  * row to row, and where none is given rows follow each other.  Rows, columns, tokens and choices are at most 2^31 - 65536
  * (TFTQ_E_SHAPE).  Sums are fp32 in an order that the arguments alone decide; results are rounded once.  Workspaces
  * are device memory, 16-byte aligned, at least as many bytes as the function beside says (TFTQ_E_SIZE), and hold
- * nothing between calls.
+ * nothing between calls.  What a function writes overlaps nothing that it reads.
  *
  * Root-mean-square norm:  h = x + residual, rounded to the rows' type;  y = h w / sqrt(mean(h^2) + eps).
  *   x         x_group rows x_stride apart, and as many again x_group_stride behind their beginning, and so on (heads inside

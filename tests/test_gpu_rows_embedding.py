@@ -79,6 +79,20 @@ def test_skewed_and_long(t):
         check(t, (torch.arange(n) // (3 * chunk)) % 40, table)
 
 
+@pytest.mark.parametrize("n, cols", [(8192, 512), (8192, 4100), (8193, 2100), (40000, 512), (270001, 512)])
+def test_long_runs(t, n, cols):
+    """Runs beside the borders of 16, 64 and 256 tokens, at sizes where those are taken; whole numbers add up exactly in any order."""
+    rows = n // 16 + 2
+    table = torch.zeros(rows, cols, device="cuda", requires_grad=True)
+    dy = torch.randint(-2, 3, (n, cols), device="cuda", dtype=torch.float32)  # sums below 2^24
+    at = torch.arange(n, device="cuda")
+    for run in (16, 64, 256):
+        for ids in (at // run, (at + run // 2) // run, at // (3 * run), (at // run).clamp(max=3), at * 0 + 7):
+            ids = ids[torch.randperm(n, device="cuda")]
+            got, = torch.autograd.grad(t.embedding(ids, table), table, dy)
+            assert torch.equal(got, torch.zeros(rows, cols, device="cuda").index_add_(0, ids, dy))
+
+
 @pytest.mark.parametrize("dtype", ref.DTYPES)
 def test_orders(t, dtype):
     """Tables inside wider ones and transposed, numbers in any order, no tokens, no columns, more dimensions."""
