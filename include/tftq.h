@@ -305,7 +305,8 @@ int tftq_newton_schulz(const tftq_ns *what, void *workspace, int64_t workspace_b
  *   residual  NULL for none; then h is x and the argument h has to be NULL
  *   weight    [cols] of weight_dtype (dtype or TFTQ_F32); NULL for ones
  *   y         [rows, cols]; or NULL, with codes [rows, cols] and scales [rows]: y in e4m3 codes that scales multiply,
- *             a row's largest magnitude / 448 (1 where that is below 2^-126)
+ *             a row's largest magnitude / 448 (1 where that is below 2^-126).  Codes are the nearest to 448 h w / max |h w|, the
+ *             even one of two that are as near (of scales above 2^-100, and of h that are no less than 2^-126 of the row's root mean square)
  * The sum of squares is fp32: rows of magnitudes beyond 1e18 pass its range.
  */
 int tftq_rms_norm(int dtype, int weight_dtype, const void *x, int64_t x_stride, int64_t x_group, int64_t x_group_stride,

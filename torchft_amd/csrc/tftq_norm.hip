@@ -8,9 +8,11 @@
 // pass: its sum of squares rides along with that of g h.
 //
 // y may leave in 8 bits: e4m3 codes with one fp32 scale a row, max |y| / 448, that multiplies them (1 where that
-// is no normal number).  Codes of 16-bit rows are taken from the fp32 y.  Of fp32 rows, whose y is good to 24 bits, one code in
-// 10^6 would then be the neighbour of the nearest, so theirs are made in 64 bits: r cancels in y / scale = 448 h w / max |h w|,
-// whose products are exact, and both sums over the row are one.  8192x2048 fp32 26 us of 22; of its codes none is off, of 13.
+// is no normal number).  A code is the nearest to y / scale = 448 h w / max |h w|, in which r cancels, an even one where two are as
+// near.  In fp32 that quotient is off by 5 2^-24 at most, so that the codes on both sides of it, 2^-21 away, differ once
+// in 10^5 elements; there products in 64 bits, which are exact, say on which side of the border it lies, or on it.  Of bf16 rows and
+// weights one in 2000 lies on a border; their products are exact in fp32 already.  8192x2048 fp32 25 us (26 with 64-bit products of all
+// elements), 8192x4096 bf16 with a residual 40.8 (39.8 without a thought of borders, 41.0 with fp32 weights, 43.6 where these are ones).
 #include "tftq_rows.h"
 
 struct NormArgs {
@@ -67,35 +69,126 @@ struct Weights {
 
 DEV float inverse_root(float mean_square, float eps) { return 1.0f / __builtin_sqrtf(mean_square + eps); }
 
-DEV float fp8_scale(float amax)
+// r as a power of two, by which h can be multiplied without rounding and without a product h w that passes fp32's range, and
+// the rest, 1 or more and below 2.  NaN stays.
+DEV void split_root(float r, float &unit, float &rest)
 {
-    const float part = amax / 448.0f;
-    return part >= 0x1p-126f ? part : 1.0f;
+    unit = r != r ? r : as_f(as_u(r) & 0x7f800000u);
+    rest = as_f((as_u(r) & 0x007fffffu) | 0x3f800000u);
 }
-// A row's scale, and what its h w are multiplied by for their codes.
-DEV void fp8_scale(double most, float r, float &scale, double &factor)
+// The largest |h unit w| of a row in 64 bits: `mine` is a lane's, rounded; where that is the row's, left(mine) is the largest part that
+// such numbers' rounding left out.  lds: 2 TEAM / 64 floats.
+template <int TEAM, class F>
+DEV double team_largest_product(float mine, float *lds, F left)
 {
-    const float part = (float)(most * r / 448.0);
-    const bool normal = part >= 0x1p-126f;
-    scale = normal ? part : 1.0f;
-    factor = normal ? 448.0 / most : (double)r;
+    constexpr int WAVES = TEAM / 64;
+    constexpr float NONE = -__builtin_inff();
+    float high = team_max<(TEAM > 64 ? 64 : TEAM)>(mine, lds), low = NONE;
+    if (TEAM <= 64) {
+        if (mine == high) low = left(high);
+        low = team_max<(TEAM > 64 ? 64 : TEAM)>(low, lds);
+    } else {
+        const float wave = high;
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = wave;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < WAVES; i++) high = fmaxf(high, lds[i]);
+        if (wave == high) {
+            if (mine == high) low = left(high);
+            low = team_max<64>(low, lds);
+        }
+        if ((threadIdx.x & 63) == 0) lds[WAVES + (threadIdx.x >> 6)] = low;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < WAVES; i++) low = fmaxf(low, lds[WAVES + i]);
+    }
+    return (double)high + (high > 0.0f && high < __builtin_inff() ? low : 0.0f);
 }
-// To fp32, cut off, the last bit set where anything was lost: the rounding to 4 bits that follows then goes as from v itself.
-DEV float cut(double v)
+
+DEV float row_scale(float part, bool &normal)
 {
-    u32x2 w = __builtin_bit_cast(u32x2, v);
-    w.x = (w.x | ((w.x & 0x1fffffffu) + 0x1fffffffu)) & 0xe0000000u;
-    return (float)__builtin_bit_cast(double, w);
+    normal = part >= 0x1p-126f;
+    return normal ? part : 1.0f;
 }
+// What a row's scale and codes are made with, from its largest |h unit w| and what that leaves of r.  Where the scale is 1 for want of a
+// normal number all codes are zeros, or NaN.
+struct RowCodes {
+    float scale, under, over;
+    double most;
+    DEV RowCodes(double largest, float rest) : most(largest)
+    {
+        const float high = (float)largest;
+        bool normal;
+        scale = row_scale(high / 448.0f * rest, normal);
+        const float by = normal ? 448.0f / high : 0.0f;
+        under = by * 0x1.fffffp-1f;
+        over = by * 0x1.000008p+0f;
+    }
+    // Of any products p = h unit w, rounded: the codes 2^-21 below and above 448 p / most, off by 5 2^-24 at most.  Where they differ,
+    // the sign of 448 h unit w - border most, two products of 53 bits at most, says which it is.  Borders are odd multiples of the step
+    // of five significant bits, 2^-10 at least.  wide(i): h unit w in 64 bits.
+    template <int EPV, class F>
+    DEV u32x2 codes(const float (&p)[EPV], F wide) const
+    {
+        u32 c[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < EPV; i += 4) {
+            u32 code = pack_fp8x4(p[i] * under, p[i + 1] * under, p[i + 2] * under, p[i + 3] * under);
+            const u32 differ = code ^ pack_fp8x4(p[i] * over, p[i + 1] * over, p[i + 2] * over, p[i + 3] * over);
+            if (differ) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const u32 mine = differ & 0xFFu << (8 * j);
+                    if (!mine) continue;
+                    const float q = __builtin_fabsf(p[i + j] * under);
+                    const float border = q < 0x1p-6f ? __builtin_rintf(q * 1024.0f) * 0x1p-10f : as_f((as_u(q) + 0x40000u) & 0xfff80000u);
+                    const double above = __builtin_fma(-(double)border, most, 448.0 * __builtin_fabs(wide(i + j)));
+                    if (above > 0.0 || (above == 0.0 && (code >> (8 * j) & 1))) code ^= mine;
+                }
+            }
+            c[i / 4] = code;
+        }
+        return u32x2{c[0], c[1]};
+    }
+};
+// Of products n = 7/8 h unit w that are exact in fp32, from the largest of them: the quotient 448 n / largest, with once more what it left
+// out.  One on a border comes out as that, any other is 2^-21 or more away (448 n and border times largest have 24 bits at most).
+struct RowCodesExact {
+    float scale, by, part;  // part: largest / 448, exact
+    DEV RowCodesExact(float largest, float rest)
+    {
+        constexpr float ONE_448TH = 1.0f / 448.0f;
+        const float first = largest * ONE_448TH;
+        bool normal;
+        part = __builtin_fmaf(__builtin_fmaf(-first, 448.0f, largest), ONE_448TH, first);
+        scale = row_scale(part * (8.0f / 7.0f) * rest, normal);
+        by = normal ? 448.0f / largest : 0.0f;
+    }
+    template <int EPV, class F>
+    DEV u32x2 codes(const float (&n)[EPV], F) const
+    {
+        u32 c[2] = {0, 0};
+        float q[EPV];
+#pragma unroll
+        for (int i = 0; i < EPV; i++) {
+            const float first = n[i] * by;
+            q[i] = __builtin_fmaf(__builtin_fmaf(-first, part, n[i]), by, first);
+        }
+#pragma unroll
+        for (int i = 0; i < EPV; i += 4) c[i / 4] = pack_fp8x4(q[i], q[i + 1], q[i + 2], q[i + 3]);
+        return u32x2{c[0], c[1]};
+    }
+};
+template <bool EXACT>
+using RowCodesOf = std::conditional_t<EXACT, RowCodesExact, RowCodes>;
+
 // EPV codes of a vector.
 template <int EPV, bool NARROW>
-DEV void store_codes(uint64_t row, const Piece &p, int cols, const float (&f)[EPV])
+DEV void store_codes(uint64_t row, const Piece &p, int cols, u32x2 c)
 {
     if (!p.in) return;
-    u32x4 c = {pack_fp8x4(f[0], f[1], f[2], f[3]), 0, 0, 0};
-    if constexpr (EPV == 8) c.y = pack_fp8x4(f[4], f[5], f[6], f[7]);
-    if (NARROW) store_bytes(row + (u32)p.at, (u32)cols, c);
-    else if constexpr (EPV == 8) *as_global<u32x2_a1>(row + (u32)p.at) = u32x2{c.x, c.y};
+    if (NARROW) store_bytes(row + (u32)p.at, (u32)cols, u32x4{c.x, c.y, 0, 0});
+    else if constexpr (EPV == 8) *as_global<u32x2_a1>(row + (u32)p.at) = c;
     else *as_global<u32_a1>(row + (u32)p.at) = c.x;
 }
 
@@ -105,9 +198,9 @@ template <class T, int TEAM, int NV, bool NARROW, bool WIDE, bool FP8>
 __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void k_rms_norm(const NormArgs a)
 {
     constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, TEAMS = TEAM > 256 ? 1 : 256 / TEAM;
-    constexpr bool EXACT = FP8 && ESZ == 4;
-    __shared__ float lds[TEAM > 64 ? TEAM / 64 : 1];
-    __shared__ double lds_most[EXACT && TEAM > 64 ? TEAM / 64 : 1];
+    // products of two 16-bit numbers are exact, those of bf16 448 times too; kept in registers where they leave eight wavefronts to a unit
+    constexpr bool LOW = ESZ == 4 || WIDE, EXACT = !LOW && std::is_same<T, bf16_tag>::value, KEEP = NV * EPV <= (WIDE ? 8 : 16);
+    __shared__ float lds[TEAM > 64 ? 2 * (TEAM / 64) : 1];
     const int lane = threadIdx.x % TEAM;
     const int64_t row = a.row0 + (int64_t)blockIdx.x * TEAMS + threadIdx.x / TEAM;
     if (row >= a.rows) return;  // a whole team; teams of several wavefronts are whole workgroups
@@ -129,7 +222,6 @@ __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void k_rms_norm(const Norm
 #pragma unroll
     for (int v = 0; v < NV; v++) weights[v].load(a.weight, piece[v], a.cols);
     float sum = 0.0f;
-    double most = 0.0;
 #pragma unroll
     for (int v = 0; v < NV; v++) {
         float f[EPV];
@@ -143,48 +235,66 @@ __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void k_rms_norm(const Norm
             store_row<ESZ, NARROW>(a.h + at, piece[v], a.cols, raw[v]);
             Elem<T>::unpack(raw[v], f);
         }
-        if constexpr (EXACT) {
-            float w[EPV];
-            weights[v].unpack(a.weight, w);
-#pragma unroll
-            for (int i = 0; i < EPV; i++) most = fmax(most, __builtin_fabs((double)f[i] * w[i]));
-        }
         if (!NARROW) count_once(f, piece[v]);
 #pragma unroll
         for (int i = 0; i < EPV; i++) sum = __builtin_fmaf(f[i], f[i], sum);
     }
-    if constexpr (EXACT) {
-        team_sum_largest<TEAM>(sum, most, lds, lds_most);
-        float scale;
-        double factor;
-        fp8_scale(most, inverse_root(sum * a.inv_cols, a.eps), scale, factor);
-        if (lane == 0) as_global<float>(a.scales)[row] = scale;
-#pragma unroll
-        for (int v = 0; v < NV; v++) {
+    const float r = inverse_root(team_sum<TEAM>(sum, lds) * a.inv_cols, a.eps);
+    if constexpr (FP8) {
+        float unit, rest, mine = 0.0f;
+        split_root(r, unit, rest);
+        if (EXACT) unit *= 0.875f;
+        float kept[KEEP ? NV : 1][EPV];
+        // else they are made again, not kept by the compiler, whose registers rows of 32768 take up (fp32 weights: 57 us of 72)
+        auto again = [&] { if (!KEEP) asm("" : "+v"(unit)); };
+        auto products = [&](int v, float (&p)[EPV]) {
             float f[EPV], w[EPV];
             Elem<T>::unpack(raw[v], f);
             weights[v].unpack(a.weight, w);
 #pragma unroll
-            for (int i = 0; i < EPV; i++) f[i] = cut((double)f[i] * w[i] * factor);
-            store_codes<EPV, NARROW>(a.codes + (uint64_t)(row * a.cols), piece[v], a.cols, f);
+            for (int i = 0; i < EPV; i++) p[i] = f[i] * unit * w[i];
+        };
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+            float(&p)[EPV] = kept[KEEP ? v : 0];
+            products(v, p);
+#pragma unroll
+            for (int i = 0; i < EPV; i++) mine = fmaxf(mine, __builtin_fabsf(p[i]));
+        }
+        std::conditional_t<LOW, double, float> most;
+        again();
+        if constexpr (LOW) {
+            most = team_largest_product<TEAM>(mine, lds, [&](float high) {
+                float low = -__builtin_inff();
+#pragma unroll
+                for (int v = 0; v < NV; v++) {
+                    float f[EPV], w[EPV];
+                    Elem<T>::unpack(raw[v], f);
+                    weights[v].unpack(a.weight, w);
+#pragma unroll
+                    for (int i = 0; i < EPV; i++)
+                        if (__builtin_fabsf(f[i] * unit * w[i]) == high)
+                            low = fmaxf(low, __builtin_fmaf(__builtin_fabsf(f[i] * unit), __builtin_fabsf(w[i]), -high));
+                }
+                return low;
+            });
+        } else most = team_largest<TEAM>(mine, lds);
+        const RowCodesOf<EXACT> row_codes(most, rest);
+        again();
+        if (lane == 0) as_global<float>(a.scales)[row] = row_codes.scale;
+#pragma unroll
+        for (int v = 0; v < NV; v++) {
+            float(&p)[EPV] = kept[KEEP ? v : 0];
+            if (!KEEP) products(v, p);
+            const u32x2 codes = row_codes.codes(p, [&](int at) {
+                float f[EPV], w[EPV];
+                Elem<T>::unpack(raw[v], f);
+                weights[v].unpack(a.weight, w);
+                return (double)(f[at] * unit) * w[at];
+            });
+            store_codes<EPV, NARROW>(a.codes + (uint64_t)(row * a.cols), piece[v], a.cols, codes);
         }
         return;
-    }
-    const float r = inverse_root(team_sum<TEAM>(sum, lds) * a.inv_cols, a.eps);
-    float inverse = 1.0f;
-    if constexpr (FP8) {
-        float amax = 0.0f;
-#pragma unroll
-        for (int v = 0; v < NV; v++) {
-            float f[EPV], w[EPV];
-            Elem<T>::unpack(raw[v], f);
-            weights[v].unpack(a.weight, w);
-#pragma unroll
-            for (int i = 0; i < EPV; i++) amax = fmaxf(amax, __builtin_fabsf(f[i] * r * w[i]));
-        }
-        const float scale = fp8_scale(team_largest<TEAM>(amax, lds));
-        inverse = 1.0f / scale;
-        if (lane == 0) as_global<float>(a.scales)[row] = scale;
     }
 #pragma unroll
     for (int v = 0; v < NV; v++) {
@@ -192,9 +302,8 @@ __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void k_rms_norm(const Norm
         Elem<T>::unpack(raw[v], f);
         weights[v].unpack(a.weight, w);
 #pragma unroll
-        for (int i = 0; i < EPV; i++) f[i] = FP8 ? f[i] * r * w[i] * inverse : f[i] * r * w[i];
-        if constexpr (FP8) store_codes<EPV, NARROW>(a.codes + (uint64_t)(row * a.cols), piece[v], a.cols, f);
-        else store_row<ESZ, NARROW>(a.y + at, piece[v], a.cols, Elem<T>::pack(f));
+        for (int i = 0; i < EPV; i++) f[i] = f[i] * r * w[i];
+        store_row<ESZ, NARROW>(a.y + at, piece[v], a.cols, Elem<T>::pack(f));
     }
 }
 
@@ -204,9 +313,8 @@ template <class T, bool WIDE, bool FP8>
 __global__ __launch_bounds__(1024) void k_rms_norm_long(const NormArgs a)
 {
     constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, STEP = 1024 * EPV;
-    constexpr bool EXACT = FP8 && ESZ == 4;
-    __shared__ float lds[16];
-    __shared__ double lds_most[EXACT ? 16 : 1];
+    constexpr bool LOW = ESZ == 4 || WIDE, EXACT = !LOW && std::is_same<T, bf16_tag>::value;
+    __shared__ float lds[32];
     const int64_t row = a.row0 + blockIdx.x;
     const uint64_t px = row_at(a.x, row, a.x_stride, a.x_group, a.x_group_stride, a.rows), pr = a.residual + (uint64_t)(row * a.residual_stride);
     const uint64_t at = (uint64_t)(row * a.cols) * ESZ, again = a.residual ? a.h + at : px;
@@ -232,51 +340,54 @@ __global__ __launch_bounds__(1024) void k_rms_norm_long(const NormArgs a)
     }
     const float r = inverse_root(team_sum<1024>(sum, lds) * a.inv_cols, a.eps);
     // every lane reads back the vectors that it wrote itself: its own stores come before its own loads
-    float scale = 1.0f, inverse = 1.0f;
-    double most = 0.0, factor = 1.0;
-    for (int pass = FP8 ? 0 : 1; pass < 2; pass++) {
-        float amax = 0.0f;
+    auto scaled = [&](const Piece &p, float by, float (&f)[EPV], float (&w)[EPV]) {
+        const u32x4 raw = load_row<ESZ, false, false>(again, p, a.cols);
+        Weights<T, false, WIDE> weights;
+        weights.load(a.weight, p, a.cols);
+        weights.unpack(a.weight, w);
+        Elem<T>::unpack(raw, f);
+#pragma unroll
+        for (int i = 0; i < EPV; i++) f[i] *= by;
+    };
+    if constexpr (FP8) {
+        float unit, rest, mine = 0.0f, f[EPV], w[EPV], p[EPV];
+        split_root(r, unit, rest);
+        if (EXACT) unit *= 0.875f;
+        for (int col = threadIdx.x * EPV; col < a.cols; col += STEP) {
+            scaled(piece_of<EPV, false>(col, a.cols), unit, f, w);
+#pragma unroll
+            for (int i = 0; i < EPV; i++) mine = fmaxf(mine, __builtin_fabsf(f[i] * w[i]));
+        }
+        std::conditional_t<LOW, double, float> most;
+        if constexpr (LOW) {
+            most = team_largest_product<1024>(mine, lds, [&](float high) {
+                float low = -__builtin_inff();
+                for (int col = threadIdx.x * EPV; col < a.cols; col += STEP) {
+                    scaled(piece_of<EPV, false>(col, a.cols), unit, f, w);
+#pragma unroll
+                    for (int i = 0; i < EPV; i++)
+                        if (__builtin_fabsf(f[i] * w[i]) == high) low = fmaxf(low, __builtin_fmaf(__builtin_fabsf(f[i]), __builtin_fabsf(w[i]), -high));
+                }
+                return low;
+            });
+        } else most = team_largest<1024>(mine, lds);
+        const RowCodesOf<EXACT> row_codes(most, rest);
+        if (threadIdx.x == 0) as_global<float>(a.scales)[row] = row_codes.scale;
+        for (int col = threadIdx.x * EPV; col < a.cols; col += STEP) {
+            const Piece here = piece_of<EPV, false>(col, a.cols);
+            scaled(here, unit, f, w);
+#pragma unroll
+            for (int i = 0; i < EPV; i++) p[i] = f[i] * w[i];
+            store_codes<EPV, false>(a.codes + (uint64_t)(row * a.cols), here, a.cols, row_codes.codes(p, [&](int at) { return (double)f[at] * w[at]; }));
+        }
+    } else {
         for (int col = threadIdx.x * EPV; col < a.cols; col += STEP) {
             const Piece p = piece_of<EPV, false>(col, a.cols);
             float f[EPV], w[EPV];
-            const u32x4 raw = load_row<ESZ, false, false>(again, p, a.cols);
-            Weights<T, false, WIDE> weights;
-            weights.load(a.weight, p, a.cols);
-            weights.unpack(a.weight, w);
-            Elem<T>::unpack(raw, f);
-            if constexpr (EXACT) {
-                if (pass == 0) {
+            scaled(p, r, f, w);
 #pragma unroll
-                    for (int i = 0; i < EPV; i++) most = fmax(most, __builtin_fabs((double)f[i] * w[i]));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < EPV; i++) f[i] = cut((double)f[i] * w[i] * factor);
-                    store_codes<EPV, false>(a.codes + (uint64_t)(row * a.cols), p, a.cols, f);
-                }
-                continue;
-            }
-#pragma unroll
-            for (int i = 0; i < EPV; i++) f[i] = f[i] * r * w[i];
-            if (!FP8) store_row<ESZ, false>(a.y + at, p, a.cols, Elem<T>::pack(f));
-            else if (pass == 0) {
-#pragma unroll
-                for (int i = 0; i < EPV; i++) amax = fmaxf(amax, __builtin_fabsf(f[i]));
-            } else {
-#pragma unroll
-                for (int i = 0; i < EPV; i++) f[i] *= inverse;
-                store_codes<EPV, false>(a.codes + (uint64_t)(row * a.cols), p, a.cols, f);
-            }
-        }
-        if (FP8 && pass == 0) {
-            if constexpr (EXACT) {
-                float none = 0.0f;
-                team_sum_largest<1024>(none, most, lds, lds_most);
-                fp8_scale(most, r, scale, factor);
-            } else {
-                scale = fp8_scale(team_largest<1024>(amax, lds));
-                inverse = 1.0f / scale;
-            }
-            if (threadIdx.x == 0) as_global<float>(a.scales)[row] = scale;
+            for (int i = 0; i < EPV; i++) f[i] *= w[i];
+            store_row<ESZ, false>(a.y + at, p, a.cols, Elem<T>::pack(f));
         }
     }
 }

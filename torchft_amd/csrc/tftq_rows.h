@@ -194,46 +194,6 @@ DEV float team_largest(float v, float *lds)
     return v;
 }
 
-// A sum, and the largest of 64-bit numbers that are not negative (NaN is none of them); lds: TEAM / 64 of each.
-template <int CTRL>
-DEV double dpp_largest(double v)
-{
-    const u32x2 w = __builtin_bit_cast(u32x2, v);
-    return fmax(v, __builtin_bit_cast(double, u32x2{as_u(dpp_mov<CTRL>(as_f(w.x))), as_u(dpp_mov<CTRL>(as_f(w.y)))}));
-}
-DEV double bcast_lane64(double v, int lane)
-{
-    const u32x2 w = __builtin_bit_cast(u32x2, v);
-    return __builtin_bit_cast(double, u32x2{as_u(bcast_lane(as_f(w.x), lane)), as_u(bcast_lane(as_f(w.y), lane))});
-}
-template <int TEAM>
-DEV void team_sum_largest(float &sum, double &most, float *lds, double *lds_most)
-{
-    sum = team_sum<(TEAM > 64 ? 64 : TEAM)>(sum, lds);
-    if (TEAM >= 2) most = dpp_largest<0xB1>(most);
-    if (TEAM >= 4) most = dpp_largest<0x4E>(most);
-    if (TEAM >= 8) most = dpp_largest<0x141>(most);
-    if (TEAM >= 16) most = dpp_largest<0x140>(most);
-    if (TEAM >= 32) {
-        const double a = fmax(bcast_lane64(most, 0), bcast_lane64(most, 16)), b = fmax(bcast_lane64(most, 32), bcast_lane64(most, 48));
-        most = TEAM > 32 ? fmax(a, b) : (threadIdx.x & 32) ? b : a;
-    }
-    if (TEAM > 64) {
-        if ((threadIdx.x & 63) == 0) {
-            lds[threadIdx.x >> 6] = sum;
-            lds_most[threadIdx.x >> 6] = most;
-        }
-        __syncthreads();
-        sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < TEAM / 64; i++) {
-            sum += lds[i];
-            most = fmax(most, lds_most[i]);
-        }
-        __syncthreads();
-    }
-}
-
 // How many lanes take a row, and how many vectors each.
 struct RowShape {
     int team, nv;

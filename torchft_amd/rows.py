@@ -88,7 +88,8 @@ def rms_norm(x: torch.Tensor, weight: "torch.Tensor | None" = None, residual: "t
 
 
 def rms_norm_fp8(x: torch.Tensor, weight: "torch.Tensor | None" = None, residual: "torch.Tensor | None" = None, eps: float = 1e-6):
-    """:func:`rms_norm` with y as :class:`FP8Rows`, rounded once from float32.  It has no gradient and refuses one."""
+    """:func:`rms_norm` with y as :class:`FP8Rows`: the codes are the nearest to ``448 h weight / max |h weight|``, the even one of two that
+    are as near.  It has no gradient and refuses one."""
     got = (_native or _module()).rms_norm(x, weight, residual, eps, True)
     rows = FP8Rows(got[0], got[1], x.dtype)
     return rows if residual is None else (rows, got[2])
