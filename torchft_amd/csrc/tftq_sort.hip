@@ -10,6 +10,7 @@
 // bits: counts of tiles of 2048, then places (three from 131072 on, where every tile would read too many counts).  Numbers
 // that another stream changes between the two would not fit the counts; places are held below n, whatever memory says.
 #include "tftq_sort.h"
+#include "tftq_fill.h"
 
 DEV u32 sort_key(const SortArgs &a, int64_t i)
 {
@@ -80,12 +81,11 @@ DEV u32 sort_prefix(u32 v, u32 *sums)
 // Workgroups from `tiles` on write zeros, a vector to a lane: they start and end in their order, so that what is written at
 // a time is one piece of memory that moves on (1050 MB at 6.6 TB/s; 5.3 with 64 KB to a workgroup, 4.7 with as many
 // workgroups as run at once and all of them side by side).
-TFTQ_HD static inline int sort_fill_rounds(int64_t bytes) { return (int)(bytes >> 34) + 1; }  // a grid has fewer than 2^32 threads
 template <int THREADS>
 DEV bool sort_fill(const SortArgs &a, int tiles)
 {
     if ((int)blockIdx.x < tiles) return false;
-    const int rounds = sort_fill_rounds(a.fill_bytes);
+    const int rounds = fill_rounds(a.fill_bytes);
     int64_t at = ((int64_t)((int)blockIdx.x - tiles) * rounds * THREADS + threadIdx.x) * 16;
     for (int r = 0; r < rounds; r++, at += THREADS * 16)
         if (at < a.fill_bytes) store_bytes(a.fill + (uint64_t)at, (u32)min((int64_t)16, a.fill_bytes - at), u32x4{0, 0, 0, 0});
@@ -304,8 +304,7 @@ bool sort_needs_keys(int64_t n, int64_t classes) { return sort_searches(n, class
 // Workgroups for so many tiles and the zeros.
 static unsigned sort_groups(const SortArgs &a, int tiles, int threads)
 {
-    const int64_t each = (int64_t)threads * 16 * sort_fill_rounds(a.fill_bytes);
-    return (unsigned)(tiles + (a.fill_bytes + each - 1) / each);
+    return (unsigned)(tiles + fill_groups(a.fill_bytes, threads));
 }
 
 static int sort_offsets(SortArgs a, hipStream_t st)
@@ -339,11 +338,11 @@ int sort_numbers(const SortArgs &in, void *workspace, hipStream_t st)
     p.counts = (uint64_t)workspace;
     p.width = width;
     const uint64_t pairs = p.counts + (uint64_t)(p.pitch + 1) * SORT_DIGITS * 4, pair = ((uint64_t)a.n * 8 + 15) & ~(uint64_t)15;
-    // the launches' shares of the zeros
-    const int64_t share = (in.fill_bytes / (2 * passes) + 4095) & ~(int64_t)4095;
-    auto next_share = [&](bool first) {
-        if (!first) a.fill += (uint64_t)a.fill_bytes;
-        a.fill_bytes = std::min(share, in.fill_bytes - (int64_t)(a.fill - in.fill));
+    int launch = 0;
+    auto next_share = [&] {  // of the zeros
+        const int64_t begin = fill_begin(in.fill_bytes, 2 * passes, launch++);
+        a.fill = in.fill + (uint64_t)begin;
+        a.fill_bytes = fill_begin(in.fill_bytes, 2 * passes, launch) - begin;
     };
     for (int pass = 0; pass < passes; pass++) {
         const bool last = pass == passes - 1;
@@ -355,11 +354,11 @@ int sort_numbers(const SortArgs &in, void *workspace, hipStream_t st)
         p.offsets = passes == 1 ? a.offsets : 0;
         p.shift = pass * width;
         void *args[] = {(void *)&a, (void *)&p}, *before[] = {(void *)&p};
-        next_share(pass == 0);
+        next_share();
         if (const int rc = (int)hipLaunchKernel((const void *)k_sort_count, dim3(sort_groups(a, p.tiles, SORT_THREADS)), dim3(SORT_THREADS), args, 0, st)) return rc;
         if (p.tiles > SORT_DIRECT)
             if (const int rc = (int)hipLaunchKernel((const void *)k_sort_before, dim3(1u << width), dim3(256), before, 0, st)) return rc;
-        next_share(false);
+        next_share();
         if (const int rc = (int)hipLaunchKernel((const void *)k_sort_place, dim3(sort_groups(a, p.tiles, SORT_THREADS)), dim3(SORT_THREADS), args, 0, st)) return rc;
     }
     return a.offsets && passes > 1 ? sort_offsets(a, st) : 0;
