@@ -21,10 +21,13 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/DynamicTypes.h>
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 
 namespace {
@@ -87,6 +90,17 @@ int64_t bytes_needed(int64_t size, const char *what)
 constexpr c10::DispatchKeySet WRAPPERS({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched,
                                         c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::BatchedNestedTensor,
                                         c10::DispatchKey::Functionalize});
+
+// Whether this thread's operations are recorded, or made up, and not only done: a trace would have the allocation of a result and not the
+// kernel that writes it.  Modes that look on are no matter.
+bool traced()
+{
+    using Modes = c10::impl::TorchDispatchModeTLS;
+    using Key = c10::impl::TorchDispatchModeKey;
+    if (torch::jit::tracer::isTracing() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch)) return true;
+    return Modes::any_modes_set() && (Modes::get_mode(Key::PROXY) || Modes::get_mode(Key::FAKE) || Modes::get_mode(Key::FUNCTIONAL));
+}
+const char *const TRACED = "Only plain tensors are supported: a trace of the call would not have its kernels";
 
 int code_of(const Tensor &t)
 {
@@ -164,11 +178,12 @@ bool wants_grad(const Tensor &t) { return t.defined() && t.requires_grad(); }
 bool wants_grad(const Maybe &t) { return t && wants_grad(*t); }
 Tensor or_none(const Maybe &t) { return t ? *t : Tensor(); }
 
-// Begins a backward pass.  Under a stream capture no gradient may go to a node of the default stream (a leaf's, made with an eager
+// Begins a backward pass, which is not traced either.  Under a stream capture no gradient may go to a node of the default stream (a leaf's, made with an eager
 // graph of the leaf that still lives): that stream would have to wait for the capture, which it cannot, and the capture breaks
 // off in ways that the process may not survive.  Refused here, where nothing has crossed yet.
 void begin_backward(const Tensor &beside)
 {
+    require(!traced(), TRACED);
     const c10::hip::HIPStream here = c10::hip::getCurrentHIPStream(beside.device().index());
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     if (here.id() == 0 || hipStreamIsCapturing(here.stream(), &status) != hipSuccess || status != hipStreamCaptureStatusActive) return;
@@ -512,6 +527,7 @@ PyObject *call(const char *name, Py_ssize_t got, Py_ssize_t want, F body)
     }
     HANDLE_TH_ERRORS
     try {
+        require(!traced(), TRACED);
         return body();
     } catch (const Refused &e) {
         PyErr_SetString(PyExc_AssertionError, e.why.c_str());

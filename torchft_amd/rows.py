@@ -11,7 +11,8 @@ All take fp32, fp16 and bf16 tensors in any order (what is not stored in rows is
 an order that the arguments alone decide, and round each result once; gradients are computed once (no second
 derivatives, no forward mode).  Kernels are enqueued on the current stream of the tensors' device; nothing synchronises the
 host, no function keeps anything from one call for the next, and all can be captured into graphs (a backward pass once no
-graph of the same leaves is left that was made on the default stream; it is refused until then).  There is no CPU or eager fallback.
+graph of the same leaves is left that was made on the default stream; it is refused until then).  A call while a trace is taken (``make_fx``,
+``torch.jit.trace``, ``torch.export``) is refused: the trace would not have its kernels.  There is no CPU or eager fallback.
 """
 
 from __future__ import annotations
