@@ -16,10 +16,13 @@
 
 #include <atomic>
 #include <string>
+#include <unordered_set>
+#include <vector>
 
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/DynamicTypes.h>
@@ -178,20 +181,38 @@ bool wants_grad(const Tensor &t) { return t.defined() && t.requires_grad(); }
 bool wants_grad(const Maybe &t) { return t && wants_grad(*t); }
 Tensor or_none(const Maybe &t) { return t ? *t : Tensor(); }
 
-// Begins a backward pass, which is not traced either.  Under a stream capture no gradient may go to a node of the default stream (a leaf's, made with an eager
-// graph of the leaf that still lives): that stream would have to wait for the capture, which it cannot, and the capture breaks
-// off in ways that the process may not survive.  Refused here, where nothing has crossed yet.
+// Begins a backward pass, which is not traced either.  Under a stream capture no gradient may go to a node of the default stream (a
+// leaf's, made with an eager graph of the leaf that still lives), neither from here nor from a node behind: that stream would have to wait for
+// the capture, which it cannot, and the capture breaks off in ways that the process may not survive.  Refused here, where nothing has crossed
+// yet.
 void begin_backward(const Tensor &beside)
 {
+    using torch::autograd::Node;
     require(!traced(), TRACED);
     const c10::hip::HIPStream here = c10::hip::getCurrentHIPStream(beside.device().index());
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     if (here.id() == 0 || hipStreamIsCapturing(here.stream(), &status) != hipSuccess || status != hipStreamCaptureStatusActive) return;
-    const std::shared_ptr<torch::autograd::Node> node = torch::autograd::get_current_node();
+    const std::shared_ptr<Node> node = torch::autograd::get_current_node();
     if (!node) return;
-    for (const torch::autograd::Edge &edge : node->next_edges()) {
-        const auto there = edge.function ? edge.function->stream() : std::nullopt;
-        require(!there || there->id() != 0, "A backward pass cannot be captured while a graph of the same tensors lives that was made on the default stream");
+    const auto *runs = torch::autograd::get_current_graph_task_exec_info();  // empty: all nodes
+    std::vector<const Node *> to_see = {node.get()};
+    std::unordered_set<const Node *> seen = {node.get()};
+    while (!to_see.empty()) {
+        const Node *from = to_see.back();
+        to_see.pop_back();
+        for (const torch::autograd::Edge &edge : from->next_edges()) {
+            Node *next = edge.function.get();
+            if (!next || !seen.insert(next).second) continue;
+            bool follow = true;  // a node whose gradient is only wanted gets one too, but hands none on
+            if (runs && !runs->empty()) {
+                const auto it = runs->find(next);
+                if (it == runs->end() || !it->second.should_execute()) continue;
+                follow = it->second.needed_;
+            }
+            const auto there = next->stream();
+            require(!there || there->id() != 0, "A backward pass cannot be captured while a graph of the same tensors lives that was made on the default stream");
+            if (follow) to_see.push_back(next);
+        }
     }
 }
 
