@@ -33,6 +33,7 @@ __global__ __launch_bounds__(256) void k_embedding(const EmbeddingArgs a)
     if (row >= a.rows) return;
     const int64_t id = a.wide ? as_global<const int64_t>(a.ids)[row] : as_global<const int32_t>(a.ids)[row];
     const bool inside = id >= 0 && id < a.vocab;
+    const float scale = inside ? a.scale : 0.0f;  // zeros outside, whatever the scale
     const uint64_t from = a.table + (uint64_t)(id * a.stride), to = a.out + (uint64_t)(row * a.cols) * ESZ;
     for (int col = lane * EPV; col < a.cols; col += U * TEAM * EPV) {
         u32x4 raw[U];
@@ -47,7 +48,7 @@ __global__ __launch_bounds__(256) void k_embedding(const EmbeddingArgs a)
             float f[EPV];
             Elem<T>::unpack(raw[u], f);
 #pragma unroll
-            for (int i = 0; i < EPV; i++) f[i] *= a.scale;
+            for (int i = 0; i < EPV; i++) f[i] *= scale;
             store_row<ESZ, NARROW>(to, piece_of<EPV, NARROW>(col + u * TEAM * EPV, a.cols), a.cols, Elem<T>::pack(f));
         }
     }
