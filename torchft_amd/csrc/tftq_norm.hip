@@ -12,7 +12,8 @@
 // near.  In fp32 that quotient is off by 5 2^-24 at most, so that the codes on both sides of it, 2^-21 away, differ once
 // in 10^5 elements; there products in 64 bits, which are exact, say on which side of the border it lies, or on it.  Of bf16 rows and
 // weights one in 2000 lies on a border; their products are exact in fp32 already.  8192x2048 fp32 25 us (26 with 64-bit products of all
-// elements), 8192x4096 bf16 with a residual 40.8 (39.8 without a thought of borders, 41.0 with fp32 weights, 43.6 where these are ones).
+// elements), 8192x4096 bf16 with a residual 40.2 (39.8 from an fp32 y, which had a quarter of the quotients on a border on the wrong side; 40.7
+// with fp32 weights, 42.7 where these are ones: one in 130 is on a border).
 #include "tftq_rows.h"
 
 struct NormArgs {
@@ -76,7 +77,7 @@ DEV void split_root(float r, float &unit, float &rest)
     unit = r != r ? r : as_f(as_u(r) & 0x7f800000u);
     rest = as_f((as_u(r) & 0x007fffffu) | 0x3f800000u);
 }
-// The largest |h unit w| of a row in 64 bits: `mine` is a lane's, rounded; where that is the row's, left(mine) is the largest part that
+// The largest |h unit w| of a row in 64 bits: `mine` is a lane's, rounded; where that is the row's, and not 0, left(mine) is the largest part that
 // such numbers' rounding left out.  lds: 2 TEAM / 64 floats.
 template <int TEAM, class F>
 DEV double team_largest_product(float mine, float *lds, F left)
@@ -85,7 +86,7 @@ DEV double team_largest_product(float mine, float *lds, F left)
     constexpr float NONE = -__builtin_inff();
     float high = team_max<(TEAM > 64 ? 64 : TEAM)>(mine, lds), low = NONE;
     if (TEAM <= 64) {
-        if (mine == high) low = left(high);
+        if (mine == high && high > 0.0f) low = left(high);
         low = team_max<(TEAM > 64 ? 64 : TEAM)>(low, lds);
     } else {
         const float wave = high;
@@ -94,7 +95,7 @@ DEV double team_largest_product(float mine, float *lds, F left)
 #pragma unroll
         for (int i = 0; i < WAVES; i++) high = fmaxf(high, lds[i]);
         if (wave == high) {
-            if (mine == high) low = left(high);
+            if (mine == high && high > 0.0f) low = left(high);
             low = team_max<64>(low, lds);
         }
         if ((threadIdx.x & 63) == 0) lds[WAVES + (threadIdx.x >> 6)] = low;
@@ -125,8 +126,7 @@ struct RowCodes {
         over = by * 0x1.000008p+0f;
     }
     // Of any products p = h unit w, rounded: the codes 2^-21 below and above 448 p / most, off by 5 2^-24 at most.  Where they differ,
-    // the sign of 448 h unit w - border most, two products of 53 bits at most, says which it is.  Borders are odd multiples of the step
-    // of five significant bits, 2^-10 at least.  wide(i): h unit w in 64 bits.
+    // the sign of 896 h unit w - (both codes' numbers) most, two products of 53 bits at most, says which it is.  wide(i): h unit w in 64 bits.
     template <int EPV, class F>
     DEV u32x2 codes(const float (&p)[EPV], F wide) const
     {
@@ -136,13 +136,14 @@ struct RowCodes {
             u32 code = pack_fp8x4(p[i] * under, p[i + 1] * under, p[i + 2] * under, p[i + 3] * under);
             const u32 differ = code ^ pack_fp8x4(p[i] * over, p[i + 1] * over, p[i + 2] * over, p[i + 3] * over);
             if (differ) {
+                float lower[4], upper[4];
+                unpack_fp8x4(code, lower);
+                unpack_fp8x4(code ^ differ, upper);
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const u32 mine = differ & 0xFFu << (8 * j);
                     if (!mine) continue;
-                    const float q = __builtin_fabsf(p[i + j] * under);
-                    const float border = q < 0x1p-6f ? __builtin_rintf(q * 1024.0f) * 0x1p-10f : as_f((as_u(q) + 0x40000u) & 0xfff80000u);
-                    const double above = __builtin_fma(-(double)border, most, 448.0 * __builtin_fabs(wide(i + j)));
+                    const double above = __builtin_fma(-(double)__builtin_fabsf(lower[j] + upper[j]), most, 896.0 * __builtin_fabs(wide(i + j)));
                     if (above > 0.0 || (above == 0.0 && (code >> (8 * j) & 1))) code ^= mine;
                 }
             }
@@ -193,13 +194,13 @@ DEV void store_codes(uint64_t row, const Piece &p, int cols, u32x2 c)
 }
 
 // One team of TEAM lanes to a row, which stays in its registers: memory is read and written once, and bounds it.  8192x4096 bf16
-// with a residual 44 us (268 MB, 6.1 TB/s), to 8 bits 39 (235 MB, 6.0); 163840x128 fp16 15.2 (84 MB, 5.5); one row 2.7.
+// with a residual 44 us (268 MB, 6.1 TB/s), to 8 bits 40 (235 MB, 5.9); 163840x128 fp16 15.2 (84 MB, 5.5); one row 2.7 (3.1 a launch among ten).
 template <class T, int TEAM, int NV, bool NARROW, bool WIDE, bool FP8>
 __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void k_rms_norm(const NormArgs a)
 {
     constexpr int ESZ = Elem<T>::ESZ, EPV = Elem<T>::EPV, TEAMS = TEAM > 256 ? 1 : 256 / TEAM;
-    // products of two 16-bit numbers are exact, those of bf16 448 times too; kept in registers where they leave eight wavefronts to a unit
-    constexpr bool LOW = ESZ == 4 || WIDE, EXACT = !LOW && std::is_same<T, bf16_tag>::value, KEEP = NV * EPV <= (WIDE ? 8 : 16);
+    // products of two 16-bit numbers are exact, those of bf16 448 times too; kept in registers where these leave eight wavefronts to a unit
+    constexpr bool LOW = ESZ == 4 || WIDE, EXACT = !LOW && std::is_same<T, bf16_tag>::value, KEEP = NV * EPV <= 16;
     __shared__ float lds[TEAM > 64 ? 2 * (TEAM / 64) : 1];
     const int lane = threadIdx.x % TEAM;
     const int64_t row = a.row0 + (int64_t)blockIdx.x * TEAMS + threadIdx.x / TEAM;
@@ -245,14 +246,25 @@ __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void k_rms_norm(const Norm
         split_root(r, unit, rest);
         if (EXACT) unit *= 0.875f;
         float kept[KEEP ? NV : 1][EPV];
-        // else they are made again, not kept by the compiler, whose registers rows of 32768 take up (fp32 weights: 57 us of 72)
-        auto again = [&] { if (!KEEP) asm("" : "+v"(unit)); };
+        auto again = [&] { if (!KEEP) asm("" : "+v"(unit)); };  // else they are made again, not kept by the compiler
         auto products = [&](int v, float (&p)[EPV]) {
             float f[EPV], w[EPV];
             Elem<T>::unpack(raw[v], f);
             weights[v].unpack(a.weight, w);
 #pragma unroll
             for (int i = 0; i < EPV; i++) p[i] = f[i] * unit * w[i];
+        };
+        // of one that is not 0, and so in the row; fp32 weights of two 16-bit vectors, 16 registers, are read again instead of kept (2048x16384
+        // bf16 with a residual 46 us, 57 with 74 registers, 74 with spills)
+        auto factors = [&](int v, int i, float &f, float &w) {
+            float all[EPV];
+            Elem<T>::unpack(raw[v], all);
+            f = all[i] * unit;
+            if (WIDE && NV == 2) w = as_global<const float>(a.weight)[piece[v].at + i];
+            else {
+                weights[v].unpack(a.weight, all);
+                w = all[i];
+            }
         };
 #pragma unroll
         for (int v = 0; v < NV; v++) {
@@ -268,13 +280,15 @@ __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void k_rms_norm(const Norm
                 float low = -__builtin_inff();
 #pragma unroll
                 for (int v = 0; v < NV; v++) {
-                    float f[EPV], w[EPV];
-                    Elem<T>::unpack(raw[v], f);
-                    weights[v].unpack(a.weight, w);
+                    float(&p)[EPV] = kept[KEEP ? v : 0];
+                    if (!KEEP) products(v, p);
 #pragma unroll
                     for (int i = 0; i < EPV; i++)
-                        if (__builtin_fabsf(f[i] * unit * w[i]) == high)
-                            low = fmaxf(low, __builtin_fmaf(__builtin_fabsf(f[i] * unit), __builtin_fabsf(w[i]), -high));
+                        if (__builtin_fabsf(p[i]) == high) {
+                            float f, w;
+                            factors(v, i, f, w);
+                            low = fmaxf(low, __builtin_fmaf(__builtin_fabsf(f), __builtin_fabsf(w), -high));
+                        }
                 }
                 return low;
             });
@@ -287,10 +301,9 @@ __global__ __launch_bounds__(TEAM > 256 ? TEAM : 256) void k_rms_norm(const Norm
             float(&p)[EPV] = kept[KEEP ? v : 0];
             if (!KEEP) products(v, p);
             const u32x2 codes = row_codes.codes(p, [&](int at) {
-                float f[EPV], w[EPV];
-                Elem<T>::unpack(raw[v], f);
-                weights[v].unpack(a.weight, w);
-                return (double)(f[at] * unit) * w[at];
+                float f, w;
+                factors(v, at, f, w);
+                return (double)f * w;
             });
             store_codes<EPV, NARROW>(a.codes + (uint64_t)(row * a.cols), piece[v], a.cols, codes);
         }
@@ -718,12 +731,15 @@ static bool narrow_row(int64_t cols, int size) { return cols * size < 16; }
 template <class T, bool WIDE, bool FP8>
 static int norm(NormArgs a, hipStream_t st)
 {
-    const RowShape shape = norm_shape((a.cols + Elem<T>::EPV - 1) / Elem<T>::EPV);
+    RowShape shape = norm_shape((a.cols + Elem<T>::EPV - 1) / Elem<T>::EPV);
+    if (WIDE && FP8 && shape.nv == 4) shape = {0, 0};  // too long with fp32 weights: 1024x32768 bf16 34 us, with a residual 58, 67 with spills; 1600x20000 55, 57
     const void *k = (const void *)k_rms_norm_long<T, WIDE, FP8>;
 #define K(TEAM, NV, NARROW) k = (const void *)k_rms_norm<T, TEAM, NV, NARROW, WIDE, FP8>
     switch (shape.team * 16 + shape.nv) {
-        SHAPE(8, 1) SHAPE(8, 2) SHAPE(16, 2) SHAPE(32, 2) SHAPE(64, 2) SHAPE(256, 1) SHAPE(512, 1) SHAPE(512, 2) SHAPE(1024, 2) SHAPE(1024, 4)
+        SHAPE(8, 1) SHAPE(8, 2) SHAPE(16, 2) SHAPE(32, 2) SHAPE(64, 2) SHAPE(256, 1) SHAPE(512, 1) SHAPE(512, 2) SHAPE(1024, 2)
     }
+    if constexpr (!(WIDE && FP8))
+        if (shape.nv == 4) K(1024, 4, false);
     if (narrow_row(a.cols, Elem<T>::ESZ)) K(8, 1, true);
 #undef K
     const int threads = shape.team == 0 ? 1024 : shape.team > 256 ? shape.team : 256, teams = shape.team == 0 ? 1 : threads / shape.team;
