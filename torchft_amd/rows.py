@@ -1,7 +1,8 @@
 """Row operators of a training step, between its linear layers (no counterpart in the reference).
 
 * :func:`rms_norm` / :func:`rms_norm_fp8`: root-mean-square norm behind the residual's addition, in the rows' type
-  with gradients, or in 8 bits with a scale a row (what :func:`dispatch` sends to experts on other GPUs);
+  with gradients, or in 8 bits with a scale a row (:func:`dispatch` moves such rows to their experts' places on the same GPU; no
+  collective here takes them, and products take their values);
 * :func:`dropout`: with a mask that a counter-based generator makes again in the backward pass, added to the residual;
 * :func:`embedding`: rows of a table, scaled; its gradient is summed over sorted tokens;
 * :func:`sort_by_expert`, :func:`dispatch`, :func:`combine`: tokens by expert, their rows there, and the experts' rows
